@@ -113,8 +113,9 @@ def _plain(state):
         factor = torch.rsqrt((x * x).mean(dim=1, keepdim=True) + EPS)
         x = x * state["gain"].float()
     top = x.abs().amax(dim=1, keepdim=True)
-    q = torch.where(top > 0, torch.round(x * (127.0 / top)), torch.zeros_like(x))
-    scale = top / 127.0
+    most = torch.full_like(top, 127.0)            # (one division each: torch takes a number's through a rounded reciprocal)
+    q = torch.where(top > 0, torch.round(x * (most / top)), torch.zeros_like(x))
+    scale = top / most
     if factor is not None:
         scale = scale * factor
     y = (q @ values.t()) * (scale * scales)
