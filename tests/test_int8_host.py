@@ -1,0 +1,87 @@
+"""What the products in 8-bit integers refuse, where no GPU is needed to say so."""
+import pytest
+import torch
+
+from llm_infer_rust_b200.kernels import int8, ops
+from llm_infer_rust_b200.kernels.ops import KernelError
+
+
+def weight(n=4, k=32):
+    return int8.Int8Weight(torch.zeros(n, int8.row_pitch(k), dtype=torch.int8)[:, :k], torch.ones(n))
+
+
+def aligned(w):
+    return w.values.data_ptr() % 16 == 0
+
+
+def test_row_pitch():
+    assert [int8.row_pitch(k) for k in (1, 16, 17, 4096)] == [16, 16, 32, 4096]
+
+
+@pytest.mark.parametrize("x", [torch.zeros(2, 32, dtype=torch.float16), torch.zeros(2, 32, dtype=torch.int8), torch.zeros(32),
+                               torch.zeros(2, 64)[:, ::2], torch.zeros(32, 2).t(), torch.zeros(1, 32).expand(3, 32), torch.zeros(2, 0)])
+def test_rows_that_are_refused(x):
+    with pytest.raises(KernelError, match="dtype|unit inner stride|columns are refused"):
+        int8.int8_linear(x, weight())
+    with pytest.raises(KernelError, match="dtype|unit inner stride|columns are refused"):
+        int8.quantize_rows(x)
+
+
+def test_more_columns_than_32_bit_sums_hold():
+    with pytest.raises(KernelError, match="131071"):
+        int8.quantize_rows(torch.zeros(1, 131072))
+    with pytest.raises(KernelError, match="131071"):
+        int8.int8_linear(int8.Int8Rows(torch.zeros(1, 131072, dtype=torch.int8), torch.ones(1)), weight())
+
+
+@pytest.mark.parametrize("w,what", [
+    (int8.Int8Weight(torch.zeros(4, 32), torch.ones(4)), "int8 values"),
+    (int8.Int8Weight(torch.zeros(4, 32, dtype=torch.int8), torch.ones(4, dtype=torch.bfloat16)), "float32 scales"),
+    (int8.Int8Weight(torch.zeros(4, 32, dtype=torch.int8), torch.ones(5)), "one scale a row"),
+    (int8.Int8Weight(torch.zeros(4, 32, dtype=torch.int8), torch.ones(8)[::2]), "one scale a row"),
+    (int8.Int8Weight(torch.zeros(32, 4, dtype=torch.int8).t(), torch.ones(4)), "unit inner stride"),
+    (int8.Int8Weight(torch.zeros(4, 33, dtype=torch.int8)[:, :32], torch.ones(4)), "multiple of 16"),
+    (int8.Int8Weight(torch.zeros(1, 32, dtype=torch.int8).expand(4, 32), torch.ones(4)), "multiple of 16"),
+    (int8.Int8Weight(torch.zeros(4, 48, dtype=torch.int8)[:, 1:33], torch.ones(4)), "multiple of 16")])
+def test_weights_that_are_refused(w, what):
+    with pytest.raises(KernelError, match=what):
+        int8.int8_linear(torch.zeros(2, 32), w)
+
+
+def test_sizes_that_do_not_fit(monkeypatch):
+    monkeypatch.setattr(ops, "_cuda", lambda *tensors: None)
+    with pytest.raises(KernelError, match="the rows have 16 columns, the weight has 32"):
+        int8.int8_linear(torch.zeros(2, 16), weight())
+    with pytest.raises(KernelError, match="gate and up rows"):
+        int8.int8_glu(torch.zeros(2, 32), weight(5))
+    for bias in (torch.zeros(4, dtype=torch.bfloat16), torch.zeros(3), torch.zeros(8)[::2]):
+        with pytest.raises(KernelError, match="the bias is float32"):
+            int8.int8_linear(torch.zeros(2, 32), weight(), bias=bias)
+    with pytest.raises(KernelError, match="gate 'relu' is refused"):
+        int8.int8_glu(torch.zeros(2, 32), weight(), glu="relu")
+    with pytest.raises(KernelError, match="dtype"):
+        int8.int8_linear(torch.zeros(2, 32), weight(), out_dtype=torch.float16)
+
+
+def test_norms_that_do_not_fit():
+    x, gain = torch.zeros(2, 32), torch.ones(32)
+    for pending in (ops.PendingNorm(x, None, torch.ones(31), 1e-6), ops.PendingNorm(x, torch.zeros(2, 32, dtype=torch.bfloat16), gain, 1e-6),
+                    ops.PendingNorm(x, torch.zeros(3, 32), gain, 1e-6), ops.PendingNorm(x, None, torch.ones(64)[::2], 1e-6)):
+        with pytest.raises(KernelError, match="norm weight|residual"):
+            int8.int8_linear(pending, weight())
+
+
+def test_there_is_no_cpu_path():
+    with pytest.raises(KernelError, match="CUDA tensors only"):
+        int8.int8_linear(torch.zeros(2, 32), weight())
+    with pytest.raises(KernelError, match="CUDA tensors only"):
+        int8.quantize_rows(torch.zeros(2, 32))
+
+
+def test_8_bit_values_of_a_checkpoint_are_laid_out():
+    values = torch.arange(-60, 60, dtype=torch.int8).view(6, 20)
+    w = int8.int8_weight_from(values, torch.ones(6, 1, dtype=torch.float64))
+    assert torch.equal(w.values, values) and w.values.stride() == (32, 1) and w.scales.shape == (6,) and w.scales.dtype == torch.float32
+    with pytest.raises(KernelError, match="N scales"):
+        int8.int8_weight_from(values, torch.ones(5))
+    assert torch.equal(w.dequantize(), values.float())
