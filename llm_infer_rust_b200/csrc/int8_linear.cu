@@ -6,68 +6,20 @@
 #include <math.h>
 
 #include "int8_rows.cuh"
+#include "int8_tcgen05.cuh"
 
 constexpr int MAX_K = 131071;
 
-enum : int { INT8_PLAIN = 0, INT8_GLU = 1 };
-
-struct Int8ProductParams {
-  const int8_t* q;           // [tokens, k], rows q_pitch bytes apart
-  const float* s;            // [tokens]
-  const int8_t* w;           // [rows, k], rows w_pitch bytes apart
-  const float* c;            // [rows]
-  const float* bias;         // [rows] or null
-  void* out;                 // [tokens, n]
-  int tokens, n, k;          // n: columns of out (INT8_GLU: w has 2 n rows)
-  long long q_pitch, w_pitch;
-  float limit, alpha;
-};
-
-// 64 tokens x 64 columns a block, four bytes of k an instruction.
-constexpr int TILE = 64, KB = 64;
-template <typename T, int MODE>
-__global__ void __launch_bounds__(256) int8_product_kernel(const Int8ProductParams P) {
-  __shared__ uint32_t qs[TILE][KB / 4 + 1], ws[(MODE == INT8_GLU ? 2 : 1) * TILE][KB / 4 + 1];
-  constexpr int HALVES = MODE == INT8_GLU ? 2 : 1;
-  const int t0 = blockIdx.y * TILE, n0 = blockIdx.x * TILE;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  int acc[HALVES][4][4] = {};
-  pdl_launch_dependents();
-  pdl_wait();
-  for (int k0 = 0; k0 < P.k; k0 += KB) {
-    for (int i = threadIdx.x; i < TILE * KB; i += 256) {
-      const int r = i / KB, k = i % KB;
-      reinterpret_cast<int8_t*>(qs[r])[k] = t0 + r < P.tokens && k0 + k < P.k ? P.q[static_cast<size_t>(t0 + r) * P.q_pitch + k0 + k] : 0;
-      for (int h = 0; h < HALVES; ++h)
-        reinterpret_cast<int8_t*>(ws[h * TILE + r])[k] =
-            n0 + r < P.n && k0 + k < P.k ? P.w[static_cast<size_t>(h * P.n + n0 + r) * P.w_pitch + k0 + k] : 0;
-    }
-    __syncthreads();
-    for (int k = 0; k < KB / 4; ++k)
-      for (int h = 0; h < HALVES; ++h)
-        for (int i = 0; i < 4; ++i)
-          for (int j = 0; j < 4; ++j)
-            acc[h][i][j] = __dp4a(static_cast<int>(qs[ty + 16 * i][k]), static_cast<int>(ws[h * TILE + tx + 16 * j][k]), acc[h][i][j]);
-    __syncthreads();
-  }
-  T* out = static_cast<T*>(P.out);
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int t = t0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (t >= P.tokens || n >= P.n) continue;
-      float y[HALVES];
-      for (int h = 0; h < HALVES; ++h) {
-        y[h] = static_cast<float>(acc[h][i][j]) * (P.s[t] * P.c[h * P.n + n]);
-        if (P.bias) y[h] += P.bias[h * P.n + n];
-      }
-      out[static_cast<size_t>(t) * P.n + n] = from_f32<T>(MODE == INT8_GLU ? glu_product(y[0], y[HALVES - 1], P.limit, P.alpha) : y[0]);
-    }
-}
-
 static int int8_product(const Int8ProductParams& P, int mode, int out_code, cudaStream_t stream) {
-  auto kernel = mode == INT8_GLU ? (out_code == B200_F32 ? int8_product_kernel<float, INT8_GLU> : int8_product_kernel<__nv_bfloat16, INT8_GLU>)
-                                 : (out_code == B200_F32 ? int8_product_kernel<float, INT8_PLAIN> : int8_product_kernel<__nv_bfloat16, INT8_PLAIN>);
-  return b200_launch(kernel, dim3((P.n + TILE - 1) / TILE, (P.tokens + TILE - 1) / TILE), dim3(256), 0, stream, 0, P);
+  static int counts[64];                       // SMs of the devices that were asked (0: not yet)
+  int device = 0, sms = 148;
+  if (cudaGetDevice(&device) == cudaSuccess && device < 64) {
+    if (counts[device] == 0) cudaDeviceGetAttribute(&counts[device], cudaDevAttrMultiProcessorCount, device);
+    if (counts[device] > 0) sms = counts[device];
+  }
+  if (mode == INT8_GLU)
+    return out_code == B200_F32 ? i8tc::product<float, INT8_GLU>(P, sms, stream) : i8tc::product<__nv_bfloat16, INT8_GLU>(P, sms, stream);
+  return out_code == B200_F32 ? i8tc::product<float, INT8_PLAIN>(P, sms, stream) : i8tc::product<__nv_bfloat16, INT8_PLAIN>(P, sms, stream);
 }
 
 // ------------------------------------------------------------------ entry points
@@ -108,6 +60,6 @@ B200_EXPORT int b200_int8_linear(const void* x, const void* residual, const void
   }
   if (n == 0) return 0;
   const Int8ProductParams P = {static_cast<const int8_t*>(q), s, static_cast<const int8_t*>(w), c, bias, out, tokens, n, k,
-                               q_pitch, w_pitch, limit, alpha};
+                               q_pitch, w_pitch, limit, alpha, err};
   return int8_product(P, mode, out_code, stream);
 }
