@@ -6,17 +6,20 @@
 #include <math.h>
 
 #include "int8_rows.cuh"
+#include "int8_stream.cuh"
 #include "int8_tcgen05.cuh"
 
 constexpr int MAX_K = 131071;
 
-static int int8_product(const Int8ProductParams& P, int mode, int out_code, cudaStream_t stream) {
-  static int counts[64];                       // SMs of the devices that were asked (0: not yet)
-  int device = 0, sms = 148;
-  if (cudaGetDevice(&device) == cudaSuccess && device < 64) {
-    if (counts[device] == 0) cudaDeviceGetAttribute(&counts[device], cudaDevAttrMultiProcessorCount, device);
-    if (counts[device] > 0) sms = counts[device];
-  }
+static int sm_count() {
+  static int counts[64];                       // of the devices that were asked (0: not yet)
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device >= 64) return 148;
+  if (counts[device] == 0) cudaDeviceGetAttribute(&counts[device], cudaDevAttrMultiProcessorCount, device);
+  return counts[device] > 0 ? counts[device] : 148;
+}
+
+static int tiled_product(const Int8ProductParams& P, int mode, int out_code, int sms, cudaStream_t stream) {
   if (mode == INT8_GLU)
     return out_code == B200_F32 ? i8tc::product<float, INT8_GLU>(P, sms, stream) : i8tc::product<__nv_bfloat16, INT8_GLU>(P, sms, stream);
   return out_code == B200_F32 ? i8tc::product<float, INT8_PLAIN>(P, sms, stream) : i8tc::product<__nv_bfloat16, INT8_PLAIN>(P, sms, stream);
@@ -40,10 +43,16 @@ B200_EXPORT int b200_int8_rows(const void* x, const void* residual, const void* 
                                int k, long long x_pitch, long long q_pitch, int x_code, int gain_code, float eps, cudaStream_t stream) {
   Int8RowsParams R;
   const int rc = rows_params(R, x, residual, gain, sum_out, q, s, tokens, k, x_pitch, q_pitch, x_code, gain_code, eps);
-  return rc != 0 ? rc : tokens == 0 ? 0 : int8_rows_launch(R, x_code, gain_code, stream);
+  return rc != 0 ? rc : tokens == 0 ? 0 : int8_rows_launch(R, x_code, gain_code, sm_count(), stream);
 }
 
-// The product; `x` not null: of its rows, which go to q, s first.
+// 1 where the product of `tokens` rows of floats takes them to 8 bits itself: no place for q and s is needed.
+B200_EXPORT int b200_int8_alone(int tokens, int k) {
+  return k >= 1 && k <= MAX_K && i8st::takes(tokens, k) && i8st::fuses(tokens, k) ? 1 : 0;
+}
+
+// The product; `x` not null: of its rows, which go to q, s first (null where
+// b200_int8_alone says so).
 B200_EXPORT int b200_int8_linear(const void* x, const void* residual, const void* gain, void* sum_out, void* q, float* s,
                                  const void* w, const float* c, const float* bias, void* out, int tokens, int n, int k,
                                  long long x_pitch, long long q_pitch, long long w_pitch, int x_code, int gain_code, int out_code,
@@ -52,14 +61,18 @@ B200_EXPORT int b200_int8_linear(const void* x, const void* residual, const void
   if (tokens < 0 || n < 0 || k < 1 || k > MAX_K || q_pitch < k || w_pitch < k || (mode != INT8_PLAIN && mode != INT8_GLU)) return B200_BAD_SIZE;
   if (!int8_aligned(q, q_pitch) || !int8_aligned(w, w_pitch)) return B200_BAD_ALIGN;
   if (tokens == 0) return 0;
+  const int sms = sm_count();
+  const bool few = n > 0 && i8st::takes(tokens, k);
+  const Int8ProductParams P = {static_cast<const int8_t*>(q), s, static_cast<const int8_t*>(w), c, bias, out, tokens, n, k,
+                               q_pitch, w_pitch, limit, alpha, err};
   if (x) {
     Int8RowsParams R;
     int rc = rows_params(R, x, residual, gain, sum_out, q, s, tokens, k, x_pitch, q_pitch, x_code, gain_code, eps);
-    if (rc == 0) rc = int8_rows_launch(R, x_code, gain_code, stream);
+    if (rc == 0 && few && i8st::fuses(tokens, k)) return i8st::product(P, &R, x_code, gain_code, mode, out_code, sms, stream);
+    if (rc == 0 && (q == nullptr || s == nullptr)) rc = B200_BAD_SIZE;
+    if (rc == 0) rc = int8_rows_launch(R, x_code, gain_code, sms, stream);
     if (rc != 0) return rc;
   }
   if (n == 0) return 0;
-  const Int8ProductParams P = {static_cast<const int8_t*>(q), s, static_cast<const int8_t*>(w), c, bias, out, tokens, n, k,
-                               q_pitch, w_pitch, limit, alpha, err};
-  return int8_product(P, mode, out_code, stream);
+  return few ? i8st::product(P, nullptr, 0, 0, mode, out_code, sms, stream) : tiled_product(P, mode, out_code, sms, stream);
 }

@@ -10,9 +10,12 @@
 // q are 0, so everything computed from the row is NaN.  Where 127 / a would overflow (a < 2^-100) row and maximum are
 // multiplied by 2^100 first, which is exact.
 //
-// Bound by the bytes of x (and the residual, twice), by latency where rows are few.  One block a row, the row in registers
-// (up to 32 elements a thread) between the reduction and the rounding.
+// Bound by the bytes of x (and the residual, twice), by latency where rows are few.  A block walks over rows; a row lies in
+// registers (up to 32 elements a thread) between the reduction and the rounding, the next row's loads are on their way
+// meanwhile.  All loads of a row are issued before its first store: a store that might alias would else hold the loads behind it.
 #pragma once
+#include <string.h>
+
 #include "common.cuh"
 
 struct Int8RowsParams {
@@ -28,13 +31,39 @@ struct Int8RowsParams {
   int wide;                  // whether 8 elements of x, residual, gain and sum_out may be moved at once
 };
 
-// N = 8 consecutive elements from `p` on (`n` of them exist, the others read as 0).
-template <typename T> __device__ __forceinline__ void int8_fetch8(const T* p, int n, bool wide, float (&v)[8]) {
+// Eight consecutive elements as they lie in memory.
+template <typename T> struct Int8Raw { uint4 v[sizeof(T) / 2]; };
+template <typename T> __device__ __forceinline__ T int8_zero();
+template <> __device__ __forceinline__ float int8_zero<float>() { return 0.0f; }
+template <> __device__ __forceinline__ __nv_bfloat16 int8_zero<__nv_bfloat16>() { return __float2bfloat16_rn(0.0f); }
+
+// The elements from `p` on, of which `n` exist (the others read as 0).
+template <typename T> __device__ __forceinline__ void int8_load8(const T* p, int n, bool wide, Int8Raw<T>& r) {
   if (wide && n >= 8) {
-    load_floats<T, 8>(p, v);
-  } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < n ? to_f32<T>(p[e]) : 0.0f;
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.v[i] = reinterpret_cast<const uint4*>(p)[i];
+  } else {
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = i < n ? p[i] : int8_zero<T>();
+    memcpy(&r, e, sizeof(r));
+  }
+}
+template <typename T> __device__ __forceinline__ void int8_floats(const Int8Raw<T>& r, float (&v)[8]) {
+  const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  } else {
+    const uint32_t u[4] = {r.v[sizeof(T) / 2 - 1].x, r.v[sizeof(T) / 2 - 1].y, r.v[sizeof(T) / 2 - 1].z, r.v[sizeof(T) / 2 - 1].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = __uint_as_float(w[i]);
+      v[4 + i] = __uint_as_float(u[i]);
+    }
   }
 }
 template <typename T> __device__ __forceinline__ void int8_store8(T* p, int n, bool wide, const float (&v)[8]) {
@@ -69,100 +98,191 @@ __device__ __forceinline__ Int8Step int8_step(uint32_t top_bits, float factor) {
 // Four elements as four bytes.  Adding 1.5 * 2^23 leaves the nearest whole number (ties to even) in the low bits.
 __device__ __forceinline__ uint32_t int8_pack4(const float* v, const Int8Step& t) {
   uint32_t b[4];
+  if (t.pre == 1.0f) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(__fadd_rn(__fmul_rn(v[e] * t.pre, t.inv), 12582912.0f));
+    for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(__fadd_rn(__fmul_rn(v[e], t.inv), 12582912.0f));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(__fadd_rn(__fmul_rn(v[e] * t.pre, t.inv), 12582912.0f));
+  }
   return t.none ? 0u : __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
 }
 
 constexpr int INT8_ROW_CHUNKS = 4;                    // chunks of 8 elements that a thread keeps
 
+// The larger of a row's maximum and |v|, NaN if either is.
+__device__ __forceinline__ float int8_top(float top, float v) {
+  asm("max.NaN.f32 %0, %0, %1;\n" : "+f"(top) : "f"(fabsf(v)));
+  return top;
+}
+// One chunk behind its loads: v = x, or behind a norm (x + residual) * gain, with what it adds to the row's sum of squares and
+// maximum; the sum is stored where sum_out is given (`n` of the elements exist).
 template <typename T, typename TG, bool NORM>
+__device__ __forceinline__ void int8_chunk(const Int8Raw<T>& x, const Int8Raw<T>& r, const Int8Raw<TG>& gain, bool add, T* sum_out, int n,
+                                           bool wide, float (&v)[8], float& ss, float& top) {
+  int8_floats<T>(x, v);
+  if (NORM) {
+    float f[8];
+    if (add) {
+      int8_floats<T>(r, f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = __fadd_rn(v[e], f[e]);
+      if (sum_out) int8_store8<T>(sum_out, n, wide, v);
+    }
+    int8_floats<TG>(gain, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      ss = fmaf(v[e], v[e], ss);
+      v[e] = __fmul_rn(v[e], f[e]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = int8_top(top, v[e]);
+}
+
+// The block's sums of squares and maximum (`turn`: which half of the scratch is free).
+// Returns the maximum's bits: as integers floats that are not negative compare as they do, and NaN is above infinity.
+template <bool NORM> __device__ __forceinline__ uint32_t int8_meet(float& ss, float top, float (*sums)[16], uint32_t (*tops)[16], int turn) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+  if (NORM) ss = warp_sum(ss);
+  if (lane == 0) { tops[turn][warp] = bits; sums[turn][warp] = ss; }
+  __syncthreads();
+  if (NORM) {
+    ss = 0.0f;
+    for (int w = 0; w < warps; ++w) ss += sums[turn][w];
+  }
+  return __reduce_max_sync(0xffffffffu, lane < warps ? tops[turn][lane] : 0u);
+}
+
+// Rows whose chunks fit the block's registers, CH a thread.
+template <typename T, typename TG, bool NORM, int CH>
 __global__ void __launch_bounds__(512) int8_rows_kernel(const Int8RowsParams P) {
-  __shared__ float sums[16];
-  __shared__ uint32_t tops[16];
+  __shared__ float sums[2][16];
+  __shared__ uint32_t tops[2][16];
   pdl_launch_dependents();
   pdl_wait();
-  const int row = blockIdx.x, threads = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const T* x = static_cast<const T*>(P.x) + static_cast<size_t>(row) * P.x_pitch;
-  const T* residual = NORM && P.residual ? static_cast<const T*>(P.residual) + static_cast<size_t>(row) * P.k : nullptr;
-  T* sum_out = NORM && P.sum_out ? static_cast<T*>(P.sum_out) + static_cast<size_t>(row) * P.k : nullptr;
+  const int threads = blockDim.x, chunks = (P.k + 7) / 8;
+  const bool wide = P.wide != 0, add = NORM && P.residual != nullptr;
   const TG* gain = static_cast<const TG*>(P.gain);
-  const int chunks = (P.k + 7) / 8;
-  const bool wide = P.wide != 0, kept = chunks <= INT8_ROW_CHUNKS * threads;
-
-  // v (behind a norm: v * gain) of one chunk; `first`: also the sum's store and the row's sum of squares
-  float ss = 0.0f;
-  uint32_t top = 0u;
-  auto fetch = [&](int c, float (&v)[8], bool first) {
-    const int at = c * 8, n = P.k - at;
-    int8_fetch8<T>(x + at, n, wide, v);
-    if (NORM) {
-      if (residual) {
-        float r[8];
-        int8_fetch8<T>(residual + at, n, wide, r);
+  Int8Raw<T> x[CH], r[CH];
+  auto load = [&](int row) {
+    const T* xs = static_cast<const T*>(P.x) + static_cast<size_t>(row) * P.x_pitch;
+    const T* rs = static_cast<const T*>(P.residual) + static_cast<size_t>(row) * P.k;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = __fadd_rn(v[e], r[e]);
-        if (first && sum_out) int8_store8<T>(sum_out + at, n, wide, v);
-      }
-      float g[8];
-      int8_fetch8<TG>(gain + at, n, wide, g);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (first) ss = fmaf(v[e], v[e], ss);
-        v[e] = __fmul_rn(v[e], g[e]);
-      }
-    }
-    if (first) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+    for (int i = 0; i < CH; ++i) {
+      const int at = (threadIdx.x + i * threads) * 8;
+      if (at >= P.k) continue;
+      int8_load8<T>(xs + at, P.k - at, wide, x[i]);
+      if (add) int8_load8<T>(rs + at, P.k - at, wide, r[i]);
     }
   };
-  float v[INT8_ROW_CHUNKS][8];
-  if (kept) {
+  load(blockIdx.x);
+  int turn = 0;
+  for (int row = blockIdx.x; row < P.tokens; row += gridDim.x, turn ^= 1) {
+    Int8Raw<TG> g[CH];
+    if (NORM)
 #pragma unroll
-    for (int i = 0; i < INT8_ROW_CHUNKS; ++i)
-      if (threadIdx.x + i * threads < chunks) fetch(threadIdx.x + i * threads, v[i], true);
-  } else {
-    for (int c = threadIdx.x; c < chunks; c += threads) fetch(c, v[0], true);
-  }
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (NORM) ss = warp_sum(ss);
-  if (lane == 0) { tops[warp] = top; sums[warp] = ss; }
-  __syncthreads();
-  top = 0u;
-  ss = 0.0f;
-  for (int w = 0; w < threads / 32; ++w) {
-    top = max(top, tops[w]);
-    ss += sums[w];
-  }
-  const Int8Step step = int8_step(top, NORM ? rsqrtf(ss / static_cast<float>(P.k) + P.eps) : 1.0f);
-  if (threadIdx.x == 0) P.s[row] = step.scale;
-  int8_t* q = P.q + static_cast<size_t>(row) * P.q_pitch;
-  if (kept) {
+      for (int i = 0; i < CH; ++i) {
+        const int at = (threadIdx.x + i * threads) * 8;
+        if (at < P.k) int8_load8<TG>(gain + at, P.k - at, wide, g[i]);
+      }
+    T* sum_out = add && P.sum_out ? static_cast<T*>(P.sum_out) + static_cast<size_t>(row) * P.k : nullptr;
+    float v[CH][8], ss = 0.0f;
+    float top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < INT8_ROW_CHUNKS; ++i)
+    for (int i = 0; i < CH; ++i) {
+      const int at = (threadIdx.x + i * threads) * 8;
+      if (at < P.k) int8_chunk<T, TG, NORM>(x[i], r[i], g[i], add, sum_out ? sum_out + at : nullptr, P.k - at, wide, v[i], ss, top);
+    }
+    if (row + static_cast<int>(gridDim.x) < P.tokens) load(row + gridDim.x);
+    const uint32_t bits = int8_meet<NORM>(ss, top, sums, tops, turn);
+    const Int8Step step = int8_step(bits, NORM ? rsqrtf(ss / static_cast<float>(P.k) + P.eps) : 1.0f);
+    if (threadIdx.x == 0) P.s[row] = step.scale;
+    int8_t* q = P.q + static_cast<size_t>(row) * P.q_pitch;
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
       if (threadIdx.x + i * threads < chunks)
         *reinterpret_cast<uint2*>(q + (threadIdx.x + i * threads) * 8) = make_uint2(int8_pack4(v[i], step), int8_pack4(v[i] + 4, step));
-  } else {
-    for (int c = threadIdx.x; c < chunks; c += threads) {
-      fetch(c, v[0], false);
-      *reinterpret_cast<uint2*>(q + c * 8) = make_uint2(int8_pack4(v[0], step), int8_pack4(v[0] + 4, step));
-    }
   }
 }
 
-template <typename T>
-static int int8_rows_typed(const Int8RowsParams& P, int gain_code, cudaStream_t stream) {
-  const int chunks = (P.k + 7) / 8;
-  int threads = (chunks + 1) / 2;                       // two chunks a thread: the row's latency, not its issue, is the time
-  threads = threads < 32 ? 32 : threads > 512 ? 512 : (threads + 31) / 32 * 32;
-  auto kernel = P.gain == nullptr ? int8_rows_kernel<T, float, false>
-                : gain_code == B200_F32 ? int8_rows_kernel<T, float, true> : int8_rows_kernel<T, __nv_bfloat16, true>;
-  return b200_launch(kernel, dim3(P.tokens), dim3(threads), 0, stream, 0, P);
+// Longer rows are read twice.
+template <typename T, typename TG, bool NORM>
+__global__ void __launch_bounds__(512) int8_long_rows_kernel(const Int8RowsParams P) {
+  __shared__ float sums[1][16];
+  __shared__ uint32_t tops[1][16];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int row = blockIdx.x, chunks = (P.k + 7) / 8;
+  const bool wide = P.wide != 0, add = NORM && P.residual != nullptr;
+  const T* xs = static_cast<const T*>(P.x) + static_cast<size_t>(row) * P.x_pitch;
+  const T* rs = static_cast<const T*>(P.residual) + static_cast<size_t>(row) * P.k;
+  const TG* gain = static_cast<const TG*>(P.gain);
+  T* sum_out = add && P.sum_out ? static_cast<T*>(P.sum_out) + static_cast<size_t>(row) * P.k : nullptr;
+  float ss = 0.0f;
+  float top = 0.0f;
+  auto fetch = [&](int c, float (&v)[8], T* store) {
+    const int at = c * 8;
+    Int8Raw<T> x, r;
+    Int8Raw<TG> g;
+    int8_load8<T>(xs + at, P.k - at, wide, x);
+    if (add) int8_load8<T>(rs + at, P.k - at, wide, r);
+    if (NORM) int8_load8<TG>(gain + at, P.k - at, wide, g);
+    int8_chunk<T, TG, NORM>(x, r, g, add, store ? store + at : nullptr, P.k - at, wide, v, ss, top);
+  };
+  for (int c = threadIdx.x; c < chunks; c += blockDim.x) {
+    float v[8];
+    fetch(c, v, sum_out);
+  }
+  const uint32_t bits = int8_meet<NORM>(ss, top, sums, tops, 0);
+  const Int8Step step = int8_step(bits, NORM ? rsqrtf(ss / static_cast<float>(P.k) + P.eps) : 1.0f);
+  if (threadIdx.x == 0) P.s[row] = step.scale;
+  int8_t* q = P.q + static_cast<size_t>(row) * P.q_pitch;
+  for (int c = threadIdx.x; c < chunks; c += blockDim.x) {
+    float v[8];
+    fetch(c, v, nullptr);
+    *reinterpret_cast<uint2*>(q + c * 8) = make_uint2(int8_pack4(v, step), int8_pack4(v + 4, step));
+  }
 }
-static int int8_rows_launch(const Int8RowsParams& P, int x_code, int gain_code, cudaStream_t stream) {
-  if (x_code == B200_F32) return int8_rows_typed<float>(P, gain_code, stream);
-  if (x_code == B200_BF16) return int8_rows_typed<__nv_bfloat16>(P, gain_code, stream);
+
+template <typename T, typename TG, bool NORM, int CH>
+static int int8_rows_kept(const Int8RowsParams& P, int threads, int sms, cudaStream_t stream) {
+  // Persistent: as many blocks as fit at once (threads, registers: found once for each size of block).
+  static int fits[17];
+  int& blocks = fits[threads / 32];
+  if (blocks == 0) {
+    int n = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, int8_rows_kernel<T, TG, NORM, CH>, threads, 0);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    blocks = n < 1 ? 1 : n;
+  }
+  const int most = sms * blocks;
+  return b200_launch(int8_rows_kernel<T, TG, NORM, CH>, dim3(P.tokens < most ? P.tokens : most), dim3(threads), 0, stream, 0, P);
+}
+template <typename T, typename TG, bool NORM>
+static int int8_rows_normed(const Int8RowsParams& P, int sms, cudaStream_t stream) {
+  const int chunks = (P.k + 7) / 8;
+  auto threads = [&](int ch) { return ((chunks + ch - 1) / ch + 31) / 32 * 32; };
+  // Few rows: the row's latency is the time, so a thread takes one chunk where it can.  Many: what counts are the bytes on their
+  // way; two chunks a thread keep them (8,192 x 4,096 behind a norm 47 us, 94 % of the copy rate), four leave room for one
+  // block an SM (12,288 columns: 3.0 TB/s), and reading rows twice, the second time out of the caches, is faster (5.2).
+  if (P.tokens <= sms) {
+    if (chunks <= 512) return int8_rows_kept<T, TG, NORM, 1>(P, threads(1), sms, stream);
+    if (chunks <= 512 * INT8_ROW_CHUNKS) return int8_rows_kept<T, TG, NORM, INT8_ROW_CHUNKS>(P, threads(INT8_ROW_CHUNKS), sms, stream);
+  } else if (chunks <= 1024) {
+    return int8_rows_kept<T, TG, NORM, 2>(P, threads(2), sms, stream);
+  }
+  return b200_launch(int8_long_rows_kernel<T, TG, NORM>, dim3(P.tokens), dim3(512), 0, stream, 0, P);
+}
+template <typename T>
+static int int8_rows_typed(const Int8RowsParams& P, int gain_code, int sms, cudaStream_t stream) {
+  if (P.gain == nullptr) return int8_rows_normed<T, float, false>(P, sms, stream);
+  return gain_code == B200_F32 ? int8_rows_normed<T, float, true>(P, sms, stream) : int8_rows_normed<T, __nv_bfloat16, true>(P, sms, stream);
+}
+static int int8_rows_launch(const Int8RowsParams& P, int x_code, int gain_code, int sms, cudaStream_t stream) {
+  if (x_code == B200_F32) return int8_rows_typed<float>(P, gain_code, sms, stream);
+  if (x_code == B200_BF16) return int8_rows_typed<__nv_bfloat16>(P, gain_code, sms, stream);
   return B200_BAD_DTYPE;
 }
 static inline bool int8_aligned(const void* p, long long pitch_bytes) {

@@ -3,55 +3,51 @@
 //
 // A tile is 128 tokens a CTA x BN columns (INT8_GLU: BN / 2 gate columns and the same BN / 2 up columns), k in blocks of 128
 // bytes.  Warps:
-//   warp 0      one lane feeds a ring of 6 stages with TMA (128-byte swizzle): a box of 128 tokens and two of 64 weight rows
+//   warp 0      one lane feeds a ring of stages with TMA (128-byte swizzle): a box of weight rows (or of gate and of up rows) for
+//               each of a stage's blocks of k
+//   warp 10     the same for the tokens
 //   warp 1      allocates tensor memory for two accumulators; one lane issues tcgen05.mma (kind::i8, K 32, four a stage)
-//   warps 2-5   read their 32 lanes of tensor memory, multiply by the scales, round, turn the tile's rows through shared
-//               memory and store whole 128-byte pieces of them
+//   warps 2-9   read their 32 lanes of tensor memory (two warps a quarter, every other 32 columns), multiply by the scales,
+//               round, turn 32 x 32 results through shared memory and store pieces of rows
 // Three ways to run it:
 //   PAIRS    CG = 2, 256 tokens x 256 columns on two CTAs (each holds its 128 tokens and half of the weight rows, the
 //            first one's MMAs read both): half the bytes per product that a CTA of its own would have to fetch, for the many
 //            tiles of prompts.  Persistent: the epilogue of a tile runs under the MMAs of the next.
-//   SINGLE   CG = 1, 128 x 128, persistent.
-//   SPLIT    CG = 1, 128 x 128, a cluster of S CTAs shares a tile's k.  Each CTA sends its sums to the CTAs that own the
+//   SINGLE   CG = 1, 128 x BN, persistent; BN is chosen so that the SMs get equal shares of the weights.
+//   SPLIT    CG = 1, 128 x BN, a cluster of S CTAs shares a tile's k.  Each CTA sends its sums to the CTAs that own the
 //            columns (distributed shared memory), which add them (integers: no order to keep) and finish.  For few tiles,
 //            whose weights else come through few SMs.
-// What lies beyond the matrices is zero-filled by TMA and masked at the store.  Every wait is bounded by the clock; one that
-// runs out flags the engine's error word, and every path reaches the end, where tensor memory is given back.
+// Token rows: a box is as high as there are tokens (to 8), and the last tile of 128 begins so that it ends with the tokens
+// (rows it shares with the tile before are not stored again): TMA takes longer to fill rows outside a matrix with zeros
+// than to fetch them.  Rows of the MMA's 128 beyond the box hold whatever lies there; sums of other rows do not see them.
+// What lies beyond the matrices otherwise is zero-filled by TMA and masked at the store.  Every wait is bounded by the clock;
+// one that runs out flags the engine's error word, and every path reaches the end, where tensor memory is given back.
 #pragma once
 #include <cuda.h>
 #include <math.h>
 #include <string.h>
+#include <type_traits>
 
-#include "common.cuh"
-
-enum : int { INT8_PLAIN = 0, INT8_GLU = 1 };
-
-struct Int8ProductParams {
-  const int8_t* q;           // [tokens, k], rows q_pitch bytes apart
-  const float* s;            // [tokens]
-  const int8_t* w;           // [rows, k], rows w_pitch bytes apart
-  const float* c;            // [rows]
-  const float* bias;         // [rows] or null
-  void* out;                 // [tokens, n]
-  int tokens, n, k;          // n: columns of out (INT8_GLU: w has 2 n rows)
-  long long q_pitch, w_pitch;
-  float limit, alpha;
-  int* err;
-};
+#include "int8_common.cuh"
 
 namespace i8tc {
 
-constexpr int BM = 128, BK = 128, STAGES = 6, THREADS = 192;
-constexpr int A_BYTES = BM * BK, W_BYTES = 128 * BK, STAGE_BYTES = A_BYTES + W_BYTES;      // 32 KB
+constexpr int BM = 128, BK = 128, MAX_STAGES = 16, EPI_WARPS = 8, PARTS = EPI_WARPS / 4, THREADS = (3 + EPI_WARPS) * 32;
 constexpr int GROUP_M = 16;                       // tiles of tokens that are walked over before the next columns
+constexpr int ACC = 256;                          // columns of tensor memory of an accumulator
+constexpr int SCALES = 8192;                      // each warp's scales and bias: [pieces][gate, up][scale, bias][32]
+template <typename T> constexpr int turn_bytes() { return EPI_WARPS * 32 * 32 * static_cast<int>(sizeof(T)); }        // a warp's 32 rows x 32 results
+template <typename T> constexpr int smem_fixed() { return 1024 + turn_bytes<T>() + SCALES + (2 * MAX_STAGES + 4) * 8 + 16; }
+constexpr int SMEM_MOST = 227 * 1024;
 
-template <int CG> struct Shape {
-  static constexpr int BN = CG == 2 ? 256 : 128;
-  static constexpr int TURN = 4 * 32 * 128;                                     // a warp's 32 rows x 128 bytes
-  static constexpr int SCALES = 4 * BN * 8;                                     // a warp's scales and bias
-  static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + TURN + SCALES + (2 * STAGES + 4) * 8 + 16;
+// How a product is cut up.
+struct Plan {
+  int way;                   // 0 PAIRS, 1 SINGLE, S > 1 a cluster of S CTAs a tile
+  int bn;                    // columns of the accumulator (INT8_GLU: half of them gate columns)
+  int box;                   // tokens that are fetched a tile
+  int sub;                   // blocks of k a stage
+  int stages, stage_bytes;
 };
-static_assert(Shape<2>::SMEM <= 227 * 1024, "shared memory of a CTA");
 
 __device__ __forceinline__ void mbar_init(uint64_t* bar, int count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(count));
@@ -64,8 +60,11 @@ __device__ __forceinline__ uint32_t cta_address(const void* p, uint32_t rank) { 
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
   return a;
 }
-__device__ __forceinline__ void mbar_arrive_at(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_addr) : "memory");
+// An accumulator is handed back when its loads have completed (the caller has waited for them): relaxed, because a release over
+// the cluster would first wait for the tile's stores.
+template <int CG> __device__ __forceinline__ void mbar_hand_back(uint64_t* bar) {
+  if constexpr (CG == 2) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cta_address(bar, 0)) : "memory");
+  else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bar)) : "memory");
 }
 template <int CG> __device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   if constexpr (CG == 2)
@@ -85,16 +84,16 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
   return (static_cast<uint64_t>(hi) << 32) | lo;
 }
 // 32-bit integer sums, signed 8-bit A and B, both K-major.
-template <int CG> __host__ __device__ constexpr uint32_t instr_desc() {
-  return (2u << 4) | (1u << 7) | (1u << 10) | ((Shape<CG>::BN >> 3) << 17) | ((CG * BM >> 4) << 24);
+template <int CG> __device__ __forceinline__ uint32_t instr_desc(int bn) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(bn >> 3) << 17) | ((CG * BM >> 4) << 24);
 }
-template <int CG> __device__ __forceinline__ void mma_i8(uint32_t tmem_c, uint64_t a, uint64_t b, uint32_t accumulate) {
+template <int CG> __device__ __forceinline__ void mma_i8(uint32_t tmem_c, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   if constexpr (CG == 2)
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n"
-                 ::"r"(tmem_c), "l"(a), "l"(b), "r"(instr_desc<CG>()), "r"(accumulate) : "memory");
+                 ::"r"(tmem_c), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
   else
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n"
-                 ::"r"(tmem_c), "l"(a), "l"(b), "r"(instr_desc<CG>()), "r"(accumulate) : "memory");
+                 ::"r"(tmem_c), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 // The barrier (of both CTAs of a pair) is arrived on when all earlier MMAs are done.
 template <int CG> __device__ __forceinline__ void mma_commit(uint64_t* bar) {
@@ -135,6 +134,19 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
     }
   }
 }
+// The feeding and issuing warps walk along as a whole and one lane issues: what comes before is then the same in every lane for
+// all the compiler knows, and addresses and descriptors are made in uniform registers, where the instructions take them.  (From
+// one lane's own registers a stage of one block cost 300 ns beside its copies and MMAs.)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}\n" : "=r"(is));
+  return is != 0;
+}
+__device__ __forceinline__ int same_in_warp(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+template <bool CLUSTER> __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* err) {
+  const bool mine = CLUSTER ? mbar_wait_cluster(bar, parity, err) : mbar_wait(bar, parity, err);
+  return __all_sync(0xffffffffu, mine ? 1 : 0) != 0;
+}
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
@@ -152,49 +164,69 @@ __device__ __forceinline__ void tile_at(int tile, int m_tiles, int n_tiles, int&
   n = in / rows;
 }
 
-template <typename T> __device__ __forceinline__ uint32_t pack_word(const float* y);
-template <> __device__ __forceinline__ uint32_t pack_word<float>(const float* y) { return __float_as_uint(y[0]); }
-template <> __device__ __forceinline__ uint32_t pack_word<__nv_bfloat16>(const float* y) {
-  const __nv_bfloat162 p = __floats2bfloat162_rn(y[0], y[1]);
-  return *reinterpret_cast<const uint32_t*>(&p);
+template <typename T> __device__ __forceinline__ uint4 pack16(const float* y);
+template <> __device__ __forceinline__ uint4 pack16<float>(const float* y) {
+  return make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
+}
+template <> __device__ __forceinline__ uint4 pack16<__nv_bfloat16>(const float* y) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(y[2 * i], y[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&p);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <typename T, int MODE, int CG, bool SPLIT>
+// Four sums with the token's scale, the channels' and their bias.
+__device__ __forceinline__ void scaled4(const int* sum, float s, float4 c, float4 b, float* y) {
+  y[0] = fmaf(static_cast<float>(sum[0]), s * c.x, b.x);
+  y[1] = fmaf(static_cast<float>(sum[1]), s * c.y, b.y);
+  y[2] = fmaf(static_cast<float>(sum[2]), s * c.z, b.z);
+  y[3] = fmaf(static_cast<float>(sum[3]), s * c.w, b.w);
+}
+
+// Where 16 bytes of a turned row lie, so that neither eight rows' same piece nor a row's pieces share banks.
+template <typename T> __device__ __forceinline__ int turned(int row, int piece) {
+  if constexpr (sizeof(T) == 4) return row * 128 + ((piece ^ (row & 7)) * 16);
+  else return row * 64 + ((piece ^ ((row >> 1) & 3)) * 16);
+}
+
+// SPLIT: CTAs that share a tile's k (1: none).
+template <typename T, int MODE, int CG, int SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
-product_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap wmap, const Int8ProductParams P) {
-  constexpr int BN = Shape<CG>::BN;
-  constexpr int OUT = MODE == INT8_GLU ? BN / 2 : BN;                           // columns of the result a tile
+product_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap wmap, const Int8ProductParams P, const Plan plan) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  unsigned char* turn = ring + STAGES * STAGE_BYTES;
-  float* scales = reinterpret_cast<float*>(turn + Shape<CG>::TURN);
-  uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<unsigned char*>(scales) + Shape<CG>::SCALES);
-  uint64_t* empty = full + STAGES;
-  uint64_t* acc_full = empty + STAGES;          // [2]
+  const int stages = plan.stages, stage_bytes = plan.stage_bytes, sub = plan.sub, a_bytes = plan.box * BK;
+  const int bn = plan.bn, out_cols = MODE == INT8_GLU ? bn / 2 : bn;      // (columns of the result a tile)
+  const int w_rows = bn / CG, w_bytes = w_rows * BK;                 // weight rows that this CTA fetches a tile
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + stages * stage_bytes);
+  uint64_t* empty = full + MAX_STAGES;
+  uint64_t* acc_full = empty + MAX_STAGES;      // [2]
   uint64_t* acc_empty = acc_full + 2;           // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  unsigned char* turn = reinterpret_cast<unsigned char*>(tmem_slot + 4);
+  float* scales = reinterpret_cast<float*>(turn + turn_bytes<T>());
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = CG == 2 || SPLIT ? cluster_rank() : 0u;
-  uint32_t ranks = 1;
-  if (SPLIT) asm volatile("mov.u32 %0, %%cluster_nctarank;\n" : "=r"(ranks));
-  const int m_tiles = (P.tokens + CG * BM - 1) / (CG * BM), n_tiles = (P.n + OUT - 1) / OUT, tiles = m_tiles * n_tiles;
+  const int warp = same_in_warp(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int rank = CG == 2 || SPLIT > 1 ? same_in_warp(static_cast<int>(cluster_rank())) : 0;
+  const int m_tiles = (P.tokens + CG * BM - 1) / (CG * BM), n_tiles = (P.n + out_cols - 1) / out_cols, tiles = m_tiles * n_tiles;
   const int all_kb = (P.k + BK - 1) / BK;
-  const int kb0 = SPLIT ? static_cast<int>(rank) * all_kb / static_cast<int>(ranks) : 0;
-  const int kb1 = SPLIT ? (static_cast<int>(rank) + 1) * all_kb / static_cast<int>(ranks) : all_kb;
-  const int first = SPLIT ? blockIdx.x / ranks : blockIdx.x / CG, step = SPLIT ? gridDim.x / ranks : gridDim.x / CG;
+  const int kb0 = SPLIT > 1 ? rank * all_kb / SPLIT : 0, kb1 = SPLIT > 1 ? (rank + 1) * all_kb / SPLIT : all_kb;
+  const int first = blockIdx.x / (SPLIT * CG), step = gridDim.x / (SPLIT * CG);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
-    for (int a = 0; a < 2; ++a) { mbar_init(acc_full + a, 1); mbar_init(acc_empty + a, 4 * CG); }
+    for (int s = 0; s < stages; ++s) { mbar_init(full + s, 2); mbar_init(empty + s, 1); }
+    for (int a = 0; a < 2; ++a) { mbar_init(acc_full + a, 1); mbar_init(acc_empty + a, EPI_WARPS * CG); }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 1) {                                                              // the whole warp allocates tensor memory
     if constexpr (CG == 2) {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(tmem_slot)), "r"(2 * BN) : "memory");
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(tmem_slot)), "r"(2 * ACC) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
     } else {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(tmem_slot)), "r"(2 * BN) : "memory");
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(tmem_slot)), "r"(2 * ACC) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
   }
@@ -202,214 +234,277 @@ product_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__
   __syncthreads();
   if (CG == 2) cluster_sync();                                                  // the pair's barriers exist
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = same_in_warp(*tmem_slot);
   pdl_launch_dependents();
 
-  // the weight rows of a tile that this CTA fetches (two boxes of 64)
+  // the weight rows of a tile that this CTA fetches (gate and up rows: two boxes, or one each of a pair's CTAs), and its
+  // tokens: the tile's, and where they are fetched
+  constexpr int BOXES = MODE == INT8_GLU && CG == 1 ? 2 : 1;
   auto weight_row = [&](int n, int box) {
-    if (MODE == INT8_GLU) return CG == 2 ? (rank ? P.n : 0) + n * OUT + box * 64 : (box ? P.n : 0) + n * OUT;
-    return n * OUT + static_cast<int>(CG == 2 ? rank : 0) * 128 + box * 64;
+    if (MODE == INT8_GLU) return ((CG == 2 ? rank : box) ? P.n : 0) + n * out_cols;
+    return n * out_cols + (CG == 2 ? rank * w_rows : 0);
   };
+  auto first_token = [&](int m) { return (m * CG + (CG == 2 ? rank : 0)) * BM; };
+  auto first_fetched = [&](int m) { return P.tokens >= BM ? min(first_token(m), P.tokens - BM) : 0; };
 
-  if (warp == 0) {
-    if (lane == 0) {
+  // SPLIT: what this CTA finishes of the cluster's tile (its share of the columns, of gate and up each half, and the tokens)
+  int m0 = 0, n0 = 0;
+  if (SPLIT > 1) tile_at(first, m_tiles, n_tiles, m0, n0);
+  const int width = bn / SPLIT, half = out_cols, own = MODE == INT8_GLU ? width / 2 : width, own0 = n0 * out_cols + rank * own;
+  const int row0 = first_fetched(m0), low = first_token(m0) - row0, high = min(BM, P.tokens - row0), quad_ints = plan.box * 4;
+  float* token_scale = scales + 512;            // behind [gate, up][scale, bias][128]
+
+  // A stage holds the tokens of its blocks of k, then the weights of them.
+  auto feed = [&](auto of_weights) {
+    constexpr bool WEIGHTS = decltype(of_weights)::value;
+    const int block_bytes = WEIGHTS ? w_bytes : a_bytes;
+    int m, n;
+    if (WEIGHTS && first < tiles) {
       // The first weights start for the second-level cache before the dependency wait; nothing is read before it.
-      int m, n;
-      if (first < tiles) {
-        tile_at(first, m_tiles, n_tiles, m, n);
-        for (int kb = kb0; kb < kb1 && kb < kb0 + STAGES; ++kb)
-          for (int box = 0; box < 2; ++box) tma_prefetch(&wmap, kb * BK, weight_row(n, box));
-      }
-      pdl_wait();
-      int it = 0;                                                               // k-blocks fetched so far, over all tiles
-      bool ok = true;
-      for (int tile = first; tile < tiles && ok; tile += step) {
-        tile_at(tile, m_tiles, n_tiles, m, n);
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = it % STAGES, use = it / STAGES;
-          if (use > 0 && !mbar_wait(empty + s, (use - 1) & 1, P.err)) { ok = false; break; }
-          unsigned char* st = ring + s * STAGE_BYTES;
-          const uint32_t bar = CG == 2 ? cta_address(full + s, 0) : smem_u32(full + s);
-          if (rank == 0 || CG == 1) mbar_expect_tx(full + s, CG * STAGE_BYTES);
-          tma_load<CG>(st, &qmap, kb * BK, (m * CG + static_cast<int>(CG == 2 ? rank : 0)) * BM, bar);
-          tma_load<CG>(st + A_BYTES, &wmap, kb * BK, weight_row(n, 0), bar);
-          tma_load<CG>(st + A_BYTES + W_BYTES / 2, &wmap, kb * BK, weight_row(n, 1), bar);
+      tile_at(first, m_tiles, n_tiles, m, n);
+      if (elect_one())
+        for (int kb = kb0; kb < kb1 && kb < kb0 + stages * sub; ++kb)
+          for (int box = 0; box < BOXES; ++box) tma_prefetch(&wmap, kb * BK, weight_row(n, box));
+      __syncwarp();
+    }
+    pdl_wait();
+    int s = 0, use = 0;                                                         // the ring's place, and how often it was filled
+    bool ok = true;
+    for (int tile = first; tile < tiles && ok; tile += step) {
+      tile_at(tile, m_tiles, n_tiles, m, n);
+      const int row = WEIGHTS ? weight_row(n, 0) : first_fetched(m);
+      for (int kb = kb0; kb < kb1; kb += sub) {
+        if (use > 0 && !mbar_wait_warp<false>(empty + s, (use - 1) & 1, P.err)) { ok = false; break; }
+        const int blocks = min(sub, kb1 - kb);
+        unsigned char* st = ring + s * stage_bytes + (WEIGHTS ? sub * a_bytes : 0);
+        const uint32_t bar = CG == 2 ? cta_address(full + s, 0) : smem_u32(full + s);
+        if (elect_one()) {
+          if (CG == 1 || rank == 0) mbar_expect_tx(full + s, CG * blocks * block_bytes);
+          for (int j = 0; j < blocks; ++j, st += block_bytes) {
+            tma_load<CG>(st, WEIGHTS ? &wmap : &qmap, (kb + j) * BK, row, bar);
+            if (WEIGHTS && BOXES == 2) tma_load<CG>(st + w_bytes / 2, &wmap, (kb + j) * BK, weight_row(n, 1), bar);
+          }
         }
+        __syncwarp();
+        if (++s == stages) { s = 0; ++use; }
       }
     }
+  };
+  if (warp == 0) {
+    feed(std::true_type());
+  } else if (warp == 2 + EPI_WARPS) {
+    feed(std::false_type());
   } else if (warp == 1) {
     pdl_wait();
-    if (lane == 0 && (CG == 1 || rank == 0)) {
-      int it = 0, local = 0;
+    if (CG == 1 || rank == 0) {
+      const uint32_t idesc = instr_desc<CG>(bn);
+      const uint64_t da = smem_desc(smem_u32(ring)), db = smem_desc(smem_u32(ring + sub * a_bytes));
+      int s = 0, use = 0, local = 0;
       bool ok = true;
       for (int tile = first; tile < tiles && ok; tile += step, ++local) {
-        const int acc = local & 1, use = local >> 1;
-        // (the epilogues have read this accumulator)
-        if (use > 0) ok = CG == 2 ? mbar_wait_cluster(acc_empty + acc, (use - 1) & 1, P.err) : mbar_wait(acc_empty + acc, (use - 1) & 1, P.err);
+        const int acc = local & 1, turns = local >> 1;
+        if (turns > 0) ok = mbar_wait_warp<CG == 2>(acc_empty + acc, (turns - 1) & 1, P.err);       // the epilogues have read this accumulator
         if (!ok) break;
         tc_fence_after();
-        const uint32_t tmem_c = tmem_base + acc * BN;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = it % STAGES;
-          ok = mbar_wait(full + s, (it / STAGES) & 1, P.err);
+        const uint32_t tmem_c = tmem_base + acc * ACC;
+        for (int kb = kb0; kb < kb1; kb += sub) {
+          ok = mbar_wait_warp<false>(full + s, use & 1, P.err);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t a = smem_u32(ring + s * STAGE_BYTES), b = a + A_BYTES;
+          const int blocks = min(sub, kb1 - kb);
+          uint64_t a = da + static_cast<uint32_t>(s * stage_bytes >> 4), b = db + static_cast<uint32_t>(s * stage_bytes >> 4);
+          if (elect_one()) {
+            for (int j = 0; j < blocks; ++j, a += static_cast<uint32_t>(a_bytes >> 4), b += static_cast<uint32_t>(w_bytes >> 4))
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k) mma_i8<CG>(tmem_c, smem_desc(a + k * 32), smem_desc(b + k * 32), (kb > kb0 || k > 0) ? 1u : 0u);
-          mma_commit<CG>(empty + s);                                            // the stage is free when these MMAs have read it
+              for (int k = 0; k < BK / 32; ++k) mma_i8<CG>(tmem_c, a + k * 2, b + k * 2, idesc, (kb > kb0 || j > 0 || k > 0) ? 1u : 0u);
+            mma_commit<CG>(empty + s);                                          // the stage is free when these MMAs have read it
+          }
+          __syncwarp();
+          if (++s == stages) { s = 0; ++use; }
         }
-        mma_commit<CG>(acc_full + acc);                                         // the tile's sums are complete
+        if (elect_one()) mma_commit<CG>(acc_full + acc);                        // the tile's sums are complete
+        __syncwarp();
       }
     }
-  } else if (!SPLIT) {
+  } else if (SPLIT == 1) {
     pdl_wait();
-    const int quarter = warp & 3;
-    unsigned char* mine = turn + quarter * (32 * 128);
-    float* sc = scales + quarter * (2 * BN);                                    // scales, then bias, in the accumulator's order
+    const int quarter = warp & 3, part = (warp - 2) >> 2;
+    constexpr int ROW = 32 * sizeof(T);                                         // bytes of a turned row
+    unsigned char* mine = turn + (warp - 2) * (32 * ROW);
+    float* sc = scales + (warp - 2) * (SCALES / 4 / EPI_WARPS);
+    constexpr int HALVES = MODE == INT8_GLU ? 2 : 1;
     int local = 0;
     T* out = static_cast<T*>(P.out);
-    const bool whole = (reinterpret_cast<uintptr_t>(out) | (static_cast<size_t>(P.n) * sizeof(T))) % 16 == 0;
-    constexpr int PIECE = 128 / sizeof(T);                                      // columns that are turned at once
+    constexpr int LANES = 32 * sizeof(T) / 16;                                  // lanes that a row's 32 results take, 16 bytes each
+    const bool whole = (reinterpret_cast<uintptr_t>(out) | (static_cast<size_t>(P.n) * sizeof(T)) | (out_cols * sizeof(T))) % 16 == 0;
+    // scales and bias of a tile's columns (and the token's scale) come from memory while the tile before is worked on
+    constexpr int PIECES = ACC / HALVES / 32 / PARTS;                           // of 32 columns, at most
+    float c_next[PIECES][HALVES], b_next[PIECES][HALVES], s_next = 0.0f;
+    auto fetch = [&](int tile) {
+      int m, n;
+      tile_at(tile, m_tiles, n_tiles, m, n);
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          const int in = (part + i * PARTS) * 32 + lane, col = n * out_cols + in;
+          const bool there = in < out_cols && col < P.n;
+          c_next[i][h] = there ? P.c[h * P.n + col] : 0.0f;
+          b_next[i][h] = there && P.bias ? P.bias[h * P.n + col] : 0.0f;
+        }
+      const int row = first_fetched(m) + quarter * 32 + lane;
+      s_next = row < P.tokens ? P.s[row] : 0.0f;
+    };
+    if (first < tiles) fetch(first);
     for (int tile = first; tile < tiles; tile += step, ++local) {
       int m, n;
       tile_at(tile, m_tiles, n_tiles, m, n);
       const int acc = local & 1;
-      const int row0 = (m * CG + static_cast<int>(CG == 2 ? rank : 0)) * BM + quarter * 32;
-      const int rows = min(32, P.tokens - row0);
+      const int row0 = first_fetched(m) + quarter * 32;
+      const int low = max(0, first_token(m) - row0), high = min(32, P.tokens - row0);       // the rows of these 32 that are stored
       __syncwarp();
-      for (int i = lane; i < BN; i += 32) {
-        const int half = MODE == INT8_GLU ? i / OUT : 0, col = n * OUT + (MODE == INT8_GLU ? i % OUT : i);
-        sc[i] = col < P.n ? P.c[half * P.n + col] : 0.0f;
-        sc[BN + i] = P.bias && col < P.n ? P.bias[half * P.n + col] : 0.0f;
-      }
-      const float s = lane < rows ? P.s[row0 + lane] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          sc[(i * HALVES + h) * 64 + lane] = c_next[i][h];
+          sc[(i * HALVES + h) * 64 + 32 + lane] = b_next[i][h];
+        }
+      const float s = s_next;
+      if (tile + step < tiles) fetch(tile + step);
       __syncwarp();
       if (!mbar_wait(acc_full + acc, (local >> 1) & 1, P.err)) break;
       tc_fence_after();
-      const uint32_t base = tmem_base + acc * BN + (static_cast<uint32_t>(quarter * 32) << 16);
+      const uint32_t base = tmem_base + acc * ACC + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll 1
-      for (int p = 0; p < OUT / PIECE; ++p) {
-        const int col0 = n * OUT + p * PIECE;
-        if (rows <= 0 || col0 >= P.n) break;                                    // (the whole warp)
+      for (int p = part, i = 0; p * 32 < out_cols; p += PARTS, ++i) {
+        const int col0 = n * out_cols + p * 32, cols = min(min(32, out_cols - p * 32), P.n - col0);
+        if (high <= low || cols <= 0) break;                                    // (the whole warp)
+        int g[32], u[MODE == INT8_GLU ? 32 : 1];
+        tmem_ld32(base + p * 32, g);
+        if constexpr (MODE == INT8_GLU) tmem_ld32(base + out_cols + p * 32, u);
+        tmem_ld_wait();
+        const float4* gs = reinterpret_cast<const float4*>(sc + i * HALVES * 64);
+        uint4 packed[LANES];                                                    // (all of them before the first store: the scales' loads pass no store)
 #pragma unroll
-        for (int h = 0; h < PIECE / 32; ++h) {
-          const int at = p * PIECE + h * 32;
-          int g[32], u[MODE == INT8_GLU ? 32 : 1];
-          tmem_ld32(base + at, g);
-          if constexpr (MODE == INT8_GLU) tmem_ld32(base + OUT + at, u);
-          tmem_ld_wait();
+        for (int e = 0; e < LANES; ++e) {
+          constexpr int N = 16 / sizeof(T);
+          float y[N];
 #pragma unroll
-          for (int e = 0; e < 32; e += 16 / sizeof(T)) {
-            uint4 piece;
-            uint32_t* words = reinterpret_cast<uint32_t*>(&piece);
-            constexpr int A_WORD = 4 / sizeof(T);
+          for (int z = 0; z < N; z += 4) {
+            const int at = e * N + z;
+            scaled4(g + at, s, gs[at / 4], P.bias ? gs[8 + at / 4] : make_float4(0.0f, 0.0f, 0.0f, 0.0f), y + z);
+            if constexpr (MODE == INT8_GLU) {
+              float up[4];
+              scaled4(u + at, s, gs[16 + at / 4], P.bias ? gs[24 + at / 4] : make_float4(0.0f, 0.0f, 0.0f, 0.0f), up);
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              float y[A_WORD];
-#pragma unroll
-              for (int z = 0; z < A_WORD; ++z) {
-                const int j = e + v * A_WORD + z;
-                y[z] = fmaf(static_cast<float>(g[j]), s * sc[at + j], sc[BN + at + j]);
-                if constexpr (MODE == INT8_GLU)
-                  y[z] = glu_product(y[z], fmaf(static_cast<float>(u[j]), s * sc[OUT + at + j], sc[BN + OUT + at + j]), P.limit, P.alpha);
-              }
-              words[v] = pack_word<T>(y);
+              for (int j = 0; j < 4; ++j) y[z + j] = gate_up(y[z + j], up[j], P.limit, P.alpha);
             }
-            const int chunk = (h * 32 + e) * static_cast<int>(sizeof(T)) / 16;
-            *reinterpret_cast<uint4*>(mine + lane * 128 + ((chunk ^ (lane & 7)) * 16)) = piece;
           }
+          packed[e] = pack16<T>(y);
         }
-        __syncwarp();
-        if (whole && col0 + PIECE <= P.n) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = i * 4 + lane / 8, chunk = lane % 8;
-            if (r < rows)
+        for (int e = 0; e < LANES; ++e) *reinterpret_cast<uint4*>(mine + turned<T>(lane, e)) = packed[e];
+        __syncwarp();
+        if (whole && cols == 32) {
+#pragma unroll
+          for (int q = 0; q < LANES; ++q) {
+            const int r = q * (32 / LANES) + lane / LANES, chunk = lane % LANES;
+            if (r >= low && r < high)
               *reinterpret_cast<uint4*>(out + static_cast<size_t>(row0 + r) * P.n + col0 + chunk * (16 / sizeof(T))) =
-                  *reinterpret_cast<const uint4*>(mine + r * 128 + ((chunk ^ (r & 7)) * 16));
+                  *reinterpret_cast<const uint4*>(mine + turned<T>(r, chunk));
           }
-        } else {
-          const int cols = min(PIECE, P.n - col0);
-          for (int r = 0; r < rows; ++r)
-            for (int c = lane; c < cols; c += 32) {
-              const int byte = c * static_cast<int>(sizeof(T));
-              out[static_cast<size_t>(row0 + r) * P.n + col0 + c] =
-                  *reinterpret_cast<const T*>(mine + r * 128 + (((byte / 16) ^ (r & 7)) * 16) + byte % 16);
-            }
+        } else if (lane < cols) {
+          const int byte = lane * static_cast<int>(sizeof(T));
+          for (int r = low; r < high; ++r)
+            out[static_cast<size_t>(row0 + r) * P.n + col0 + lane] = *reinterpret_cast<const T*>(mine + turned<T>(r, byte / 16) + byte % 16);
         }
         __syncwarp();
       }
       tc_fence_before();                                                        // the loads of this accumulator are done
       __syncwarp();
-      if (lane == 0) mbar_arrive_at(CG == 2 ? cta_address(acc_empty + acc, 0) : cta_address(acc_empty + acc, cluster_rank()));
+      if (lane == 0) mbar_hand_back<CG>(acc_empty + acc);
     }
   } else {
+    // One tile a cluster: scales and bias of the columns that this CTA will finish, then the tokens' scales.
     pdl_wait();
-    if (first < tiles) mbar_wait(acc_full, 0, P.err);                           // (one tile a cluster)
+    for (int i = threadIdx.x - 64; i < own; i += 32 * EPI_WARPS)
+#pragma unroll
+      for (int h = 0; h < (MODE == INT8_GLU ? 2 : 1); ++h) {
+        const bool in = own0 + i < P.n;
+        scales[h * 256 + i] = in ? P.c[h * P.n + own0 + i] : 0.0f;
+        scales[h * 256 + 128 + i] = in && P.bias ? P.bias[h * P.n + own0 + i] : 0.0f;
+      }
+    for (int i = threadIdx.x - 64; i < high; i += 32 * EPI_WARPS) token_scale[i] = P.s[row0 + i];
+    if (first < tiles) mbar_wait(acc_full, 0, P.err);
     tc_fence_after();
   }
 
-  if constexpr (SPLIT) {
-    // Everybody's MMAs have read their rings, which take the others' sums now: [from][columns / 4][128 rows][4].
+  if constexpr (SPLIT > 1) {
+    // Everybody's MMAs have read their rings, which take the others' sums now: [from][columns / 4][tokens of the box][4].
+    int* sums = reinterpret_cast<int*>(ring);
     __syncwarp();
     cluster_sync();
-    int* sums = reinterpret_cast<int*>(ring);
-    const int width = BN / static_cast<int>(ranks);                             // columns that a CTA owns (of gate and up each half)
-    const int half = MODE == INT8_GLU ? OUT : BN, own = MODE == INT8_GLU ? width / 2 : width;
-    int m, n;
-    tile_at(first, m_tiles, n_tiles, m, n);
-    const int rows = min(BM, P.tokens - m * BM);
-    constexpr int QUAD = BM * 4;                                                // ints of four columns
-    if (warp >= 2) {
-      const int quarter = warp & 3, row = quarter * 32 + lane;
-      if (quarter * 32 < rows) {
-        const uint32_t base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    if (warp >= 2 && warp < 2 + EPI_WARPS) {
+      const int row = (warp & 3) * 32 + lane;
+      if ((warp & 3) * 32 < high) {
+        const uint32_t base = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
 #pragma unroll 1
-        for (int c = 0; c < BN; c += 32) {
+        for (int c = ((warp - 2) >> 2) * 32; c < bn; c += PARTS * 32) {
           int v[32];
           tmem_ld32(base + c, v);
           tmem_ld_wait();
+          int up = MODE == INT8_GLU && c >= half ? own : 0, to = (c - (up ? half : 0)) / own, at = c - (up ? half : 0) - to * own;
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
-            const int col = c + e, in = MODE == INT8_GLU ? col % half : col;
-            const int to = in / own, quad = ((MODE == INT8_GLU && col >= half ? own : 0) + in % own) / 4;
-            const uint32_t dst = cta_address(sums + (rank * (width / 4) + quad) * QUAD + row * 4, to);
-            if (row < rows)
+            if (c + e < bn && row < high) {
+              const uint32_t dst = cta_address(sums + (rank * (width / 4) + (up + at) / 4) * quad_ints + row * 4, to);
               asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst), "r"(v[e]), "r"(v[e + 1]), "r"(v[e + 2]), "r"(v[e + 3]) : "memory");
+            }
+            if ((at += 4) == own) {
+              at = 0;
+              if (++to == SPLIT) { to = 0; up = own; }
+            }
           }
         }
       }
     }
     __syncwarp();
     cluster_sync();
-    pdl_wait();                                                                 // (every thread reads scales from here on)
+    // A warp takes 8 tokens x 16 columns at a time: a lane four columns of a token.
     T* out = static_cast<T*>(P.out);
-    const int quads = own / 4;
-    for (int i = threadIdx.x; i < rows * quads; i += THREADS) {
-      const int row = i / quads, quad = i % quads;
-      const int col = n * OUT + static_cast<int>(rank) * own + quad * 4;
-      if (col >= P.n) continue;
-      const float s = P.s[m * BM + row];
+    const bool whole = (reinterpret_cast<uintptr_t>(out) | (static_cast<size_t>(P.n) * sizeof(T))) % (4 * sizeof(T)) == 0;
+    const int quads = own / 4, across = (quads + 3) / 4, blocks = (high - low + 7) / 8 * across;
+    for (int i = warp; i < blocks; i += THREADS / 32) {
+      const int row = low + i / across * 8 + (lane & 7), quad = i % across * 4 + (lane >> 3), col = own0 + quad * 4;
+      if (row >= high || quad >= quads || col >= P.n) continue;
       float y[2][4];
 #pragma unroll
       for (int h = 0; h < (MODE == INT8_GLU ? 2 : 1); ++h) {
-        int4 t = make_int4(0, 0, 0, 0);
-        for (uint32_t from = 0; from < ranks; ++from) {
-          const int4 v = *reinterpret_cast<const int4*>(sums + (from * (width / 4) + h * quads + quad) * QUAD + row * 4);
-          t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w;
-        }
-        const int a[4] = {t.x, t.y, t.z, t.w};
+        int t[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int at = h * P.n + min(col + e, P.n - 1);
-          y[h][e] = fmaf(static_cast<float>(a[e]), s * P.c[at], P.bias ? P.bias[at] : 0.0f);
+        for (int from = 0; from < SPLIT; ++from) {
+          const int4 v = *reinterpret_cast<const int4*>(sums + (from * (width / 4) + h * quads + quad) * quad_ints + row * 4);
+          t[0] += v.x; t[1] += v.y; t[2] += v.z; t[3] += v.w;
         }
+        scaled4(t, token_scale[row], *reinterpret_cast<const float4*>(scales + h * 256 + quad * 4),
+                *reinterpret_cast<const float4*>(scales + h * 256 + 128 + quad * 4), y[h]);
       }
-      T* dst = out + static_cast<size_t>(m * BM + row) * P.n + col;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (col + e < P.n) dst[e] = from_f32<T>(MODE == INT8_GLU ? glu_product(y[0][e], y[1][e], P.limit, P.alpha) : y[0][e]);
+        if (MODE == INT8_GLU) y[0][e] = gate_up(y[0][e], y[1][e], P.limit, P.alpha);
+      T* dst = out + static_cast<size_t>(row0 + row) * P.n + col;
+      if (whole && col + 4 <= P.n) {
+        __align__(16) T r[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = from_f32<T>(y[0][e]);
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(r);
+        else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(r);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < P.n) dst[e] = from_f32<T>(y[0][e]);
+      }
     }
   }
   // Everybody meets here on every path; then the allocating warp gives the tensor memory back.
@@ -419,8 +514,8 @@ product_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__
   if (CG == 2) cluster_sync();                                                  // (the pair's MMAs and arrivals are over)
   if (warp == 1) {
     tc_fence_after();
-    if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(2 * BN) : "memory");
-    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(2 * BN) : "memory");
+    if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(2 * ACC) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(2 * ACC) : "memory");
   }
 }
 
@@ -450,40 +545,75 @@ static int tensor_map(CUtensorMap* map, const void* matrix, long long rows, long
   return r == CUDA_SUCCESS ? 0 : 1000 + static_cast<int>(r);
 }
 
-template <typename T, int MODE, int CG, bool SPLIT>
-static int launch(const Int8ProductParams& P, int blocks, int cluster, cudaStream_t stream) {
+template <typename T, int MODE, int CG, int SPLIT>
+static int launch(const Int8ProductParams& P, const Plan& plan, int blocks, int cluster, cudaStream_t stream) {
   static bool configured = false;
   if (!configured) {
-    const cudaError_t e = cudaFuncSetAttribute(product_kernel<T, MODE, CG, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<CG>::SMEM);
+    const cudaError_t e = cudaFuncSetAttribute(product_kernel<T, MODE, CG, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST);
     if (e != cudaSuccess) return static_cast<int>(e);
     configured = true;
   }
   CUtensorMap qmap, wmap;
-  int rc = tensor_map(&qmap, P.q, P.tokens, P.k, P.q_pitch, BM);
-  if (rc == 0) rc = tensor_map(&wmap, P.w, static_cast<long long>(P.n) * (MODE == INT8_GLU ? 2 : 1), P.k, P.w_pitch, 64);
+  int rc = tensor_map(&qmap, P.q, P.tokens, P.k, P.q_pitch, plan.box);
+  if (rc == 0) rc = tensor_map(&wmap, P.w, static_cast<long long>(P.n) * (MODE == INT8_GLU ? 2 : 1), P.k, P.w_pitch,
+                                 CG == 2 || MODE == INT8_GLU ? plan.bn / 2 : plan.bn);
   if (rc != 0) return rc;
-  return b200_launch(product_kernel<T, MODE, CG, SPLIT>, dim3(blocks), dim3(THREADS), Shape<CG>::SMEM, stream, cluster, qmap, wmap, P);
+  return b200_launch(product_kernel<T, MODE, CG, SPLIT>, dim3(blocks), dim3(THREADS), smem_fixed<T>() + plan.stages * plan.stage_bytes, stream,
+                     cluster, qmap, wmap, P, plan);
 }
 
-// Which way a product goes (0 PAIRS, 1 SINGLE, S > 1 a cluster of S CTAs a tile).
-static inline int route(int tokens, int n, int k, int mode, int sms) {
-  const long long m1 = (tokens + 127) / 128, out1 = mode == INT8_GLU ? 64 : 128;
-  const long long tiles = m1 * ((n + out1 - 1) / out1), pairs = (tokens + 255ll) / 256 * ((n + 2 * out1 - 1) / (2 * out1));
-  if (tokens > 128 && pairs * 2 >= sms) return 0;
-  const int kb = (k + BK - 1) / BK;
-  int split = 1;
-  while (split < 8 && tiles * split * 2 <= sms && split * 2 <= kb) split *= 2;
-  return split;
+// Stages of as much k as leaves the ring four of them: a stage costs the threads that feed and issue about 190 ns beside its
+// copies and MMAs (300 ns with one block of k and few columns).
+static void set_stages(Plan& p, int rows_a_cta, int fixed) {
+  const int block = (p.box + rows_a_cta) * BK, room = SMEM_MOST - fixed;
+  p.sub = p.way == 0 ? 1 : room / (4 * block);
+  if (p.sub < 1) p.sub = 1;
+  if (p.sub > 4) p.sub = 4;
+  p.stage_bytes = p.sub * block;
+  p.stages = room / p.stage_bytes;
+  if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+}
+
+// How a product is cut up (see the top of the file): what its fullest SM takes, in us.  A block of k of one CTA takes what its
+// bytes take at 92 GB/s, but 125 ns at least; of a pair's CTA at 118 GB/s, or the MMA's 2 bn cycles.  (One CTA a tile, 4,096 k,
+// 64 tokens: 96 tiles of 64 columns 9.5 us, 48 of 128 11.9, 192 of 32 in two rounds 12.0.)  Sharing k costs about 2 us more with
+// two CTAs and 4.5 with four.
+static inline Plan make_plan(int tokens, int n, int k, int mode, int sms, int fixed) {
+  Plan p = {};
+  const int glu = mode == INT8_GLU ? 2 : 1, kb = (k + BK - 1) / BK;
+  const long long cols = static_cast<long long>(n) * glu, m_tiles = (tokens + BM - 1) / BM;
+  p.box = tokens >= BM ? BM : (tokens + 7) / 8 * 8;
+  double best = 0.0;
+  for (int split = 1; split <= 4 && split <= kb; split *= 2)
+    for (int bn = 256; bn >= 32; bn -= 16) {
+      if (bn % (4 * glu * split) != 0) continue;
+      const long long rounds = (m_tiles * ((cols + bn - 1) / bn) * split + sms - 1) / sms;
+      if (split > 1 && rounds > 1) continue;
+      const double block = (p.box + bn) * BK / 92e3;
+      const double cost = static_cast<double>(rounds * ((kb + split - 1) / split)) * (block > 0.125 ? block : 0.125) +
+                          (split == 4 ? 5.4 : split == 2 ? 2.2 : 0.0) + bn * 0.008;
+      if (best == 0.0 || cost < best) { best = cost; p.way = split; p.bn = bn; }
+    }
+  if (tokens > BM)
+    for (int bn = 256; bn >= 128; bn -= 32) {
+      const long long rounds = ((tokens + 255ll) / 256 * ((cols + bn - 1) / bn) + sms / 2 - 1) / (sms / 2);
+      const double bytes = (BM + bn / 2) * BK / 118e3, mma = bn * 2 / 1.85e3;
+      const double cost = static_cast<double>(rounds * kb) * (bytes > mma ? bytes : mma) + bn * 0.008;
+      if (cost < best) { best = cost; p.way = 0; p.bn = bn; }
+    }
+  set_stages(p, p.way == 0 ? p.bn / 2 : p.bn, fixed);
+  return p;
 }
 
 template <typename T, int MODE> static int product(const Int8ProductParams& P, int sms, cudaStream_t stream) {
-  const int way = route(P.tokens, P.n, P.k, MODE, sms);
-  const int tall = way == 0 ? 256 : 128, wide = (way == 0 ? 256 : 128) / (MODE == INT8_GLU ? 2 : 1);
+  const Plan plan = make_plan(P.tokens, P.n, P.k, MODE, sms, smem_fixed<T>());
+  const int tall = plan.way == 0 ? 2 * BM : BM, wide = plan.bn / (MODE == INT8_GLU ? 2 : 1);
   const long long tiles = static_cast<long long>((P.tokens + tall - 1) / tall) * ((P.n + wide - 1) / wide);
-  if (tiles > 0x3fffffff) return B200_BAD_SIZE;
-  if (way == 0) return launch<T, MODE, 2, false>(P, 2 * static_cast<int>(tiles < sms / 2 ? tiles : sms / 2), 2, stream);
-  if (way == 1) return launch<T, MODE, 1, false>(P, static_cast<int>(tiles < sms ? tiles : sms), 0, stream);
-  return launch<T, MODE, 1, true>(P, static_cast<int>(tiles) * way, way, stream);
+  if (tiles > 0x0fffffff || plan.stages < 2) return B200_BAD_SIZE;
+  const int t = static_cast<int>(tiles);
+  if (plan.way == 0) return launch<T, MODE, 2, 1>(P, plan, 2 * (t < sms / 2 ? t : sms / 2), 2, stream);
+  if (plan.way == 1) return launch<T, MODE, 1, 1>(P, plan, t < sms ? t : sms, 0, stream);
+  return plan.way == 2 ? launch<T, MODE, 1, 2>(P, plan, 2 * t, 2, stream) : launch<T, MODE, 1, 4>(P, plan, 4 * t, 4, stream);
 }
 
 }  // namespace i8tc

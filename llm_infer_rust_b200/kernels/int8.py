@@ -127,37 +127,54 @@ def _source(x):
     return src, residual, gain, kept, x.eps
 
 
+_sizes = ops._bind("byte_product_sizes")
+
+
 def _product(x, weight: Int8Weight, bias, out_dtype, mode: int, glu: str, limit: float, alpha: float) -> torch.Tensor:
-    _check_8_bit(weight, "weights")
+    w, w_scales = weight
     if isinstance(x, Int8Rows):
-        _check_8_bit(x, "rows")
         src = residual = gain = kept = None
         eps, (values, scales) = 0.0, x
+        _check_8_bit(x, "rows")
+        _check_8_bit(weight, "weights")
         tokens, k = values.shape
         _check_k(k)
-        pitch, out_dtype, x_pitch, x_code = values.stride(0), out_dtype or torch.bfloat16, 0, 0
-        ops._cuda(values, scales, weight.values, weight.scales, bias)
+        rows, w_pitch, pitch, out_dtype, x_pitch, x_code = w.shape[0], w.stride(0), values.stride(0), out_dtype or torch.bfloat16, 0, 0
+        ops._cuda(values, scales, w, w_scales, bias)
     else:
-        src, residual, gain, kept, eps = _source(x)
-        ops._cuda(src, residual, gain, kept, weight.values, weight.scales, bias)
-        tokens, k = src.shape
-        pitch, out_dtype, x_pitch, x_code = row_pitch(k), out_dtype or src.dtype, src.stride(0) if tokens > 1 else k, ops._code(src)
-        # the tokens in 8 bits and their scales, between the two kernels of the call
-        values = ops._empty((tokens * pitch + 4 * tokens,), torch.int8, src.device)
-        scales = values.data_ptr() + tokens * pitch
-    rows = weight.values.shape[0]
-    if weight.values.shape[1] != k:
-        raise KernelError(f"the rows have {k} columns, the weight has {weight.values.shape[1]}")
-    if mode == _GLU and rows % 2:
-        raise KernelError("gate and up rows of a gated product are as many")
+        if isinstance(x, ops.PendingNorm):
+            src, residual, gain, kept, eps = _source(x)
+        else:
+            src, residual, gain, kept, eps = x, None, None, None, 0.0
+        sizes = _sizes(src, w, w_scales)
+        if sizes is None:                        # (something is not as it should be, or there is nothing to do)
+            _check_8_bit(weight, "weights")
+            _source(src)
+            ops._cuda(src, w, w_scales)
+            sizes = (*src.shape, w.shape[0], src.stride(0) if src.shape[0] > 1 else src.shape[1], w.stride(0), ops._code(src))
+        ops._cuda(residual, gain, kept, bias)
+        tokens, k, rows, x_pitch, w_pitch, x_code = sizes
+        _check_k(k)
+        pitch, out_dtype, values, scales = row_pitch(k), out_dtype or src.dtype, None, None
+    if w.shape[1] != k:
+        raise KernelError(f"the rows have {k} columns, the weight has {w.shape[1]}")
+    n = rows
+    if mode == _GLU:
+        if rows % 2:
+            raise KernelError("gate and up rows of a gated product are as many")
+        n = rows // 2
     if bias is not None and (bias.dtype != torch.float32 or bias.numel() != rows or not bias.is_contiguous()):
         raise KernelError("the bias is float32, one element an output channel")
-    n = rows // 2 if mode == _GLU else rows
-    out = ops._empty((tokens, n), out_dtype, weight.values.device)
-    rc = _lib(glu).b200_int8_linear(src, residual, gain, kept, values, scales, weight.values, weight.scales, bias, out, tokens, n, k,
-                                    x_pitch, pitch, weight.values.stride(0), x_code, 0 if gain is None else ops._code(gain),
-                                    ops._code(out), mode, eps, float(limit), float(alpha), ops.error_word(out.device), ops._stream())
-    ops._ok(rc, "int8_linear", 0 if not tokens else int(src is not None) + int(n > 0))
+    lib, device = _lib(glu), w.device
+    out = ops._empty((tokens, n), out_dtype, device)
+    if values is None and (not n or not lib.b200_int8_alone(tokens, k)):
+        # the tokens in 8 bits and their scales, between the two kernels of the call
+        values = ops._empty((tokens * pitch + 4 * tokens,), torch.int8, device)
+        scales = values.data_ptr() + tokens * pitch
+    rc = lib.b200_int8_linear(src, residual, gain, kept, values, scales, w, w_scales, bias, out, tokens, n, k, x_pitch, pitch, w_pitch,
+                              x_code, 0 if gain is None else ops._code(gain), ops._code(out), mode, eps, float(limit), float(alpha),
+                              ops.error_word(device), ops._stream())
+    ops._ok(rc, "int8_linear", 0 if not tokens else (0 if src is None else 1) + (1 if n and (src is None or values is not None) else 0))
     return out
 
 
