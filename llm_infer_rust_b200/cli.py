@@ -31,6 +31,7 @@ Engine options (names and defaults follow the reference's command line):
                             max_position_embeddings (8192)
   --page-size N             tokens per cache page (16)
   --dtype NAME              auto (the checkpoint's), bfloat16 or float32
+  --int8-projections        hold and multiply the layers' projections in 8-bit integers
   --device NAME             auto or cuda; there is no CPU path (auto)
   --log-level LEVEL         error, warn, info, debug or trace (info)
   --tp-size N               must be 1: the engine runs on one GPU
@@ -79,6 +80,7 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--max-seq-len", type=int, default=None)
     p.add_argument("--page-size", type=int, default=16)
     p.add_argument("--dtype", default="auto", choices=["auto", "bfloat16", "float32"])
+    p.add_argument("--int8-projections", action="store_true")
     p.add_argument("--device", default="auto", choices=["auto", "cuda"])
     p.add_argument("--log-level", default="info", type=lambda v: "warn" if v.lower() == "warning" else v.lower(),
                    choices=["trace", "debug", "info", "warn", "error"])
@@ -150,7 +152,8 @@ def main(argv: Optional[List[str]] = None) -> int:
                     max_prefill_tokens_per_batch=args.max_prefill_tokens_per_batch,
                     chunked_prefill_size=args.chunked_prefill_size, cuda_graph_bs=args.cuda_graph_bs,
                     prefill_cuda_graph_max_tokens=args.prefill_cuda_graph_max_tokens,
-                    cpu_gpu_overlap=not args.disable_cpu_gpu_overlap, seed=args.seed, log_level=args.log_level)
+                    cpu_gpu_overlap=not args.disable_cpu_gpu_overlap, seed=args.seed, log_level=args.log_level,
+                    int8_projections=args.int8_projections)
     params = SamplingParams(args.temperature, args.top_k, args.top_p, args.ignore_eos, args.max_tokens,
                             args.seed if args.seed else None)
     for prompt, result in zip(prompts, engine.generate(prompts, params)):

@@ -26,7 +26,7 @@ from ..config.registry import resolve_architecture
 from ..config.spec import ConfigError
 from ..kernels import ops
 from ..kernels.build import load_host_runtime
-from ..parts import DecoderModel
+from ..parts import DecoderModel, int8_projections as with_int8_projections
 from ..sampling import Sampler, SamplingParams
 from ..weights.loader import load_weights, read_model_config
 from ..weights.random_init import bind_random_weights
@@ -137,12 +137,14 @@ class Engine:
                  cuda_graph_bs: Optional[int] = 0, prefill_cuda_graph_max_tokens: int = 0,
                  eos_token_ids: Optional[Sequence[int]] = None, cpu_gpu_overlap: bool = True,
                  seed: int = 0, log_level: str = "info", random_weights_config: Optional[dict] = None,
-                 random_weights_seed: int = 0, keep_float32_tensors: Optional[bool] = None):
+                 random_weights_seed: int = 0, keep_float32_tensors: Optional[bool] = None, int8_projections: bool = False):
         """``model_path``: a folder with config.json and model.safetensors.  With ``model_path`` None and
         ``random_weights_config`` (the keys of a config.json) the weights are drawn on the device from
         ``random_weights_seed`` and no file is read: for sizes whose checkpoint would take long to write.
         ``keep_float32_tensors``: what a bfloat16 engine does with tensors stored in 32-bit (None: they stay float32
         in a checkpoint that declares itself 16-bit and are converted otherwise; see weights/loader.py).
+        ``int8_projections``: the layers' attention and gated feed-forward projections are held and multiplied in 8-bit
+        integers, with a scale for each output channel and each token (see parts/int8.py for which have that form).
         ``log_level``: error, warn(ing), info, debug or trace, for the package's logger."""
         self.model_path = model_path
         self.log_level = log_level
@@ -165,6 +167,8 @@ class Engine:
         self.config = self.arch.parse_config(raw)
         self.raw_config = raw
         spec = self.arch.model_spec(self.config)
+        if int8_projections:
+            spec = with_int8_projections(spec)
 
         self._setup_device(device)
         if dtype == "auto":

@@ -196,7 +196,7 @@ class GQAttention(Part):
         rope = self.rope
         q = torch.empty((tokens, self.nh * self.d), dtype=x.dtype, device=x.device)
         slots = ctx.slots[cache.group] if cache.writes else None
-        if ops.few_row_takes(tokens, p["qkv_proj"], self.env.dtype, ops.EPI_QKV, self.d):
+        if self._fuses_heads(tokens):
             # few tokens: norm (if pending), projection, per-head norm, rotation and cache store in one kernel
             ops.few_row_linear(x, p["qkv_proj"], ops.EPI_QKV, qkv=dict(
                 head_dim=self.d, num_heads=self.nh, num_kv_heads=self.nkv, q_out=q, k_cache=cache.k, v_cache=cache.v,
@@ -204,9 +204,7 @@ class GQAttention(Part):
                 cos=rope.cos if rope else None, sin=rope.sin if rope else None,
                 rot_dim=rope.rot_dim if rope else 0, positions=ctx.positions, slots=slots), lazy=True)
         else:
-            if isinstance(x, ops.PendingNorm):
-                x = x.materialize()
-            qkv = ops.linear(x, p["qkv_proj"])
+            qkv = self._project_heads(x)
             ops.qkv_post(qkv, q, cache.k, cache.v, p.get("q_norm"), p.get("k_norm"),
                          float(self.qk_eps or 0.0), rope.cos if rope else None, rope.sin if rope else None,
                          rope.rot_dim if rope else 0, ctx.positions, slots, self.nh, self.nkv, self.d)
@@ -225,7 +223,16 @@ class GQAttention(Part):
             ops.decode_attention(q, cache.k, cache.v, out, scratch, ctx.block_tables[g], ctx.cu_q,
                                  ctx.kv_len, ctx.decode_rows, ctx.num_decode, self.nh, self.nkv, self.d,
                                  page, self.window, self.scale, splits)
-        return ops.linear(out, p["o_proj"], lazy=True)
+        return self._project_out(out)
+
+    def _fuses_heads(self, tokens: int) -> bool:
+        return ops.few_row_takes(tokens, self.params["qkv_proj"], self.env.dtype, ops.EPI_QKV, self.d)
+
+    def _project_heads(self, x):
+        return ops.linear(x.materialize() if isinstance(x, ops.PendingNorm) else x, self.params["qkv_proj"])
+
+    def _project_out(self, out):
+        return ops.linear(out, self.params["o_proj"], lazy=True)
 
 
 class GatedConvAttention(Part):

@@ -85,3 +85,27 @@ def test_8_bit_values_of_a_checkpoint_are_laid_out():
     with pytest.raises(KernelError, match="N scales"):
         int8.int8_weight_from(values, torch.ones(5))
     assert torch.equal(w.dequantize(), values.float())
+
+
+def test_which_parts_have_a_form_in_8_bits():
+    from llm_infer_rust_b200 import ConfigError, LayerSpec, ModelSpec, PartSpec, Qwen3Config, RunEntry
+    from llm_infer_rust_b200.parts import int8_projections, registered
+    raw = {"model_type": "qwen3", "architectures": ["Qwen3ForCausalLM"], "num_hidden_layers": 2, "hidden_size": 32,
+           "num_attention_heads": 2, "num_key_value_heads": 1, "head_dim": 16, "intermediate_size": 48, "vocab_size": 61}
+    spec = Qwen3Config.parse(raw).model_spec()
+    held = int8_projections(spec)
+    for before, layer in zip(spec.layers, held.layers):
+        assert layer["mixer"].kind == "gqa_attention_int8" and layer["mixer"].params == before["mixer"].params
+        assert layer["feed_forward"].kind == "swiglu_int8" and layer["input_norm"] == before["input_norm"]
+        assert layer["mixer"].kind in registered("mixer") and layer["feed_forward"].kind in registered("feed_forward")
+    assert held.lm_head == spec.lm_head and held.run_list == spec.run_list and held != spec
+    other = LayerSpec(PartSpec("pre_norm_input_conv"), {"mixer": PartSpec("decay_retention", {})})
+    with pytest.raises(ConfigError, match="no layer of X has projections with a form in 8-bit"):
+        int8_projections(ModelSpec("X", 10, 8, 16, PartSpec("token_embedding"), (other,), (RunEntry(0),), PartSpec("rms_norm"),
+                                   PartSpec("linear_head")))
+
+
+def test_the_command_line_names_them():
+    from llm_infer_rust_b200 import cli
+    assert cli.parse_args(["--model-path", "m", "--int8-projections"]).int8_projections
+    assert not cli.parse_args(["--model-path", "m"]).int8_projections and "--int8-projections" in cli.USAGE
