@@ -236,30 +236,36 @@ PyObject* mm_t(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// byte_product_sizes(x, values, scales) -> (tokens, k, rows, elements between x's rows, bytes between the weights' rows, x is
-// bfloat16) where everything is as a product in 8 bits takes it, else None (the wrapper then says what is wrong): one call for some
-// twenty attributes of three tensors, each of which costs Python a tenth of a microsecond.
+// byte_product_sizes(x, values, scales, residual, gain, kept, bias) -> (tokens, k, rows, elements between x's rows, bytes between the
+// weights' rows, x's type, gain's type) where everything is as a product in 8 bits takes it (the last four may be None), else None
+// (the wrapper then says what is wrong): one call for some thirty attributes of up to seven tensors, each of which costs Python a
+// tenth of a microsecond.
 PyObject* byte_product_sizes(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 3) {
-    PyErr_SetString(PyExc_TypeError, "byte_product_sizes(x, values, scales)");
+  if (n != 7) {
+    PyErr_SetString(PyExc_TypeError, "byte_product_sizes(x, values, scales, residual, gain, kept, bias)");
     return nullptr;
   }
-  for (int i = 0; i < 3; ++i)
+  const at::Tensor* t[7] = {};
+  for (int i = 0; i < 7; ++i) {
+    if (i > 2 && args[i] == Py_None) continue;
     if (!THPVariable_Check(args[i])) Py_RETURN_NONE;
-  const at::Tensor& x = THPVariable_Unpack(args[0]);
-  const at::Tensor& w = THPVariable_Unpack(args[1]);
-  const at::Tensor& c = THPVariable_Unpack(args[2]);
-  const bool half = x.scalar_type() == at::kBFloat16;
-  if (!x.is_cuda() || !w.is_cuda() || !c.is_cuda() || !(half || x.scalar_type() == at::kFloat) || w.scalar_type() != at::kChar ||
-      c.scalar_type() != at::kFloat || x.dim() != 2 || w.dim() != 2 || c.dim() != 1)
-    Py_RETURN_NONE;
+    t[i] = &THPVariable_Unpack(args[i]);
+    if (!t[i]->is_cuda()) Py_RETURN_NONE;
+  }
+  const at::Tensor &x = *t[0], &w = *t[1], &c = *t[2];
+  auto code = [](const at::Tensor& v) { return v.scalar_type() == at::kBFloat16 ? 1 : v.scalar_type() == at::kFloat ? 0 : -1; };
+  if (code(x) < 0 || w.scalar_type() != at::kChar || code(c) != 0 || x.dim() != 2 || w.dim() != 2 || c.dim() != 1) Py_RETURN_NONE;
   const I tokens = x.size(0), k = x.size(1), rows = w.size(0), between = tokens > 1 ? x.stride(0) : k;
   if (k < 1 || w.size(1) != k || c.size(0) != rows || rows < 1 || (k > 1 && (x.stride(1) != 1 || w.stride(1) != 1)) || between < k ||
       c.stride(0) != 1 || w.stride(0) < k || w.stride(0) % 16 != 0 || reinterpret_cast<std::uintptr_t>(w.const_data_ptr()) % 16 != 0)
     Py_RETURN_NONE;
-  return Py_BuildValue("LLLLLi", static_cast<long long>(tokens), static_cast<long long>(k), static_cast<long long>(rows),
-                       static_cast<long long>(between), static_cast<long long>(w.stride(0)), static_cast<int>(half));
+  for (int i = 3; i < 6; i += 2)                 // the residual and where its sum goes: as x is, row after row
+    if (t[i] != nullptr && (t[i]->sizes() != x.sizes() || t[i]->scalar_type() != x.scalar_type() || !t[i]->is_contiguous())) Py_RETURN_NONE;
+  if (t[4] != nullptr && (code(*t[4]) < 0 || t[4]->numel() != k || !t[4]->is_contiguous())) Py_RETURN_NONE;
+  if (t[6] != nullptr && (code(*t[6]) != 0 || t[6]->numel() != rows || !t[6]->is_contiguous())) Py_RETURN_NONE;
+  return Py_BuildValue("LLLLLii", static_cast<long long>(tokens), static_cast<long long>(k), static_cast<long long>(rows),
+                       static_cast<long long>(between), static_cast<long long>(w.stride(0)), code(x), t[4] != nullptr ? code(*t[4]) : 0);
   END_HANDLE_TH_ERRORS
 }
 
@@ -414,7 +420,7 @@ PyMethodDef methods[] = {
     {"all_cuda", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(all_cuda)), METH_FASTCALL, "whether every tensor (None counts as one) is on a GPU"},
     {"all_contiguous", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(all_contiguous)), METH_FASTCALL, "whether every tensor (None counts as one) is contiguous"},
     {"empty", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(empty)), METH_FASTCALL, "empty(shape, dtype, device)"},
-    {"byte_product_sizes", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(byte_product_sizes)), METH_FASTCALL, "byte_product_sizes(x, values, scales): its sizes, or None"},
+    {"byte_product_sizes", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(byte_product_sizes)), METH_FASTCALL, "the sizes of a product in 8 bits, or None"},
     {"mm_t", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mm_t)), METH_FASTCALL, "mm_t(x, w): x . w^T"},
     {nullptr, nullptr, 0, nullptr}};
 

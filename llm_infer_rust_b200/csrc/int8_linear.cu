@@ -51,6 +51,12 @@ B200_EXPORT int b200_int8_alone(int tokens, int k) {
   return k >= 1 && k <= MAX_K && i8st::takes(tokens, k) && i8st::fuses(tokens, k) ? 1 : 0;
 }
 
+// How the tiled product is cut up: 1,000 times the way (0: pairs of CTAs, else the CTAs that share a tile's k) plus the columns.
+B200_EXPORT int b200_int8_plan(int tokens, int n, int k, int mode, int sms, int quads) {
+  const i8tc::Plan p = i8tc::make_plan(tokens, n, k, mode, sms, quads, i8tc::smem_fixed<__nv_bfloat16>());
+  return 1000 * p.way + p.bn;
+}
+
 // The product; `x` not null: of its rows, which go to q, s first (null where
 // b200_int8_alone says so).
 B200_EXPORT int b200_int8_linear(const void* x, const void* residual, const void* gain, void* sum_out, void* q, float* s,

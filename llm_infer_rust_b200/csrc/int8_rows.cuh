@@ -142,7 +142,7 @@ __device__ __forceinline__ void int8_chunk(const Int8Raw<T>& x, const Int8Raw<T>
 
 // The block's sums of squares and maximum (`turn`: which half of the scratch is free).
 // Returns the maximum's bits: as integers floats that are not negative compare as they do, and NaN is above infinity.
-template <bool NORM> __device__ __forceinline__ uint32_t int8_meet(float& ss, float top, float (*sums)[16], uint32_t (*tops)[16], int turn) {
+template <bool NORM> __device__ __forceinline__ uint32_t int8_meet(float& ss, float top, float (*sums)[32], uint32_t (*tops)[32], int turn) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
   if (NORM) ss = warp_sum(ss);
@@ -156,17 +156,19 @@ template <bool NORM> __device__ __forceinline__ uint32_t int8_meet(float& ss, fl
 }
 
 // Rows whose chunks fit the block's registers, CH a thread.
-template <typename T, typename TG, bool NORM, int CH>
-__global__ void __launch_bounds__(512) int8_rows_kernel(const Int8RowsParams P) {
-  __shared__ float sums[2][16];
-  __shared__ uint32_t tops[2][16];
+template <typename T, typename TG, bool NORM, int CH, int MOST = 512>
+__global__ void __launch_bounds__(MOST) int8_rows_kernel(const Int8RowsParams P) {
+  __shared__ float sums[2][32];
+  __shared__ uint32_t tops[2][32];
   pdl_launch_dependents();
   pdl_wait();
   const int threads = blockDim.x, chunks = (P.k + 7) / 8;
   const bool wide = P.wide != 0, add = NORM && P.residual != nullptr;
   const TG* gain = static_cast<const TG*>(P.gain);
-  Int8Raw<T> x[CH], r[CH];
-  auto load = [&](int row) {
+  constexpr int AHEAD = 1;
+  Int8Raw<T> x[AHEAD][CH], r[AHEAD][CH];
+  auto load = [&](int row, Int8Raw<T> (&x)[CH], Int8Raw<T> (&r)[CH]) {
+    if (row >= P.tokens) return;
     const T* xs = static_cast<const T*>(P.x) + static_cast<size_t>(row) * P.x_pitch;
     const T* rs = static_cast<const T*>(P.residual) + static_cast<size_t>(row) * P.k;
 #pragma unroll
@@ -177,9 +179,8 @@ __global__ void __launch_bounds__(512) int8_rows_kernel(const Int8RowsParams P) 
       if (add) int8_load8<T>(rs + at, P.k - at, wide, r[i]);
     }
   };
-  load(blockIdx.x);
   int turn = 0;
-  for (int row = blockIdx.x; row < P.tokens; row += gridDim.x, turn ^= 1) {
+  auto take = [&](int row, Int8Raw<T> (&x)[CH], Int8Raw<T> (&r)[CH]) {
     Int8Raw<TG> g[CH];
     if (NORM)
 #pragma unroll
@@ -195,8 +196,9 @@ __global__ void __launch_bounds__(512) int8_rows_kernel(const Int8RowsParams P) 
       const int at = (threadIdx.x + i * threads) * 8;
       if (at < P.k) int8_chunk<T, TG, NORM>(x[i], r[i], g[i], add, sum_out ? sum_out + at : nullptr, P.k - at, wide, v[i], ss, top);
     }
-    if (row + static_cast<int>(gridDim.x) < P.tokens) load(row + gridDim.x);
+    load(row + AHEAD * gridDim.x, x, r);
     const uint32_t bits = int8_meet<NORM>(ss, top, sums, tops, turn);
+    turn ^= 1;
     const Int8Step step = int8_step(bits, NORM ? rsqrtf(ss / static_cast<float>(P.k) + P.eps) : 1.0f);
     if (threadIdx.x == 0) P.s[row] = step.scale;
     int8_t* q = P.q + static_cast<size_t>(row) * P.q_pitch;
@@ -204,14 +206,61 @@ __global__ void __launch_bounds__(512) int8_rows_kernel(const Int8RowsParams P) 
     for (int i = 0; i < CH; ++i)
       if (threadIdx.x + i * threads < chunks)
         *reinterpret_cast<uint2*>(q + (threadIdx.x + i * threads) * 8) = make_uint2(int8_pack4(v[i], step), int8_pack4(v[i] + 4, step));
+  };
+#pragma unroll
+  for (int a = 0; a < AHEAD; ++a) load(blockIdx.x + a * gridDim.x, x[a], r[a]);
+  for (int row = blockIdx.x; row < P.tokens; row += AHEAD * gridDim.x)
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a)
+      if (row + a * static_cast<int>(gridDim.x) < P.tokens) take(row + a * gridDim.x, x[a], r[a]);
+}
+
+// Many long bfloat16 rows without a norm: eight chunks a thread, kept AS THEY LIE IN MEMORY and taken apart once for the maximum and
+// once for the rounding.  With two chunks a thread, what every thread does once a row (the reduction, the division, addresses) was
+// two thirds of 15 instructions an element and bound the kernel: 8,192 x 4,096 20.4 -> 17.1 us (5.9 TB/s), 8,192 x 12,288 64 -> 47 us
+// (6.4 TB/s).  Short rows and few rows lose by it (8,192 x 1,024 6.7 -> 9.0 us, 300 x 4,096 2.5 -> 2.8), rows behind a norm too, whose
+// two inputs leave room for few threads (8,192 x 4,096 45 -> 47 us).
+template <typename T>
+__global__ void __launch_bounds__(256) int8_many_rows_kernel(const Int8RowsParams P) {
+  constexpr int CH = 8;
+  __shared__ float sums[1][32];
+  __shared__ uint32_t tops[1][32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int row = blockIdx.x, threads = blockDim.x;
+  const T* xs = static_cast<const T*>(P.x) + static_cast<size_t>(row) * P.x_pitch;
+  Int8Raw<T> x[CH];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int at = (threadIdx.x + i * threads) * 8;
+    if (at < P.k) int8_load8<T>(xs + at, 8, true, x[i]);        // (whole chunks: the launch sees to it)
+  }
+  float v[8], ss = 0.0f, top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < CH; ++i)
+    if ((threadIdx.x + i * threads) * 8 < P.k) {
+      int8_floats<T>(x[i], v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = int8_top(top, v[e]);
+    }
+  const Int8Step step = int8_step(int8_meet<false>(ss, top, sums, tops, 0), 1.0f);
+  if (threadIdx.x == 0) P.s[row] = step.scale;
+  int8_t* q = P.q + static_cast<size_t>(row) * P.q_pitch;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int at = (threadIdx.x + i * threads) * 8;
+    if (at < P.k) {
+      int8_floats<T>(x[i], v);
+      *reinterpret_cast<uint2*>(q + at) = make_uint2(int8_pack4(v, step), int8_pack4(v + 4, step));
+    }
   }
 }
 
 // Longer rows are read twice.
 template <typename T, typename TG, bool NORM>
 __global__ void __launch_bounds__(512) int8_long_rows_kernel(const Int8RowsParams P) {
-  __shared__ float sums[1][16];
-  __shared__ uint32_t tops[1][16];
+  __shared__ float sums[1][32];
+  __shared__ uint32_t tops[1][32];
   pdl_launch_dependents();
   pdl_wait();
   const int row = blockIdx.x, chunks = (P.k + 7) / 8;
@@ -246,32 +295,39 @@ __global__ void __launch_bounds__(512) int8_long_rows_kernel(const Int8RowsParam
   }
 }
 
-template <typename T, typename TG, bool NORM, int CH>
+template <typename T, typename TG, bool NORM, int CH, int MOST = 512>
 static int int8_rows_kept(const Int8RowsParams& P, int threads, int sms, cudaStream_t stream) {
   // Persistent: as many blocks as fit at once (threads, registers: found once for each size of block).
-  static int fits[17];
+  static int fits[33];
   int& blocks = fits[threads / 32];
   if (blocks == 0) {
     int n = 0;
-    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, int8_rows_kernel<T, TG, NORM, CH>, threads, 0);
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, int8_rows_kernel<T, TG, NORM, CH, MOST>, threads, 0);
     if (e != cudaSuccess) return static_cast<int>(e);
     blocks = n < 1 ? 1 : n;
   }
   const int most = sms * blocks;
-  return b200_launch(int8_rows_kernel<T, TG, NORM, CH>, dim3(P.tokens < most ? P.tokens : most), dim3(threads), 0, stream, 0, P);
+  return b200_launch(int8_rows_kernel<T, TG, NORM, CH, MOST>, dim3(P.tokens < most ? P.tokens : most), dim3(threads), 0, stream, 0, P);
 }
 template <typename T, typename TG, bool NORM>
 static int int8_rows_normed(const Int8RowsParams& P, int sms, cudaStream_t stream) {
   const int chunks = (P.k + 7) / 8;
   auto threads = [&](int ch) { return ((chunks + ch - 1) / ch + 31) / 32 * 32; };
-  // Few rows: the row's latency is the time, so a thread takes one chunk where it can.  Many: what counts are the bytes on their
-  // way; two chunks a thread keep them (8,192 x 4,096 behind a norm 47 us, 94 % of the copy rate), four leave room for one
-  // block an SM (12,288 columns: 3.0 TB/s), and reading rows twice, the second time out of the caches, is faster (5.2).
+  if constexpr (sizeof(T) == 2 && !NORM)
+    if (P.tokens > 8 * sms && P.wide && P.k % 8 == 0 && chunks >= 512 && chunks <= 2048)
+      return b200_launch(int8_many_rows_kernel<T>, dim3(P.tokens), dim3(threads(8)), 0, stream, 0, P);
+  // Few rows: the row's latency is the time, so a thread takes as little as 512 of them allow.  Many: what counts are the bytes on
+  // their way; two chunks a thread keep them (8,192 x 4,096 behind a norm 45 us; four chunks, half the threads: 61), and rows longer
+  // than that are faster read twice, the second time out of the caches (8,192 x 12,288 behind a norm 130 us, 5.4 TB/s), but for float32
+  // without a norm, where 1,024 threads still keep theirs (2,048 x 12,288: 20 us, read twice 25).
   if (P.tokens <= sms) {
     if (chunks <= 512) return int8_rows_kept<T, TG, NORM, 1>(P, threads(1), sms, stream);
+    if (chunks <= 1024) return int8_rows_kept<T, TG, NORM, 2>(P, threads(2), sms, stream);
     if (chunks <= 512 * INT8_ROW_CHUNKS) return int8_rows_kept<T, TG, NORM, INT8_ROW_CHUNKS>(P, threads(INT8_ROW_CHUNKS), sms, stream);
   } else if (chunks <= 1024) {
     return int8_rows_kept<T, TG, NORM, 2>(P, threads(2), sms, stream);
+  } else if (!NORM && sizeof(T) == 4 && chunks <= 2048) {
+    return int8_rows_kept<T, TG, false, 2, 1024>(P, threads(2), sms, stream);
   }
   return b200_launch(int8_long_rows_kernel<T, TG, NORM>, dim3(P.tokens), dim3(512), 0, stream, 0, P);
 }

@@ -152,28 +152,23 @@ __global__ void __launch_bounds__(THREADS, 1) stream_kernel(const Int8ProductPar
     }
     cp_async_commit();
   };
+  if constexpr (!FUSED) {
+    const int pieces = plan.x_pitch / 16;
+    for (int i = threadIdx.x; i < P.tokens * pieces; i += THREADS) {
+      const int row = i / pieces, at = (i - row * pieces) * 16, left = P.k - at;         // (what lies beyond the row reads as 0)
+      const int8_t* from = P.q + row * P.q_pitch + (left > 0 ? at : 0);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_u32(xs + row * plan.x_pitch + at)), "l"(from), "r"(max(0, min(16, left))));
+    }
+    cp_async_commit();
+  }
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d) copy(d);
 
   if constexpr (FUSED) {
     tokens_to_8_bits<T, TG, NORM>(R, xs, plan.x_pitch, token_scale, sums, tops);
   } else {
-    const int pieces = plan.x_pitch / 16;
-    for (int i = threadIdx.x; i < P.tokens * pieces; i += THREADS) {
-      const int row = i / pieces, at = (i - row * pieces) * 16;
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (at < P.k) v = *reinterpret_cast<const uint4*>(P.q + row * P.q_pitch + at);
-      if (at + 16 > P.k) {                                                      // (what lies beyond the row does not count)
-        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int left = P.k - at - 4 * j;
-          w[j] &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
-        }
-      }
-      *reinterpret_cast<uint4*>(xs + row * plan.x_pitch + at) = v;
-    }
     if (threadIdx.x < P.tokens) token_scale[threadIdx.x] = P.s[threadIdx.x];
+    cp_async_wait<DEPTH>();                                                     // (the tokens; the weights behind them are on their way)
   }
   __syncthreads();
 

@@ -406,11 +406,11 @@ product_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__
 #pragma unroll
         for (int e = 0; e < LANES; ++e) *reinterpret_cast<uint4*>(mine + turned<T>(lane, e)) = packed[e];
         __syncwarp();
-        if (whole && cols == 32) {
+        if (whole) {                                                            // (whole pieces of 16 bytes, up to the last column too)
 #pragma unroll
           for (int q = 0; q < LANES; ++q) {
             const int r = q * (32 / LANES) + lane / LANES, chunk = lane % LANES;
-            if (r >= low && r < high)
+            if (r >= low && r < high && chunk * static_cast<int>(16 / sizeof(T)) < cols)
               *reinterpret_cast<uint4*>(out + static_cast<size_t>(row0 + r) * P.n + col0 + chunk * (16 / sizeof(T))) =
                   *reinterpret_cast<const uint4*>(mine + turned<T>(r, chunk));
           }
@@ -574,39 +574,71 @@ static void set_stages(Plan& p, int rows_a_cta, int fixed) {
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
 }
 
-// How a product is cut up (see the top of the file): what its fullest SM takes, in us.  A block of k of one CTA takes what its
-// bytes take at 92 GB/s, but 125 ns at least; of a pair's CTA at 118 GB/s, or the MMA's 2 bn cycles.  (One CTA a tile, 4,096 k,
-// 64 tokens: 96 tiles of 64 columns 9.5 us, 48 of 128 11.9, 192 of 32 in two rounds 12.0.)  Sharing k costs about 2 us more with
-// two CTAs and 4.5 with four.
-static inline Plan make_plan(int tokens, int n, int k, int mode, int sms, int fixed) {
+// How a product is cut up (see the top of the file): the way that takes its fullest SM the least, by a model of it in us.  `quads`:
+// clusters of four CTAs that run side by side.
+//   a block of k      what its bytes take at 126 GB/s an SM, 0.19 us at least (a pair's: or its MMAs' time)
+//   a tile's epilogue 0.0024 us a column, 0.4 us more where warps find pieces of less than 32 columns; it hides behind the next tile
+//   sharing k         1.4 us with two CTAs, 3.8 us with four (with the cluster's launch; the exchange itself is below 1 us)
+// Fitted to 140 products of 20 to 2,048 tokens that were run all ways (behind rows to 8 bits, cold weights): the way chosen takes 1.6 %
+// longer than the best one on average.  (Of it, 64 columns / 128 / 32 in two rounds, 64 tokens, 4,096 k, 6,144 columns: 9.5 / 11.9 /
+// 12.0 us; 100 tokens, 12,288 k, 4,096 columns: 128 columns shared by four 16.1, 64 by two 16.6, 32 by none 18.9, pairs of 190 tokens
+// 26.9 us at 24,576 gated columns where single tiles take 30.6.)
+static inline Plan make_plan(int tokens, int n, int k, int mode, int sms, int quads, int fixed) {
   Plan p = {};
   const int glu = mode == INT8_GLU ? 2 : 1, kb = (k + BK - 1) / BK;
   const long long cols = static_cast<long long>(n) * glu, m_tiles = (tokens + BM - 1) / BM;
   p.box = tokens >= BM ? BM : (tokens + 7) / 8 * 8;
   double best = 0.0;
+  auto consider = [&](int way, int bn, long long tiles, long long side_by_side, double block, int blocks, double more) {
+    const long long rounds = (tiles + side_by_side - 1) / side_by_side;
+    const double products = blocks * block, epilogue = 0.0024 * bn + (bn / glu % 32 ? 0.4 : 0.0);
+    const double cost = way > 1 ? rounds * (products + epilogue / 2 + more)
+                                : products + (rounds - 1) * (products > epilogue ? products : epilogue) + epilogue + more;
+    if (best == 0.0 || cost < best) { best = cost; p.way = way; p.bn = bn; }
+  };
   for (int split = 1; split <= 4 && split <= kb; split *= 2)
     for (int bn = 256; bn >= 32; bn -= 16) {
       if (bn % (4 * glu * split) != 0) continue;
-      const long long rounds = (m_tiles * ((cols + bn - 1) / bn) * split + sms - 1) / sms;
-      if (split > 1 && rounds > 1) continue;
-      const double block = (p.box + bn) * BK / 92e3;
-      const double cost = static_cast<double>(rounds * ((kb + split - 1) / split)) * (block > 0.125 ? block : 0.125) +
-                          (split == 4 ? 5.4 : split == 2 ? 2.2 : 0.0) + bn * 0.008;
-      if (best == 0.0 || cost < best) { best = cost; p.way = split; p.bn = bn; }
+      const double block = (p.box + bn) * BK / 126e3;
+      consider(split, bn, m_tiles * ((cols + bn - 1) / bn), split == 1 ? sms : split == 2 ? sms / 2 : quads, block > 0.19 ? block : 0.19,
+               (kb + split - 1) / split, split == 1 ? 0.0 : split == 2 ? 1.4 : 3.8);
     }
   if (tokens > BM)
     for (int bn = 256; bn >= 128; bn -= 32) {
-      const long long rounds = ((tokens + 255ll) / 256 * ((cols + bn - 1) / bn) + sms / 2 - 1) / (sms / 2);
-      const double bytes = (BM + bn / 2) * BK / 118e3, mma = bn * 2 / 1.85e3;
-      const double cost = static_cast<double>(rounds * kb) * (bytes > mma ? bytes : mma) + bn * 0.008;
-      if (cost < best) { best = cost; p.way = 0; p.bn = bn; }
+      const double bytes = (BM + bn / 2) * BK / 126e3, mma = bn * 0.0011;
+      consider(0, bn, (tokens + 255ll) / 256 * ((cols + bn - 1) / bn), sms / 2, bytes > mma ? bytes : mma, kb, 0.12);
     }
   set_stages(p, p.way == 0 ? p.bn / 2 : p.bn, fixed);
   return p;
 }
 
+// Clusters of four CTAs of the split kernel that run side by side (1 where the device does not say).
+template <typename T, int MODE> static int quads_side_by_side() {
+  static int known[64];                        // plus one, of the devices that were asked
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device >= 64) return 1;
+  if (known[device] == 0) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(4);
+    config.blockDim = dim3(THREADS);
+    config.dynamicSmemBytes = SMEM_MOST;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 4;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    int n = 0;
+    if (cudaFuncSetAttribute(product_kernel<T, MODE, 1, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, product_kernel<T, MODE, 1, 4>, &config) != cudaSuccess || n < 1)
+      n = 1;
+    known[device] = n + 1;
+  }
+  return known[device] - 1;
+}
+
 template <typename T, int MODE> static int product(const Int8ProductParams& P, int sms, cudaStream_t stream) {
-  const Plan plan = make_plan(P.tokens, P.n, P.k, MODE, sms, smem_fixed<T>());
+  const Plan plan = make_plan(P.tokens, P.n, P.k, MODE, sms, quads_side_by_side<T, MODE>(), smem_fixed<T>());
   const int tall = plan.way == 0 ? 2 * BM : BM, wide = plan.bn / (MODE == INT8_GLU ? 2 : 1);
   const long long tiles = static_cast<long long>((P.tokens + tall - 1) / tall) * ((P.n + wide - 1) / wide);
   if (tiles > 0x0fffffff || plan.stages < 2) return B200_BAD_SIZE;

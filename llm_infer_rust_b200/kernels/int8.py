@@ -131,51 +131,60 @@ _sizes = ops._bind("byte_product_sizes")
 
 
 def _product(x, weight: Int8Weight, bias, out_dtype, mode: int, glu: str, limit: float, alpha: float) -> torch.Tensor:
+    if ops._held is not None or ops._chain is not None:
+        ops.flush_chain()                        # (what waits in the chain may be what is read here)
     w, w_scales = weight
+    values = scales = residual = gain = kept = None
+    eps, gain_code = 0.0, 0
     if isinstance(x, Int8Rows):
-        src = residual = gain = kept = None
-        eps, (values, scales) = 0.0, x
+        src, (values, scales) = None, x
         _check_8_bit(x, "rows")
         _check_8_bit(weight, "weights")
         tokens, k = values.shape
-        _check_k(k)
         rows, w_pitch, pitch, out_dtype, x_pitch, x_code = w.shape[0], w.stride(0), values.stride(0), out_dtype or torch.bfloat16, 0, 0
+        _check_sizes(k, w, bias)
         ops._cuda(values, scales, w, w_scales, bias)
     else:
-        if isinstance(x, ops.PendingNorm):
-            src, residual, gain, kept, eps = _source(x)
+        if not isinstance(x, ops.PendingNorm):
+            src = x
+        elif x.rows is None:
+            src, residual, gain, kept, eps = x.x, x.residual, x.weight, x.residual_out, x.eps
         else:
-            src, residual, gain, kept, eps = x, None, None, None, 0.0
-        sizes = _sizes(src, w, w_scales)
-        if sizes is None:                        # (something is not as it should be, or there is nothing to do)
+            src = x.materialize()                # (the norm's own kernel picks rows)
+        sizes = _sizes(src, w, w_scales, residual, gain, kept, bias)
+        if sizes is None:                        # something is not as it should be, or there is nothing to do
             _check_8_bit(weight, "weights")
-            _source(src)
-            ops._cuda(src, w, w_scales)
-            sizes = (*src.shape, w.shape[0], src.stride(0) if src.shape[0] > 1 else src.shape[1], w.stride(0), ops._code(src))
-        ops._cuda(residual, gain, kept, bias)
-        tokens, k, rows, x_pitch, w_pitch, x_code = sizes
+            _source(x if gain is not None else src)
+            ops._cuda(src, w, w_scales, residual, gain, kept, bias)
+            _check_sizes(src.shape[1], w, bias)
+            sizes = (*src.shape, w.shape[0], src.stride(0) if src.shape[0] > 1 else src.shape[1], w.stride(0), ops._code(src),
+                     0 if gain is None else ops._code(gain))
+        tokens, k, rows, x_pitch, w_pitch, x_code, gain_code = sizes
+        pitch, out_dtype = row_pitch(k), out_dtype or src.dtype
         _check_k(k)
-        pitch, out_dtype, values, scales = row_pitch(k), out_dtype or src.dtype, None, None
-    if w.shape[1] != k:
-        raise KernelError(f"the rows have {k} columns, the weight has {w.shape[1]}")
     n = rows
     if mode == _GLU:
         if rows % 2:
             raise KernelError("gate and up rows of a gated product are as many")
         n = rows // 2
-    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != rows or not bias.is_contiguous()):
-        raise KernelError("the bias is float32, one element an output channel")
     lib, device = _lib(glu), w.device
     out = ops._empty((tokens, n), out_dtype, device)
-    if values is None and (not n or not lib.b200_int8_alone(tokens, k)):
+    if values is None and (tokens > 8 or not n or not lib.b200_int8_alone(tokens, k)):
         # the tokens in 8 bits and their scales, between the two kernels of the call
         values = ops._empty((tokens * pitch + 4 * tokens,), torch.int8, device)
         scales = values.data_ptr() + tokens * pitch
     rc = lib.b200_int8_linear(src, residual, gain, kept, values, scales, w, w_scales, bias, out, tokens, n, k, x_pitch, pitch, w_pitch,
-                              x_code, 0 if gain is None else ops._code(gain), ops._code(out), mode, eps, float(limit), float(alpha),
-                              ops.error_word(device), ops._stream())
+                              x_code, gain_code, ops._code(out), mode, eps, float(limit), float(alpha), ops.error_word(device), ops._stream())
     ops._ok(rc, "int8_linear", 0 if not tokens else (0 if src is None else 1) + (1 if n and (src is None or values is not None) else 0))
     return out
+
+
+def _check_sizes(k: int, w: torch.Tensor, bias) -> None:
+    _check_k(k)
+    if w.shape[1] != k:
+        raise KernelError(f"the rows have {k} columns, the weight has {w.shape[1]}")
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != w.shape[0] or not bias.is_contiguous()):
+        raise KernelError("the bias is float32, one element an output channel")
 
 
 def int8_linear(x, weight: Int8Weight, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
