@@ -30,6 +30,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <iterator>
 #include <vector>
 
 #if !defined(__x86_64__) && !defined(__aarch64__)
@@ -236,36 +237,71 @@ PyObject* mm_t(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// byte_product_sizes(x, values, scales, residual, gain, kept, bias) -> (tokens, k, rows, elements between x's rows, bytes between the
-// weights' rows, x's type, gain's type) where everything is as a product in 8 bits takes it (the last four may be None), else None
-// (the wrapper then says what is wrong): one call for some thirty attributes of up to seven tensors, each of which costs Python a
-// tenth of a microsecond.
-PyObject* byte_product_sizes(PyObject*, PyObject* const* args, Py_ssize_t n) {
+// byte_product(product, alone, x, values, scales, residual, gain, kept, bias, dtype, mode, eps, limit, alpha, error word, stream)
+//   -> (out, code, kernels)
+// A product in 8 bits (csrc/int8_linear.cu, whose two entry points come first) as one call: what the tensors must be (the four from
+// `residual` on may be None), the output, the place for the tokens in 8 bits where the product needs one, and the launch.  None, and
+// nothing done, where something is not as it should be (the wrapper then says what) or this thread records its calls.  A decode
+// step's products take the host longer than the GPU otherwise: 6.8 us through Python, of which 2.8 are the launch.
+PyObject* byte_product(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 7) {
-    PyErr_SetString(PyExc_TypeError, "byte_product_sizes(x, values, scales, residual, gain, kept, bias)");
+  if (n != 16 || Py_TYPE(args[0]) != &entry_type || Py_TYPE(args[1]) != &entry_type || !(args[9] == Py_None || THPDtype_Check(args[9])) ||
+      !PyLong_Check(args[10]) || !PyFloat_Check(args[11]) || !PyFloat_Check(args[12]) || !PyFloat_Check(args[13]) ||
+      !THPVariable_Check(args[14]) || !PyLong_Check(args[15])) {
+    PyErr_SetString(PyExc_TypeError, "byte_product(product, alone, x, values, scales, residual, gain, kept, bias, dtype, mode, eps, limit, alpha, "
+                                     "error word, stream)");
     return nullptr;
   }
+  if (recording != nullptr) Py_RETURN_NONE;
   const at::Tensor* t[7] = {};
   for (int i = 0; i < 7; ++i) {
-    if (i > 2 && args[i] == Py_None) continue;
-    if (!THPVariable_Check(args[i])) Py_RETURN_NONE;
-    t[i] = &THPVariable_Unpack(args[i]);
+    PyObject* a = args[i + 2];
+    if (i > 2 && a == Py_None) continue;
+    if (!THPVariable_Check(a)) Py_RETURN_NONE;
+    t[i] = &THPVariable_Unpack(a);
     if (!t[i]->is_cuda()) Py_RETURN_NONE;
   }
   const at::Tensor &x = *t[0], &w = *t[1], &c = *t[2];
-  auto code = [](const at::Tensor& v) { return v.scalar_type() == at::kBFloat16 ? 1 : v.scalar_type() == at::kFloat ? 0 : -1; };
-  if (code(x) < 0 || w.scalar_type() != at::kChar || code(c) != 0 || x.dim() != 2 || w.dim() != 2 || c.dim() != 1) Py_RETURN_NONE;
-  const I tokens = x.size(0), k = x.size(1), rows = w.size(0), between = tokens > 1 ? x.stride(0) : k;
-  if (k < 1 || w.size(1) != k || c.size(0) != rows || rows < 1 || (k > 1 && (x.stride(1) != 1 || w.stride(1) != 1)) || between < k ||
-      c.stride(0) != 1 || w.stride(0) < k || w.stride(0) % 16 != 0 || reinterpret_cast<std::uintptr_t>(w.const_data_ptr()) % 16 != 0)
+  auto code_of = [](at::ScalarType s) -> I { return s == at::kBFloat16 ? 1 : s == at::kFloat ? 0 : -1; };
+  auto code = [&](const at::Tensor& v) { return code_of(v.scalar_type()); };
+  const at::ScalarType type = args[9] == Py_None ? x.scalar_type() : reinterpret_cast<THPDtype*>(args[9])->scalar_type;
+  if (code(x) < 0 || code_of(type) < 0 || w.scalar_type() != at::kChar || code(c) != 0 || x.dim() != 2 || w.dim() != 2 || c.dim() != 1) Py_RETURN_NONE;
+  const I mode = PyLong_AsLongLong(args[10]), stream = PyLong_AsLongLong(args[15]);
+  if (PyErr_Occurred()) return nullptr;
+  const I tokens = x.size(0), k = x.size(1), rows = w.size(0), between = tokens > 1 ? x.stride(0) : k, w_pitch = w.stride(0);
+  if (tokens < 1 || k < 1 || k > 131071 || w.size(1) != k || c.size(0) != rows || rows < 1 || (mode != 0 && rows % 2 != 0) || between < k ||
+      (k > 1 && (x.stride(1) != 1 || w.stride(1) != 1)) || (rows > 1 && c.stride(0) != 1) || w_pitch < k || w_pitch % 16 != 0 ||
+      reinterpret_cast<std::uintptr_t>(w.const_data_ptr()) % 16 != 0 || tokens > INT32_MAX || rows > INT32_MAX)
     Py_RETURN_NONE;
   for (int i = 3; i < 6; i += 2)                 // the residual and where its sum goes: as x is, row after row
     if (t[i] != nullptr && (t[i]->sizes() != x.sizes() || t[i]->scalar_type() != x.scalar_type() || !t[i]->is_contiguous())) Py_RETURN_NONE;
   if (t[4] != nullptr && (code(*t[4]) < 0 || t[4]->numel() != k || !t[4]->is_contiguous())) Py_RETURN_NONE;
   if (t[6] != nullptr && (code(*t[6]) != 0 || t[6]->numel() != rows || !t[6]->is_contiguous())) Py_RETURN_NONE;
-  return Py_BuildValue("LLLLLii", static_cast<long long>(tokens), static_cast<long long>(k), static_cast<long long>(rows),
-                       static_cast<long long>(between), static_cast<long long>(w.stride(0)), code(x), t[4] != nullptr ? code(*t[4]) : 0);
+  if ((t[3] != nullptr || t[5] != nullptr) && t[4] == nullptr) Py_RETURN_NONE;
+  const I columns = mode != 0 ? rows / 2 : rows, pitch = (k + 15) / 16 * 16;
+  const float floats[MAX_FLOATS] = {static_cast<float>(PyFloat_AS_DOUBLE(args[11])), static_cast<float>(PyFloat_AS_DOUBLE(args[12])),
+                                    static_cast<float>(PyFloat_AS_DOUBLE(args[13]))};
+  I* const err = THPVariable_Unpack(args[14]).is_cuda() ? reinterpret_cast<I*>(THPVariable_Unpack(args[14]).mutable_data_ptr()) : nullptr;
+  void* const product = reinterpret_cast<Entry*>(args[0])->fn;
+  void* const alone = reinterpret_cast<Entry*>(args[1])->fn;
+  at::Tensor out, place;
+  int rc;
+  bool placed = false;
+  {
+    pybind11::gil_scoped_release free;
+    out = at::empty({tokens, columns}, x.options().dtype(type).requires_grad(false));
+    I ints[MAX_INTS] = {tokens, k};
+    auto address = [](const at::Tensor* v) { return v != nullptr ? reinterpret_cast<I>(v->const_data_ptr()) : 0; };
+    placed = invoke(alone, ints, 2, floats) == 0;
+    if (placed) place = at::empty({tokens * pitch + 4 * tokens}, x.options().dtype(at::kChar).requires_grad(false));
+    const I q = placed ? address(&place) : 0;
+    const I all[] = {address(&x), address(t[3]), address(t[4]), address(t[5]), q, placed ? q + tokens * pitch : 0, address(&w), address(&c),
+                     address(t[6]), address(&out), tokens, columns, k, between, pitch, w_pitch, code(x), t[4] != nullptr ? code(*t[4]) : 0,
+                     code_of(type), mode, reinterpret_cast<I>(err), stream};
+    std::copy(std::begin(all), std::end(all), ints);
+    rc = invoke(product, ints, static_cast<int>(std::size(all)), floats);
+  }
+  return Py_BuildValue("Nii", THPVariable_Wrap(out), rc, placed ? 2 : 1);
   END_HANDLE_TH_ERRORS
 }
 
@@ -420,7 +456,7 @@ PyMethodDef methods[] = {
     {"all_cuda", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(all_cuda)), METH_FASTCALL, "whether every tensor (None counts as one) is on a GPU"},
     {"all_contiguous", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(all_contiguous)), METH_FASTCALL, "whether every tensor (None counts as one) is contiguous"},
     {"empty", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(empty)), METH_FASTCALL, "empty(shape, dtype, device)"},
-    {"byte_product_sizes", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(byte_product_sizes)), METH_FASTCALL, "the sizes of a product in 8 bits, or None"},
+    {"byte_product", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(byte_product)), METH_FASTCALL, "a product in 8 bits: (out, code, kernels), or None"},
     {"mm_t", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mm_t)), METH_FASTCALL, "mm_t(x, w): x . w^T"},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -597,7 +597,7 @@ static inline Plan make_plan(int tokens, int n, int k, int mode, int sms, int qu
     if (best == 0.0 || cost < best) { best = cost; p.way = way; p.bn = bn; }
   };
   for (int split = 1; split <= 4 && split <= kb; split *= 2)
-    for (int bn = 256; bn >= 32; bn -= 16) {
+    for (int bn = 256; bn >= 32; bn -= bn > 128 ? 32 : 16) {
       if (bn % (4 * glu * split) != 0) continue;
       const double block = (p.box + bn) * BK / 126e3;
       consider(split, bn, m_tiles * ((cols + bn - 1) / bn), split == 1 ? sms : split == 2 ? sms / 2 : quads, block > 0.19 ? block : 0.19,

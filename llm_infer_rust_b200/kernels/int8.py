@@ -18,7 +18,7 @@ from typing import NamedTuple, Optional, Union
 import torch
 
 from . import ops
-from .build import load_entry_points
+from .build import load_call_binding, load_entry_points
 from .ops import KernelError
 
 MAX_K = 131071              # 128 * 128 * K stays below 2^31
@@ -127,64 +127,68 @@ def _source(x):
     return src, residual, gain, kept, x.eps
 
 
-_sizes = ops._bind("byte_product_sizes")
+_byte_product = None             # of the compiled binding, which is loaded at the first product
 
 
 def _product(x, weight: Int8Weight, bias, out_dtype, mode: int, glu: str, limit: float, alpha: float) -> torch.Tensor:
+    global _byte_product
     if ops._held is not None or ops._chain is not None:
         ops.flush_chain()                        # (what waits in the chain may be what is read here)
     w, w_scales = weight
     values = scales = residual = gain = kept = None
-    eps, gain_code = 0.0, 0
+    eps = 0.0
     if isinstance(x, Int8Rows):
         src, (values, scales) = None, x
-        _check_8_bit(x, "rows")
-        _check_8_bit(weight, "weights")
-        tokens, k = values.shape
-        rows, w_pitch, pitch, out_dtype, x_pitch, x_code = w.shape[0], w.stride(0), values.stride(0), out_dtype or torch.bfloat16, 0, 0
-        _check_sizes(k, w, bias)
-        ops._cuda(values, scales, w, w_scales, bias)
+    elif not isinstance(x, ops.PendingNorm):
+        src = x
+    elif x.rows is None:
+        src, residual, gain, kept, eps = x.x, x.residual, x.weight, x.residual_out, x.eps
     else:
-        if not isinstance(x, ops.PendingNorm):
-            src = x
-        elif x.rows is None:
-            src, residual, gain, kept, eps = x.x, x.residual, x.weight, x.residual_out, x.eps
-        else:
-            src = x.materialize()                # (the norm's own kernel picks rows)
-        sizes = _sizes(src, w, w_scales, residual, gain, kept, bias)
-        if sizes is None:                        # something is not as it should be, or there is nothing to do
-            _check_8_bit(weight, "weights")
-            _source(x if gain is not None else src)
-            ops._cuda(src, w, w_scales, residual, gain, kept, bias)
-            _check_sizes(src.shape[1], w, bias)
-            sizes = (*src.shape, w.shape[0], src.stride(0) if src.shape[0] > 1 else src.shape[1], w.stride(0), ops._code(src),
-                     0 if gain is None else ops._code(gain))
-        tokens, k, rows, x_pitch, w_pitch, x_code, gain_code = sizes
-        pitch, out_dtype = row_pitch(k), out_dtype or src.dtype
-        _check_k(k)
-    n = rows
+        src = x.materialize()                    # (the norm's own kernel picks rows)
+    lib = _lib(glu)
+    if src is not None and w.is_cuda:
+        if _byte_product is None:
+            _byte_product = load_call_binding().byte_product
+        got = _byte_product(lib.b200_int8_linear, lib.b200_int8_alone, src, w, w_scales, residual, gain, kept, bias, out_dtype, mode,
+                            eps, float(limit), float(alpha), ops.error_word(w.device), ops._stream())
+        if got is not None:
+            out, rc, kernels = got
+            ops._ok(rc, "int8_linear", kernels)
+            return out
+    # Rows that are in 8 bits already, a layer's calls that are being kept, nothing to do, or something that is not as it should be.
+    _check_8_bit(weight, "weights")
+    if src is None:
+        _check_8_bit(x, "rows")
+        tokens, k = values.shape
+        pitch, out_dtype, x_pitch, x_code = values.stride(0), out_dtype or torch.bfloat16, 0, 0
+    else:
+        _source(x if gain is not None else src)
+        tokens, k = src.shape
+        pitch, out_dtype, x_pitch, x_code = row_pitch(k), out_dtype or src.dtype, src.stride(0) if tokens > 1 else k, ops._code(src)
+    _check_k(k)
+    rows = n = w.shape[0]
+    if w.shape[1] != k:
+        raise KernelError(f"the rows have {k} columns, the weight has {w.shape[1]}")
     if mode == _GLU:
         if rows % 2:
             raise KernelError("gate and up rows of a gated product are as many")
         n = rows // 2
-    lib, device = _lib(glu), w.device
-    out = ops._empty((tokens, n), out_dtype, device)
-    if values is None and (tokens > 8 or not n or not lib.b200_int8_alone(tokens, k)):
-        # the tokens in 8 bits and their scales, between the two kernels of the call
-        values = ops._empty((tokens * pitch + 4 * tokens,), torch.int8, device)
-        scales = values.data_ptr() + tokens * pitch
-    rc = lib.b200_int8_linear(src, residual, gain, kept, values, scales, w, w_scales, bias, out, tokens, n, k, x_pitch, pitch, w_pitch,
-                              x_code, gain_code, ops._code(out), mode, eps, float(limit), float(alpha), ops.error_word(device), ops._stream())
-    ops._ok(rc, "int8_linear", 0 if not tokens else (0 if src is None else 1) + (1 if n and (src is None or values is not None) else 0))
-    return out
-
-
-def _check_sizes(k: int, w: torch.Tensor, bias) -> None:
-    _check_k(k)
-    if w.shape[1] != k:
-        raise KernelError(f"the rows have {k} columns, the weight has {w.shape[1]}")
-    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != w.shape[0] or not bias.is_contiguous()):
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != rows or not bias.is_contiguous()):
         raise KernelError("the bias is float32, one element an output channel")
+    if out_dtype not in ops._CODES:
+        raise KernelError(f"dtype {out_dtype} is not supported (float32 and bfloat16 are)")
+    ops._cuda(src, residual, gain, kept, values, scales, w, w_scales, bias)
+    out = ops._empty((tokens, n), out_dtype, w.device)
+    if values is None:
+        # the tokens in 8 bits and their scales, between the two kernels of the call
+        values = ops._empty((tokens * pitch + 4 * tokens,), torch.int8, w.device)
+        scales = values.data_ptr() + tokens * pitch
+    rc = lib.b200_int8_linear(src, residual, gain, kept, values, scales, w, w_scales, bias, out, tokens, n, k, x_pitch, pitch, w.stride(0),
+                              x_code, 0 if gain is None else ops._code(gain), ops._code(out), mode, eps, float(limit), float(alpha),
+                              ops.error_word(w.device), ops._stream())
+    both = src is not None and n and not lib.b200_int8_alone(tokens, k)
+    ops._ok(rc, "int8_linear", 0 if not tokens else 2 if both else int(src is not None or n > 0))
+    return out
 
 
 def int8_linear(x, weight: Int8Weight, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
