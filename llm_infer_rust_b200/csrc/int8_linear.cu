@@ -32,9 +32,9 @@ static int rows_params(Int8RowsParams& R, const void* x, const void* residual, c
   if (tokens < 0 || k < 1 || k > MAX_K || x_pitch < k || q_pitch < k) return B200_BAD_SIZE;
   if (!int8_aligned(q, q_pitch)) return B200_BAD_ALIGN;
   const long long e = x_code == B200_F32 ? 4 : 2;
-  const bool wide = int8_aligned(x, x_pitch * e) && int8_aligned(residual, residual ? k * e : 0) && int8_aligned(gain, 0) &&
+  const bool whole = k % 8 == 0 && int8_aligned(x, x_pitch * e) && int8_aligned(residual, residual ? k * e : 0) && int8_aligned(gain, 0) &&
                     int8_aligned(sum_out, sum_out ? k * e : 0);
-  R = {x, residual, gain, sum_out, static_cast<int8_t*>(q), s, tokens, k, x_pitch, q_pitch, eps, wide};
+  R = {x, residual, gain, sum_out, static_cast<int8_t*>(q), s, tokens, k, x_pitch, q_pitch, eps, whole};
   return 0;
 }
 

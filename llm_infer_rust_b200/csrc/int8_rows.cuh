@@ -28,7 +28,7 @@ struct Int8RowsParams {
   int tokens, k;
   long long x_pitch, q_pitch;
   float eps;
-  int wide;                  // whether 8 elements of x, residual, gain and sum_out may be moved at once
+  int whole;                 // whether every row of x, residual, gain and sum_out is whole eights of elements at multiples of 16 bytes
 };
 
 // Eight consecutive elements as they lie in memory.
@@ -37,16 +37,59 @@ template <typename T> __device__ __forceinline__ T int8_zero();
 template <> __device__ __forceinline__ float int8_zero<float>() { return 0.0f; }
 template <> __device__ __forceinline__ __nv_bfloat16 int8_zero<__nv_bfloat16>() { return __float2bfloat16_rn(0.0f); }
 
-// The elements from `p` on, of which `n` exist (the others read as 0).
-template <typename T> __device__ __forceinline__ void int8_load8(const T* p, int n, bool wide, Int8Raw<T>& r) {
-  if (wide && n >= 8) {
+// The words w[0 .. N) of what begins `bytes` (an even number below 20) behind w's start.  (Branches on a number that all threads
+// share: word by word selections cost three times the instructions.)
+template <int BY, int N, int M> __device__ __forceinline__ void int8_shift_by(uint32_t (&w)[M], uint32_t bits) {
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.v[i] = reinterpret_cast<const uint4*>(p)[i];
+  for (int i = 0; i < N; ++i) w[i] = i + BY + 1 < M ? __funnelshift_r(w[i + BY], w[i + BY + 1], bits) : w[i + BY] >> bits;
+}
+template <int N, int M> __device__ __forceinline__ void int8_shift(uint32_t (&w)[M], int bytes) {
+  const uint32_t bits = (bytes & 2) * 8;
+  switch (bytes >> 2) {
+    case 0: int8_shift_by<0, N>(w, bits); break;
+    case 1: int8_shift_by<1, N>(w, bits); break;
+    case 2: int8_shift_by<2, N>(w, bits); break;
+    case 3: int8_shift_by<3, N>(w, bits); break;
+    default: int8_shift_by<4, N>(w, bits); break;
+  }
+}
+
+// Eight elements in a row from `p` on, of which `n` exist (the others read as 0).  WHOLE: all of them do, at a multiple of 16 bytes.
+// Else the aligned 16-byte pieces that hold them are fetched and shifted into place: rows whose length is no multiple of eight begin
+// anywhere, and element by element they took three times as long.  (No piece without an element of the row is touched.)
+template <typename T, bool WHOLE> __device__ __forceinline__ void int8_load8(const T* p, int n, Int8Raw<T>& r) {
+  constexpr int PIECES = sizeof(T) / 2;
+  if constexpr (WHOLE) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) r.v[i] = reinterpret_cast<const uint4*>(p)[i];
   } else {
-    T e[8];
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15u), bytes = off + min(n, 8) * static_cast<int>(sizeof(T));
+    const uint4* from = reinterpret_cast<const uint4*>(p - off / static_cast<int>(sizeof(T)));
+    if (off == 0 && n >= 8) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = i < n ? p[i] : int8_zero<T>();
-    memcpy(&r, e, sizeof(r));
+      for (int i = 0; i < PIECES; ++i) r.v[i] = from[i];
+      return;
+    }
+    uint32_t w[PIECES * 4 + 5];
+#pragma unroll
+    for (int i = 0; i <= PIECES; ++i) {
+      const uint4 v = i * 16 < bytes ? from[i] : make_uint4(0u, 0u, 0u, 0u);
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+    w[PIECES * 4 + 4] = 0u;
+    int8_shift<PIECES * 4, PIECES * 4 + 5>(w, off);
+    if (n < 8) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (sizeof(T) == 2) {
+          if (e >= n) w[e / 2] &= e % 2 ? 0x0000ffffu : 0u;
+        } else {
+          if (e >= n) w[e] = 0u;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) r.v[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
   }
 }
 template <typename T> __device__ __forceinline__ void int8_floats(const Int8Raw<T>& r, float (&v)[8]) {
@@ -66,18 +109,55 @@ template <typename T> __device__ __forceinline__ void int8_floats(const Int8Raw<
     }
   }
 }
-template <typename T> __device__ __forceinline__ void int8_store8(T* p, int n, bool wide, const float (&v)[8]) {
-  if (wide && n >= 8) {
-    __align__(16) T r[8];
+// Eight floats as T, in words.
+template <typename T> __device__ __forceinline__ void int8_words(const float (&v)[8], uint32_t (&w)[sizeof(T) * 2]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = from_f32<T>(v[e]);
+  for (int e = 0; e < static_cast<int>(sizeof(T)) * 2; ++e) {
+    if constexpr (sizeof(T) == 2) {
+      const __nv_bfloat162 pair = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+      memcpy(&w[e], &pair, 4);
+    } else {
+      w[e] = __float_as_uint(v[e]);
+    }
+  }
+}
+// The chunk at column `at` of a row of k elements.  WHOLE: as in int8_load8.  Else every lane of the warp calls (those beyond the row
+// store nothing): where the row begins off a multiple of 16 bytes, a lane stores the aligned pieces that begin in the chunk before,
+// with that lane's last bytes in front; the pieces at the ends of the warp's stretch are stored element by element.
+template <typename T, bool WHOLE> __device__ __forceinline__ void int8_store8(T* row, int at, int k, const float (&v)[8]) {
+  constexpr int N = sizeof(T) * 2, SIZE = sizeof(T);
+  uint32_t w[N];
+  int8_words<T>(v, w);
+  if constexpr (WHOLE) {
 #pragma unroll
-    for (int e = 0; e < 8; e += 16 / static_cast<int>(sizeof(T)))
-      *reinterpret_cast<uint4*>(p + e) = *reinterpret_cast<const uint4*>(r + e);
+    for (int i = 0; i < N; i += 4) *reinterpret_cast<uint4*>(row + at + i * 4 / SIZE) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
   } else {
+    const int lane = threadIdx.x & 31, off = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15u), n = k - at;
+    if (off == 0) {                                             // (all lanes' rows are this one)
+      if (n >= 8) return int8_store8<T, true>(row, at, k, v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < n) p[e] = from_f32<T>(v[e]);
+      for (int e = 0; e < 8; ++e)
+        if (e < n) row[at + e] = from_f32<T>(v[e]);
+      return;
+    }
+    uint32_t c[N + 5];                                          // the chunk before this one's last 16 bytes, then this one
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = __shfl_up_sync(0xffffffffu, w[N - 4 + i], 1);
+#pragma unroll
+    for (int i = 0; i < N; ++i) c[4 + i] = w[i];
+    c[N + 4] = 0u;
+    int8_shift<N, N + 5>(c, 16 - off);                          // to the first aligned piece
+    T* aligned = row + at - off / SIZE;
+    const bool full = n >= 8, joins = full && lane > 0;               // its first piece lies in two chunks' elements
+    const bool joined = lane < 31 && n >= 16;                                       // ... and so does what is behind its last
+    if (joins) *reinterpret_cast<uint4*>(aligned) = make_uint4(c[0], c[1], c[2], c[3]);
+    if (full && N == 8) *reinterpret_cast<uint4*>(aligned + 16 / SIZE) = make_uint4(c[N - 4], c[N - 3], c[N - 2], c[N - 1]);
+    const int head = (16 - off) / SIZE, tail = 8 - off / SIZE;
+    if (!joins || !joined) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < n && ((!joins && (!full || e < head)) || (full && !joined && e >= tail))) row[at + e] = from_f32<T>(v[e]);
+    }
   }
 }
 
@@ -115,20 +195,20 @@ __device__ __forceinline__ float int8_top(float top, float v) {
   asm("max.NaN.f32 %0, %0, %1;\n" : "+f"(top) : "f"(fabsf(v)));
   return top;
 }
-// One chunk behind its loads: v = x, or behind a norm (x + residual) * gain, with what it adds to the row's sum of squares and
-// maximum; the sum is stored where sum_out is given (`n` of the elements exist).
-template <typename T, typename TG, bool NORM>
-__device__ __forceinline__ void int8_chunk(const Int8Raw<T>& x, const Int8Raw<T>& r, const Int8Raw<TG>& gain, bool add, T* sum_out, int n,
-                                           bool wide, float (&v)[8], float& ss, float& top) {
+// One chunk behind its loads: v = x, or behind a residual add x + residual ...
+template <typename T> __device__ __forceinline__ void int8_sum(const Int8Raw<T>& x, const Int8Raw<T>& r, bool add, float (&v)[8]) {
   int8_floats<T>(x, v);
+  if (add) {
+    float f[8];
+    int8_floats<T>(r, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = __fadd_rn(v[e], f[e]);
+  }
+}
+// ... and what it adds to the row's sum of squares and maximum; behind a norm v becomes v * gain.
+template <typename TG, bool NORM> __device__ __forceinline__ void int8_gain(const Int8Raw<TG>& gain, float (&v)[8], float& ss, float& top) {
   if (NORM) {
     float f[8];
-    if (add) {
-      int8_floats<T>(r, f);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = __fadd_rn(v[e], f[e]);
-      if (sum_out) int8_store8<T>(sum_out, n, wide, v);
-    }
     int8_floats<TG>(gain, f);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -155,19 +235,19 @@ template <bool NORM> __device__ __forceinline__ uint32_t int8_meet(float& ss, fl
   return __reduce_max_sync(0xffffffffu, lane < warps ? tops[turn][lane] : 0u);
 }
 
-// Rows whose chunks fit the block's registers, CH a thread.
-template <typename T, typename TG, bool NORM, int CH, int MOST = 512>
+// Rows whose chunks fit the block's registers, CH a thread.  WHOLE: there are whole chunks alone, all at multiples of 16 bytes.
+// (8,192 x 4,096 behind a norm with that question asked chunk by chunk 45 us, so 38: 6.2 TB/s, 95 % of the copy rate.)
+template <typename T, typename TG, bool NORM, int CH, bool WHOLE, int MOST = 512>
 __global__ void __launch_bounds__(MOST) int8_rows_kernel(const Int8RowsParams P) {
   __shared__ float sums[2][32];
   __shared__ uint32_t tops[2][32];
   pdl_launch_dependents();
   pdl_wait();
-  const int threads = blockDim.x, chunks = (P.k + 7) / 8;
-  const bool wide = P.wide != 0, add = NORM && P.residual != nullptr;
+  const int threads = blockDim.x;
+  const bool add = NORM && P.residual != nullptr;
   const TG* gain = static_cast<const TG*>(P.gain);
-  constexpr int AHEAD = 1;
-  Int8Raw<T> x[AHEAD][CH], r[AHEAD][CH];
-  auto load = [&](int row, Int8Raw<T> (&x)[CH], Int8Raw<T> (&r)[CH]) {
+  Int8Raw<T> x[CH], r[CH];
+  auto load = [&](int row) {
     if (row >= P.tokens) return;
     const T* xs = static_cast<const T*>(P.x) + static_cast<size_t>(row) * P.x_pitch;
     const T* rs = static_cast<const T*>(P.residual) + static_cast<size_t>(row) * P.k;
@@ -175,44 +255,41 @@ __global__ void __launch_bounds__(MOST) int8_rows_kernel(const Int8RowsParams P)
     for (int i = 0; i < CH; ++i) {
       const int at = (threadIdx.x + i * threads) * 8;
       if (at >= P.k) continue;
-      int8_load8<T>(xs + at, P.k - at, wide, x[i]);
-      if (add) int8_load8<T>(rs + at, P.k - at, wide, r[i]);
+      int8_load8<T, WHOLE>(xs + at, P.k - at, x[i]);
+      if (add) int8_load8<T, WHOLE>(rs + at, P.k - at, r[i]);
     }
   };
   int turn = 0;
-  auto take = [&](int row, Int8Raw<T> (&x)[CH], Int8Raw<T> (&r)[CH]) {
+  load(blockIdx.x);
+  for (int row = blockIdx.x; row < P.tokens; row += gridDim.x, turn ^= 1) {
     Int8Raw<TG> g[CH];
     if (NORM)
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int at = (threadIdx.x + i * threads) * 8;
-        if (at < P.k) int8_load8<TG>(gain + at, P.k - at, wide, g[i]);
+        if (at < P.k) int8_load8<TG, WHOLE>(gain + at, P.k - at, g[i]);
       }
     T* sum_out = add && P.sum_out ? static_cast<T*>(P.sum_out) + static_cast<size_t>(row) * P.k : nullptr;
-    float v[CH][8], ss = 0.0f;
-    float top = 0.0f;
+    float v[CH][8], ss = 0.0f, top = 0.0f;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int at = (threadIdx.x + i * threads) * 8;
-      if (at < P.k) int8_chunk<T, TG, NORM>(x[i], r[i], g[i], add, sum_out ? sum_out + at : nullptr, P.k - at, wide, v[i], ss, top);
+      const int at = (threadIdx.x + i * threads) * 8, warp_at = at - (threadIdx.x & 31) * 8;
+      if (WHOLE ? at >= P.k : warp_at >= P.k) continue;
+      if (WHOLE || at < P.k) int8_sum<T>(x[i], r[i], add, v[i]);
+      if (NORM && sum_out) int8_store8<T, WHOLE>(sum_out, at, P.k, v[i]);
+      if (WHOLE || at < P.k) int8_gain<TG, NORM>(g[i], v[i], ss, top);
     }
-    load(row + AHEAD * gridDim.x, x, r);
+    load(row + gridDim.x);
     const uint32_t bits = int8_meet<NORM>(ss, top, sums, tops, turn);
-    turn ^= 1;
     const Int8Step step = int8_step(bits, NORM ? rsqrtf(ss / static_cast<float>(P.k) + P.eps) : 1.0f);
     if (threadIdx.x == 0) P.s[row] = step.scale;
     int8_t* q = P.q + static_cast<size_t>(row) * P.q_pitch;
 #pragma unroll
-    for (int i = 0; i < CH; ++i)
-      if (threadIdx.x + i * threads < chunks)
-        *reinterpret_cast<uint2*>(q + (threadIdx.x + i * threads) * 8) = make_uint2(int8_pack4(v[i], step), int8_pack4(v[i] + 4, step));
-  };
-#pragma unroll
-  for (int a = 0; a < AHEAD; ++a) load(blockIdx.x + a * gridDim.x, x[a], r[a]);
-  for (int row = blockIdx.x; row < P.tokens; row += AHEAD * gridDim.x)
-#pragma unroll
-    for (int a = 0; a < AHEAD; ++a)
-      if (row + a * static_cast<int>(gridDim.x) < P.tokens) take(row + a * gridDim.x, x[a], r[a]);
+    for (int i = 0; i < CH; ++i) {
+      const int at = (threadIdx.x + i * threads) * 8;
+      if (at < P.k) *reinterpret_cast<uint2*>(q + at) = make_uint2(int8_pack4(v[i], step), int8_pack4(v[i] + 4, step));
+    }
+  }
 }
 
 // Many long bfloat16 rows without a norm: eight chunks a thread, kept AS THEY LIE IN MEMORY and taken apart once for the maximum and
@@ -233,7 +310,7 @@ __global__ void __launch_bounds__(256) int8_many_rows_kernel(const Int8RowsParam
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     const int at = (threadIdx.x + i * threads) * 8;
-    if (at < P.k) int8_load8<T>(xs + at, 8, true, x[i]);        // (whole chunks: the launch sees to it)
+    if (at < P.k) int8_load8<T, true>(xs + at, 8, x[i]);        // (whole chunks: the launch sees to it)
   }
   float v[8], ss = 0.0f, top = 0.0f;
 #pragma unroll
@@ -257,79 +334,88 @@ __global__ void __launch_bounds__(256) int8_many_rows_kernel(const Int8RowsParam
 }
 
 // Longer rows are read twice.
-template <typename T, typename TG, bool NORM>
+template <typename T, typename TG, bool NORM, bool WHOLE>
 __global__ void __launch_bounds__(512) int8_long_rows_kernel(const Int8RowsParams P) {
   __shared__ float sums[1][32];
   __shared__ uint32_t tops[1][32];
   pdl_launch_dependents();
   pdl_wait();
-  const int row = blockIdx.x, chunks = (P.k + 7) / 8;
-  const bool wide = P.wide != 0, add = NORM && P.residual != nullptr;
+  const int row = blockIdx.x, lane = threadIdx.x & 31;
+  const bool add = NORM && P.residual != nullptr;
   const T* xs = static_cast<const T*>(P.x) + static_cast<size_t>(row) * P.x_pitch;
   const T* rs = static_cast<const T*>(P.residual) + static_cast<size_t>(row) * P.k;
   const TG* gain = static_cast<const TG*>(P.gain);
   T* sum_out = add && P.sum_out ? static_cast<T*>(P.sum_out) + static_cast<size_t>(row) * P.k : nullptr;
-  float ss = 0.0f;
-  float top = 0.0f;
-  auto fetch = [&](int c, float (&v)[8], T* store) {
-    const int at = c * 8;
+  float ss = 0.0f, top = 0.0f;
+  auto fetch = [&](int at, float (&v)[8], bool store) {
     Int8Raw<T> x, r;
     Int8Raw<TG> g;
-    int8_load8<T>(xs + at, P.k - at, wide, x);
-    if (add) int8_load8<T>(rs + at, P.k - at, wide, r);
-    if (NORM) int8_load8<TG>(gain + at, P.k - at, wide, g);
-    int8_chunk<T, TG, NORM>(x, r, g, add, store ? store + at : nullptr, P.k - at, wide, v, ss, top);
+    const bool in = at < P.k;
+    if (in) {
+      int8_load8<T, WHOLE>(xs + at, P.k - at, x);
+      if (add) int8_load8<T, WHOLE>(rs + at, P.k - at, r);
+      if (NORM) int8_load8<TG, WHOLE>(gain + at, P.k - at, g);
+      int8_sum<T>(x, r, add, v);
+    }
+    if (NORM && store && (!WHOLE || in)) int8_store8<T, WHOLE>(sum_out, at, P.k, v);
+    if (in) int8_gain<TG, NORM>(g, v, ss, top);
   };
-  for (int c = threadIdx.x; c < chunks; c += blockDim.x) {
+  for (int at = threadIdx.x * 8; at - lane * 8 < P.k; at += blockDim.x * 8) {        // (whole warps)
     float v[8];
-    fetch(c, v, sum_out);
+    fetch(at, v, sum_out != nullptr);
   }
   const uint32_t bits = int8_meet<NORM>(ss, top, sums, tops, 0);
   const Int8Step step = int8_step(bits, NORM ? rsqrtf(ss / static_cast<float>(P.k) + P.eps) : 1.0f);
   if (threadIdx.x == 0) P.s[row] = step.scale;
   int8_t* q = P.q + static_cast<size_t>(row) * P.q_pitch;
-  for (int c = threadIdx.x; c < chunks; c += blockDim.x) {
+  for (int at = threadIdx.x * 8; at < P.k; at += blockDim.x * 8) {
     float v[8];
-    fetch(c, v, nullptr);
-    *reinterpret_cast<uint2*>(q + c * 8) = make_uint2(int8_pack4(v, step), int8_pack4(v + 4, step));
+    fetch(at, v, false);
+    *reinterpret_cast<uint2*>(q + at) = make_uint2(int8_pack4(v, step), int8_pack4(v + 4, step));
   }
 }
 
-template <typename T, typename TG, bool NORM, int CH, int MOST = 512>
-static int int8_rows_kept(const Int8RowsParams& P, int threads, int sms, cudaStream_t stream) {
+template <typename T, typename TG, bool NORM, int CH, bool WHOLE, int MOST = 512>
+static int int8_rows_blocks(const Int8RowsParams& P, int threads, int sms, cudaStream_t stream) {
   // Persistent: as many blocks as fit at once (threads, registers: found once for each size of block).
   static int fits[33];
   int& blocks = fits[threads / 32];
   if (blocks == 0) {
     int n = 0;
-    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, int8_rows_kernel<T, TG, NORM, CH, MOST>, threads, 0);
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, int8_rows_kernel<T, TG, NORM, CH, WHOLE, MOST>, threads, 0);
     if (e != cudaSuccess) return static_cast<int>(e);
     blocks = n < 1 ? 1 : n;
   }
   const int most = sms * blocks;
-  return b200_launch(int8_rows_kernel<T, TG, NORM, CH, MOST>, dim3(P.tokens < most ? P.tokens : most), dim3(threads), 0, stream, 0, P);
+  return b200_launch(int8_rows_kernel<T, TG, NORM, CH, WHOLE, MOST>, dim3(P.tokens < most ? P.tokens : most), dim3(threads), 0, stream, 0, P);
+}
+template <typename T, typename TG, bool NORM, int CH, int MOST = 512>
+static int int8_rows_kept(const Int8RowsParams& P, int threads, int sms, cudaStream_t stream) {
+  return P.whole ? int8_rows_blocks<T, TG, NORM, CH, true, MOST>(P, threads, sms, stream)
+                                : int8_rows_blocks<T, TG, NORM, CH, false, MOST>(P, threads, sms, stream);
 }
 template <typename T, typename TG, bool NORM>
 static int int8_rows_normed(const Int8RowsParams& P, int sms, cudaStream_t stream) {
   const int chunks = (P.k + 7) / 8;
   auto threads = [&](int ch) { return ((chunks + ch - 1) / ch + 31) / 32 * 32; };
   if constexpr (sizeof(T) == 2 && !NORM)
-    if (P.tokens > 8 * sms && P.wide && P.k % 8 == 0 && chunks >= 512 && chunks <= 2048)
+    if (P.tokens > 8 * sms && P.whole && chunks >= 512 && chunks <= 2048)
       return b200_launch(int8_many_rows_kernel<T>, dim3(P.tokens), dim3(threads(8)), 0, stream, 0, P);
   // Few rows: the row's latency is the time, so a thread takes as little as 512 of them allow.  Many: what counts are the bytes on
-  // their way; two chunks a thread keep them (8,192 x 4,096 behind a norm 45 us; four chunks, half the threads: 61), and rows longer
-  // than that are faster read twice, the second time out of the caches (8,192 x 12,288 behind a norm 130 us, 5.4 TB/s), but for float32
-  // without a norm, where 1,024 threads still keep theirs (2,048 x 12,288: 20 us, read twice 25).
+  // their way; two chunks a thread keep them (behind a norm 8,192 x 4,096 38 us; four chunks, half the threads: a third slower), in up
+  // to 1,024 threads (8,192 x 12,288 bfloat16 behind a norm 117 us, 6.0 TB/s; read twice, the second time out of the caches, 126),
+  // but for float32 behind a norm, which is faster read twice (226 us, 254 kept).
   if (P.tokens <= sms) {
     if (chunks <= 512) return int8_rows_kept<T, TG, NORM, 1>(P, threads(1), sms, stream);
     if (chunks <= 1024) return int8_rows_kept<T, TG, NORM, 2>(P, threads(2), sms, stream);
     if (chunks <= 512 * INT8_ROW_CHUNKS) return int8_rows_kept<T, TG, NORM, INT8_ROW_CHUNKS>(P, threads(INT8_ROW_CHUNKS), sms, stream);
   } else if (chunks <= 1024) {
     return int8_rows_kept<T, TG, NORM, 2>(P, threads(2), sms, stream);
-  } else if (!NORM && sizeof(T) == 4 && chunks <= 2048) {
-    return int8_rows_kept<T, TG, false, 2, 1024>(P, threads(2), sms, stream);
+  } else if constexpr (NORM == (sizeof(T) == 2)) {
+    if (chunks <= 2048) return int8_rows_kept<T, TG, NORM, 2, 1024>(P, threads(2), sms, stream);
   }
-  return b200_launch(int8_long_rows_kernel<T, TG, NORM>, dim3(P.tokens), dim3(512), 0, stream, 0, P);
+  return P.whole ? b200_launch(int8_long_rows_kernel<T, TG, NORM, true>, dim3(P.tokens), dim3(512), 0, stream, 0, P)
+                                : b200_launch(int8_long_rows_kernel<T, TG, NORM, false>, dim3(P.tokens), dim3(512), 0, stream, 0, P);
 }
 template <typename T>
 static int int8_rows_typed(const Int8RowsParams& P, int gain_code, int sms, cudaStream_t stream) {

@@ -51,10 +51,10 @@ __device__ __forceinline__ void tokens_to_8_bits(const Int8RowsParams& R, int8_t
   const int slots = R.tokens <= 1 ? 1 : R.tokens <= 2 ? 2 : R.tokens <= 4 ? 4 : 8, warps = WARPS / slots;
   const int token = warp / warps, threads = warps * 32, me = (warp % warps) * 32 + lane;
   const int chunks = x_pitch / 8;                                // (columns beyond k: zeros)
-  const bool wide = R.wide != 0, here = token < R.tokens;
+  const bool whole = R.whole != 0, here = token < R.tokens;
   float v[INT8_ROW_CHUNKS][8];
   float ss = 0.0f, most = 0.0f;
-  if (here) {
+  if (here) {                                                    // (whole warps)
     const T* x = static_cast<const T*>(R.x) + static_cast<size_t>(token) * R.x_pitch;
     const T* residual = NORM && R.residual ? static_cast<const T*>(R.residual) + static_cast<size_t>(token) * R.k : nullptr;
     T* sum_out = NORM && R.sum_out && blockIdx.x == 0 ? static_cast<T*>(R.sum_out) + static_cast<size_t>(token) * R.k : nullptr;
@@ -65,15 +65,26 @@ __device__ __forceinline__ void tokens_to_8_bits(const Int8RowsParams& R, int8_t
     for (int i = 0; i < INT8_ROW_CHUNKS; ++i) {
       const int at = (me + i * threads) * 8;
       if (at >= R.k) continue;
-      int8_load8<T>(x + at, R.k - at, wide, raw[i]);
-      if (NORM && residual) int8_load8<T>(residual + at, R.k - at, wide, add[i]);
-      if (NORM) int8_load8<TG>(gain + at, R.k - at, wide, g[i]);
+      if (whole) {
+        int8_load8<T, true>(x + at, 8, raw[i]);
+        if (NORM && residual) int8_load8<T, true>(residual + at, 8, add[i]);
+        if (NORM) int8_load8<TG, true>(gain + at, 8, g[i]);
+      } else {
+        int8_load8<T, false>(x + at, R.k - at, raw[i]);
+        if (NORM && residual) int8_load8<T, false>(residual + at, R.k - at, add[i]);
+        if (NORM) int8_load8<TG, false>(gain + at, R.k - at, g[i]);
+      }
     }
 #pragma unroll
     for (int i = 0; i < INT8_ROW_CHUNKS; ++i) {
       const int at = (me + i * threads) * 8;
-      if (at < R.k)
-        int8_chunk<T, TG, NORM>(raw[i], add[i], g[i], residual != nullptr, sum_out ? sum_out + at : nullptr, R.k - at, wide, v[i], ss, most);
+      if (at - lane * 8 >= R.k) continue;
+      if (at < R.k) int8_sum<T>(raw[i], add[i], residual != nullptr, v[i]);
+      if (NORM && sum_out) {
+        if (!whole) int8_store8<T, false>(sum_out, at, R.k, v[i]);
+        else if (at < R.k) int8_store8<T, true>(sum_out, at, R.k, v[i]);
+      }
+      if (at < R.k) int8_gain<TG, NORM>(g[i], v[i], ss, most);
     }
   }
   uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));

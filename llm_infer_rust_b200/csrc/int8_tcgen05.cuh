@@ -578,6 +578,7 @@ static void set_stages(Plan& p, int rows_a_cta, int fixed) {
 // clusters of four CTAs that run side by side.
 //   a block of k      what its bytes take at 126 GB/s an SM, 0.19 us at least (a pair's: or its MMAs' time)
 //   a tile's epilogue 0.0024 us a column, 0.4 us more where warps find pieces of less than 32 columns; it hides behind the next tile
+//   the weights       no less than at 8.4 TB/s (a part of them comes while the rows go to 8 bits)
 //   sharing k         1.4 us with two CTAs, 3.8 us with four (with the cluster's launch; the exchange itself is below 1 us)
 // Fitted to 140 products of 20 to 2,048 tokens that were run all ways (behind rows to 8 bits, cold weights): the way chosen takes 1.6 %
 // longer than the best one on average.  (Of it, 64 columns / 128 / 32 in two rounds, 64 tokens, 4,096 k, 6,144 columns: 9.5 / 11.9 /
@@ -588,12 +589,13 @@ static inline Plan make_plan(int tokens, int n, int k, int mode, int sms, int qu
   const int glu = mode == INT8_GLU ? 2 : 1, kb = (k + BK - 1) / BK;
   const long long cols = static_cast<long long>(n) * glu, m_tiles = (tokens + BM - 1) / BM;
   p.box = tokens >= BM ? BM : (tokens + 7) / 8 * 8;
+  const double memory = static_cast<double>(cols) * k / 8.4e6;
   double best = 0.0;
   auto consider = [&](int way, int bn, long long tiles, long long side_by_side, double block, int blocks, double more) {
     const long long rounds = (tiles + side_by_side - 1) / side_by_side;
     const double products = blocks * block, epilogue = 0.0024 * bn + (bn / glu % 32 ? 0.4 : 0.0);
-    const double cost = way > 1 ? rounds * (products + epilogue / 2 + more)
-                                : products + (rounds - 1) * (products > epilogue ? products : epilogue) + epilogue + more;
+    const double all = products * (way > 1 ? rounds : 1) + (way > 1 ? 0.0 : (rounds - 1) * (products > epilogue ? products : epilogue));
+    const double cost = (all > memory ? all : memory) + (way > 1 ? rounds * (epilogue / 2 + more) : epilogue + more);
     if (best == 0.0 || cost < best) { best = cost; p.way = way; p.bn = bn; }
   };
   for (int split = 1; split <= 4 && split <= kb; split *= 2)

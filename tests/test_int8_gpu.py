@@ -351,3 +351,46 @@ def test_weights_in_8_bits():
         assert torch.equal(m.int8_linear(x, again), m.int8_linear(x, held))
     laid = m.int8_weight_from(held.values, held.scales)
     assert laid.values.data_ptr() == held.values.data_ptr()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("tokens,k", [(2, 9), (3, 15), (5, 257), (400, 264), (64, 1999), (400, 2051), (1300, 1999), (7, 4095), (200, 4100), (1300, 4095),
+                                      (3, 8191), (160, 8201), (160, 12289), (1200, 12288), (2, 33333), (170, 16395)])
+def test_rows_that_begin_anywhere(tokens, k, dtype):
+    """Row lengths that are no multiple of eight, with and without a norm; sums are written to their rows and nowhere else."""
+    m, o = int8(), ops()
+    x, residual, gain = activations(tokens, k, dtype).contiguous(), rnd(tokens, k, dtype=dtype, seed=3), 1.0 + 0.3 * rnd(k, seed=4)
+    q, s = plain_rows(x.float())
+    rows = m.quantize_rows(x)
+    assert torch.equal(rows.values, q) and torch.equal(rows.scales, s)
+    v = x.float() + residual.float()
+    q, s = plain_rows(v * gain)
+    want = s.double() * (v.double().square().mean(dim=1) + 1e-5).rsqrt()
+    for lead in (16, 1):                                       # outputs at a multiple of 16 bytes and off it
+        whole = torch.full((tokens * k + 64,), 99.0, dtype=dtype, device=DEV)
+        kept = whole[lead:lead + tokens * k]
+        pitch = m.row_pitch(k)
+        values = torch.full((tokens * pitch + 32,), 77, dtype=torch.int8, device=DEV)
+        scales = torch.zeros(tokens, device=DEV)
+        rc = m._lib().b200_int8_rows(x, residual, gain, kept, values[16:], scales, tokens, k, k, pitch, o._code(x), 0, 1e-5, o._stream())
+        assert rc == 0
+        assert torch.equal(kept.view(tokens, k), v.to(dtype))
+        assert (whole[:lead] == 99).all() and (whole[lead + tokens * k:] == 99).all()
+        got = values[16:16 + tokens * pitch].view(tokens, pitch)[:, :k]
+        assert torch.equal(got, q) and (values[:16] == 77).all() and (values[16 + tokens * pitch:] == 77).all()
+        assert ((scales.double() - want).abs() <= 2.0 ** -18 * want).all()
+
+
+@pytest.mark.parametrize("tokens,k", [(1, 1999), (2, 1023), (4, 777), (7, 333), (8, 1001), (3, 5001)])
+def test_few_rows_that_begin_anywhere_behind_a_norm(tokens, k):
+    """The same inside the kernel for few tokens."""
+    m, o = int8(), ops()
+    for dtype in (BF16, F32):
+        x, residual, gain = activations(tokens, k, dtype).contiguous(), rnd(tokens, k, dtype=dtype, seed=3), 1.0 + 0.3 * rnd(k, seed=4)
+        w, pending = weight(70, k), o.PendingNorm(x, residual, gain, 1e-6)
+        y = m.int8_linear(pending, w, out_dtype=F32)
+        v = x.float() + residual.float()
+        q, s = plain_rows(v * gain)
+        rows = m.Int8Rows(q, s.double() * (v.double().square().mean(dim=1) + 1e-6).rsqrt())
+        check(y, *floats(rows, w), F32, rel=2.0 ** -18)
+        assert torch.equal(pending.residual_out, v.to(dtype))

@@ -109,3 +109,39 @@ def test_the_command_line_names_them():
     from llm_infer_rust_b200 import cli
     assert cli.parse_args(["--model-path", "m", "--int8-projections"]).int8_projections
     assert not cli.parse_args(["--model-path", "m"]).int8_projections and "--int8-projections" in cli.USAGE
+
+
+def plan(*sizes):
+    """(CTAs that share a tile's k, 0: pairs, columns of a tile) on 148 SMs that hold 36 clusters of four."""
+    import llm_infer_rust_b200.kernels.build as build
+    got = build.load_cuda_library("int8_linear.cu").b200_int8_plan(*sizes, 148, 36)
+    return got // 1000, got % 1000
+
+
+def test_how_products_are_cut_up():
+    """The ways that were fastest, or within a few hundredths of it, of all that were measured; (tokens, columns, k, gated)."""
+    assert plan(8192, 6144, 4096, 0) == plan(2048, 4096, 12288, 0) == (0, 256)          # many tiles: pairs of CTAs
+    assert plan(190, 12288, 4096, 1)[0] == plan(777, 2816, 1024, 1)[0] == 0
+    assert plan(1500, 8192, 5120, 0) == (0, 224)                                        # (three rounds of narrower tiles)
+    assert plan(100, 4096, 12288, 0) == (4, 128)                                        # long k, few columns: shared
+    assert plan(64, 4096, 4096, 0)[0] == 2 and plan(300, 4096, 4096, 0)[1] == 128
+    assert plan(45, 12288, 4096, 1)[0] == plan(64, 10240, 5120, 0)[0] == 1              # one round over the SMs
+
+
+def test_plans_are_ones_that_the_kernels_take():
+    import random
+    rng = random.Random(5)
+    for _ in range(400):
+        mode = rng.randint(0, 1)
+        tokens, n, k = (int(2 ** rng.uniform(0, b)) for b in (14, 15, 17))
+        way, bn = plan(tokens, n, min(k, 131071), mode)
+        assert way in (0, 1, 2, 4) and 32 <= bn <= 256
+        assert bn % 32 == 0 and tokens > 128 if way == 0 else bn % 16 == 0 and bn % (4 * way * (1 + mode)) == 0
+        assert way <= max(1, -(-k // 128))
+
+
+def test_which_tokens_need_no_kernel_in_front():
+    import llm_infer_rust_b200.kernels.build as build
+    alone = build.load_cuda_library("int8_linear.cu").b200_int8_alone
+    assert all(alone(t, k) for t, k in ((1, 1), (1, 16384), (2, 8192), (3, 4096), (4, 4096), (8, 2048)))
+    assert not any(alone(t, k) for t, k in ((1, 16392), (2, 8200), (5, 2056), (8, 2056), (9, 64), (0, 0), (1, 131072)))
