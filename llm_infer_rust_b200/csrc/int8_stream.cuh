@@ -183,6 +183,8 @@ __global__ void __launch_bounds__(THREADS, 1) stream_kernel(const Int8ProductPar
   }
   __syncthreads();
 
+  // The scales (and bias) of the result that this thread finishes first come while the unit's products run.
+  const int rows = glu ? 8 : 16, mine_first = wk * 32 + lane, mine_row = mine_first & (rows - 1);
   int slot = 0, turn = 0;
   for (int unit = first; unit < plan.units; unit += stride, turn ^= 1) {
     int acc[NT][4];
@@ -190,6 +192,16 @@ __global__ void __launch_bounds__(THREADS, 1) stream_kernel(const Int8ProductPar
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[j][e] = 0;
+    const int col = unit * rows + mine_row;
+    float c0 = 0.0f, c1 = 0.0f, b0 = 0.0f, b1 = 0.0f;
+    if (mine_first < P.tokens * rows && col < P.n) {
+      c0 = P.c[col];
+      if (glu) c1 = P.c[P.n + col];
+      if (P.bias) {
+        b0 = P.bias[col];
+        if (glu) b1 = P.bias[P.n + col];
+      }
+    }
     for (int i = 0; i < plan.steps; ++i) {
       const int at = (wk + i * plan.wk) * 64 + t * 16;
       uint4 x[NT];
@@ -213,18 +225,18 @@ __global__ void __launch_bounds__(THREADS, 1) stream_kernel(const Int8ProductPar
 #pragma unroll
       for (int e = 0; e < 4; ++e) mine[(j * 8 + t * 2 + (e & 1)) * 16 + g + (e >> 1) * 8] = acc[j][e];
     asm volatile("bar.sync %0, %1;\n" ::"r"(1 + wn), "r"(plan.wk * 32) : "memory");       // the group's warps
-    const int rows = glu ? 8 : 16;
-    for (int i = wk * 32 + lane; i < P.tokens * rows; i += plan.wk * 32) {
-      const int r = glu ? i & 7 : i & 15, token = glu ? i >> 3 : i >> 4, col = unit * rows + r;
+    // (a thread's further results are of other tokens, in the same column: their number is a multiple of the rows)
+    for (int i = mine_first; i < P.tokens * rows; i += plan.wk * 32) {
       if (col >= P.n) continue;
-      const int* from = red + (turn * WARPS + wn * plan.wk) * NT * 128 + token * 16 + r;
+      const int token = glu ? i >> 3 : i >> 4;
+      const int* from = red + (turn * WARPS + wn * plan.wk) * NT * 128 + token * 16 + mine_row;
       int sum = 0, up = 0;
       for (int w = 0; w < plan.wk; ++w) {
         sum += from[w * NT * 128];
         if (glu) up += from[w * NT * 128 + 8];
       }
-      float z = fmaf(static_cast<float>(sum), token_scale[token] * P.c[col], P.bias ? P.bias[col] : 0.0f);
-      if (glu) z = gate_up(z, fmaf(static_cast<float>(up), token_scale[token] * P.c[P.n + col], P.bias ? P.bias[P.n + col] : 0.0f), P.limit, P.alpha);
+      float z = fmaf(static_cast<float>(sum), token_scale[token] * c0, b0);
+      if (glu) z = gate_up(z, fmaf(static_cast<float>(up), token_scale[token] * c1, b1), P.limit, P.alpha);
       const size_t at = static_cast<size_t>(token) * P.n + col;
       if (out_f32) static_cast<float*>(P.out)[at] = z;
       else static_cast<__nv_bfloat16*>(P.out)[at] = __float2bfloat16_rn(z);
@@ -254,9 +266,11 @@ static inline Plan make_plan(int n, int k, int mode, int sms) {
   long long best = 0;
   for (int wn = 1; wn <= 4; wn *= 2) {
     const int wk = WARPS / wn, share = (steps + wk - 1) / wk;
-    // Rounds of the fullest group, each its steps and about four more for the sums' meeting.  (One token, WN = 1, 2, 4, us:
-    // 24,576 x 4,096 gated 27.7, 22.0, 20.1; 6,144 x 4,096 8.2, 7.5, 6.7; 4,096 x 12,288 11.6, 10.9, 11.4; 4,096 x 1,024 4.3, 3.2,
-    // 3.3; 151,936 x 4,096 108, 95, 95.)
+    // Rounds of the fullest group, each its steps and about four more for the sums' meeting and a late group's wait; from sixteen
+    // units an SM on rounds even out, and a unit that all warps share is the fastest.  (One token, WN = 1, 2, 4, us: 24,576 x 4,096
+    // gated 19.3, 18.9, 18.1; 6,144 x 4,096 7.2, 6.9, 6.3; 4,096 x 12,288 11.2, 10.7, 11.4; 4,096 x 1,024 3.7, 2.8, 2.8; 151,936 x 4,096
+    // 92.0, 94.1, 94.7.)
+    if (wn > 1 && p.units >= 16 * sms) break;
     const long long groups = static_cast<long long>(sms) * wn, cost = (p.units + groups - 1) / groups * (share + 4);
     if (best == 0 || cost < best) {
       best = cost;
