@@ -67,6 +67,7 @@ B200_EXPORT int b200_int8_linear(const void* x, const void* residual, const void
   if (tokens < 0 || n < 0 || k < 1 || k > MAX_K || q_pitch < k || w_pitch < k || (mode != INT8_PLAIN && mode != INT8_GLU)) return B200_BAD_SIZE;
   if (!int8_aligned(q, q_pitch) || !int8_aligned(w, w_pitch)) return B200_BAD_ALIGN;
   if (tokens == 0) return 0;
+  if (!x && (!q || !s)) return B200_BAD_SIZE;
   const int sms = sm_count();
   const bool few = n > 0 && i8st::takes(tokens, k);
   const Int8ProductParams P = {static_cast<const int8_t*>(q), s, static_cast<const int8_t*>(w), c, bias, out, tokens, n, k,

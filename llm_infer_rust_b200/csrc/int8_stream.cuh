@@ -8,14 +8,14 @@
 //             sum over k does not care about the order of k, so the 16 bytes serve two instructions as they come, and the
 //             tokens are read the same way.  (tcgen05 needs no faster rate here: 16 x 64 weights an SM every 44 cycles
 //             are all that memory gives, two of these instructions.)
-//   tokens    at most 8 a tile of the multiply, in shared memory for the whole kernel.  FUSED: they arrive as floats; 16 / T
-//             warps a token take them (behind the residual add and the norm) to 8 bits, in every CTA again: cheaper than
+//   tokens    at most 8 a tile of the multiply, in shared memory for the whole kernel.  FUSED: they arrive as floats; 16
+//             warps over the tokens (to a power of two) take each (behind the residual add and the norm) to 8 bits, in every CTA again: cheaper than
 //             a kernel in front while a thread holds its share in registers (16,384 floats in all).
 //   split     a CTA's 16 warps are WN groups of WK warps.  A group owns 16 weight rows at a time (INT8_GLU: 8 gate rows and the
 //             same 8 up rows), its warps share k (warp s takes the steps s, s + WK, ...) and their sums meet in shared memory
 //             (integers: any order); groups do not wait for one another, and the next rows' weights are on their way.
-// One CTA an SM; rows are dealt out over all groups of all CTAs.  Before the dependency wait the first weights start for the second-level cache; nothing is
-// read before it.
+// One CTA an SM; rows are dealt out over all groups of all CTAs.  Before the dependency wait the first weights start for the
+// second-level cache; nothing is read before it.
 #pragma once
 #include "int8_common.cuh"
 #include "int8_rows.cuh"

@@ -10,7 +10,7 @@
 //   warps 2-9   read their 32 lanes of tensor memory (two warps a quarter, every other 32 columns), multiply by the scales,
 //               round, turn 32 x 32 results through shared memory and store pieces of rows
 // Three ways to run it:
-//   PAIRS    CG = 2, 256 tokens x 256 columns on two CTAs (each holds its 128 tokens and half of the weight rows, the
+//   PAIRS    CG = 2, 256 tokens x up to 256 columns on two CTAs (each holds its 128 tokens and half of the weight rows, the
 //            first one's MMAs read both): half the bytes per product that a CTA of its own would have to fetch, for the many
 //            tiles of prompts.  Persistent: the epilogue of a tile runs under the MMAs of the next.
 //   SINGLE   CG = 1, 128 x BN, persistent; BN is chosen so that the SMs get equal shares of the weights.

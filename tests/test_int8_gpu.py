@@ -394,3 +394,19 @@ def test_few_rows_that_begin_anywhere_behind_a_norm(tokens, k):
         rows = m.Int8Rows(q, s.double() * (v.double().square().mean(dim=1) + 1e-6).rsqrt())
         check(y, *floats(rows, w), F32, rel=2.0 ** -18)
         assert torch.equal(pending.residual_out, v.to(dtype))
+
+
+def test_more_results_than_32_bits_count():
+    """16,500 tokens x 131,200 columns: results, and 40,000 rows of 60,000: inputs, beyond 2^31 elements."""
+    m = int8()
+    x, w = activations(16500, 32, BF16).contiguous(), weight(131200, 32)
+    y = m.int8_linear(x, w)
+    assert y.numel() > 2 ** 31
+    for a, b in ((0, 3), (8000, 8009), (16490, 16500)):
+        assert torch.equal(y[a:b], m.int8_linear(x[a:b], w))
+    del y, x
+    x = torch.zeros(40000, 60000, dtype=BF16, device=DEV)
+    x[39990:] = activations(10, 60000, BF16)
+    rows = m.quantize_rows(x)
+    q, s = plain_rows(x[39990:].float())
+    assert torch.equal(rows.values[39990:], q) and torch.equal(rows.scales[39990:], s) and not rows.scales[:39990].any()

@@ -145,3 +145,35 @@ def test_which_tokens_need_no_kernel_in_front():
     alone = build.load_cuda_library("int8_linear.cu").b200_int8_alone
     assert all(alone(t, k) for t, k in ((1, 1), (1, 16384), (2, 8192), (3, 4096), (4, 4096), (8, 2048)))
     assert not any(alone(t, k) for t, k in ((1, 16392), (2, 8200), (5, 2056), (8, 2056), (9, 64), (0, 0), (1, 131072)))
+
+
+def test_the_compiled_call_asks_for_its_arguments():
+    from llm_infer_rust_b200.kernels.build import load_call_binding, load_entry_points
+    lib, call = load_entry_points("int8_linear.cu"), load_call_binding().byte_product
+    x, w = torch.zeros(2, 32), weight()
+    good = [lib.b200_int8_linear, lib.b200_int8_alone, x, w.values, w.scales, None, None, None, None, None, 0, 0.0, 0.0, 1.0,
+            torch.zeros(1, dtype=torch.int32), 0]
+    assert call(*good) is None                               # (nothing is on a GPU: the wrapper says so)
+    for at, wrong in ((0, len), (1, None), (9, "float32"), (10, 0.5), (11, 1), (14, None), (15, None)):
+        with pytest.raises(TypeError):
+            call(*good[:at], wrong, *good[at + 1:])
+    with pytest.raises(TypeError):
+        call(*good[:-1])
+
+
+def test_entry_points_refuse_what_they_cannot_run():
+    from llm_infer_rust_b200.kernels.build import load_entry_points
+    lib = load_entry_points("int8_linear.cu")
+    x, q, s, w, c, out = torch.zeros(2, 32), torch.zeros(2, 32, dtype=torch.int8), torch.zeros(2), torch.zeros(4, 32, dtype=torch.int8), torch.ones(4), torch.zeros(2, 4)
+
+    def call(tokens=2, n=4, k=32, x_pitch=32, q_pitch=32, w_pitch=32, x_code=0, gain_code=0, out_code=0, mode=0, x=x, q=q, w=w, gain=None):
+        return lib.b200_int8_linear(x, None, gain, None, q, s, w, c, None, out, tokens, n, k, x_pitch, q_pitch, w_pitch, x_code, gain_code, out_code,
+                                    mode, 0.0, 0.0, 1.0, None, 0)
+    assert call(tokens=0) == 0
+    assert call(x_code=2, tokens=20) == -1 and call(out_code=7) == -1 and call(gain=c, gain_code=3, tokens=20) == -1
+    assert call(k=0) == call(k=131072) == call(tokens=-1) == call(n=-1) == call(mode=2) == call(w_pitch=16) == call(q_pitch=16) == -2
+    assert call(x=None, q=None) == -2
+    assert call(w=w.view(-1)[1:]) == -3 and call(q_pitch=40) == -3 and call(w_pitch=40) == -3
+    assert lib.b200_int8_rows(x, None, None, None, q, s, 0, 32, 32, 32, 0, 0, 0.0, 0) == 0
+    assert lib.b200_int8_rows(x, None, None, None, q, s, 2, 32, 31, 32, 0, 0, 0.0, 0) == -2
+    assert lib.b200_int8_rows(x, None, None, None, q, s, 2, 32, 32, 33, 0, 0, 0.0, 0) == -3
