@@ -33,9 +33,6 @@ struct Int8RowsParams {
 
 // Eight consecutive elements as they lie in memory.
 template <typename T> struct Int8Raw { uint4 v[sizeof(T) / 2]; };
-template <typename T> __device__ __forceinline__ T int8_zero();
-template <> __device__ __forceinline__ float int8_zero<float>() { return 0.0f; }
-template <> __device__ __forceinline__ __nv_bfloat16 int8_zero<__nv_bfloat16>() { return __float2bfloat16_rn(0.0f); }
 
 // The words w[0 .. N) of what begins `bytes` (an even number below 20) behind w's start.  (Branches on a number that all threads
 // share: word by word selections cost three times the instructions.)
@@ -56,8 +53,9 @@ template <int N, int M> __device__ __forceinline__ void int8_shift(uint32_t (&w)
 
 // Eight elements in a row from `p` on, of which `n` exist (the others read as 0).  WHOLE: all of them do, at a multiple of 16 bytes.
 // Else the aligned 16-byte pieces that hold them are fetched and shifted into place: rows whose length is no multiple of eight begin
-// anywhere, and element by element they took three times as long.  (No piece without an element of the row is touched.)
-template <typename T, bool WHOLE> __device__ __forceinline__ void int8_load8(const T* p, int n, Int8Raw<T>& r) {
+// anywhere, and element by element they took three times as long.  (No piece without an element of the row is touched: of the eight
+// the first `lead` do not exist either; what they read as is the caller's affair.)
+template <typename T, bool WHOLE> __device__ __forceinline__ void int8_load8(const T* p, int n, Int8Raw<T>& r, int lead = 0) {
   constexpr int PIECES = sizeof(T) / 2;
   if constexpr (WHOLE) {
 #pragma unroll
@@ -65,7 +63,7 @@ template <typename T, bool WHOLE> __device__ __forceinline__ void int8_load8(con
   } else {
     const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15u), bytes = off + min(n, 8) * static_cast<int>(sizeof(T));
     const uint4* from = reinterpret_cast<const uint4*>(p - off / static_cast<int>(sizeof(T)));
-    if (off == 0 && n >= 8) {
+    if (off == 0 && n >= 8 && lead == 0) {
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) r.v[i] = from[i];
       return;
@@ -73,7 +71,8 @@ template <typename T, bool WHOLE> __device__ __forceinline__ void int8_load8(con
     uint32_t w[PIECES * 4 + 5];
 #pragma unroll
     for (int i = 0; i <= PIECES; ++i) {
-      const uint4 v = i * 16 < bytes ? from[i] : make_uint4(0u, 0u, 0u, 0u);
+      const bool any = i * 16 < bytes && i * 16 + 16 > off + lead * static_cast<int>(sizeof(T));
+      const uint4 v = any ? from[i] : make_uint4(0u, 0u, 0u, 0u);
       w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
     }
     w[PIECES * 4 + 4] = 0u;
@@ -161,6 +160,96 @@ template <typename T, bool WHOLE> __device__ __forceinline__ void int8_store8(T*
   }
 }
 
+// Rows that are not whole, AS THEY LIE: a thread's eight elements begin at a multiple of 16 bytes, so at columns c, c + 8, ... with
+// -16 bytes < c <= 0, and nothing is shifted on its way in or out but the gain (which lies otherwise to every row) and the 8-bit
+// results, that begin at a multiple of 16 bytes in every row.  With x, the residual and the sum shifted to columns 0, 8, ... the
+// instructions bound the kernel: 8,192 x 1,999 bfloat16 behind a norm 46.5 -> 28.0 us (3.8 TB/s; whole rows of 2,000 20), float32
+// 69 -> 44, 4,042 x 4,407 55 -> 35, without a norm 17.5 -> 15.5.
+
+// How many elements lie between the multiple of 16 bytes at or before p and p.
+template <typename T, bool WHOLE> __device__ __forceinline__ int int8_lead(const T* p) {
+  return WHOLE ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15u) / static_cast<int>(sizeof(T));
+}
+// Columns c .. c + 8 of a row of k elements (those that are none are read as anything; int8_trim).  LIES: row + c is a multiple of 16
+// bytes.
+template <typename T, bool WHOLE, bool LIES = true> __device__ __forceinline__ void int8_fetch(const T* row, int c, int k, Int8Raw<T>& r) {
+  constexpr int PIECES = sizeof(T) / 2, PER = 16 / sizeof(T);
+  if constexpr (WHOLE) {
+    int8_load8<T, true>(row + c, 8, r);
+  } else {
+    if (LIES || c >= k) {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) r.v[i] = c + i * PER < k ? reinterpret_cast<const uint4*>(row + c)[i] : make_uint4(0u, 0u, 0u, 0u);
+    } else {
+      int8_load8<T, false>(row + c, k - c, r, max(-c, 0));
+    }
+  }
+}
+// What lies beside the row becomes 0.
+template <bool WHOLE> __device__ __forceinline__ void int8_trim(float (&v)[8], int c, int k) {
+  if (!WHOLE && (c < 0 || c + 8 > k)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (static_cast<unsigned>(c + e) >= static_cast<unsigned>(k)) v[e] = 0.0f;
+  }
+}
+// Columns c .. c + 8 as they go out, rounded to T.
+template <typename T, bool WHOLE> __device__ __forceinline__ void int8_put_sum(T* row, int c, int k, const float (&v)[8]) {
+  constexpr int PIECES = sizeof(T) / 2, PER = 16 / sizeof(T);
+  if constexpr (WHOLE) {
+    int8_store8<T, true>(row, c, k, v);
+  } else {
+    const bool lies = (reinterpret_cast<uintptr_t>(row + c) & 15u) == 0;
+    uint32_t w[sizeof(T) * 2];
+    int8_words<T>(v, w);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int at = c + i * PER;
+      if (lies && at >= 0 && at + PER <= k) {
+        reinterpret_cast<uint4*>(row + c)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+          if (at + e >= 0 && at + e < k) row[at + e] = from_f32<T>(v[i * PER + e]);
+      }
+    }
+  }
+}
+// A thread's column in its i-th chunk of CH: not WHOLE, a warp's chunks follow one another.
+template <bool WHOLE, int CH> __device__ __forceinline__ int int8_column(int i, int lead) {
+  return WHOLE ? static_cast<int>(threadIdx.x + i * blockDim.x) * 8
+               : static_cast<int>((threadIdx.x & ~31u) * CH + i * 32 + (threadIdx.x & 31)) * 8 - lead;
+}
+// Whether a thread (not WHOLE: the whole warp) has nothing at its column c.
+template <bool WHOLE> __device__ __forceinline__ bool int8_beyond(int c, int k) {
+  return WHOLE ? c >= k : c - static_cast<int>(threadIdx.x & 31) * 8 >= k;
+}
+// The 8-bit results of a warp's chunks, the first at column c.  Not WHOLE: every lane calls; c + lead is a multiple of eight, a lane
+// stores eight results from there on, the last of them the next lane's first, and where two warps meet they go byte by byte.  ALONE:
+// the warp has the whole row.
+template <int CH, bool ALONE>
+__device__ __forceinline__ void int8_put(int8_t* row, int c, int lead, int k, const uint32_t (&low)[CH], const uint32_t (&high)[CH]) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t bits = (lead & 3) * 8;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int at = c + lead + i * 256;
+    const uint32_t low2 = __shfl_sync(0xffffffffu, i + 1 < CH && lane == 0 ? low[i + 1 < CH ? i + 1 : i] : low[i], lane + 1);
+    const uint32_t high2 = __shfl_sync(0xffffffffu, i + 1 < CH && lane == 0 ? high[i + 1 < CH ? i + 1 : i] : high[i], lane + 1);
+    const uint32_t w0 = lead < 4 ? low[i] : high[i], w1 = lead < 4 ? high[i] : low2, w2 = lead < 4 ? low2 : high2;
+    if (at < k && (ALONE || i + 1 < CH || lane < 31 || lead == 0))
+      *reinterpret_cast<uint2*>(row + at) = make_uint2(__funnelshift_r(w0, w1, bits), __funnelshift_r(w1, w2, bits));
+  }
+  if (!ALONE && lead > 0) {
+    const bool head = lane < lead;
+    const uint32_t l0 = __shfl_sync(0xffffffffu, low[0], 0), h0 = __shfl_sync(0xffffffffu, high[0], 0);
+    const uint32_t l1 = __shfl_sync(0xffffffffu, low[CH - 1], 31), h1 = __shfl_sync(0xffffffffu, high[CH - 1], 31);
+    const int at = c - lane * 8 + (head ? 0 : CH * 256 - 8) + lane;
+    const uint32_t word = lane < 4 ? (head ? l0 : l1) : (head ? h0 : h1);
+    if (lane < 8 && at >= 0 && at < k) row[at] = static_cast<int8_t>(word >> (lane & 3) * 8);
+  }
+}
+
 // What a row's maximum (as bits of a float that is not negative) makes of its elements: q = rint(v * pre * inv).
 struct Int8Step {
   float pre, inv, scale;
@@ -206,7 +295,8 @@ template <typename T> __device__ __forceinline__ void int8_sum(const Int8Raw<T>&
   }
 }
 // ... and what it adds to the row's sum of squares and maximum; behind a norm v becomes v * gain.
-template <typename TG, bool NORM> __device__ __forceinline__ void int8_gain(const Int8Raw<TG>& gain, float (&v)[8], float& ss, float& top) {
+template <typename TG, bool NORM, bool WHOLE>
+__device__ __forceinline__ void int8_gain(const Int8Raw<TG>& gain, float (&v)[8], int c, int k, float& ss, float& top) {
   if (NORM) {
     float f[8];
     int8_floats<TG>(gain, f);
@@ -215,6 +305,7 @@ template <typename TG, bool NORM> __device__ __forceinline__ void int8_gain(cons
       ss = fmaf(v[e], v[e], ss);
       v[e] = __fmul_rn(v[e], f[e]);
     }
+    int8_trim<WHOLE>(v, c, k);                                  // (what is read beside the gain may be no number)
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) top = int8_top(top, v[e]);
@@ -222,10 +313,12 @@ template <typename TG, bool NORM> __device__ __forceinline__ void int8_gain(cons
 
 // The block's sums of squares and maximum (`turn`: which half of the scratch is free).
 // Returns the maximum's bits: as integers floats that are not negative compare as they do, and NaN is above infinity.
-template <bool NORM> __device__ __forceinline__ uint32_t int8_meet(float& ss, float top, float (*sums)[32], uint32_t (*tops)[32], int turn) {
+template <bool NORM, bool ALONE = false>
+__device__ __forceinline__ uint32_t int8_meet(float& ss, float top, float (*sums)[32], uint32_t (*tops)[32], int turn) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
   if (NORM) ss = warp_sum(ss);
+  if constexpr (ALONE) return bits;
   if (lane == 0) { tops[turn][warp] = bits; sums[turn][warp] = ss; }
   __syncthreads();
   if (NORM) {
@@ -235,15 +328,16 @@ template <bool NORM> __device__ __forceinline__ uint32_t int8_meet(float& ss, fl
   return __reduce_max_sync(0xffffffffu, lane < warps ? tops[turn][lane] : 0u);
 }
 
-// Rows whose chunks fit the block's registers, CH a thread.  WHOLE: there are whole chunks alone, all at multiples of 16 bytes.
+// Rows whose chunks fit the block's registers, CH a thread (ALONE: a warp's, of which there are blockDim.y).  WHOLE: there are whole chunks alone, all at multiples of 16 bytes.
 // (8,192 x 4,096 behind a norm with that question asked chunk by chunk 45 us, so 38: 6.2 TB/s, 95 % of the copy rate.)
-template <typename T, typename TG, bool NORM, int CH, bool WHOLE, int MOST = 512>
+template <typename T, typename TG, bool NORM, int CH, bool WHOLE, int MOST = 512, bool ALONE = false>
 __global__ void __launch_bounds__(MOST) int8_rows_kernel(const Int8RowsParams P) {
   __shared__ float sums[2][32];
   __shared__ uint32_t tops[2][32];
   pdl_launch_dependents();
   pdl_wait();
-  const int threads = blockDim.x;
+  const int first = ALONE ? blockIdx.x * blockDim.y + threadIdx.y : blockIdx.x;
+  const int step_rows = ALONE ? gridDim.x * blockDim.y : gridDim.x;
   const bool add = NORM && P.residual != nullptr;
   const TG* gain = static_cast<const TG*>(P.gain);
   Int8Raw<T> x[CH], r[CH];
@@ -251,44 +345,57 @@ __global__ void __launch_bounds__(MOST) int8_rows_kernel(const Int8RowsParams P)
     if (row >= P.tokens) return;
     const T* xs = static_cast<const T*>(P.x) + static_cast<size_t>(row) * P.x_pitch;
     const T* rs = static_cast<const T*>(P.residual) + static_cast<size_t>(row) * P.k;
+    const int lead = int8_lead<T, WHOLE>(xs);
+    const bool alike = lead == int8_lead<T, WHOLE>(rs);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int at = (threadIdx.x + i * threads) * 8;
-      if (at >= P.k) continue;
-      int8_load8<T, WHOLE>(xs + at, P.k - at, x[i]);
-      if (add) int8_load8<T, WHOLE>(rs + at, P.k - at, r[i]);
+      const int c = int8_column<WHOLE, CH>(i, lead);
+      if (int8_beyond<WHOLE>(c, P.k)) continue;
+      int8_fetch<T, WHOLE>(xs, c, P.k, x[i]);
+      if (add && alike) int8_fetch<T, WHOLE>(rs, c, P.k, r[i]);
+      else if (add) int8_fetch<T, WHOLE, false>(rs, c, P.k, r[i]);
     }
   };
-  int turn = 0;
-  load(blockIdx.x);
-  for (int row = blockIdx.x; row < P.tokens; row += gridDim.x, turn ^= 1) {
-    Int8Raw<TG> g[CH];
-    if (NORM)
+  Int8Raw<TG> g[CH];
+  int turn = 0, held = -1;                    // (rows that lie alike need the gain once: the launch sees to it that a block's rows do)
+  load(first);
+  for (int row = first; row < P.tokens; row += step_rows, turn ^= 1) {
+    const int lead = int8_lead<T, WHOLE>(static_cast<const T*>(P.x) + static_cast<size_t>(row) * P.x_pitch);
+    if (NORM && (WHOLE || lead != held)) {
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
-        const int at = (threadIdx.x + i * threads) * 8;
-        if (at < P.k) int8_load8<TG, WHOLE>(gain + at, P.k - at, g[i]);
+        const int c = int8_column<WHOLE, CH>(i, lead);
+        if (!int8_beyond<WHOLE>(c, P.k)) int8_fetch<TG, WHOLE, false>(gain, c, P.k, g[i]);
       }
+      held = lead;
+    }
     T* sum_out = add && P.sum_out ? static_cast<T*>(P.sum_out) + static_cast<size_t>(row) * P.k : nullptr;
     float v[CH][8], ss = 0.0f, top = 0.0f;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int at = (threadIdx.x + i * threads) * 8, warp_at = at - (threadIdx.x & 31) * 8;
-      if (WHOLE ? at >= P.k : warp_at >= P.k) continue;
-      if (WHOLE || at < P.k) int8_sum<T>(x[i], r[i], add, v[i]);
-      if (NORM && sum_out) int8_store8<T, WHOLE>(sum_out, at, P.k, v[i]);
-      if (WHOLE || at < P.k) int8_gain<TG, NORM>(g[i], v[i], ss, top);
+      const int c = int8_column<WHOLE, CH>(i, lead);
+      if (int8_beyond<WHOLE>(c, P.k)) continue;
+      int8_sum<T>(x[i], r[i], add, v[i]);
+      int8_trim<WHOLE>(v[i], c, P.k);
+      if (NORM && sum_out) int8_put_sum<T, WHOLE>(sum_out, c, P.k, v[i]);
+      int8_gain<TG, NORM, WHOLE>(g[i], v[i], c, P.k, ss, top);
     }
-    load(row + gridDim.x);
-    const uint32_t bits = int8_meet<NORM>(ss, top, sums, tops, turn);
+    load(row + step_rows);
+    const uint32_t bits = int8_meet<NORM, ALONE>(ss, top, sums, tops, turn);
     const Int8Step step = int8_step(bits, NORM ? rsqrtf(ss / static_cast<float>(P.k) + P.eps) : 1.0f);
     if (threadIdx.x == 0) P.s[row] = step.scale;
     int8_t* q = P.q + static_cast<size_t>(row) * P.q_pitch;
+    uint32_t low[CH], high[CH];
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int at = (threadIdx.x + i * threads) * 8;
-      if (at < P.k) *reinterpret_cast<uint2*>(q + at) = make_uint2(int8_pack4(v[i], step), int8_pack4(v[i] + 4, step));
+      const int c = int8_column<WHOLE, CH>(i, lead);
+      low[i] = high[i] = 0u;
+      if (int8_beyond<WHOLE>(c, P.k)) continue;
+      low[i] = int8_pack4(v[i], step);
+      high[i] = int8_pack4(v[i] + 4, step);
+      if (WHOLE) *reinterpret_cast<uint2*>(q + c) = make_uint2(low[i], high[i]);
     }
+    if (!WHOLE) int8_put<CH, ALONE>(q, int8_column<WHOLE, CH>(0, lead), lead, P.k, low, high);
   }
 }
 
@@ -304,18 +411,18 @@ __global__ void __launch_bounds__(256) int8_many_rows_kernel(const Int8RowsParam
   __shared__ uint32_t tops[1][32];
   pdl_launch_dependents();
   pdl_wait();
-  const int row = blockIdx.x, threads = blockDim.x;
+  const int row = blockIdx.x;
   const T* xs = static_cast<const T*>(P.x) + static_cast<size_t>(row) * P.x_pitch;
   Int8Raw<T> x[CH];
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
-    const int at = (threadIdx.x + i * threads) * 8;
-    if (at < P.k) int8_load8<T, true>(xs + at, 8, x[i]);        // (whole chunks: the launch sees to it)
+    const int c = int8_column<true, CH>(i, 0);
+    if (!int8_beyond<true>(c, P.k)) int8_fetch<T, true>(xs, c, P.k, x[i]);
   }
   float v[8], ss = 0.0f, top = 0.0f;
 #pragma unroll
   for (int i = 0; i < CH; ++i)
-    if ((threadIdx.x + i * threads) * 8 < P.k) {
+    if (!int8_beyond<true>(int8_column<true, CH>(i, 0), P.k)) {
       int8_floats<T>(x[i], v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = int8_top(top, v[e]);
@@ -325,11 +432,10 @@ __global__ void __launch_bounds__(256) int8_many_rows_kernel(const Int8RowsParam
   int8_t* q = P.q + static_cast<size_t>(row) * P.q_pitch;
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
-    const int at = (threadIdx.x + i * threads) * 8;
-    if (at < P.k) {
-      int8_floats<T>(x[i], v);
-      *reinterpret_cast<uint2*>(q + at) = make_uint2(int8_pack4(v, step), int8_pack4(v + 4, step));
-    }
+    const int c = int8_column<true, CH>(i, 0);
+    if (int8_beyond<true>(c, P.k)) continue;
+    int8_floats<T>(x[i], v);
+    *reinterpret_cast<uint2*>(q + c) = make_uint2(int8_pack4(v, step), int8_pack4(v + 4, step));
   }
 }
 
@@ -340,41 +446,57 @@ __global__ void __launch_bounds__(512) int8_long_rows_kernel(const Int8RowsParam
   __shared__ uint32_t tops[1][32];
   pdl_launch_dependents();
   pdl_wait();
-  const int row = blockIdx.x, lane = threadIdx.x & 31;
+  const int row = blockIdx.x;
   const bool add = NORM && P.residual != nullptr;
   const T* xs = static_cast<const T*>(P.x) + static_cast<size_t>(row) * P.x_pitch;
   const T* rs = static_cast<const T*>(P.residual) + static_cast<size_t>(row) * P.k;
   const TG* gain = static_cast<const TG*>(P.gain);
   T* sum_out = add && P.sum_out ? static_cast<T*>(P.sum_out) + static_cast<size_t>(row) * P.k : nullptr;
   float ss = 0.0f, top = 0.0f;
-  auto fetch = [&](int at, float (&v)[8], bool store) {
+  const int lead = int8_lead<T, WHOLE>(xs);
+  const bool alike = lead == int8_lead<T, WHOLE>(rs);
+  auto fetch = [&](int c, float (&v)[8], bool store) {
     Int8Raw<T> x, r;
     Int8Raw<TG> g;
-    const bool in = at < P.k;
-    if (in) {
-      int8_load8<T, WHOLE>(xs + at, P.k - at, x);
-      if (add) int8_load8<T, WHOLE>(rs + at, P.k - at, r);
-      if (NORM) int8_load8<TG, WHOLE>(gain + at, P.k - at, g);
-      int8_sum<T>(x, r, add, v);
-    }
-    if (NORM && store && (!WHOLE || in)) int8_store8<T, WHOLE>(sum_out, at, P.k, v);
-    if (in) int8_gain<TG, NORM>(g, v, ss, top);
+    int8_fetch<T, WHOLE>(xs, c, P.k, x);
+    if (add && alike) int8_fetch<T, WHOLE>(rs, c, P.k, r);
+    else if (add) int8_fetch<T, WHOLE, false>(rs, c, P.k, r);
+    if (NORM) int8_fetch<TG, WHOLE, false>(gain, c, P.k, g);
+    int8_sum<T>(x, r, add, v);
+    int8_trim<WHOLE>(v, c, P.k);
+    if (NORM && store) int8_put_sum<T, WHOLE>(sum_out, c, P.k, v);
+    int8_gain<TG, NORM, WHOLE>(g, v, c, P.k, ss, top);
   };
-  for (int at = threadIdx.x * 8; at - lane * 8 < P.k; at += blockDim.x * 8) {        // (whole warps)
+  for (int c = threadIdx.x * 8 - lead; !int8_beyond<WHOLE>(c, P.k); c += blockDim.x * 8) {
     float v[8];
-    fetch(at, v, sum_out != nullptr);
+    fetch(c, v, sum_out != nullptr);
   }
   const uint32_t bits = int8_meet<NORM>(ss, top, sums, tops, 0);
   const Int8Step step = int8_step(bits, NORM ? rsqrtf(ss / static_cast<float>(P.k) + P.eps) : 1.0f);
   if (threadIdx.x == 0) P.s[row] = step.scale;
   int8_t* q = P.q + static_cast<size_t>(row) * P.q_pitch;
-  for (int at = threadIdx.x * 8; at < P.k; at += blockDim.x * 8) {
+  for (int c = threadIdx.x * 8 - lead; !int8_beyond<WHOLE>(c, P.k); c += blockDim.x * 8) {
     float v[8];
-    fetch(at, v, false);
-    *reinterpret_cast<uint2*>(q + at) = make_uint2(int8_pack4(v, step), int8_pack4(v + 4, step));
+    fetch(c, v, false);
+    const uint32_t low[1] = {int8_pack4(v, step)}, high[1] = {int8_pack4(v + 4, step)};
+    if (WHOLE) *reinterpret_cast<uint2*>(q + c) = make_uint2(low[0], high[0]);
+    else int8_put<1, false>(q, c, lead, P.k, low, high);
   }
 }
 
+template <typename T, typename TG, bool NORM, int CH, bool WHOLE>
+static int int8_rows_warps(const Int8RowsParams& P, int sms, cudaStream_t stream) {
+  static int blocks;
+  const auto kernel = int8_rows_kernel<T, TG, NORM, CH, WHOLE, 256, true>;
+  if (blocks == 0) {
+    int n = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, 256, 0);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    blocks = n < 1 ? 1 : n;
+  }
+  const int want = (P.tokens + 7) / 8, most = sms * blocks;
+  return b200_launch(kernel, dim3(want < most ? want : most), dim3(32, 8), 0, stream, 0, P);
+}
 template <typename T, typename TG, bool NORM, int CH, bool WHOLE, int MOST = 512>
 static int int8_rows_blocks(const Int8RowsParams& P, int threads, int sms, cudaStream_t stream) {
   // Persistent: as many blocks as fit at once (threads, registers: found once for each size of block).
@@ -386,7 +508,7 @@ static int int8_rows_blocks(const Int8RowsParams& P, int threads, int sms, cudaS
     if (e != cudaSuccess) return static_cast<int>(e);
     blocks = n < 1 ? 1 : n;
   }
-  const int most = sms * blocks;
+  const int most = WHOLE ? sms * blocks : sms * blocks & ~7;                    // (rows eight apart lie alike)
   return b200_launch(int8_rows_kernel<T, TG, NORM, CH, WHOLE, MOST>, dim3(P.tokens < most ? P.tokens : most), dim3(threads), 0, stream, 0, P);
 }
 template <typename T, typename TG, bool NORM, int CH, int MOST = 512>
@@ -396,7 +518,7 @@ static int int8_rows_kept(const Int8RowsParams& P, int threads, int sms, cudaStr
 }
 template <typename T, typename TG, bool NORM>
 static int int8_rows_normed(const Int8RowsParams& P, int sms, cudaStream_t stream) {
-  const int chunks = (P.k + 7) / 8;
+  const int chunks = (P.k + (P.whole ? 0 : 16 / static_cast<int>(sizeof(T)) - 1) + 7) / 8;
   auto threads = [&](int ch) { return ((chunks + ch - 1) / ch + 31) / 32 * 32; };
   if constexpr (sizeof(T) == 2 && !NORM)
     if (P.tokens > 8 * sms && P.whole && chunks >= 512 && chunks <= 2048)
@@ -409,6 +531,14 @@ static int int8_rows_normed(const Int8RowsParams& P, int sms, cudaStream_t strea
     if (chunks <= 512) return int8_rows_kept<T, TG, NORM, 1>(P, threads(1), sms, stream);
     if (chunks <= 1024) return int8_rows_kept<T, TG, NORM, 2>(P, threads(2), sms, stream);
     if (chunks <= 512 * INT8_ROW_CHUNKS) return int8_rows_kept<T, TG, NORM, INT8_ROW_CHUNKS>(P, threads(INT8_ROW_CHUNKS), sms, stream);
+  } else if (chunks <= 64) {
+    // Short rows take a warp each: two warps that meet over a row cost more than the row (8,192 x 512 bfloat16 5.4 -> 3.8 us, behind a
+    // norm 8.5 -> 6.3, 8,192 x 64 5.3 -> 2.5).  Up to 128 chunks that holds for bfloat16 (8,192 x 1,024 6.2 -> 5.7, behind a norm
+    // 11.1 -> 10.3) where there are many rows (200 x 1,024 behind a norm 2.2 -> 2.5) that are whole, of the others up to 96.
+    return P.whole ? int8_rows_warps<T, TG, NORM, 2, true>(P, sms, stream) : int8_rows_warps<T, TG, NORM, 2, false>(P, sms, stream);
+  } else if (P.tokens > 4 * sms && chunks <= (P.whole ? sizeof(T) == 2 ? 128 : 0 : 96)) {
+    if (!P.whole) return int8_rows_warps<T, TG, NORM, 3, false>(P, sms, stream);
+    if constexpr (sizeof(T) == 2) return int8_rows_warps<T, TG, NORM, 4, true>(P, sms, stream);
   } else if (chunks <= 1024) {
     return int8_rows_kept<T, TG, NORM, 2>(P, threads(2), sms, stream);
   } else if constexpr (NORM == (sizeof(T) == 2)) {

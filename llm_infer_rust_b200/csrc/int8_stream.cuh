@@ -84,7 +84,7 @@ __device__ __forceinline__ void tokens_to_8_bits(const Int8RowsParams& R, int8_t
         if (!whole) int8_store8<T, false>(sum_out, at, R.k, v[i]);
         else if (at < R.k) int8_store8<T, true>(sum_out, at, R.k, v[i]);
       }
-      if (at < R.k) int8_gain<TG, NORM>(g[i], v[i], ss, most);
+      if (at < R.k) int8_gain<TG, NORM, true>(g[i], v[i], at, R.k, ss, most);
     }
   }
   uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));

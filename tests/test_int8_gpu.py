@@ -381,6 +381,40 @@ def test_rows_that_begin_anywhere(tokens, k, dtype):
         assert ((scales.double() - want).abs() <= 2.0 ** -18 * want).all()
 
 
+@pytest.mark.parametrize("dtype,gain_dtype", [(BF16, BF16), (F32, BF16), (BF16, F32), (F32, F32)])
+@pytest.mark.parametrize("tokens,k", [(200, 3), (700, 64), (700, 250), (700, 507), (2000, 512), (700, 533), (700, 536), (700, 767), (700, 1000),
+                                      (2000, 1024), (700, 1001), (1300, 2049), (1300, 8187), (170, 16400)])
+def test_rows_beside_anything(tokens, k, dtype, gain_dtype):
+    """Short and long rows of many tokens; x, the residual, the gain and the sums begin at unlike places, between and beside them there
+    is nothing but NaN, and none of it counts or is written."""
+    m, o = int8(), ops()
+    nan = float("nan")
+    for apart, lead, begin in ((0, 8, (0, 0, 0)), (0, 3, (1, 1, 2)), (5, 2, (3, 6, 1)), (8, 8, (1, 0, 5))):
+        pitch_x = k + apart
+        space = torch.full((tokens * pitch_x + 32,), nan, dtype=dtype, device=DEV)
+        x = space[lead:lead + tokens * pitch_x].view(tokens, pitch_x)[:, :k]
+        x.copy_(activations(tokens, k, dtype))
+        residual, gain, kept = (torch.full((size + 64,), nan, dtype=t, device=DEV)[16 + at:16 + at + size]
+                                for size, t, at in zip((tokens * k, k, tokens * k), (dtype, gain_dtype, dtype), begin))
+        residual.copy_(rnd(tokens * k, dtype=dtype, seed=3))
+        gain.copy_((1.0 + 0.3 * rnd(k, seed=4)).to(gain_dtype))
+        pitch, scales = m.row_pitch(k), torch.zeros(tokens, device=DEV)
+        values = torch.full((tokens, pitch), 77, dtype=torch.int8, device=DEV)
+        q, s = plain_rows(x.float())
+        rc = m._lib().b200_int8_rows(x, None, None, None, values, scales, tokens, k, pitch_x, pitch, o._code(x), 0, 0.0, o._stream())
+        assert rc == 0 and torch.equal(values[:, :k], q) and torch.equal(scales, s)
+        v = x.float() + residual.float().view(tokens, k)
+        q, s = plain_rows(v * gain.float())
+        rc = m._lib().b200_int8_rows(x, residual, gain, kept, values, scales, tokens, k, pitch_x, pitch, o._code(x), o._code(gain), 1e-5,
+                                     o._stream())
+        want = s.double() * (v.double().square().mean(dim=1) + 1e-5).rsqrt()
+        assert rc == 0 and torch.equal(values[:, :k], q) and torch.equal(kept.view(tokens, k), v.to(dtype))
+        assert ((scales.double() - want).abs() <= 2.0 ** -18 * want).all()
+        for t, at in ((residual, begin[0]), (kept, begin[2])):
+            around = t.as_strided((tokens * k + 64,), (1,), 0)
+            assert around[:16 + at].isnan().all() and around[16 + at + tokens * k:].isnan().all()
+
+
 @pytest.mark.parametrize("tokens,k", [(1, 1999), (2, 1023), (4, 777), (7, 333), (8, 1001), (3, 5001)])
 def test_few_rows_that_begin_anywhere_behind_a_norm(tokens, k):
     """The same inside the kernel for few tokens."""
