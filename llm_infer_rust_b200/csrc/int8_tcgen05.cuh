@@ -192,8 +192,30 @@ template <typename T> __device__ __forceinline__ int turned(int row, int piece) 
   else return row * 64 + ((piece ^ ((row >> 1) & 3)) * 16);
 }
 
-// SPLIT: CTAs that share a tile's k (1: none).
-template <typename T, int MODE, int CG, int SPLIT>
+// Rows low .. high and the first `cols` columns of 32 x 32 turned results to where the first belongs, word by word of W, the loads
+// of eight ahead of their stores.  (Rows off 16 bytes: 7,052 x 768 -> 3,252 bfloat16 in words of eight bytes 35.4 -> 22.0 us,
+// -> 3,251 result by result 28.4, loads and stores in turn 35.4.  Words of two results gained nothing over single ones.)
+template <typename W, typename T>
+__device__ __forceinline__ void store_rows(const unsigned char* turn, T* out, int n, int low, int high, int cols) {
+  constexpr int ACROSS = 32 * sizeof(T) / sizeof(W), ROWS = 32 / ACROSS;
+  const int lane = threadIdx.x & 31, at = lane % ACROSS * static_cast<int>(sizeof(W) / sizeof(T)), byte = at * static_cast<int>(sizeof(T));
+  if (at >= cols) return;
+#pragma unroll 1
+  for (int r0 = lane / ACROSS; r0 < high; r0 += 8 * ROWS) {
+    W y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = *reinterpret_cast<const W*>(turn + turned<T>(r0 + i * ROWS, byte / 16) + byte % 16);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = r0 + i * ROWS;
+      if (r >= low && r < high) *reinterpret_cast<W*>(out + static_cast<size_t>(r) * n + at) = y[i];
+    }
+  }
+}
+
+// SPLIT: CTAs that share a tile's k (1: none).  WHOLE (looked at without a split): pieces of 16 bytes of the result lie at multiples of
+// 16 bytes.  (Both kinds of store in one kernel cost whole results 4 %.)
+template <typename T, int MODE, int CG, int SPLIT, bool WHOLE>
 __global__ void __launch_bounds__(THREADS, 1)
 product_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap wmap, const Int8ProductParams P, const Plan plan) {
   extern __shared__ unsigned char smem_raw[];
@@ -336,7 +358,6 @@ product_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__
     int local = 0;
     T* out = static_cast<T*>(P.out);
     constexpr int LANES = 32 * sizeof(T) / 16;                                  // lanes that a row's 32 results take, 16 bytes each
-    const bool whole = (reinterpret_cast<uintptr_t>(out) | (static_cast<size_t>(P.n) * sizeof(T)) | (out_cols * sizeof(T))) % 16 == 0;
     // scales and bias of a tile's columns (and the token's scale) come from memory while the tile before is worked on
     constexpr int PIECES = ACC / HALVES / 32 / PARTS;                           // of 32 columns, at most
     float c_next[PIECES][HALVES], b_next[PIECES][HALVES], s_next = 0.0f;
@@ -406,18 +427,20 @@ product_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__
 #pragma unroll
         for (int e = 0; e < LANES; ++e) *reinterpret_cast<uint4*>(mine + turned<T>(lane, e)) = packed[e];
         __syncwarp();
-        if (whole) {                                                            // (whole pieces of 16 bytes, up to the last column too)
+        T* to = out + static_cast<size_t>(row0) * P.n + col0;
+        if constexpr (WHOLE && sizeof(T) == 2) {                                // (whole pieces of 16 bytes, up to the last column too)
 #pragma unroll
           for (int q = 0; q < LANES; ++q) {
             const int r = q * (32 / LANES) + lane / LANES, chunk = lane % LANES;
-            if (r >= low && r < high && chunk * static_cast<int>(16 / sizeof(T)) < cols)
-              *reinterpret_cast<uint4*>(out + static_cast<size_t>(row0 + r) * P.n + col0 + chunk * (16 / sizeof(T))) =
-                  *reinterpret_cast<const uint4*>(mine + turned<T>(r, chunk));
+            if (r >= low && r < high && chunk * 8 < cols)
+              *reinterpret_cast<uint4*>(to + static_cast<size_t>(r) * P.n + chunk * 8) = *reinterpret_cast<const uint4*>(mine + turned<T>(r, chunk));
           }
-        } else if (lane < cols) {
-          const int byte = lane * static_cast<int>(sizeof(T));
-          for (int r = low; r < high; ++r)
-            out[static_cast<size_t>(row0 + r) * P.n + col0 + lane] = *reinterpret_cast<const T*>(mine + turned<T>(r, byte / 16) + byte % 16);
+        } else if constexpr (WHOLE) {
+          store_rows<uint4, T>(mine, to, P.n, low, high, cols);
+        } else if (sizeof(T) == 2 && ((reinterpret_cast<uintptr_t>(to) / 2 | P.n | cols) & 3) == 0) {
+          store_rows<uint2, T>(mine, to, P.n, low, high, cols);
+        } else {
+          store_rows<T, T>(mine, to, P.n, low, high, cols);
         }
         __syncwarp();
       }
@@ -545,11 +568,11 @@ static int tensor_map(CUtensorMap* map, const void* matrix, long long rows, long
   return r == CUDA_SUCCESS ? 0 : 1000 + static_cast<int>(r);
 }
 
-template <typename T, int MODE, int CG, int SPLIT>
+template <typename T, int MODE, int CG, int SPLIT, bool WHOLE>
 static int launch(const Int8ProductParams& P, const Plan& plan, int blocks, int cluster, cudaStream_t stream) {
   static bool configured = false;
   if (!configured) {
-    const cudaError_t e = cudaFuncSetAttribute(product_kernel<T, MODE, CG, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST);
+    const cudaError_t e = cudaFuncSetAttribute(product_kernel<T, MODE, CG, SPLIT, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST);
     if (e != cudaSuccess) return static_cast<int>(e);
     configured = true;
   }
@@ -558,7 +581,7 @@ static int launch(const Int8ProductParams& P, const Plan& plan, int blocks, int 
   if (rc == 0) rc = tensor_map(&wmap, P.w, static_cast<long long>(P.n) * (MODE == INT8_GLU ? 2 : 1), P.k, P.w_pitch,
                                  CG == 2 || MODE == INT8_GLU ? plan.bn / 2 : plan.bn);
   if (rc != 0) return rc;
-  return b200_launch(product_kernel<T, MODE, CG, SPLIT>, dim3(blocks), dim3(THREADS), smem_fixed<T>() + plan.stages * plan.stage_bytes, stream,
+  return b200_launch(product_kernel<T, MODE, CG, SPLIT, WHOLE>, dim3(blocks), dim3(THREADS), smem_fixed<T>() + plan.stages * plan.stage_bytes, stream,
                      cluster, qmap, wmap, P, plan);
 }
 
@@ -631,8 +654,8 @@ template <typename T, int MODE> static int quads_side_by_side() {
     config.attrs = &attr;
     config.numAttrs = 1;
     int n = 0;
-    if (cudaFuncSetAttribute(product_kernel<T, MODE, 1, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST) != cudaSuccess ||
-        cudaOccupancyMaxActiveClusters(&n, product_kernel<T, MODE, 1, 4>, &config) != cudaSuccess || n < 1)
+    if (cudaFuncSetAttribute(product_kernel<T, MODE, 1, 4, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, product_kernel<T, MODE, 1, 4, true>, &config) != cudaSuccess || n < 1)
       n = 1;
     known[device] = n + 1;
   }
@@ -645,9 +668,11 @@ template <typename T, int MODE> static int product(const Int8ProductParams& P, i
   const long long tiles = static_cast<long long>((P.tokens + tall - 1) / tall) * ((P.n + wide - 1) / wide);
   if (tiles > 0x0fffffff || plan.stages < 2) return B200_BAD_SIZE;
   const int t = static_cast<int>(tiles);
-  if (plan.way == 0) return launch<T, MODE, 2, 1>(P, plan, 2 * (t < sms / 2 ? t : sms / 2), 2, stream);
-  if (plan.way == 1) return launch<T, MODE, 1, 1>(P, plan, t < sms ? t : sms, 0, stream);
-  return plan.way == 2 ? launch<T, MODE, 1, 2>(P, plan, 2 * t, 2, stream) : launch<T, MODE, 1, 4>(P, plan, 4 * t, 4, stream);
+  const bool whole = (reinterpret_cast<uintptr_t>(P.out) | (static_cast<size_t>(P.n) * sizeof(T)) | (wide * sizeof(T))) % 16 == 0;
+  const int pairs = 2 * (t < sms / 2 ? t : sms / 2), ctas = t < sms ? t : sms;
+  if (plan.way == 0) return whole ? launch<T, MODE, 2, 1, true>(P, plan, pairs, 2, stream) : launch<T, MODE, 2, 1, false>(P, plan, pairs, 2, stream);
+  if (plan.way == 1) return whole ? launch<T, MODE, 1, 1, true>(P, plan, ctas, 0, stream) : launch<T, MODE, 1, 1, false>(P, plan, ctas, 0, stream);
+  return plan.way == 2 ? launch<T, MODE, 1, 2, true>(P, plan, 2 * t, 2, stream) : launch<T, MODE, 1, 4, true>(P, plan, 4 * t, 4, stream);
 }
 
 }  // namespace i8tc

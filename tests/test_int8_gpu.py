@@ -276,6 +276,35 @@ def test_outputs_at_any_address():
             assert torch.equal(out, m.int8_glu(rows, w, out_dtype=out_dtype) if mode else m.int8_linear(rows, w, out_dtype=out_dtype))
 
 
+@pytest.mark.parametrize("mode", [0, 1])
+@pytest.mark.parametrize("tokens,k,n", [(300, 96, 1540), (300, 96, 1541), (300, 96, 1542), (700, 256, 324), (700, 256, 323), (2100, 64, 2052),
+                                        (2100, 64, 2051)])
+def test_results_of_any_width_at_any_address(tokens, k, n, mode):
+    """Rows of results that begin at multiples of 16, 8, 4 and 2 bytes, against the definition, with nothing written beside them."""
+    m, o = int8(), ops()
+    rows, w = m.quantize_rows(activations(tokens, k, BF16)), weight(n * (1 + mode), k)
+    want, size = floats(rows, w)
+    if mode:
+        want = gated(want, "silu", 0.0, 1.0)
+    for out_dtype in (BF16, F32):
+        first = None
+        for at in (16, 20, 18, 17):
+            space = torch.full((tokens * n + 64,), 123.0, dtype=out_dtype, device=DEV)
+            out = space[at:at + tokens * n].view(tokens, n)
+            rc = m._lib().b200_int8_linear(None, None, None, None, rows.values, rows.scales, w.values, w.scales, None, out, tokens, n, k, 0,
+                                           rows.values.stride(0), w.values.stride(0), 0, 0, o._code(out), mode, 0.0, 0.0, 1.0,
+                                           o.error_word(out.device), o._stream())
+            assert rc == 0 and (space[:at] == 123).all() and (space[at + tokens * n:] == 123).all()
+            if first is None:
+                first = out
+                if not mode:
+                    check(out, want, size, out_dtype)
+                else:                                           # both factors 2^-21, the gate's own functions 2^-19 of what they give
+                    g, u = size.chunk(2, dim=1)
+                    check(out, want, g * u + g + u, out_dtype, rel=2.0 ** -18)
+            assert torch.equal(out, first)
+
+
 def test_rows_are_alike_whatever_runs_beside_them():
     """A token's result has the same bits alone and among others (sums are exact, scales are its own)."""
     m = int8()
