@@ -10,8 +10,8 @@
 // q are 0, so everything computed from the row is NaN.  Where 127 / a would overflow (a < 2^-100) row and maximum are
 // multiplied by 2^100 first, which is exact.
 //
-// Bound by the bytes of x (and the residual, twice), by latency where rows are few.  A block walks over rows; a row lies in
-// registers (up to 32 elements a thread) between the reduction and the rounding, the next row's loads are on their way
+// Bound by the bytes of x (and the residual, twice), by latency where rows are few.  A block (short rows: a warp) walks over rows; a
+// row lies in registers (up to 32 elements a thread) between the reduction and the rounding, the next row's loads are on their way
 // meanwhile.  All loads of a row are issued before its first store: a store that might alias would else hold the loads behind it.
 #pragma once
 #include <string.h>
@@ -328,7 +328,8 @@ __device__ __forceinline__ uint32_t int8_meet(float& ss, float top, float (*sums
   return __reduce_max_sync(0xffffffffu, lane < warps ? tops[turn][lane] : 0u);
 }
 
-// Rows whose chunks fit the block's registers, CH a thread (ALONE: a warp's, of which there are blockDim.y).  WHOLE: there are whole chunks alone, all at multiples of 16 bytes.
+// Rows whose chunks fit the block's registers, CH a thread (ALONE: a warp's, of which a block has blockDim.y).  WHOLE: there are whole
+// chunks alone, all at multiples of 16 bytes.
 // (8,192 x 4,096 behind a norm with that question asked chunk by chunk 45 us, so 38: 6.2 TB/s, 95 % of the copy rate.)
 template <typename T, typename TG, bool NORM, int CH, bool WHOLE, int MOST = 512, bool ALONE = false>
 __global__ void __launch_bounds__(MOST) int8_rows_kernel(const Int8RowsParams P) {

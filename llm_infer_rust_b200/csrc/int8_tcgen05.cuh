@@ -6,7 +6,7 @@
 //   warp 0      one lane feeds a ring of stages with TMA (128-byte swizzle): a box of weight rows (or of gate and of up rows) for
 //               each of a stage's blocks of k
 //   warp 10     the same for the tokens
-//   warp 1      allocates tensor memory for two accumulators; one lane issues tcgen05.mma (kind::i8, K 32, four a stage)
+//   warp 1      allocates tensor memory for two accumulators; one lane issues tcgen05.mma (kind::i8, K 32, four a block)
 //   warps 2-9   read their 32 lanes of tensor memory (two warps a quarter, every other 32 columns), multiply by the scales,
 //               round, turn 32 x 32 results through shared memory and store pieces of rows
 // Three ways to run it:
