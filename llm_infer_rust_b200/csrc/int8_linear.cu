@@ -51,6 +51,13 @@ B200_EXPORT int b200_int8_alone(int tokens, int k) {
   return k >= 1 && k <= MAX_K && i8st::takes(tokens, k) && i8st::fuses(tokens, k) ? 1 : 0;
 }
 
+// The shared memory that the streaming kernel asks for at launch with `tokens` rows of k columns (0: the tiled kernel takes them), and the
+// most that it may ask for.
+B200_EXPORT int b200_int8_stream_bytes(int tokens, int k) {
+  return tokens >= 1 && k >= 1 && k <= MAX_K && i8st::takes(tokens, k) ? i8st::smem_of(tokens, k) : 0;
+}
+B200_EXPORT int b200_int8_stream_limit() { return i8st::DYNAMIC_MOST; }
+
 // How the tiled product is cut up: 1,000 times the way (0: pairs of CTAs, else the CTAs that share a tile's k) plus the columns.
 B200_EXPORT int b200_int8_plan(int tokens, int n, int k, int mode, int sms, int quads) {
   const i8tc::Plan p = i8tc::make_plan(tokens, n, k, mode, sms, quads, i8tc::smem_fixed<__nv_bfloat16>());

@@ -25,7 +25,9 @@ namespace i8st {
 constexpr int THREADS = 512, WARPS = 16, DEPTH = 6;
 constexpr int RING = DEPTH * 2 * THREADS * 16;                   // 96 KB
 constexpr int MOST_TOKENS = 16;
-constexpr int SMEM_MOST = 227 * 1024;
+// What a launch may ask for: of the 227 KB of a block one is left to the arrays that the kernel declares itself.  takes() goes by it and
+// the kernel's limit is set to it: a size above the limit would be refused at launch.
+constexpr int DYNAMIC_MOST = 226 * 1024;
 
 struct Plan {
   int wn, wk, steps;         // groups, shares of k, steps of 64 k a share
@@ -257,7 +259,7 @@ static inline bool fuses(int tokens, int k) {
   const int slots = tokens <= 1 ? 1 : tokens <= 2 ? 2 : tokens <= 4 ? 4 : 8;
   return tokens <= 8 && (k + 7) / 8 <= INT8_ROW_CHUNKS * THREADS / slots;
 }
-static inline bool takes(int tokens, int k) { return tokens <= MOST_TOKENS && smem_of(tokens, k) <= SMEM_MOST; }
+static inline bool takes(int tokens, int k) { return tokens <= MOST_TOKENS && smem_of(tokens, k) <= DYNAMIC_MOST; }
 
 static inline Plan make_plan(int n, int k, int mode, int sms) {
   Plan p;
@@ -285,7 +287,7 @@ template <typename T, typename TG, bool NORM, bool FUSED, int NT>
 static int launch_one(const Int8ProductParams& P, const Int8RowsParams& R, int mode, int out_code, int sms, cudaStream_t stream) {
   static bool configured = false;
   if (!configured) {
-    const cudaError_t e = cudaFuncSetAttribute(stream_kernel<T, TG, NORM, FUSED, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST - 1024);
+    const cudaError_t e = cudaFuncSetAttribute(stream_kernel<T, TG, NORM, FUSED, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, DYNAMIC_MOST);
     if (e != cudaSuccess) return static_cast<int>(e);
     configured = true;
   }
