@@ -268,10 +268,11 @@ PyObject* byte_product(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (code(x) < 0 || code_of(type) < 0 || w.scalar_type() != at::kChar || code(c) != 0 || x.dim() != 2 || w.dim() != 2 || c.dim() != 1) Py_RETURN_NONE;
   const I mode = PyLong_AsLongLong(args[10]), stream = PyLong_AsLongLong(args[15]);
   if (PyErr_Occurred()) return nullptr;
+  constexpr I MOST_ROWS = INT32_MAX - 65536;     // (what the entry points take)
   const I tokens = x.size(0), k = x.size(1), rows = w.size(0), between = tokens > 1 ? x.stride(0) : k, w_pitch = w.stride(0);
   if (tokens < 1 || k < 1 || k > 131071 || w.size(1) != k || c.size(0) != rows || rows < 1 || (mode != 0 && rows % 2 != 0) || between < k ||
       (k > 1 && (x.stride(1) != 1 || w.stride(1) != 1)) || (rows > 1 && c.stride(0) != 1) || w_pitch < k || w_pitch % 16 != 0 ||
-      reinterpret_cast<std::uintptr_t>(w.const_data_ptr()) % 16 != 0 || tokens > INT32_MAX || rows > INT32_MAX)
+      reinterpret_cast<std::uintptr_t>(w.const_data_ptr()) % 16 != 0 || tokens > MOST_ROWS || rows > MOST_ROWS)
     Py_RETURN_NONE;
   for (int i = 3; i < 6; i += 2)                 // the residual and where its sum goes: as x is, row after row
     if (t[i] != nullptr && (t[i]->sizes() != x.sizes() || t[i]->scalar_type() != x.scalar_type() || !t[i]->is_contiguous())) Py_RETURN_NONE;

@@ -10,6 +10,9 @@
 #include "int8_tcgen05.cuh"
 
 constexpr int MAX_K = 131071;
+// Tokens and weight rows of a call.  Kernels count them in 32-bit integers and step past the end by what a grid takes at once: up to
+// 9,472 rows to 8 bits, a tile of 256.
+constexpr int MAX_ROWS = 2147483647 - 65536;
 
 static int sm_count() {
   static int counts[64];                       // of the devices that were asked (0: not yet)
@@ -29,7 +32,7 @@ static int tiled_product(const Int8ProductParams& P, int mode, int out_code, int
 static int rows_params(Int8RowsParams& R, const void* x, const void* residual, const void* gain, void* sum_out, void* q, float* s,
                        int tokens, int k, long long x_pitch, long long q_pitch, int x_code, int gain_code, float eps) {
   if ((x_code != B200_F32 && x_code != B200_BF16) || (gain && gain_code != B200_F32 && gain_code != B200_BF16)) return B200_BAD_DTYPE;
-  if (tokens < 0 || k < 1 || k > MAX_K || x_pitch < k || q_pitch < k) return B200_BAD_SIZE;
+  if (tokens < 0 || tokens > MAX_ROWS || k < 1 || k > MAX_K || x_pitch < k || q_pitch < k) return B200_BAD_SIZE;
   if (!int8_aligned(q, q_pitch)) return B200_BAD_ALIGN;
   const long long e = x_code == B200_F32 ? 4 : 2;
   const bool whole = k % 8 == 0 && int8_aligned(x, x_pitch * e) && int8_aligned(residual, residual ? k * e : 0) && int8_aligned(gain, 0) &&
@@ -71,7 +74,9 @@ B200_EXPORT int b200_int8_linear(const void* x, const void* residual, const void
                                  long long x_pitch, long long q_pitch, long long w_pitch, int x_code, int gain_code, int out_code,
                                  int mode, float eps, float limit, float alpha, int* err, cudaStream_t stream) {
   if (out_code != B200_F32 && out_code != B200_BF16) return B200_BAD_DTYPE;
-  if (tokens < 0 || n < 0 || k < 1 || k > MAX_K || q_pitch < k || w_pitch < k || (mode != INT8_PLAIN && mode != INT8_GLU)) return B200_BAD_SIZE;
+  if (tokens < 0 || tokens > MAX_ROWS || n < 0 || n > MAX_ROWS / (mode == INT8_GLU ? 2 : 1) || k < 1 || k > MAX_K || q_pitch < k || w_pitch < k ||
+      (mode != INT8_PLAIN && mode != INT8_GLU))
+    return B200_BAD_SIZE;
   if (!int8_aligned(q, q_pitch) || !int8_aligned(w, w_pitch)) return B200_BAD_ALIGN;
   if (tokens == 0) return 0;
   if (!x && (!q || !s)) return B200_BAD_SIZE;

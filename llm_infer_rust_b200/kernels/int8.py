@@ -22,6 +22,7 @@ from .build import load_call_binding, load_entry_points
 from .ops import KernelError
 
 MAX_K = 131071              # 128 * 128 * K stays below 2^31
+MAX_ROWS = 2 ** 31 - 1 - 65536   # tokens, or rows of a weight: the kernels count them (and a step past their end) in 32 bits
 _PLAIN, _GLU = 0, 1
 
 
@@ -54,12 +55,18 @@ def _lib(glu: str = "silu"):
     return load_entry_points("int8_linear.cu", ops._GLU_DEFINES[glu] or None)
 
 
+def _check_count(rows: int) -> None:
+    if rows > MAX_ROWS:
+        raise KernelError(f"{rows} rows are refused: at most {MAX_ROWS} a call")
+
+
 def _check_8_bit(m, what: str) -> None:
     values, scales = m.values, m.scales
     if values.dtype != torch.int8 or scales.dtype != torch.float32:
         raise KernelError(f"{what} in 8 bits are int8 values with float32 scales")
     if values.dim() != 2 or values.stride(1) != 1 or scales.dim() != 1 or scales.numel() != values.shape[0] or not scales.is_contiguous():
         raise KernelError(f"{what} in 8 bits are values [rows, K] with a unit inner stride and one scale a row")
+    _check_count(values.shape[0])
     if values.stride(0) % 16 or values.data_ptr() % 16 or values.stride(0) < values.shape[1]:
         raise KernelError(f"the rows of {what} in 8 bits lie a multiple of 16 bytes apart")
 
@@ -68,6 +75,7 @@ def _check_rows(x: torch.Tensor, what: str) -> None:
     ops._code(x)
     if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
         raise KernelError(f"{what} takes rows [T, K] with a unit inner stride")
+    _check_count(x.shape[0])
 
 
 def _check_k(k: int) -> None:

@@ -20,3 +20,38 @@ def test_what_the_streaming_kernel_takes_fits_its_launch():
     # rows of these widths lie between what a block has and what a launch may ask for: the tiled kernel takes them
     assert all(asks(t, k) == 0 for t, k in ((16, 6272), (15, 6656), (14, 7168), (13, 7680), (10, 9984), (8, 14592)))
     assert all(asks(t, k) > 0 for t, k in ((16, 6208), (15, 6592), (14, 7104), (13, 7616), (10, 9920), (8, 14528)))
+
+
+def entry_points():
+    return build.load_entry_points("int8_linear.cu")
+
+
+def linear_call(**kw):
+    """b200_int8_linear on two rows of 32 (memory of the host: nothing may be launched)."""
+    a = dict(x=torch.zeros(2, 32), residual=None, gain=None, kept=None, q=torch.zeros(2, 32, dtype=torch.int8), s=torch.zeros(2),
+             w=torch.zeros(4, 32, dtype=torch.int8), c=torch.ones(4), bias=None, out=torch.zeros(2, 4), tokens=2, n=4, k=32, x_pitch=32, q_pitch=32,
+             w_pitch=32, x_code=0, gain_code=0, out_code=0, mode=0, eps=0.0, limit=0.0, alpha=1.0, err=torch.zeros(1, dtype=torch.int32), stream=0)
+    a.update(kw)
+    return entry_points().b200_int8_linear(*a.values())
+
+
+def test_entry_points_refuse_more_rows_than_they_count():
+    """A step past the last row must stay below 2^31 too."""
+    for many in (2 ** 31 - 1, 2 ** 31 - 65536):
+        assert linear_call(tokens=many) == linear_call(n=many) == -2
+        assert entry_points().b200_int8_rows(torch.zeros(2, 32), None, None, None, torch.zeros(2, 32, dtype=torch.int8), torch.zeros(2), many, 32, 32, 32,
+                                             0, 0, 0.0, 0) == -2
+    assert linear_call(n=2 ** 30, mode=1) == -2                   # (gate and up rows together)
+
+
+def test_more_rows_than_the_kernels_count_are_refused():
+    from llm_infer_rust_b200.kernels import int8
+    from llm_infer_rust_b200.kernels.ops import KernelError
+    w = int8.Int8Weight(torch.zeros(4, 16, dtype=torch.int8)[:, :1], torch.ones(4))
+    for many in (2 ** 31 - 65536, 2 ** 32 + 5):                   # (memory of no device: the sizes alone count)
+        x = torch.empty(many, 1, dtype=torch.bfloat16, device="meta")
+        rows = int8.Int8Rows(torch.empty(many, 16, dtype=torch.int8, device="meta")[:, :1], torch.empty(many, device="meta"))
+        for call in (lambda: int8.int8_linear(x, w), lambda: int8.quantize_rows(x), lambda: int8.int8_linear(rows, w),
+                     lambda: int8.int8_linear(torch.zeros(2, 1), int8.Int8Weight(*rows))):
+            with pytest.raises(KernelError, match="rows are refused"):
+                call()
