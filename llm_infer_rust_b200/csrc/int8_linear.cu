@@ -46,7 +46,8 @@ B200_EXPORT int b200_int8_rows(const void* x, const void* residual, const void* 
                                int k, long long x_pitch, long long q_pitch, int x_code, int gain_code, float eps, cudaStream_t stream) {
   Int8RowsParams R;
   const int rc = rows_params(R, x, residual, gain, sum_out, q, s, tokens, k, x_pitch, q_pitch, x_code, gain_code, eps);
-  return rc != 0 ? rc : tokens == 0 ? 0 : int8_rows_launch(R, x_code, gain_code, sm_count(), stream);
+  if (rc != 0 || tokens == 0) return rc;
+  return !x || !q || !s ? B200_BAD_SIZE : int8_rows_launch(R, x_code, gain_code, sm_count(), stream);
 }
 
 // 1 where the product of `tokens` rows of floats takes them to 8 bits itself: no place for q and s is needed.
@@ -79,19 +80,22 @@ B200_EXPORT int b200_int8_linear(const void* x, const void* residual, const void
     return B200_BAD_SIZE;
   if (!int8_aligned(q, q_pitch) || !int8_aligned(w, w_pitch)) return B200_BAD_ALIGN;
   if (tokens == 0) return 0;
-  if (!x && (!q || !s)) return B200_BAD_SIZE;
+  if ((!x && (!q || !s)) || (n > 0 && (!w || !c || !out))) return B200_BAD_SIZE;
   const int sms = sm_count();
   const bool few = n > 0 && i8st::takes(tokens, k);
   const Int8ProductParams P = {static_cast<const int8_t*>(q), s, static_cast<const int8_t*>(w), c, bias, out, tokens, n, k,
                                q_pitch, w_pitch, limit, alpha, err};
+  const bool no_word = n > 0 && !err;           // (where a wait that runs out is flagged)
   if (x) {
     Int8RowsParams R;
     int rc = rows_params(R, x, residual, gain, sum_out, q, s, tokens, k, x_pitch, q_pitch, x_code, gain_code, eps);
+    if (rc == 0 && no_word) rc = B200_BAD_SIZE;
     if (rc == 0 && few && i8st::fuses(tokens, k)) return i8st::product(P, &R, x_code, gain_code, mode, out_code, sms, stream);
     if (rc == 0 && (q == nullptr || s == nullptr)) rc = B200_BAD_SIZE;
     if (rc == 0) rc = int8_rows_launch(R, x_code, gain_code, sms, stream);
     if (rc != 0) return rc;
   }
   if (n == 0) return 0;
+  if (no_word) return B200_BAD_SIZE;
   return few ? i8st::product(P, nullptr, 0, 0, mode, out_code, sms, stream) : tiled_product(P, mode, out_code, sms, stream);
 }

@@ -55,3 +55,15 @@ def test_more_rows_than_the_kernels_count_are_refused():
                      lambda: int8.int8_linear(torch.zeros(2, 1), int8.Int8Weight(*rows))):
             with pytest.raises(KernelError, match="rows are refused"):
                 call()
+
+
+def test_entry_points_refuse_null_operands():
+    rows = lambda x=torch.zeros(2, 32), q=torch.zeros(2, 32, dtype=torch.int8), s=torch.zeros(2): \
+        entry_points().b200_int8_rows(x, None, None, None, q, s, 2, 32, 32, 32, 0, 0, 0.0, 0)
+    assert rows(x=None) == rows(q=None) == rows(s=None) == -2
+    for tokens in (2, 20):                                        # (the streaming kernel and the tiled one)
+        for name in ("w", "c", "out", "err"):
+            assert linear_call(tokens=tokens, **{name: None}) == -2, (tokens, name)
+        assert linear_call(tokens=tokens, x=None, s=None) == linear_call(tokens=tokens, x=None, q=None) == -2
+    assert linear_call(tokens=20, q=None) == linear_call(tokens=20, s=None) == -2      # (two tokens alone need no place for them)
+    assert linear_call(tokens=0, x=None, q=None, s=None, w=None, c=None, out=None, err=None) == 0
