@@ -19,6 +19,18 @@ struct Int8ProductParams {
   int* err;
 };
 
+// The device that a call runs on.
+struct Int8Device { int index, sms; };
+
+// A kernel's limit of dynamic shared memory is a device's own: set at its first launch on each (beyond 64 devices at every launch).
+template <typename Kernel> static int int8_launch_limit(Kernel kernel, int bytes, const Int8Device& device, bool (&set)[64]) {
+  const bool kept = device.index >= 0 && device.index < 64;
+  if (kept && set[device.index]) return 0;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && kept) set[device.index] = true;
+  return static_cast<int>(e);
+}
+
 // What joins gate and up (see glu_product of common.cuh for the forms), each a factor over 1 + exp: tanh(z) = 2 / (1 + exp(-2 z)) - 1.
 // The fast exponential and quotient are off by a few 2^-22, without the branches of the exact ones, which keep the
 // elements of a row from overlapping (a tile of 128 x 128 took 7 us with them, more than its products).

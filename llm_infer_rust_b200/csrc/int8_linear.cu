@@ -14,18 +14,19 @@ constexpr int MAX_K = 131071;
 // 9,472 rows to 8 bits, a tile of 256.
 constexpr int MAX_ROWS = 2147483647 - 65536;
 
-static int sm_count() {
-  static int counts[64];                       // of the devices that were asked (0: not yet)
+static Int8Device current_device() {
+  static int counts[64];                       // SMs of the devices that were asked (0: not yet)
   int device = 0;
-  if (cudaGetDevice(&device) != cudaSuccess || device >= 64) return 148;
+  if (cudaGetDevice(&device) != cudaSuccess) return {-1, 148};
+  if (device >= 64) return {device, 148};
   if (counts[device] == 0) cudaDeviceGetAttribute(&counts[device], cudaDevAttrMultiProcessorCount, device);
-  return counts[device] > 0 ? counts[device] : 148;
+  return {device, counts[device] > 0 ? counts[device] : 148};
 }
 
-static int tiled_product(const Int8ProductParams& P, int mode, int out_code, int sms, cudaStream_t stream) {
+static int tiled_product(const Int8ProductParams& P, int mode, int out_code, const Int8Device& device, cudaStream_t stream) {
   if (mode == INT8_GLU)
-    return out_code == B200_F32 ? i8tc::product<float, INT8_GLU>(P, sms, stream) : i8tc::product<__nv_bfloat16, INT8_GLU>(P, sms, stream);
-  return out_code == B200_F32 ? i8tc::product<float, INT8_PLAIN>(P, sms, stream) : i8tc::product<__nv_bfloat16, INT8_PLAIN>(P, sms, stream);
+    return out_code == B200_F32 ? i8tc::product<float, INT8_GLU>(P, device, stream) : i8tc::product<__nv_bfloat16, INT8_GLU>(P, device, stream);
+  return out_code == B200_F32 ? i8tc::product<float, INT8_PLAIN>(P, device, stream) : i8tc::product<__nv_bfloat16, INT8_PLAIN>(P, device, stream);
 }
 
 // ------------------------------------------------------------------ entry points
@@ -47,7 +48,7 @@ B200_EXPORT int b200_int8_rows(const void* x, const void* residual, const void* 
   Int8RowsParams R;
   const int rc = rows_params(R, x, residual, gain, sum_out, q, s, tokens, k, x_pitch, q_pitch, x_code, gain_code, eps);
   if (rc != 0 || tokens == 0) return rc;
-  return !x || !q || !s ? B200_BAD_SIZE : int8_rows_launch(R, x_code, gain_code, sm_count(), stream);
+  return !x || !q || !s ? B200_BAD_SIZE : int8_rows_launch(R, x_code, gain_code, current_device().sms, stream);
 }
 
 // 1 where the product of `tokens` rows of floats takes them to 8 bits itself: no place for q and s is needed.
@@ -81,7 +82,7 @@ B200_EXPORT int b200_int8_linear(const void* x, const void* residual, const void
   if (!int8_aligned(q, q_pitch) || !int8_aligned(w, w_pitch)) return B200_BAD_ALIGN;
   if (tokens == 0) return 0;
   if ((!x && (!q || !s)) || (n > 0 && (!w || !c || !out))) return B200_BAD_SIZE;
-  const int sms = sm_count();
+  const Int8Device device = current_device();
   const bool few = n > 0 && i8st::takes(tokens, k);
   const Int8ProductParams P = {static_cast<const int8_t*>(q), s, static_cast<const int8_t*>(w), c, bias, out, tokens, n, k,
                                q_pitch, w_pitch, limit, alpha, err};
@@ -90,12 +91,12 @@ B200_EXPORT int b200_int8_linear(const void* x, const void* residual, const void
     Int8RowsParams R;
     int rc = rows_params(R, x, residual, gain, sum_out, q, s, tokens, k, x_pitch, q_pitch, x_code, gain_code, eps);
     if (rc == 0 && no_word) rc = B200_BAD_SIZE;
-    if (rc == 0 && few && i8st::fuses(tokens, k)) return i8st::product(P, &R, x_code, gain_code, mode, out_code, sms, stream);
+    if (rc == 0 && few && i8st::fuses(tokens, k)) return i8st::product(P, &R, x_code, gain_code, mode, out_code, device, stream);
     if (rc == 0 && (q == nullptr || s == nullptr)) rc = B200_BAD_SIZE;
-    if (rc == 0) rc = int8_rows_launch(R, x_code, gain_code, sms, stream);
+    if (rc == 0) rc = int8_rows_launch(R, x_code, gain_code, device.sms, stream);
     if (rc != 0) return rc;
   }
   if (n == 0) return 0;
   if (no_word) return B200_BAD_SIZE;
-  return few ? i8st::product(P, nullptr, 0, 0, mode, out_code, sms, stream) : tiled_product(P, mode, out_code, sms, stream);
+  return few ? i8st::product(P, nullptr, 0, 0, mode, out_code, device, stream) : tiled_product(P, mode, out_code, device, stream);
 }

@@ -284,33 +284,30 @@ static inline Plan make_plan(int n, int k, int mode, int sms) {
 }
 
 template <typename T, typename TG, bool NORM, bool FUSED, int NT>
-static int launch_one(const Int8ProductParams& P, const Int8RowsParams& R, int mode, int out_code, int sms, cudaStream_t stream) {
-  static bool configured = false;
-  if (!configured) {
-    const cudaError_t e = cudaFuncSetAttribute(stream_kernel<T, TG, NORM, FUSED, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, DYNAMIC_MOST);
-    if (e != cudaSuccess) return static_cast<int>(e);
-    configured = true;
-  }
-  const Plan plan = make_plan(P.n, P.k, mode, sms);
-  return b200_launch(stream_kernel<T, TG, NORM, FUSED, NT>, dim3(plan.units < sms ? plan.units : sms), dim3(THREADS), smem_of(P.tokens, P.k), stream,
+static int launch_one(const Int8ProductParams& P, const Int8RowsParams& R, int mode, int out_code, const Int8Device& device, cudaStream_t stream) {
+  static bool set[64];
+  const int rc = int8_launch_limit(stream_kernel<T, TG, NORM, FUSED, NT>, DYNAMIC_MOST, device, set);
+  if (rc != 0) return rc;
+  const Plan plan = make_plan(P.n, P.k, mode, device.sms);
+  return b200_launch(stream_kernel<T, TG, NORM, FUSED, NT>, dim3(plan.units < device.sms ? plan.units : device.sms), dim3(THREADS), smem_of(P.tokens, P.k), stream,
                      0, P, R, plan, mode, static_cast<int>(out_code == B200_F32));
 }
 
 // `R`: the tokens as floats (null: P.q and P.s are there already).
-static int product(const Int8ProductParams& P, const Int8RowsParams* R, int x_code, int gain_code, int mode, int out_code, int sms, cudaStream_t stream) {
+static int product(const Int8ProductParams& P, const Int8RowsParams* R, int x_code, int gain_code, int mode, int out_code, const Int8Device& device, cudaStream_t stream) {
   const Int8RowsParams none = {};
   if (R == nullptr)
-    return P.tokens > 8 ? launch_one<float, float, false, false, 2>(P, none, mode, out_code, sms, stream)
-                        : launch_one<float, float, false, false, 1>(P, none, mode, out_code, sms, stream);
+    return P.tokens > 8 ? launch_one<float, float, false, false, 2>(P, none, mode, out_code, device, stream)
+                        : launch_one<float, float, false, false, 1>(P, none, mode, out_code, device, stream);
   const bool wide_x = x_code == B200_F32, wide_g = gain_code == B200_F32;
   if (R->gain == nullptr)
-    return wide_x ? launch_one<float, float, false, true, 1>(P, *R, mode, out_code, sms, stream)
-                  : launch_one<__nv_bfloat16, float, false, true, 1>(P, *R, mode, out_code, sms, stream);
+    return wide_x ? launch_one<float, float, false, true, 1>(P, *R, mode, out_code, device, stream)
+                  : launch_one<__nv_bfloat16, float, false, true, 1>(P, *R, mode, out_code, device, stream);
   if (wide_x)
-    return wide_g ? launch_one<float, float, true, true, 1>(P, *R, mode, out_code, sms, stream)
-                  : launch_one<float, __nv_bfloat16, true, true, 1>(P, *R, mode, out_code, sms, stream);
-  return wide_g ? launch_one<__nv_bfloat16, float, true, true, 1>(P, *R, mode, out_code, sms, stream)
-                : launch_one<__nv_bfloat16, __nv_bfloat16, true, true, 1>(P, *R, mode, out_code, sms, stream);
+    return wide_g ? launch_one<float, float, true, true, 1>(P, *R, mode, out_code, device, stream)
+                  : launch_one<float, __nv_bfloat16, true, true, 1>(P, *R, mode, out_code, device, stream);
+  return wide_g ? launch_one<__nv_bfloat16, float, true, true, 1>(P, *R, mode, out_code, device, stream)
+                : launch_one<__nv_bfloat16, __nv_bfloat16, true, true, 1>(P, *R, mode, out_code, device, stream);
 }
 
 }  // namespace i8st

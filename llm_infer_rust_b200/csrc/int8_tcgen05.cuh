@@ -569,15 +569,12 @@ static int tensor_map(CUtensorMap* map, const void* matrix, long long rows, long
 }
 
 template <typename T, int MODE, int CG, int SPLIT, bool WHOLE>
-static int launch(const Int8ProductParams& P, const Plan& plan, int blocks, int cluster, cudaStream_t stream) {
-  static bool configured = false;
-  if (!configured) {
-    const cudaError_t e = cudaFuncSetAttribute(product_kernel<T, MODE, CG, SPLIT, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST);
-    if (e != cudaSuccess) return static_cast<int>(e);
-    configured = true;
-  }
+static int launch(const Int8ProductParams& P, const Plan& plan, int blocks, int cluster, const Int8Device& device, cudaStream_t stream) {
+  static bool set[64];
+  int rc = int8_launch_limit(product_kernel<T, MODE, CG, SPLIT, WHOLE>, SMEM_MOST, device, set);
+  if (rc != 0) return rc;
   CUtensorMap qmap, wmap;
-  int rc = tensor_map(&qmap, P.q, P.tokens, P.k, P.q_pitch, plan.box);
+  rc = tensor_map(&qmap, P.q, P.tokens, P.k, P.q_pitch, plan.box);
   if (rc == 0) rc = tensor_map(&wmap, P.w, static_cast<long long>(P.n) * (MODE == INT8_GLU ? 2 : 1), P.k, P.w_pitch,
                                  CG == 2 || MODE == INT8_GLU ? plan.bn / 2 : plan.bn);
   if (rc != 0) return rc;
@@ -638,10 +635,9 @@ static inline Plan make_plan(int tokens, int n, int k, int mode, int sms, int qu
 }
 
 // Clusters of four CTAs of the split kernel that run side by side (1 where the device does not say).
-template <typename T, int MODE> static int quads_side_by_side() {
+template <typename T, int MODE> static int quads_side_by_side(int device) {
   static int known[64];                        // plus one, of the devices that were asked
-  int device = 0;
-  if (cudaGetDevice(&device) != cudaSuccess || device >= 64) return 1;
+  if (device < 0 || device >= 64) return 1;
   if (known[device] == 0) {
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(4);
@@ -662,17 +658,18 @@ template <typename T, int MODE> static int quads_side_by_side() {
   return known[device] - 1;
 }
 
-template <typename T, int MODE> static int product(const Int8ProductParams& P, int sms, cudaStream_t stream) {
-  const Plan plan = make_plan(P.tokens, P.n, P.k, MODE, sms, quads_side_by_side<T, MODE>(), smem_fixed<T>());
+template <typename T, int MODE> static int product(const Int8ProductParams& P, const Int8Device& device, cudaStream_t stream) {
+  const int sms = device.sms;
+  const Plan plan = make_plan(P.tokens, P.n, P.k, MODE, sms, quads_side_by_side<T, MODE>(device.index), smem_fixed<T>());
   const int tall = plan.way == 0 ? 2 * BM : BM, wide = plan.bn / (MODE == INT8_GLU ? 2 : 1);
   const long long tiles = static_cast<long long>((P.tokens + tall - 1) / tall) * ((P.n + wide - 1) / wide);
   if (tiles > 0x0fffffff || plan.stages < 2) return B200_BAD_SIZE;
   const int t = static_cast<int>(tiles);
   const bool whole = (reinterpret_cast<uintptr_t>(P.out) | (static_cast<size_t>(P.n) * sizeof(T)) | (wide * sizeof(T))) % 16 == 0;
   const int pairs = 2 * (t < sms / 2 ? t : sms / 2), ctas = t < sms ? t : sms;
-  if (plan.way == 0) return whole ? launch<T, MODE, 2, 1, true>(P, plan, pairs, 2, stream) : launch<T, MODE, 2, 1, false>(P, plan, pairs, 2, stream);
-  if (plan.way == 1) return whole ? launch<T, MODE, 1, 1, true>(P, plan, ctas, 0, stream) : launch<T, MODE, 1, 1, false>(P, plan, ctas, 0, stream);
-  return plan.way == 2 ? launch<T, MODE, 1, 2, true>(P, plan, 2 * t, 2, stream) : launch<T, MODE, 1, 4, true>(P, plan, 4 * t, 4, stream);
+  if (plan.way == 0) return whole ? launch<T, MODE, 2, 1, true>(P, plan, pairs, 2, device, stream) : launch<T, MODE, 2, 1, false>(P, plan, pairs, 2, device, stream);
+  if (plan.way == 1) return whole ? launch<T, MODE, 1, 1, true>(P, plan, ctas, 0, device, stream) : launch<T, MODE, 1, 1, false>(P, plan, ctas, 0, device, stream);
+  return plan.way == 2 ? launch<T, MODE, 1, 2, true>(P, plan, 2 * t, 2, device, stream) : launch<T, MODE, 1, 4, true>(P, plan, 4 * t, 4, device, stream);
 }
 
 }  // namespace i8tc

@@ -67,3 +67,33 @@ def test_entry_points_refuse_null_operands():
         assert linear_call(tokens=tokens, x=None, s=None) == linear_call(tokens=tokens, x=None, q=None) == -2
     assert linear_call(tokens=20, q=None) == linear_call(tokens=20, s=None) == -2      # (two tokens alone need no place for them)
     assert linear_call(tokens=0, x=None, q=None, s=None, w=None, c=None, out=None, err=None) == 0
+
+
+FAKE = r"""
+#include <cuda_runtime.h>
+#include <cstdio>
+static int calls = 0, refuse = 0;
+template <typename K> static cudaError_t fake_attribute(K, cudaFuncAttribute, int) { ++calls; return refuse ? cudaErrorInvalidValue : cudaSuccess; }
+#define cudaFuncSetAttribute fake_attribute
+#include "int8_common.cuh"
+__global__ void kernel() {}
+int main() {
+  bool set[64] = {};
+  for (int device : {0, 0, 1, 0, 63, 1, 63, 64, 64, -1, 2, 2}) {
+    refuse = device == 2 && calls == 6;
+    const int rc = int8_launch_limit(kernel, 1000, Int8Device{device, 148}, set);
+    std::printf("%d:%d ", rc, calls);
+  }
+}
+"""
+
+
+def test_a_launch_limit_is_set_once_a_device(tmp_path):
+    """Against a fake of the runtime's call: every device that a kernel is launched on has its limit, one that was refused is asked again."""
+    import subprocess
+    source, program = tmp_path / "limit.cu", tmp_path / "limit"
+    source.write_text(FAKE)
+    subprocess.run([build.find_nvcc(), *build.ARCH_FLAGS, "-std=c++17", "-I", build.CSRC, "-o", str(program), str(source)], check=True,
+                   stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
+    said = subprocess.run([str(program)], check=True, stdout=subprocess.PIPE, text=True).stdout
+    assert said.split() == "0:1 0:1 0:2 0:2 0:3 0:3 0:3 0:4 0:5 0:6 1:7 0:8".split()
