@@ -31,17 +31,38 @@ template <typename Kernel> static int int8_launch_limit(Kernel kernel, int bytes
   return static_cast<int>(e);
 }
 
+// g / (1 + exp(x)).
+// EXACT, for results in float32: good to 8 units of 2^-24 (4.8 at most among 56 million; the fast functions 65), and without a branch: those of
+// expf and of a true quotient keep the elements of a row from overlapping (45 tokens at 2 x 12,288 x 4,096 34.2 us so, 23.7 this way and with the fast
+// functions; 8,192 at 2 x 2,816 x 1,024 89 us, so 62).
+//   exponential   2^p with p = x log2(e) rounded.  What the rounding left, e (by a fused multiply-add, log2(e) in two floats), makes it
+//                 2^(p + e) = 2^p (1 + e ln 2) to second order.
+//   quotient      times the hardware's reciprocal behind a Newton step.
+// Results in bfloat16 take the fast exponential and quotient: 2 + 1.173 |x| units in the last place at an exponent of x, so 2^-18 of the result
+// at 16 and 2^-16 at 87, far below their own rounding of 2^-8 (the other way costs them 5 to 10 % where the epilogue bounds: 777 at 2 x 2,816 x
+// 1,024 12.4 us, so 13.0).  From an exponent of about 87.3 on, where the factor is below 2e-36, both give 0.
+template <bool EXACT> __device__ __forceinline__ float gate_over(float g, float x) {
+  if constexpr (EXACT) {
+    const float at = fminf(fmaxf(x, -100.0f), 88.5f);  // (beyond: 1 and 0 all the same, and every step stays finite; a NaN comes back with g)
+    const float p = __fmul_rn(at, 1.44269502f), e = fmaf(at, 1.92596299e-8f, fmaf(at, 1.44269502f, -p));
+    float t, y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(t) : "f"(p));
+    const float d = 1.0f + fmaf(t, e * 0.693147181f, t);
+    asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(d));
+    return g * fmaf(fmaf(-d, y, 1.0f), y, y);
+  } else {
+    return __fdividef(g, 1.0f + __expf(x));
+  }
+}
 // What joins gate and up (see glu_product of common.cuh for the forms), each a factor over 1 + exp: tanh(z) = 2 / (1 + exp(-2 z)) - 1.
-// The fast exponential and quotient are off by a few 2^-22, without the branches of the exact ones, which keep the
-// elements of a row from overlapping (a tile of 128 x 128 took 7 us with them, more than its products).
-__device__ __forceinline__ float gate_up(float g, float u, float limit, float alpha) {
+template <bool EXACT> __device__ __forceinline__ float gate_up(float g, float u, float limit, float alpha) {
 #if defined(GLU_CLAMPED_SWISH)
   g = g > limit ? limit : g;                          // (comparisons, not minima: NaN stays)
   u = (u > limit ? limit : u < -limit ? -limit : u) + 1.0f;
-  return __fdividef(g, 1.0f + __expf(-alpha * g)) * u;
+  return gate_over<EXACT>(g, -alpha * g) * u;
 #elif defined(GLU_GELU_TANH)
-  return __fdividef(g, 1.0f + __expf(-1.5957691216057308f * (g + 0.044715f * g * g * g))) * u;
+  return gate_over<EXACT>(g, -1.5957691216057308f * (g + 0.044715f * g * g * g)) * u;
 #else
-  return __fdividef(g, 1.0f + __expf(-g)) * u;
+  return gate_over<EXACT>(g, -g) * u;
 #endif
 }

@@ -238,7 +238,10 @@ __global__ void __launch_bounds__(THREADS, 1) stream_kernel(const Int8ProductPar
         if (glu) up += from[w * NT * 128 + 8];
       }
       float z = fmaf(static_cast<float>(sum), token_scale[token] * c0, b0);
-      if (glu) z = gate_up(z, fmaf(static_cast<float>(up), token_scale[token] * c1, b1), P.limit, P.alpha);
+      if (glu) {
+        const float u = fmaf(static_cast<float>(up), token_scale[token] * c1, b1);
+        z = out_f32 ? gate_up<true>(z, u, P.limit, P.alpha) : gate_up<false>(z, u, P.limit, P.alpha);
+      }
       const size_t at = static_cast<size_t>(token) * P.n + col;
       if (out_f32) static_cast<float*>(P.out)[at] = z;
       else static_cast<__nv_bfloat16*>(P.out)[at] = __float2bfloat16_rn(z);

@@ -419,7 +419,7 @@ product_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__
               float up[4];
               scaled4(u + at, s, gs[16 + at / 4], P.bias ? gs[24 + at / 4] : make_float4(0.0f, 0.0f, 0.0f, 0.0f), up);
 #pragma unroll
-              for (int j = 0; j < 4; ++j) y[z + j] = gate_up(y[z + j], up[j], P.limit, P.alpha);
+              for (int j = 0; j < 4; ++j) y[z + j] = gate_up<sizeof(T) == 4>(y[z + j], up[j], P.limit, P.alpha);
             }
           }
           packed[e] = pack16<T>(y);
@@ -515,7 +515,7 @@ product_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (MODE == INT8_GLU) y[0][e] = gate_up(y[0][e], y[1][e], P.limit, P.alpha);
+        if (MODE == INT8_GLU) y[0][e] = gate_up<sizeof(T) == 4>(y[0][e], y[1][e], P.limit, P.alpha);
       T* dst = out + static_cast<size_t>(row0 + row) * P.n + col;
       if (whole && col + 4 <= P.n) {
         __align__(16) T r[4];
