@@ -86,6 +86,7 @@ class DecoderModel:
                 for name in part.missing_params()]
 
     def parameter_bytes(self) -> int:
+        """Bytes of the parameters' elements in the form in which they are held, without what a part keeps beside them."""
         seen, total = set(), 0
         for part in self._owners().values():
             for t in part.params.values():
@@ -93,6 +94,26 @@ class DecoderModel:
                     seen.add(t.data_ptr())
                     total += t.numel() * t.element_size()
         return total
+
+    def held_bytes(self) -> int:
+        """Bytes of memory that the parts hold: the parameters, what lies between their rows, and what is made of them or kept beside
+        them (scales of 8-bit matrices, tables of positions)."""
+        held = {}
+
+        def add(value):
+            if isinstance(value, torch.Tensor):
+                storage = value.untyped_storage()
+                held[storage.data_ptr()] = storage.nbytes()
+            elif isinstance(value, dict):
+                for v in value.values():
+                    add(v)
+            elif isinstance(value, (list, tuple)):
+                for v in value:
+                    add(v)
+
+        for part in list(self._owners().values()) + list(self.position_encodings.values()):
+            add(vars(part))
+        return sum(held.values())
 
     # ------------------------------------------------------------------ one step
     def _repeated(self, first, h, residual, caches):
