@@ -526,8 +526,11 @@ static int int8_rows_normed(const Int8RowsParams& P, int sms, cudaStream_t strea
       return b200_launch(int8_many_rows_kernel<T>, dim3(P.tokens), dim3(threads(8)), 0, stream, 0, P);
   // Few rows: the row's latency is the time, so a thread takes as little as 512 of them allow.  Many: what counts are the bytes on
   // their way; two chunks a thread keep them (behind a norm 8,192 x 4,096 38 us; four chunks, half the threads: a third slower), in up
-  // to 1,024 threads (8,192 x 12,288 bfloat16 behind a norm 117 us, 6.0 TB/s; read twice, the second time out of the caches, 126),
-  // but for float32 behind a norm, which is faster read twice (226 us, 254 kept).
+  // to 1,024 threads (8,192 x 12,288 bfloat16 behind a norm 117 us, 6.0 TB/s; read twice, the second time out of the caches, 126;
+  // without a norm, 160 / 300 / 600 / 1,184 rows of 12,288 2.7 / 3.8 / 6.0 / 9.0 us, read twice 4.0 / 4.6 / 6.7 / 10.1, of 16,384 3.2 / 4.9 / 7.3 /
+  // 10.7, read twice 5.0 / 6.1 / 8.6 / 12.8), but for float32 behind a norm, which is faster read twice (226 us, 254 kept), and for bfloat16 rows without
+  // a norm that are not whole, which are where there are many of them or they are long (300 / 1,184 / 8,192 of 12,289 7.1 / 14.1 / 83.6 us, kept
+  // 6.0 / 17.3 / 110.8; of 9,001 5.5 / 11.5 / 68.4, kept 3.5 / 9.8 / 61.0).
   if (P.tokens <= sms) {
     if (chunks <= 512) return int8_rows_kept<T, TG, NORM, 1>(P, threads(1), sms, stream);
     if (chunks <= 1024) return int8_rows_kept<T, TG, NORM, 2>(P, threads(2), sms, stream);
@@ -544,6 +547,8 @@ static int int8_rows_normed(const Int8RowsParams& P, int sms, cudaStream_t strea
     return int8_rows_kept<T, TG, NORM, 2>(P, threads(2), sms, stream);
   } else if constexpr (NORM == (sizeof(T) == 2)) {
     if (chunks <= 2048) return int8_rows_kept<T, TG, NORM, 2, 1024>(P, threads(2), sms, stream);
+  } else if constexpr (!NORM) {
+    if (chunks <= 2048 && P.whole) return int8_rows_blocks<T, TG, NORM, 2, true, 1024>(P, threads(2), sms, stream);
   }
   return P.whole ? b200_launch(int8_long_rows_kernel<T, TG, NORM, true>, dim3(P.tokens), dim3(512), 0, stream, 0, P)
                                 : b200_launch(int8_long_rows_kernel<T, TG, NORM, false>, dim3(P.tokens), dim3(512), 0, stream, 0, P);

@@ -36,3 +36,13 @@ def test_products_where_another_kernel_takes_over(tokens, k, dtype):
             assert got.dtype == dtype
             assert ((got.double() - want).abs() <= 2.0 ** -16 * g * (u + 1.0) + (2.0 ** -8 if dtype == T.BF16 else 0.0) * want.abs()).all()
         assert torch.equal(pending.residual_out, v.to(dtype))
+
+
+@pytest.mark.parametrize("dtype", [T.BF16, T.F32])
+@pytest.mark.parametrize("tokens,k", [(148, 8200), (149, 8200), (300, 12288), (1184, 16384), (1185, 9000), (160, 16392), (150, 8192), (200, 8193), (500, 16377)])
+def test_rows_where_another_kernel_takes_over(tokens, k, dtype):
+    """Long rows: kept in registers in few or many threads, or read twice."""
+    x = T.activations(tokens, k, dtype)
+    rows = T.int8().quantize_rows(x)
+    q, s = T.plain_rows(x.float())
+    assert torch.equal(rows.values, q) and torch.equal(rows.scales, s)
