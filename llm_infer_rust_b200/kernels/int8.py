@@ -10,6 +10,9 @@ zeros has scale 0; a row that holds a NaN or an infinity has scale NaN, so all o
 Weights are kept in 8 bits (half the bytes that a decode step of bfloat16 weights reads, and the tensor cores' faster
 products for prompts); what a product reads of its activations is bfloat16 or float32, a ``PendingNorm`` (the residual add
 and the RMS norm in front of a block then run on the way to 8 bits), or rows that are in 8 bits already.
+
+A token's results are the same bits alone and among others, but for those behind a norm: there the row's scale has a float sum of
+squares whose order goes by the number of tokens (each such scale is within 2^-18 of the true one).
 """
 from __future__ import annotations
 
