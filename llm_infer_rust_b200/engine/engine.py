@@ -144,7 +144,8 @@ class Engine:
         ``keep_float32_tensors``: what a bfloat16 engine does with tensors stored in 32-bit (None: they stay float32
         in a checkpoint that declares itself 16-bit and are converted otherwise; see weights/loader.py).
         ``int8_projections``: the layers' attention and gated feed-forward projections are held and multiplied in 8-bit
-        integers, with a scale for each output channel and each token (see parts/int8.py for which have that form).
+        integers, with a scale for each output channel and each token (see parts/int8.py for which have that form; decode steps of
+        small models, whose bfloat16 layers run in fewer kernels, are slower so).
         ``log_level``: error, warn(ing), info, debug or trace, for the package's logger."""
         self.model_path = model_path
         self.log_level = log_level
