@@ -528,7 +528,7 @@ static int int8_rows_normed(const Int8RowsParams& P, int sms, cudaStream_t strea
   // their way; two chunks a thread keep them (behind a norm 8,192 x 4,096 38 us; four chunks, half the threads: a third slower), in up
   // to 1,024 threads (8,192 x 12,288 bfloat16 behind a norm 117 us, 6.0 TB/s; read twice, the second time out of the caches, 126;
   // without a norm, 160 / 300 / 600 / 1,184 rows of 12,288 2.7 / 3.8 / 6.0 / 9.0 us, read twice 4.0 / 4.6 / 6.7 / 10.1, of 16,384 3.2 / 4.9 / 7.3 /
-  // 10.7, read twice 5.0 / 6.1 / 8.6 / 12.8), but for float32 behind a norm, which is faster read twice (226 us, 254 kept), and for bfloat16 rows without
+  // 10.7, read twice 5.0 / 6.1 / 8.6 / 12.8), but for float32 behind a norm, which is faster read twice (600 / 8,192 rows of 12,288 24 / 206 us, kept 27 / 302), and for bfloat16 rows without
   // a norm that are not whole, which are where there are many of them or they are long (300 / 1,184 / 8,192 of 12,289 7.1 / 14.1 / 83.6 us, kept
   // 6.0 / 17.3 / 110.8; of 9,001 5.5 / 11.5 / 68.4, kept 3.5 / 9.8 / 61.0).
   if (P.tokens <= sms) {
