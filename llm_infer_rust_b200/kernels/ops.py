@@ -13,7 +13,7 @@ import ctypes
 import gc
 import os
 import sys
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -66,6 +66,12 @@ def _cuda(*tensors: Optional[torch.Tensor]) -> None:
 def _cuda_only(*tensors: Optional[torch.Tensor]) -> None:
     if not _all_cuda(*tensors):
         raise KernelError("the kernels run on CUDA tensors only; there is no CPU path")
+
+
+def _on_current(device: torch.device) -> None:
+    """Checks that a call's tensors are on the current device, whose stream it launches on."""
+    if device.index != _current_device():
+        raise KernelError(f"the tensors are on {device}, which is not the current device: use torch.cuda.device({device.index})")
 
 
 def _contig(*tensors: Optional[torch.Tensor]) -> None:
@@ -1617,6 +1623,46 @@ def sample(logits: torch.Tensor, params: torch.Tensor, uniforms: Optional[torch.
                                                       uniforms, error_word(logits.device), _stream())
     _ok(rc, "sample")
     return out
+
+
+class TokenLogprobs(NamedTuple):
+    """Of every row of logits: ``logprobs`` float32 [rows], the log probability of its given token (None: none was given);
+    ``entropy`` float32 [rows], in nats; ``top_ids`` int32 and ``top_logprobs`` float32 [rows, top], the most likely tokens."""
+    logprobs: Optional[torch.Tensor]
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+MAX_TOP_LOGPROBS = 32
+
+
+def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0) -> TokenLogprobs:
+    """Log probabilities under softmax(logits), float32 [rows, vocab] with any row stride: of ``tokens`` (int32, one a row) and of the
+    ``top`` (up to 32) most likely tokens, most likely first, equal ones by the lower id; and the entropy.
+
+    -inf is a token that cannot come.  A row that holds a NaN or +inf, or -inf alone, has NaN for all its numbers (its ids still go
+    by the logits that are no NaN; where those are too few they are -1).  A token outside the vocabulary has NaN and sets the
+    error word (``check_errors``)."""
+    _cuda(logits, tokens)
+    if logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
+        raise KernelError("token_logprobs takes float32 logits [rows, vocab] with unit inner stride")
+    rows, vocab = logits.shape
+    if not 0 <= top <= min(MAX_TOP_LOGPROBS, vocab):
+        raise KernelError(f"{top} alternatives are refused: 0 to {MAX_TOP_LOGPROBS}, and no more than there are logits in a row ({vocab})")
+    if tokens is not None and (tokens.dtype != torch.int32 or tokens.dim() != 1 or tokens.numel() != rows or not tokens.is_contiguous()):
+        raise KernelError("token_logprobs takes one int32 token a row")
+    if tokens is not None and tokens.device != logits.device:
+        raise KernelError("the tokens are on another device than the logits")
+    device = logits.device
+    _on_current(device)
+    chosen = None if tokens is None else _empty((rows,), torch.float32, device)
+    entropy = _empty((rows,), torch.float32, device)
+    ids, best = _empty((rows, top), torch.int32, device), _empty((rows, top), torch.float32, device)
+    rc = load_entry_points("logprobs.cu").b200_token_logprobs(logits, logits.stride(0) if rows > 1 else vocab, rows, vocab, tokens, top, chosen,
+                                                              entropy, ids, best, error_word(device), _stream())
+    _ok(rc, "token_logprobs", int(rows > 0))
+    return TokenLogprobs(chosen, entropy, ids, best)
 
 
 # --------------------------------------------------------------------------- float32 residual stream, one-gain norms
