@@ -82,3 +82,81 @@ struct PrefixItem {
   int begin, end, kvh, slot;
   bool shared;
 };
+
+// A vector's splits joined, a warp a vector: grid (vectors / MERGE_WARPS), blocks of MERGE_WARPS warps.  The splits' weights
+// 2^(m - max) stand in the lanes; a lane owns groups of four dims.  `pitch`: floats of a split's output (a multiple of 4).
+constexpr int MERGE_WARPS = 4;
+template <typename T, int PITCH>
+__global__ void __launch_bounds__(MERGE_WARPS * 32)
+prefix_merge_kernel(T* __restrict__ out, const PrefixCall c, int hd) {
+  constexpr int MOST = 128;                     // splits in all
+  const int lane = threadIdx.x & 31;
+  pdl_launch_dependents();
+  pdl_wait();
+  const long long vec = static_cast<long long>(blockIdx.x) * MERGE_WARPS + (threadIdx.x >> 5);
+  if (vec >= static_cast<long long>(c.n_rows) * c.nh) return;
+  const int splits = prefix_splits(c);
+  const float2* ml = c.part_ml + vec * splits;
+  const float* acc = c.part_acc + vec * splits * PITCH;
+  float2 mine[MOST / 32];
+  float m = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < MOST / 32; ++k) {
+    mine[k] = make_float2(-INFINITY, 0.0f);
+    if (k * 32 + lane < splits) mine[k] = ml[k * 32 + lane];
+    m = fmaxf(m, mine[k].x);
+  }
+  m = warp_max(m);
+  float l = 0.0f, f[MOST / 32];
+#pragma unroll
+  for (int k = 0; k < MOST / 32; ++k) {
+    f[k] = mine[k].x == -INFINITY ? 0.0f : exp2f(mine[k].x - m);
+    l = fmaf(mine[k].y, f[k], l);
+  }
+  l = warp_sum(l);
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  const int row = static_cast<int>(vec / c.nh), head = static_cast<int>(vec % c.nh);
+  T* dst = out + (static_cast<long long>(c.cu_q[c.rows[row]]) * c.nh + head) * hd;
+  constexpr int PER = (PITCH + 127) / 128;
+  float4 o[PER];
+#pragma unroll
+  for (int n = 0; n < PER; ++n) o[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+  for (int k = 0; k < MOST / 32; ++k) {
+    const int some = min(32, splits - 32 * k);
+#pragma unroll 4
+    for (int s = 0; s < some; ++s) {
+      const float w = __shfl_sync(0xffffffffu, f[k], s);
+      if (w == 0.0f) continue;                  // (nothing was written where a split saw no key)
+      const float* src = acc + static_cast<long long>(32 * k + s) * PITCH;
+#pragma unroll
+      for (int n = 0; n < PER; ++n) {
+        const int dim = n * 128 + lane * 4;
+        if (PITCH % 128 == 0 || dim < PITCH) {
+          const float4 a = __ldcg(reinterpret_cast<const float4*>(src + dim));
+          o[n].x = fmaf(w, a.x, o[n].x);
+          o[n].y = fmaf(w, a.y, o[n].y);
+          o[n].z = fmaf(w, a.z, o[n].z);
+          o[n].w = fmaf(w, a.w, o[n].w);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < PER; ++n) {
+    const int dim = n * 128 + lane * 4;
+    const float y[4] = {o[n].x * inv, o[n].y * inv, o[n].z * inv, o[n].w * inv};
+#pragma unroll
+    for (int e = 0; e < 4; e += 2)              // (head sizes are even)
+      if (dim + e < hd) {
+        dst[dim + e] = from_f32<T>(y[e]);
+        dst[dim + e + 1] = from_f32<T>(y[e + 1]);
+      }
+  }
+}
+template <typename T, int PITCH>
+static inline int prefix_merge(void* out, const PrefixCall& c, int hd, cudaStream_t stream) {
+  const long long vectors = static_cast<long long>(c.n_rows) * c.nh;
+  return b200_launch(prefix_merge_kernel<T, PITCH>, dim3(static_cast<unsigned>((vectors + MERGE_WARPS - 1) / MERGE_WARPS)), dim3(MERGE_WARPS * 32), 0,
+                     stream, 0, static_cast<T*>(out), c, hd);
+}

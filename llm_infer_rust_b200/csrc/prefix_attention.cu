@@ -266,27 +266,6 @@ prefix_any_kernel(const T* __restrict__ q, const T* __restrict__ kc, const T* __
   attend<T>(q, kc, vc, c, it, hd, wide, sm);
 }
 
-// grid (n_rows, nh): a vector's splits joined.
-template <typename T>
-__global__ void prefix_merge_kernel(T* __restrict__ out, const PrefixCall c, int hd) {
-  const int splits = prefix_splits(c);
-  const long long base = (static_cast<long long>(blockIdx.x) * c.nh + blockIdx.y) * splits;
-  float m = -INFINITY;
-  for (int s = 0; s < splits; ++s) m = fmaxf(m, c.part_ml[base + s].x);
-  T* dst = out + (static_cast<long long>(c.cu_q[c.rows[blockIdx.x]]) * c.nh + blockIdx.y) * hd;
-  for (int dim = threadIdx.x; dim < hd; dim += blockDim.x) {
-    float l = 0.0f, o = 0.0f;
-    for (int s = 0; s < splits; ++s) {
-      const float2 ml = c.part_ml[base + s];
-      if (ml.x == -INFINITY) continue;
-      const float f = fast_exp2(ml.x - m);
-      l += ml.y * f;
-      o += c.part_acc[(base + s) * D + dim] * f;
-    }
-    dst[dim] = from_f32<T>(l > 0.0f ? o / l : 0.0f);
-  }
-}
-
 template <typename T>
 static int launch(const void* q, const void* kc, const void* vc, void* out, const PrefixCall& c, int hd, cudaStream_t stream) {
   static bool seen[16];
@@ -300,8 +279,7 @@ static int launch(const void* q, const void* kc, const void* vc, void* out, cons
   prefix_any_kernel<T><<<static_cast<unsigned>(ctas), THREADS, SMEM, stream>>>(static_cast<const T*>(q), static_cast<const T*>(kc), static_cast<const T*>(vc), c, hd, wide);
   rc = b200_check_launch();
   if (rc != 0) return rc;
-  prefix_merge_kernel<T><<<dim3(c.n_rows, c.nh), hd >= 128 ? 128 : hd >= 64 ? 64 : 32, 0, stream>>>(static_cast<T*>(out), c, hd);
-  return b200_check_launch();
+  return prefix_merge<T, D>(out, c, hd, stream);
 }
 
 B200_EXPORT int b200_prefix_attention_smem() { return SMEM; }

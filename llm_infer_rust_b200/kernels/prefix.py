@@ -17,11 +17,19 @@ from .build import load_entry_points
 from .ops import KernelError
 
 _TILE = 32                    # query vectors of a CTA of the all-sizes kernel
+_MMA_TILE = {False: 32, True: 16}   # of the mma.sync kernel, by whether a head is wider than 128
+_TC_VECTORS = 128             # of a tile of the tcgen05 kernel; a CTA takes one or two
 _KEYS_PER_CTA_AT_LEAST = 64
+_MOST_SPLITS = 64             # of the shared keys, and of the own ones
 
 
 def _lib(head_dim: int):
     return load_entry_points("prefix_attention.cu", {"HEAD_DIM": ops.padded_head_dim(head_dim)})
+
+
+def _on_tcgen05(head_dim: int, vectors: int, most_shared: int) -> bool:
+    """Whether a group's shared keys go to the tcgen05 kernel (``vectors``: its query vectors of a KV head)."""
+    return head_dim == 128 and vectors > 32 and most_shared >= 256
 
 
 def _split(most_shared: int, most_own: int, shared_ctas: int, own_ctas: int, room: int, least: int) -> tuple:
@@ -71,13 +79,40 @@ def prefix_attention(q, k_cache, v_cache, out, block_table, cu_q, kv_len, rows, 
     per = num_heads // num_kv_heads
     most_rows = max(1, min(most_rows, n_rows))
     lib = _lib(head_dim)
-    tiles = -(-most_rows * per // _TILE)
-    per_sm = max(1, 227 * 1024 // (lib.b200_prefix_attention_smem() + 1024))
-    shared, own = _split(most_shared, most_own, n_groups * num_kv_heads * tiles, n_rows * num_kv_heads * -(-per // _TILE),
-                         per_sm * ops._sm_count(q.device), _KEYS_PER_CTA_AT_LEAST)
-    # the splits' parts, between the two kernels of the call
-    scratch = ops._empty((n_rows * num_heads * (shared + own) * (ops.padded_head_dim(head_dim) + 2),), torch.float32, q.device)
-    rc = lib.b200_prefix_attention(q, k_cache, v_cache, out, scratch, block_table, block_table.shape[1], cu_q, kv_len, rows, n_rows, groups, n_groups,
-                                   num_heads, num_kv_heads, page_size, k_cache.shape[0], float(scale), shared, own, tiles, code, head_dim,
-                                   ops.error_word(q.device), ops._stream())
-    ops._ok(rc, "prefix_attention", 2)
+    # (the splits' parts stand between the kernels of the call, in memory of the call's own)
+    err, stream, sms = ops.error_word(q.device), ops._stream(), ops._sm_count(q.device)
+    common = (block_table, block_table.shape[1], cu_q, kv_len, rows, n_rows, groups, n_groups, num_heads, num_kv_heads, page_size,
+              k_cache.shape[0], float(scale))
+
+    def parts(splits):
+        return ops._empty((n_rows * num_heads * splits * (ops.padded_head_dim(head_dim) + 2),), torch.float32, q.device)
+
+    if not ops.decode_uses_tensor_cores(q.dtype, num_heads, num_kv_heads, head_dim, page_size) or q.data_ptr() % 16:
+        lib = _lib(head_dim)
+        tiles = -(-most_rows * per // _TILE)
+        per_sm = max(1, 227 * 1024 // (lib.b200_prefix_attention_smem() + 1024))
+        shared, own = _split(most_shared, most_own, n_groups * num_kv_heads * tiles, n_rows * num_kv_heads * -(-per // _TILE), per_sm * sms,
+                             _KEYS_PER_CTA_AT_LEAST)
+        rc = lib.b200_prefix_attention(q, k_cache, v_cache, out, parts(shared + own), *common, shared, own, tiles, code, head_dim, err, stream)
+        ops._ok(rc, "prefix_attention", 2)
+        return
+    box_rows = min(page_size, 32)
+    kmap, vmap = ops.kv_tensor_map(k_cache, box_rows), ops.kv_tensor_map(v_cache, box_rows)
+    lib = load_entry_points("prefix_mma.cu", {"HEAD_DIM": head_dim})
+    own_ctas = n_rows * num_kv_heads
+    if n_groups and _on_tcgen05(head_dim, most_rows * per, most_shared):
+        two = most_rows * per > _TC_VECTORS
+        tiles = -(-most_rows * per // (2 * _TC_VECTORS if two else _TC_VECTORS))
+        ctas = max(1, min(-(-most_shared // (128 if two else 256)), sms // (n_groups * num_kv_heads * tiles), _MOST_SPLITS if two else _MOST_SPLITS // 2))
+        shared = ctas if two else 2 * ctas
+        own = _split(0, most_own, 0, own_ctas, sms, _KEYS_PER_CTA_AT_LEAST)[1]
+        scratch = parts(shared + own)
+        rc = load_entry_points("prefix_tcgen05.cu").b200_prefix_tcgen05(q, kmap, vmap, scratch, *common, shared, own, tiles, int(two), err, stream)
+        ops._ok(rc, "prefix_tcgen05")
+        covered, tiles = tiles * (2 * _TC_VECTORS if two else _TC_VECTORS), 1
+    else:
+        covered, tiles = 0, -(-most_rows * per // _MMA_TILE[head_dim > 128])
+        shared, own = _split(most_shared, most_own, n_groups * num_kv_heads * tiles, own_ctas, sms, _KEYS_PER_CTA_AT_LEAST)
+        scratch = parts(shared + own)
+    rc = lib.b200_prefix_attention_mma(q, kmap, vmap, out, scratch, *common, shared, own, tiles, covered, err, stream)
+    ops._ok(rc, "prefix_attention_mma", 2)
