@@ -11,6 +11,7 @@
 //                                       of its own, and the rings are a stage of keys deeper.
 // Bound by the special-function unit and the products from about 128 vectors on, by the copies below.
 #include "attention_tcgen05.cuh"
+#include "kv_map.cuh"
 #include "prefix.cuh"
 
 constexpr int COPY_WARPS = 2;
@@ -253,30 +254,32 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
 // Vectors of a group that a CTA takes: `two` tiles or one.
 B200_EXPORT int b200_prefix_tcgen05_vectors(int two) { return two != 0 ? 2 * BQ : BQ; }
 
-// The first `tiles` tiles of every group's vectors against its shared keys, in `ctas` CTAs a tile and KV head, whose parts go to slots
-// 0 .. splits_shared - 1 (splits_shared = ctas, or 2 ctas with one tile a CTA).  The kernel of b200_prefix_attention_mma follows.
-// Other arguments as there.
-B200_EXPORT int b200_prefix_tcgen05(const void* q, const void* k_map, const void* v_map, float* scratch, const int* block_table, int table_stride,
+// The first `tiles` tiles (of one or `two` times 128) of every group's vectors against its shared keys, whose parts go to slots
+// 0 .. splits_shared - 1 of [n_rows * nh][splits_shared], at the start of `scratch` (splits_shared is the number of CTAs, or with one
+// tile a CTA twice that).  The kernels of b200_prefix_attention_mma follow.  Other arguments as there.
+B200_EXPORT int b200_prefix_tcgen05(const void* q, const void* k_cache, const void* v_cache, float* scratch, const int* block_table, int table_stride,
                                     const int* cu_q, const int* kv_len, const int* rows, int n_rows, const int* groups, int n_groups, int nh, int nkv,
-                                    int page_size, int pages, float scale, int splits_shared, int splits_own, int tiles, int two, int* err,
+                                    int page_size, int pages, float scale, int splits_shared, int tiles, int two, int* err,
                                     cudaStream_t stream) {
   if (n_rows <= 0 || n_groups <= 0) return 0;
   if (nh <= 0 || nkv <= 0 || nkv > 65535 || nh % nkv != 0 || page_size <= 0 || (page_size & (page_size - 1)) != 0 || pages <= 0 || table_stride <= 0) return B200_BAD_SIZE;
-  if (splits_shared < 1 || splits_own < 1 || splits_shared + splits_own > 128 || tiles < 1 || (two == 0 && splits_shared % 2 != 0) ||
+  if (splits_shared < 1 || tiles < 1 || (two == 0 && splits_shared % 2 != 0) ||
       static_cast<long long>(n_groups) * tiles > 65535)
     return B200_BAD_SIZE;
   if (!(scale > 0.0f)) return B200_BAD_SIZE;                         // maxima and masks are taken of the unscaled scores
   if (reinterpret_cast<uintptr_t>(q) % 16 != 0) return B200_BAD_ALIGN;
   const PrefixCall c = {block_table, cu_q, kv_len, rows, reinterpret_cast<const int2*>(groups), scratch,
-                        reinterpret_cast<float2*>(scratch + static_cast<size_t>(n_rows) * nh * (splits_shared + splits_own) * D), err, table_stride, n_rows,
-                        n_groups, nh, nkv, page_size, pages, splits_shared, splits_own, tiles, scale * 1.4426950408889634f};
+                        reinterpret_cast<float2*>(scratch + static_cast<size_t>(n_rows) * nh * splits_shared * D), err, table_stride, n_rows,
+                        n_groups, nh, nkv, page_size, pages, splits_shared, 0, tiles, scale * 1.4426950408889634f};
   static bool seen[2][16];
   auto* kernel = two != 0 ? prefix_tcgen05_kernel<true> : prefix_tcgen05_kernel<false>;
-  const int rc = prefix_smem_limit(kernel, SMEM, seen[two != 0]);
-  if (rc != 0) return rc;
   CUtensorMap kmap, vmap;
-  memcpy(&kmap, k_map, sizeof(kmap));
-  memcpy(&vmap, v_map, sizeof(vmap));
+  const int box_rows = page_size < 32 ? page_size : 32;
+  const long long lines = static_cast<long long>(pages) * nkv * page_size;
+  int rc = make_kv_tensor_map(&kmap, k_cache, lines, D, box_rows);
+  if (rc == 0) rc = make_kv_tensor_map(&vmap, v_cache, lines, D, box_rows);
+  if (rc == 0) rc = prefix_smem_limit(kernel, SMEM, seen[two != 0]);
+  if (rc != 0) return rc;
   return b200_launch(kernel, dim3(two != 0 ? splits_shared : splits_shared / 2, nkv, n_groups * tiles), dim3(THREADS), SMEM, stream, 0, kmap, vmap,
-                     static_cast<const bf16*>(q), c, page_size < 32 ? page_size : 32);
+                     static_cast<const bf16*>(q), c, box_rows);
 }

@@ -10,6 +10,8 @@ with keys below the group's ``shared`` read through the block table of the group
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import ops
@@ -17,10 +19,10 @@ from .build import load_entry_points
 from .ops import KernelError
 
 _TILE = 32                    # query vectors of a CTA of the all-sizes kernel
-_MMA_TILE = {False: 32, True: 16}   # of the mma.sync kernel, by whether a head is wider than 128
 _TC_VECTORS = 128             # of a tile of the tcgen05 kernel; a CTA takes one or two
 _KEYS_PER_CTA_AT_LEAST = 64
-_MOST_SPLITS = 64             # of the shared keys, and of the own ones
+_MOST_SPLITS = 64             # of the shared keys
+_MOST_ENTRIES = 400           # rows and groups of a call that the tensor-core kernels take
 
 
 def _lib(head_dim: int):
@@ -84,35 +86,30 @@ def prefix_attention(q, k_cache, v_cache, out, block_table, cu_q, kv_len, rows, 
     common = (block_table, block_table.shape[1], cu_q, kv_len, rows, n_rows, groups, n_groups, num_heads, num_kv_heads, page_size,
               k_cache.shape[0], float(scale))
 
-    def parts(splits):
-        return ops._empty((n_rows * num_heads * splits * (ops.padded_head_dim(head_dim) + 2),), torch.float32, q.device)
-
-    if not ops.decode_uses_tensor_cores(q.dtype, num_heads, num_kv_heads, head_dim, page_size) or q.data_ptr() % 16:
+    if not ops.decode_uses_tensor_cores(q.dtype, num_heads, num_kv_heads, head_dim, page_size) or (q.data_ptr() | out.data_ptr()) % 16 \
+            or n_rows + n_groups > _MOST_ENTRIES:
         lib = _lib(head_dim)
         tiles = -(-most_rows * per // _TILE)
         per_sm = max(1, 227 * 1024 // (lib.b200_prefix_attention_smem() + 1024))
         shared, own = _split(most_shared, most_own, n_groups * num_kv_heads * tiles, n_rows * num_kv_heads * -(-per // _TILE), per_sm * sms,
                              _KEYS_PER_CTA_AT_LEAST)
-        rc = lib.b200_prefix_attention(q, k_cache, v_cache, out, parts(shared + own), *common, shared, own, tiles, code, head_dim, err, stream)
+        scratch = ops._empty((n_rows * num_heads * (shared + own) * (ops.padded_head_dim(head_dim) + 2),), torch.float32, q.device)
+        rc = lib.b200_prefix_attention(q, k_cache, v_cache, out, scratch, *common, shared, own, tiles, code, head_dim, err, stream)
         ops._ok(rc, "prefix_attention", 2)
         return
-    box_rows = min(page_size, 32)
-    kmap, vmap = ops.kv_tensor_map(k_cache, box_rows), ops.kv_tensor_map(v_cache, box_rows)
     lib = load_entry_points("prefix_mma.cu", {"HEAD_DIM": head_dim})
-    own_ctas = n_rows * num_kv_heads
+    covered = shared = 0
     if n_groups and _on_tcgen05(head_dim, most_rows * per, most_shared):
         two = most_rows * per > _TC_VECTORS
-        tiles = -(-most_rows * per // (2 * _TC_VECTORS if two else _TC_VECTORS))
+        covered = _TC_VECTORS * (2 if two else 1)
+        tiles = -(-most_rows * per // covered)
         ctas = max(1, min(-(-most_shared // (128 if two else 256)), sms // (n_groups * num_kv_heads * tiles), _MOST_SPLITS if two else _MOST_SPLITS // 2))
-        shared = ctas if two else 2 * ctas
-        own = _split(0, most_own, 0, own_ctas, sms, _KEYS_PER_CTA_AT_LEAST)[1]
-        scratch = parts(shared + own)
-        rc = load_entry_points("prefix_tcgen05.cu").b200_prefix_tcgen05(q, kmap, vmap, scratch, *common, shared, own, tiles, int(two), err, stream)
+        shared, covered = ctas * (1 if two else 2), covered * tiles
+    floats = lib.library.b200_prefix_scratch_floats
+    floats.restype = ctypes.c_longlong
+    scratch = ops._empty((floats(n_rows, n_groups, num_heads, num_kv_heads, shared, sms),), torch.float32, q.device)
+    if covered:
+        rc = load_entry_points("prefix_tcgen05.cu").b200_prefix_tcgen05(q, k_cache, v_cache, scratch, *common, shared, tiles, int(two), err, stream)
         ops._ok(rc, "prefix_tcgen05")
-        covered, tiles = tiles * (2 * _TC_VECTORS if two else _TC_VECTORS), 1
-    else:
-        covered, tiles = 0, -(-most_rows * per // _MMA_TILE[head_dim > 128])
-        shared, own = _split(most_shared, most_own, n_groups * num_kv_heads * tiles, own_ctas, sms, _KEYS_PER_CTA_AT_LEAST)
-        scratch = parts(shared + own)
-    rc = lib.b200_prefix_attention_mma(q, kmap, vmap, out, scratch, *common, shared, own, tiles, covered, err, stream)
+    rc = lib.b200_prefix_attention_mma(q, k_cache, v_cache, out, scratch, *common, shared, covered, sms, err, stream)
     ops._ok(rc, "prefix_attention_mma", 2)
