@@ -24,48 +24,178 @@ constexpr int THREADS = WARPS * 32;
 constexpr int MOST_ENTRIES = 400;                // rows and groups of a call, whose places in the sequence stand in shared memory
 constexpr size_t RING = static_cast<size_t>(WARPS) * STAGES * TILE_BYTES;
 constexpr size_t QUERIES = static_cast<size_t>(WARPS) * VT * LD * sizeof(bf16);
+constexpr size_t FIXED = 1024 + RING + QUERIES + WARPS * STAGES * 8;
 
-// A group's or a row's place in the sequence of blocks (of one KV head).
+// The places of a call's groups, then rows, in the sequence of blocks (of one KV head), in shared memory.
 struct Entries {
-  int start[MOST_ENTRIES + 1];                   // its first block
-  int keys[MOST_ENTRIES];                        // a group's shared keys, a row's keys
-  int low[MOST_ENTRIES];                         // a group's first row; a row's first own key
-  int where[MOST_ENTRIES];                       // the tiles of the groups before; a row's place in the block table
-  int token[MOST_ENTRIES];                       // a row's token
-  int sums[WARPS + 1];
+  int* start;                                    // [entries + 1]: the first block
+  int* keys;                                     // a group's shared keys, a row's keys
+  int* low;                                      // a group's first row; a row's first own key
+  int* where;                                    // the tiles of the groups before; a row's place in the block table
+  int* token;                                    // a row's token
+  int blocks, items, group_tiles;                // in all (of one KV head)
 };
-constexpr size_t SMEM = 1024 + RING + QUERIES + sizeof(Entries) + WARPS * STAGES * 8;
-static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
-
-// What the joining kernel has to know of the sequence (in device memory, written by the first CTA).
-struct Sequence {
-  int blocks;                                    // of one KV head
-  int items;                                     // of one KV head
-  int workers;
-  int group_tiles;                               // of all groups
-  int start[MOST_ENTRIES + 1];
-  int tiles_before[MOST_ENTRIES];
-};
+__host__ __device__ constexpr int entries_bytes(int n_entries) { return (5 * n_entries + 1 + 8) * 4; }
+static_assert(WARPS <= 8, "a sum a warp");
+static_assert(FIXED + entries_bytes(MOST_ENTRIES) <= 227 * 1024, "shared memory of one CTA");
 
 struct StreamCall {
   PrefixCall c;                                  // part_acc, part_ml: of the tcgen05 kernel, [n_rows * nh][splits_shared]
   float* acc;                                    // [parts][16][D]
   float2* ml;                                    // [parts][16]
-  Sequence* sequence;
   int covered;                                   // vectors of each group that the tcgen05 kernel serves
 };
 
 __device__ __forceinline__ int tiles_of(const StreamCall& k, int rows, int group) { return (max(0, rows * group - k.covered) + VT - 1) / VT; }
 
-// The stretch that block s of the whole sequence is in: stretch w begins at block floor(w total / workers).
-__device__ __forceinline__ int worker_of(long long s, long long total, int workers) { return static_cast<int>(((s + 1) * workers - 1) / total); }
+// Sums of `v` over the CTA's threads before this one; `sum` becomes that of all.  `sh`: one int a warp.
+template <int WARPS_HERE>
+__device__ __forceinline__ int sums_before(int v, int& sum, int* sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int upto = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int less = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += less;
+  }
+  if (lane == 31) sh[warp] = upto;
+  __syncthreads();
+  int before = 0;
+  sum = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS_HERE; ++w) {
+    if (w == warp) before = sum;
+    sum += sh[w];
+  }
+  __syncthreads();
+  return before + upto - v;
+}
+
+// Fills in `at` (a whole CTA).  What the kernels wait for here is two loads one behind the other, a row's number and its length.
+template <int WARPS_HERE>
+__device__ __forceinline__ void lay_out(const StreamCall& k, Entries& at, int* memory) {
+  constexpr int N = WARPS_HERE * 32;
+  const PrefixCall& c = k.c;
+  const int n_entries = c.n_groups + c.n_rows, group = c.nh / c.nkv;
+  at.start = memory;
+  at.keys = at.start + n_entries + 1;
+  at.low = at.keys + n_entries;
+  at.where = at.low + n_entries;
+  at.token = at.where + n_entries;
+  int* sh = at.token + n_entries;
+  const int most = static_cast<int>(min(static_cast<long long>(c.table_stride) * c.page_size, static_cast<long long>(INT_MAX)));
+  auto checked = [&](int keys) {                   // no more keys than a block table has places for
+    if (keys > most) atomicOr(c.err, B200_ERR_SLOT_RANGE);
+    return min(max(keys, 0), most);
+  };
+  for (int x = threadIdx.x; x < max(c.n_groups, c.n_rows); x += N) {
+    const bool is_row = x < c.n_rows, is_group = x < c.n_groups;
+    const int row = is_row ? c.rows[x] : 0;
+    const int2 here = is_group ? c.groups[x] : make_int2(0, 0);
+    const int behind = is_group && x + 1 < c.n_groups ? c.groups[x + 1].x : c.n_rows;
+    const int keys = is_row ? c.kv_len[row] : 0, token = is_row ? c.cu_q[row] : 0;
+    if (is_group) {
+      const int first = min(max(here.x, 0), c.n_rows), rows = min(max(behind, first), c.n_rows) - first;
+      at.keys[x] = rows > 0 ? checked(here.y) : 0;
+      at.low[x] = first;
+      at.where[x] = tiles_of(k, rows, group);
+    }
+    if (is_row) {
+      at.where[c.n_groups + x] = row;
+      at.keys[c.n_groups + x] = checked(keys);
+      at.token[c.n_groups + x] = token;
+    }
+  }
+  __syncthreads();
+  at.blocks = at.group_tiles = 0;
+  for (int e0 = 0; e0 < n_entries; e0 += N) {
+    const int e = e0 + static_cast<int>(threadIdx.x);
+    int v = 0, tiles = 0;
+    if (e < c.n_groups) {
+      tiles = at.where[e];
+      v = tiles * ((at.keys[e] + KB - 1) / KB);
+    } else if (e < n_entries) {
+      int lo = 0, hi = c.n_groups;                 // the groups that begin at or before the row: it is the last one's
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (at.low[mid] <= e - c.n_groups) lo = mid + 1; else hi = mid;
+      }
+      const int keys = at.keys[e], low = lo == 0 ? 0 : min(keys, at.keys[lo - 1]);
+      at.low[e] = low;
+      v = keys > low ? (keys + KB - 1) / KB - low / KB : 0;
+    }
+    int sum, before = sums_before<WARPS_HERE>(v, sum, sh);
+    if (e < n_entries) at.start[e] = at.blocks + before;
+    at.blocks += sum;
+    if (e0 < c.n_groups) {
+      before = sums_before<WARPS_HERE>(tiles, sum, sh);
+      if (e < c.n_groups) at.where[e] = at.group_tiles + before;
+      at.group_tiles += sum;
+    }
+  }
+  if (threadIdx.x == 0) at.start[n_entries] = at.blocks;
+  at.items = at.group_tiles + c.n_rows;
+  __syncthreads();
+}
+
+// The sequence of all KV heads' blocks in equal stretches, the first `longer` of them one block longer.
+struct Stretches {
+  int workers, blocks, longer;
+  __device__ __forceinline__ Stretches(int total, int most) {
+    workers = max(1, min(total, most));
+    blocks = total / workers;
+    longer = total - blocks * workers;
+  }
+  __device__ __forceinline__ int begin(int w) const { return w * blocks + min(w, longer); }
+  __device__ __forceinline__ int of(int s) const {
+    const int edge = longer * (blocks + 1);
+    return s < edge ? s / (blocks + 1) : longer + (s - edge) / blocks;
+  }
+};
 
 // Where a worker stands: `left` blocks of an item from key first_key on.
 struct Place {
-  long long s;
-  int kvh, first_key, end, lowest, left, item, i0, vector0, vectors, table_row;
-  bool shared;
+  int s, kvh, first_key, end, lowest, left, item, i0, vector0, vectors, table_row;
 };
+// (not inlined: it is asked in three places, and a kernel this short waits for its instructions)
+__device__ __noinline__ Place locate(const Entries& at, int s, int s_end, int n_groups, int n_rows, int group, int covered) {
+  Place p;
+  p.s = s;
+  p.kvh = s / at.blocks;
+  const int pos = s - p.kvh * at.blocks, lane = threadIdx.x & 31;
+  int e = -1;                                      // the entries that begin at or before pos: the last of them holds it
+  for (int e0 = 0; e0 < n_groups + n_rows; e0 += 32) {
+    const unsigned begun = __ballot_sync(0xffffffffu, e0 + lane < n_groups + n_rows && at.start[e0 + lane] <= pos);
+    e += __popc(begun);
+    if (begun != 0xffffffffu) break;
+  }
+  int block = pos - at.start[e], of;
+  p.end = at.keys[e];
+  if (e < n_groups) {
+    of = (p.end + KB - 1) / KB;
+    const int tile = block / of;
+    block -= tile * of;
+    p.item = p.kvh * at.items + at.where[e] + tile;
+    p.lowest = 0;
+    p.i0 = at.low[e];
+    const int next = e + 1 < n_groups ? max(at.low[e + 1], p.i0) : n_rows;
+    p.vector0 = covered + tile * VT;
+    p.vectors = min(VT, (next - p.i0) * group - p.vector0);
+    p.table_row = at.where[n_groups + p.i0];
+    p.first_key = block * KB;
+  } else {
+    p.lowest = at.low[e];
+    of = (p.end + KB - 1) / KB - p.lowest / KB;
+    p.i0 = e - n_groups;
+    p.item = p.kvh * at.items + at.group_tiles + p.i0;
+    p.vector0 = 0;
+    p.vectors = group;
+    p.table_row = at.where[e];
+    p.first_key = (p.lowest / KB + block) * KB;
+  }
+  p.left = min(of - block, s_end - s);
+  return p;
+}
 
 // The page of this lane's sub-block, inside the pool (the sink's where the table names none that is, or where the sub-block ends
 // below `lowest`: those keys are another table's).
@@ -80,9 +210,9 @@ __device__ __forceinline__ int lane_page_checked(const PrefixCall& c, const Plac
 
 // One block of 32 keys against the 16 vectors whose queries are `qa` (or stand at `qs`): as block_mma of attention_mma.cuh, with the
 // last key that a vector sees (last0, last1: of rows lane / 4 and lane / 4 + 8; -1: none) and the item's first.
-template <bool MASKED>
 __device__ __forceinline__ void item_block(const uint32_t (&qa)[kQueriesInRegisters ? D / 16 : 1][4], const bf16* qs, const unsigned char* ks,
-                                           const unsigned char* vs, int first_key, int lowest, int last0, int last1, float scale_log2, WarpAcc& st) {
+                                           const unsigned char* vs, bool masked, int first_key, int lowest, int last0, int last1, float scale_log2,
+                                           WarpAcc& st) {
   const int lane = threadIdx.x & 31;
   const int mi = lane >> 3, r8 = lane & 7;
   float s[4][4];
@@ -107,25 +237,25 @@ __device__ __forceinline__ void item_block(const uint32_t (&qa)[kQueriesInRegist
   }
   const int t2 = (lane & 3) * 2;
   float mx0 = -INFINITY, mx1 = -INFINITY;
+  if (masked) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int key = first_key + n * 8 + t2 + e;
+        s[n][e] = key >= lowest && key <= last0 ? s[n][e] : -INFINITY;
+        s[n][2 + e] = key >= lowest && key <= last1 ? s[n][2 + e] : -INFINITY;
+      }
+    }
+  }
 #pragma unroll
   for (int n = 0; n < 4; ++n) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      if (MASKED) {
-        const int key = first_key + n * 8 + t2 + e;
-        s[n][e] = key >= lowest && key <= last0 ? s[n][e] * scale_log2 : -INFINITY;
-        s[n][2 + e] = key >= lowest && key <= last1 ? s[n][2 + e] * scale_log2 : -INFINITY;
-      } else {
-        s[n][e] *= scale_log2;
-        s[n][2 + e] *= scale_log2;
-      }
-      mx0 = fmaxf(mx0, s[n][e]);
-      mx1 = fmaxf(mx1, s[n][2 + e]);
-    }
+    mx0 = fmaxf(mx0, fmaxf(s[n][0], s[n][1]));
+    mx1 = fmaxf(mx1, fmaxf(s[n][2], s[n][3]));
   }
   mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1)); mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
   mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1)); mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-  const float m0 = fmaxf(st.m[0], mx0), m1 = fmaxf(st.m[1], mx1);
+  const float m0 = fmaxf(st.m[0], mx0 * scale_log2), m1 = fmaxf(st.m[1], mx1 * scale_log2);      // (the scale is positive)
   const float base0 = m0 == -INFINITY ? 0.0f : m0, base1 = m1 == -INFINITY ? 0.0f : m1;
   const float c0 = fast_exp2(st.m[0] - base0), c1 = fast_exp2(st.m[1] - base1);       // (0 on the first visible block)
   float sum0 = 0.0f, sum1 = 0.0f;
@@ -133,8 +263,8 @@ __device__ __forceinline__ void item_block(const uint32_t (&qa)[kQueriesInRegist
   for (int n = 0; n < 4; ++n) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      s[n][e] = fast_exp2(s[n][e] - base0);
-      s[n][2 + e] = fast_exp2(s[n][2 + e] - base1);
+      s[n][e] = fast_exp2(fmaf(s[n][e], scale_log2, -base0));
+      s[n][2 + e] = fast_exp2(fmaf(s[n][2 + e], scale_log2, -base1));
       sum0 += s[n][e];
       sum1 += s[n][2 + e];
     }
@@ -169,228 +299,101 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   bf16* queries = reinterpret_cast<bf16*>(tiles + RING);
   uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<unsigned char*>(queries) + QUERIES);      // [WARPS][STAGES]
-  Entries& at = *reinterpret_cast<Entries*>(bars + WARPS * STAGES);
   const PrefixCall& c = k.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x < WARPS * STAGES) mbar_init(bars + threadIdx.x, 1);
   asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   // Behind the tcgen05 kernel of the same call, which has waited for the kernels before it, this one begins beside it, and waits
-  // for its end at its own: whoever waits for this kernel then waits for both.
-  pdl_launch_dependents();
+  // for its end at its own: whoever waits for this kernel then waits for both.  The joining kernel may come as soon as what was
+  // launched before the call has ended.
   if (k.covered == 0) pdl_wait();
+  pdl_launch_dependents();
+  Entries at;
+  lay_out<WARPS>(k, at, reinterpret_cast<int*>(bars + WARPS * STAGES));
 
-  // ---- the sequence: groups, then rows
   const int group = c.nh / c.nkv;
-  const int n_entries = c.n_groups + c.n_rows;
-  for (int g = threadIdx.x; g < c.n_groups; g += THREADS) {
-    const int2 rows = rows_of_group(c, g);
-    at.keys[g] = rows.y > 0 ? shared_of_group(c, g) : 0;
-    at.low[g] = rows.x;
-    at.where[g] = tiles_of(k, rows.y, group);
-  }
-  for (int i = threadIdx.x; i < c.n_rows; i += THREADS) {
-    const int e = c.n_groups + i, row = c.rows[i];
-    at.where[e] = row;
-    at.keys[e] = keys_of_row(c, row);
-    at.token[e] = c.cu_q[row];
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < c.n_rows; i += THREADS) {
-    int lo = 0, hi = c.n_groups;                   // the groups that begin at or before row i
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (at.low[mid] <= i) lo = mid + 1; else hi = mid;
-    }
-    // (groups that begin at one row: the last of them has it)
-    at.low[c.n_groups + i] = lo == 0 ? 0 : min(at.keys[c.n_groups + i], at.keys[lo - 1]);
-  }
-  __syncthreads();
-  auto blocks_of = [&](int e) {
-    if (e < c.n_groups) return at.where[e] * ((at.keys[e] + KB - 1) / KB);
-    return at.keys[e] > at.low[e] ? (at.keys[e] + KB - 1) / KB - at.low[e] / KB : 0;
-  };
-  // exclusive sums: a thread's own stretch of the entries, then the warps', then the CTA's
-  const int each = (n_entries + THREADS - 1) / THREADS, e0 = min(n_entries, static_cast<int>(threadIdx.x) * each), e1 = min(n_entries, e0 + each);
-  int mine = 0;
-  for (int e = e0; e < e1; ++e) mine += blocks_of(e);
-  int upto = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int before = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += before;
-  }
-  if (lane == 31) at.sums[warp] = upto;
-  __syncthreads();
-  int sum = upto - mine;
-  for (int w = 0; w < warp; ++w) sum += at.sums[w];
-  for (int e = e0; e < e1; ++e) {
-    at.start[e] = sum;
-    sum += blocks_of(e);
-  }
-  if (e0 < n_entries && e1 == n_entries) at.start[n_entries] = sum;
-  __syncthreads();
-  if (warp == 0) {                                 // the tiles of the groups before each one
-    int before = 0;
-    for (int g0 = 0; g0 < c.n_groups; g0 += 32) {
-      const int here = g0 + lane < c.n_groups ? at.where[g0 + lane] : 0;
-      int tiles_upto = here;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int less = __shfl_up_sync(0xffffffffu, tiles_upto, o);
-        if (lane >= o) tiles_upto += less;
-      }
-      if (g0 + lane < c.n_groups) at.where[g0 + lane] = before + tiles_upto - here;
-      before += __shfl_sync(0xffffffffu, tiles_upto, 31);
-    }
-    if (lane == 0) at.sums[WARPS] = before;
-  }
-  __syncthreads();
-  const int blocks = at.start[n_entries], group_tiles = at.sums[WARPS], items = group_tiles + c.n_rows;
-  const long long total = static_cast<long long>(blocks) * c.nkv;
-  const int workers = static_cast<int>(min(static_cast<long long>(gridDim.x) * WARPS, max(total, 1ll)));
-  if (blockIdx.x == 0) {
-    for (int e = threadIdx.x; e <= n_entries; e += THREADS) k.sequence->start[e] = at.start[e];
-    for (int g = threadIdx.x; g < c.n_groups; g += THREADS) k.sequence->tiles_before[g] = at.where[g];
-    if (threadIdx.x == 0) {
-      k.sequence->blocks = blocks;
-      k.sequence->items = items;
-      k.sequence->workers = workers;
-      k.sequence->group_tiles = group_tiles;
-    }
-  }
-
+  const Stretches stretches(at.blocks * c.nkv, static_cast<int>(gridDim.x) * WARPS);
   const int worker = warp * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x);      // (few stretches: on as many SMs as can be)
-  const long long s_end = worker < workers ? (worker + 1) * total / workers : 0;
-  auto locate = [&](long long s) {
-    Place p;
-    p.s = s;
-    p.kvh = static_cast<int>(s / blocks);
-    const int pos = static_cast<int>(s - static_cast<long long>(p.kvh) * blocks);
-    int lo = 0, hi = n_entries;                    // the entries that begin at or before pos: the last of them holds it
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (at.start[mid] <= pos) lo = mid + 1; else hi = mid;
-    }
-    const int e = lo - 1;
-    int block = pos - at.start[e], of;
-    p.shared = e < c.n_groups;
-    p.end = at.keys[e];
-    if (p.shared) {
-      of = (p.end + KB - 1) / KB;
-      const int tile = block / of;
-      block -= tile * of;
-      p.item = p.kvh * items + at.where[e] + tile;
-      p.lowest = 0;
-      p.i0 = at.low[e];
-      const int next = e + 1 < c.n_groups ? max(at.low[e + 1], p.i0) : c.n_rows;
-      p.vector0 = k.covered + tile * VT;
-      p.vectors = min(VT, (next - p.i0) * group - p.vector0);
-      p.table_row = at.where[c.n_groups + p.i0];
-      p.first_key = block * KB;
-    } else {
-      p.lowest = at.low[e];
-      of = (p.end + KB - 1) / KB - p.lowest / KB;
-      p.item = p.kvh * items + group_tiles + e - c.n_groups;
-      p.i0 = e - c.n_groups;
-      p.vector0 = 0;
-      p.vectors = group;
-      p.table_row = at.where[e];
-      p.first_key = (p.lowest / KB + block) * KB;
-    }
-    p.left = static_cast<int>(min(static_cast<long long>(of - block), s_end - s));
-    return p;
-  };
-
-  long long s = worker < workers ? worker * total / workers : 0;
-  if (s < s_end) {
+  const int s_begin = worker < stretches.workers ? stretches.begin(worker) : 0, s_end = worker < stretches.workers ? stretches.begin(worker + 1) : 0;
+  if (s_begin < s_end) {
     unsigned char* ring = tiles + static_cast<size_t>(warp) * STAGES * TILE_BYTES;
     uint64_t* full = bars + warp * STAGES;
     bf16* qs = queries + warp * VT * LD;
-    // the queries of an item into shared memory
+    // the queries of an item into shared memory: two lanes a vector
     auto fetch_queries = [&](const Place& p) {
-      for (int x = lane; x < VT * (D / 8); x += 32) {
-        const int r = x / (D / 8), part = x - r * (D / 8);
-        const int vec = p.vector0 + min(r, p.vectors - 1);
-        const int token = at.token[c.n_groups + p.i0 + vec / group];
-        cp_async16(qs + r * LD + part * 8, q + (static_cast<long long>(token) * c.nh + p.kvh * group + vec % group) * D + part * 8, r < p.vectors);
-      }
+      const int r = lane >> 1, vec = p.vector0 + min(r, p.vectors - 1), row = vec / group;
+      const int token = at.token[c.n_groups + p.i0 + row];
+      const bf16* src = q + (static_cast<long long>(token) * c.nh + p.kvh * group + vec - row * group) * D;
+      for (int part = lane & 1; part < D / 8; part += 2) cp_async16(qs + r * LD + part * 8, src + part * 8, r < p.vectors);
       cp_async_commit();
     };
-    Place now = locate(s), ahead = now;
+    Place now = locate(at, s_begin, s_end, c.n_groups, c.n_rows, group, k.covered), ahead = now, next = now;
     int page = lane_page_checked(c, ahead, box_rows, lane);
-    int fetch_stage = 0;
-    // The next block of the stretch on its way, whatever item it is of; the page numbers of the one behind it are asked for.
-    auto fetch_next = [&]() {
-      if (ahead.s >= s_end) return;
-      fetch_block(ring + fetch_stage * TILE_BYTES, &kmap, &vmap, page, c.page_size, c.nkv, ahead.kvh, box_rows, ahead.first_key, ahead.end, full + fetch_stage, lane);
-      fetch_stage = fetch_stage + 1 == STAGES ? 0 : fetch_stage + 1;
-      ++ahead.s;
-      ahead.first_key += KB;
-      if (--ahead.left == 0 && ahead.s < s_end) ahead = locate(ahead.s);
-      if (ahead.s < s_end) page = lane_page_checked(c, ahead, box_rows, lane);
-    };
     fetch_queries(now);
-#pragma unroll
-    for (int x = 0; x < STAGES - 1; ++x) fetch_next();
-    int stage = 0;
+    uint32_t qa[kQueriesInRegisters ? D / 16 : 1][4];
+    WarpAcc st;
+    int last[2], all_see = 0, done = 0;            // `done`: blocks of the item behind us
+    int fetch_stage = 0, stage = 0;
     uint32_t parity = 0;
-    bool alive = true;                             // (a wait that ran out ends the warp's work; the error word says so)
-    while (alive) {
-      uint32_t qa[kQueriesInRegisters ? D / 16 : 1][4];
-      cp_async_wait<0>();
-      __syncwarp();
-      const long long behind = now.s + now.left;
-      Place next = now;
-      if constexpr (kQueriesInRegisters) {
-#pragma unroll
-        for (int x = 0; x < D / 16; ++x) ldmatrix_x4(qa[x], qs + (lane & 15) * LD + x * 16 + (lane >> 4) * 8);
+    for (int tick = 1 - STAGES;; ++tick) {
+      // the next block of the stretch on its way, whatever item it is of; the page numbers of the one behind it are asked for
+      if (ahead.s < s_end) {
+        fetch_block(ring + fetch_stage * TILE_BYTES, &kmap, &vmap, page, c.page_size, c.nkv, ahead.kvh, box_rows, ahead.first_key, ahead.end,
+                    full + fetch_stage, lane);
+        fetch_stage = fetch_stage + 1 == STAGES ? 0 : fetch_stage + 1;
+        ++ahead.s;
+        ahead.first_key += KB;
+        if (--ahead.left == 0 && ahead.s < s_end) ahead = locate(at, ahead.s, s_end, c.n_groups, c.n_rows, group, k.covered);
+        if (ahead.s < s_end) page = lane_page_checked(c, ahead, box_rows, lane);
+      }
+      if (tick < 0) continue;
+      if (done == 0) {                             // an item begins
+        cp_async_wait<0>();
         __syncwarp();
-        if (behind < s_end) {
-          next = locate(behind);
-          fetch_queries(next);
-        }
-      }
-      // the last key that this lane's two vectors see, and the least of all vectors'
-      int last[2], all_see = INT_MAX;
+        if constexpr (kQueriesInRegisters) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int r = x * 8 + (lane >> 2);
-        last[x] = -1;
-        if (r < now.vectors) {
-          last[x] = min(now.end, at.keys[c.n_groups + now.i0 + (now.vector0 + r) / group]) - 1;
-          all_see = min(all_see, last[x]);
-        }
-      }
-      all_see = __reduce_min_sync(0xffffffffu, all_see);
-      WarpAcc st;
-      st.init();
-      for (int x = 0; x < now.left; ++x) {
-        fetch_next();
-        if (!mbar_wait(full + stage, parity, c.err)) {
-          // Give the copies that are still in flight a bounded time to land before the warp leaves.
-          for (int t = 0; t < STAGES; ++t) mbar_wait(full + t, t < stage ? parity ^ 1u : parity, c.err);
-          alive = false;
-          break;
-        }
-        unsigned char* t = ring + stage * TILE_BYTES;
-        const int first_key = now.first_key + x * KB;
-        if (first_key + KB > now.end || first_key < now.lowest) {
-          // Value rows that are not the item's: whatever the page holds there must not reach P V.
-          if (first_key + lane >= now.end || first_key + lane < now.lowest) {
-            const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-            for (int v = 0; v < VALUE_CHUNKS; ++v) *reinterpret_cast<uint4*>(t + V_OFFSET + (v >> 3) * HALF_BYTES + lane * 128 + (v & 7) * 16) = zero;
+          for (int x = 0; x < D / 16; ++x) ldmatrix_x4(qa[x], qs + (lane & 15) * LD + x * 16 + (lane >> 4) * 8);
+          __syncwarp();
+          if (now.s + now.left < s_end) {
+            next = locate(at, now.s + now.left, s_end, c.n_groups, c.n_rows, group, k.covered);
+            fetch_queries(next);
           }
         }
-        __syncwarp();
-        if (first_key + KB - 1 > all_see || first_key < now.lowest)
-          item_block<true>(qa, qs, t, t + V_OFFSET, first_key, now.lowest, last[0], last[1], c.scale_log2, st);
-        else
-          item_block<false>(qa, qs, t, t + V_OFFSET, first_key, now.lowest, last[0], last[1], c.scale_log2, st);
-        __syncwarp();                              // every lane is done reading before the stage is refilled
-        if (++stage == STAGES) { stage = 0; parity ^= 1u; }
+        // the last key that this lane's two vectors see, and the least of all vectors'
+        all_see = INT_MAX;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int r = x * 8 + (lane >> 2);
+          last[x] = -1;
+          if (r < now.vectors) {
+            last[x] = min(now.end, at.keys[c.n_groups + now.i0 + (now.vector0 + r) / group]) - 1;
+            all_see = min(all_see, last[x]);
+          }
+        }
+        all_see = __reduce_min_sync(0xffffffffu, all_see);
+        st.init();
       }
-      // this stretch's part of the item
+      if (!mbar_wait(full + stage, parity, c.err)) {
+        // Give the copies that are still in flight a bounded time to land before the warp leaves; the error word is flagged.
+        for (int t = 0; t < STAGES; ++t) mbar_wait(full + t, t < stage ? parity ^ 1u : parity, c.err);
+        break;
+      }
+      unsigned char* t = ring + stage * TILE_BYTES;
+      const int first_key = now.first_key + done * KB;
+      if (first_key + KB > now.end || first_key < now.lowest) {
+        // Value rows that are not the item's: whatever the page holds there must not reach P V.
+        if (first_key + lane >= now.end || first_key + lane < now.lowest) {
+          const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 1
+          for (int v = 0; v < VALUE_CHUNKS; ++v) *reinterpret_cast<uint4*>(t + V_OFFSET + (v >> 3) * HALF_BYTES + lane * 128 + (v & 7) * 16) = zero;
+        }
+      }
+      __syncwarp();
+      item_block(qa, qs, t, t + V_OFFSET, first_key + KB - 1 > all_see || first_key < now.lowest, first_key, now.lowest, last[0], last[1], c.scale_log2, st);
+      __syncwarp();                                // every lane is done reading before the stage is refilled
+      if (++stage == STAGES) { stage = 0; parity ^= 1u; }
+      if (++done < now.left) continue;
+      // the item ends here, or the stretch: its part
       const long long part = static_cast<long long>(worker) + now.item;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -405,97 +408,149 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
           if ((lane & 3) == 0) k.ml[part * VT + r] = make_float2(st.m[half], l);
         }
       }
-      if (behind >= s_end) break;
+      if (now.s + now.left >= s_end) break;
       if constexpr (!kQueriesInRegisters) {
-        next = locate(behind);
+        next = locate(at, now.s + now.left, s_end, c.n_groups, c.n_rows, group, k.covered);
         fetch_queries(next);
       }
       now = next;
+      done = 0;
     }
   }
   if (k.covered > 0) pdl_wait();
 }
 
-// A vector's parts joined, a warp a vector: those of its row's item, of its group's tile, and of the tcgen05 kernel's splits.
-constexpr int JOIN_WARPS = 4;
+// A row's vectors of one KV head joined out of their parts: those of the row's item, of its group's tile, and of the tcgen05 kernel's
+// splits.  grid (n_rows * nkv).  The warps share a vector's parts, as many to a vector as there are.
+constexpr int JOIN_WARPS = 8;
 __global__ void __launch_bounds__(JOIN_WARPS * 32)
-prefix_join_kernel(bf16* __restrict__ out, const StreamCall k) {
+prefix_join_kernel(bf16* __restrict__ out, const StreamCall k, int most_workers) {
+  extern __shared__ int join_memory[];
   const PrefixCall& c = k.c;
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int ROW = D + 4;                       // what a warp leaves of a vector: outputs, maximum, sum
+  float* left = reinterpret_cast<float*>(join_memory);               // [JOIN_WARPS][ROW]
+  // The stream kernel began when everything before the call had ended, so the call's index arrays may be read beside it.
+  Entries at;
+  lay_out<JOIN_WARPS>(k, at, join_memory + JOIN_WARPS * ROW);
+  const int group = c.nh / c.nkv;
+  const int i = static_cast<int>(blockIdx.x) / c.nkv, kvh = static_cast<int>(blockIdx.x) - i * c.nkv;
+  const Stretches stretches(at.blocks * c.nkv, most_workers);
+  // the parts of a run of blocks of an item: first and number
+  auto parts_of_item = [&](int first, int blocks, int item, long long& part) {
+    if (blocks <= 0) return 0;
+    const int s = kvh * at.blocks + first;
+    const int w0 = stretches.of(s);
+    part = static_cast<long long>(w0) + kvh * at.items + item;
+    return stretches.of(s + blocks - 1) - w0 + 1;
+  };
+  const int e = c.n_groups + i;
+  long long own_part = 0;
+  const int own_count = parts_of_item(at.start[e], at.start[e + 1] - at.start[e], at.group_tiles + i, own_part);
+  const int g = group_of_row(c, i);
+  const int first_row = g >= 0 ? at.low[g] : 0;
+  const int tiles = g >= 0 ? (g + 1 < c.n_groups ? at.where[g + 1] : at.group_tiles) - at.where[g] : 0;
+  const int tile_blocks = tiles > 0 ? (at.start[g + 1] - at.start[g]) / tiles : 0;
+  bf16* dst = out + (static_cast<long long>(at.token[e]) * c.nh + kvh * group) * D;
   pdl_launch_dependents();
   pdl_wait();
-  const int vec = static_cast<int>(blockIdx.x) * JOIN_WARPS + (threadIdx.x >> 5);
-  if (vec >= c.n_rows * c.nh) return;
-  const int group = c.nh / c.nkv;
-  const int i = vec / c.nh, head = vec % c.nh, kvh = head / group;
-  constexpr int PER = (D + 127) / 128;
-  float4 o[PER];
+
+  const int sharers = group >= JOIN_WARPS ? 1 : JOIN_WARPS / group;      // warps of a vector
+  constexpr int PER = (D + 127) / 128, BATCH = 8 / PER;
+  for (int r0 = 0; r0 < group; r0 += JOIN_WARPS / sharers) {
+    const int r = r0 + warp / sharers, share = warp % sharers;
+    float4 o[PER];
 #pragma unroll
-  for (int n = 0; n < PER; ++n) o[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float m = -INFINITY, l = 0.0f;
-  // `count` parts, `step` vectors from one to the next
-  auto join = [&](const float* acc, const float2* ml, int count, int step) {
-    for (int p0 = 0; p0 < count; p0 += 32) {
-      float2 mine = make_float2(-INFINITY, 0.0f);
-      if (p0 + lane < count) mine = __ldcg(ml + static_cast<long long>(p0 + lane) * step);
-      const float most = fmaxf(m, warp_max(mine.x));
-      if (most == -INFINITY) continue;
-      const float f = m == -INFINITY ? 0.0f : exp2f(m - most), w = mine.x == -INFINITY ? 0.0f : exp2f(mine.x - most);
-      m = most;
-      l = fmaf(l, f, warp_sum(mine.y * w));
+    for (int n = 0; n < PER; ++n) o[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float m = -INFINITY, l = 0.0f;
+    // this warp's share of `count` parts, `step` vectors from one to the next
+    auto join = [&](const float* acc, const float2* ml, int count, int step) {
+      for (int p0 = share; p0 < count; p0 += 32 * sharers) {
+        const int p_mine = p0 + lane * sharers;
+        float2 mine = make_float2(-INFINITY, 0.0f);
+        if (p_mine < count) mine = __ldcg(ml + static_cast<long long>(p_mine) * step);
+        const float most = fmaxf(m, warp_max(mine.x));
+        if (most == -INFINITY) continue;
+        const float f = m == -INFINITY ? 0.0f : exp2f(m - most), w = mine.x == -INFINITY ? 0.0f : exp2f(mine.x - most);
+        m = most;
+        l = fmaf(l, f, warp_sum(mine.y * w));
 #pragma unroll
-      for (int n = 0; n < PER; ++n) { o[n].x *= f; o[n].y *= f; o[n].z *= f; o[n].w *= f; }
-      const int some = min(32, count - p0);
-#pragma unroll 4
-      for (int p = 0; p < some; ++p) {
-        const float wp = __shfl_sync(0xffffffffu, w, p);
-        const float* src = acc + static_cast<long long>(p0 + p) * step * D;
+        for (int n = 0; n < PER; ++n) { o[n].x *= f; o[n].y *= f; o[n].z *= f; o[n].w *= f; }
+        const int some = min(32, (count - p0 + sharers - 1) / sharers);
+        // (all of a batch's loads before its sums: one after the other a part took 580 cycles)
+        for (int b0 = 0; b0 < some; b0 += BATCH) {
+          float4 a[BATCH][PER];
 #pragma unroll
-        for (int n = 0; n < PER; ++n) {
-          const int dim = n * 128 + lane * 4;
-          if ((D % 128 == 0 || dim < D) && wp > 0.0f) {      // (nothing was written where a split saw no key)
-            const float4 a = __ldcg(reinterpret_cast<const float4*>(src + dim));
-            o[n].x = fmaf(wp, a.x, o[n].x);
-            o[n].y = fmaf(wp, a.y, o[n].y);
-            o[n].z = fmaf(wp, a.z, o[n].z);
-            o[n].w = fmaf(wp, a.w, o[n].w);
+          for (int b = 0; b < BATCH; ++b)
+#pragma unroll
+            for (int n = 0; n < PER; ++n)
+              if (D % 128 == 0 || n * 128 + lane * 4 < D)
+                a[b][n] = __ldcg(reinterpret_cast<const float4*>(acc + static_cast<long long>(p0 + min(b0 + b, some - 1) * sharers) * step * D + n * 128 + lane * 4));
+#pragma unroll
+          for (int b = 0; b < BATCH; ++b) {
+            const float wp = __shfl_sync(0xffffffffu, w, (b0 + b) & 31);
+            if (b0 + b < some && wp > 0.0f) {      // (where a split saw no key nothing was written)
+#pragma unroll
+              for (int n = 0; n < PER; ++n) {
+                o[n].x = fmaf(wp, a[b][n].x, o[n].x);
+                o[n].y = fmaf(wp, a[b][n].y, o[n].y);
+                o[n].z = fmaf(wp, a[b][n].z, o[n].z);
+                o[n].w = fmaf(wp, a[b][n].w, o[n].w);
+              }
+            }
           }
         }
       }
+    };
+    if (r < group) {
+      if (g >= 0) {
+        const int v = (i - first_row) * group + r;
+        if (v < k.covered) {
+          const long long place = (static_cast<long long>(i) * c.nh + kvh * group + r) * c.splits_shared;
+          join(c.part_acc + place * D, c.part_ml + place, c.splits_shared, 1);
+        } else {
+          long long part = 0;
+          const int tile = (v - k.covered) / VT, count = parts_of_item(at.start[g] + tile * tile_blocks, tile_blocks, at.where[g] + tile, part);
+          part = part * VT + (v - k.covered) % VT;
+          join(k.acc + part * D, k.ml + part, count, VT);
+        }
+      }
+      join(k.acc + (own_part * VT + r) * D, k.ml + own_part * VT + r, own_count, VT);
     }
-  };
-  const Sequence& q = *k.sequence;
-  const long long total = static_cast<long long>(q.blocks) * c.nkv;
-  auto join_item = [&](int first, int blocks, int item, int r) {
-    if (blocks <= 0) return;
-    const long long s = static_cast<long long>(kvh) * q.blocks + first;
-    const int w0 = worker_of(s, total, q.workers), w1 = worker_of(s + blocks - 1, total, q.workers);
-    const long long part = static_cast<long long>(w0) + kvh * static_cast<long long>(q.items) + item;
-    join(k.acc + (part * VT + r) * D, k.ml + part * VT + r, w1 - w0 + 1, VT);
-  };
-  const int e = c.n_groups + i;
-  join_item(q.start[e], q.start[e + 1] - q.start[e], q.group_tiles + i, head % group);
-  const int g = group_of_row(c, i);
-  if (g >= 0) {
-    const int2 rows = rows_of_group(c, g);
-    const int v = (i - rows.x) * group + head % group;
-    if (v < k.covered) {
-      const long long place = static_cast<long long>(vec) * c.splits_shared;
-      join(c.part_acc + place * D, c.part_ml + place, c.splits_shared, 1);
-    } else {
-      const int tiles = tiles_of(k, rows.y, group), tile = (v - k.covered) / VT;
-      const int blocks = (q.start[g + 1] - q.start[g]) / max(tiles, 1);
-      join_item(q.start[g] + tile * blocks, blocks, q.tiles_before[g] + tile, (v - k.covered) % VT);
-    }
-  }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-  bf16* dst = out + (static_cast<long long>(c.cu_q[c.rows[i]]) * c.nh + head) * D;
+    if (sharers > 1) {
+      __syncthreads();
 #pragma unroll
-  for (int n = 0; n < PER; ++n) {
-    const int dim = n * 128 + lane * 4;
-    if (D % 128 == 0 || dim < D) {
-      const uint2 two = make_uint2(pack_bf16(o[n].x * inv, o[n].y * inv), pack_bf16(o[n].z * inv, o[n].w * inv));
-      *reinterpret_cast<uint2*>(dst + dim) = two;
+      for (int n = 0; n < PER; ++n)
+        if (D % 128 == 0 || n * 128 + lane * 4 < D) *reinterpret_cast<float4*>(left + warp * ROW + n * 128 + lane * 4) = o[n];
+      if (lane == 0) { left[warp * ROW + D] = m; left[warp * ROW + D + 1] = l; }
+      __syncthreads();
+      if (share == 0) {
+        for (int x = 1; x < sharers; ++x) {
+          const float* other = left + (warp + x) * ROW;
+          const float most = fmaxf(m, other[D]);
+          const float f = m == -INFINITY ? 0.0f : exp2f(m - most), w = other[D] == -INFINITY ? 0.0f : exp2f(other[D] - most);
+          m = most;
+          l = l * f + other[D + 1] * w;
+#pragma unroll
+          for (int n = 0; n < PER; ++n)
+            if (D % 128 == 0 || n * 128 + lane * 4 < D) {
+              const float4 a = *reinterpret_cast<const float4*>(other + n * 128 + lane * 4);
+              o[n].x = fmaf(w, a.x, o[n].x * f);
+              o[n].y = fmaf(w, a.y, o[n].y * f);
+              o[n].z = fmaf(w, a.z, o[n].z * f);
+              o[n].w = fmaf(w, a.w, o[n].w * f);
+            }
+        }
+      }
+    }
+    if (share == 0 && r < group) {
+      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+      for (int n = 0; n < PER; ++n) {
+        const int dim = n * 128 + lane * 4;
+        if (D % 128 == 0 || dim < D)
+          *reinterpret_cast<uint2*>(dst + r * D + dim) = make_uint2(pack_bf16(o[n].x * inv, o[n].y * inv), pack_bf16(o[n].z * inv, o[n].w * inv));
+      }
     }
   }
 }
@@ -512,7 +567,7 @@ B200_EXPORT int b200_prefix_most_entries() { return MOST_ENTRIES; }
 // Floats of scratch: the tcgen05 kernel's part first (splits_shared > 0).
 B200_EXPORT long long b200_prefix_scratch_floats(int n_rows, int n_groups, int nh, int nkv, int splits_shared, int sms) {
   const long long vectors = static_cast<long long>(n_rows) * nh * splits_shared, parts = parts_of(n_rows, n_groups, nh, nkv, sms) * VT;
-  return vectors * (D + 2) + parts * (D + 2) + align4(sizeof(Sequence) / 4) + 8;
+  return align4(vectors * (D + 2)) + parts * (D + 2);
 }
 
 // q, out [tokens, nh * D]; k_cache, v_cache [pages, nkv, page_size, D]; `groups`: (first row, shared keys) each.  `scratch` holds
@@ -525,6 +580,10 @@ B200_EXPORT int b200_prefix_attention_mma(const void* q, const void* k_cache, co
   if (n_rows <= 0) return 0;
   if (nh <= 0 || nkv <= 0 || nh % nkv != 0 || nh / nkv > 16 || page_size <= 0 || (page_size & (page_size - 1)) != 0 || pages <= 0 || table_stride <= 0 || n_groups < 0)
     return B200_BAD_SIZE;
+  // (blocks are counted in 32 bits)
+  const long long most_blocks = (static_cast<long long>(table_stride) * page_size / KB + 2) * nkv *
+                                ((static_cast<long long>(n_rows) * (nh / nkv) + VT - 1) / VT + n_groups + n_rows);
+  if (most_blocks > INT32_MAX / 2) return B200_BAD_SIZE;
   if (splits_shared < 0 || covered < 0 || (covered > 0) != (splits_shared > 0) || sms < 1 || n_rows + n_groups > MOST_ENTRIES) return B200_BAD_SIZE;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(scratch)) % 16 != 0) return B200_BAD_ALIGN;
   StreamCall k;
@@ -532,7 +591,6 @@ B200_EXPORT int b200_prefix_attention_mma(const void* q, const void* k_cache, co
   float2* part_ml = reinterpret_cast<float2*>(scratch + vectors * D);
   k.acc = scratch + align4(vectors * (D + 2));
   k.ml = reinterpret_cast<float2*>(k.acc + parts * D);
-  k.sequence = reinterpret_cast<Sequence*>(k.ml + parts);
   k.covered = covered;
   k.c = {block_table, cu_q, kv_len, rows, reinterpret_cast<const int2*>(groups), scratch, part_ml, err, table_stride, n_rows, n_groups, nh, nkv,
          page_size, pages, splits_shared, 0, 1, scale * 1.4426950408889634f};
@@ -543,11 +601,11 @@ B200_EXPORT int b200_prefix_attention_mma(const void* q, const void* k_cache, co
   if (rc == 0) rc = make_kv_tensor_map(&vmap, v_cache, lines, D, box_rows);
   if (rc != 0) return rc;
   static bool seen[16];
-  rc = prefix_smem_limit(prefix_stream_kernel, static_cast<int>(SMEM), seen);
+  rc = prefix_smem_limit(prefix_stream_kernel, static_cast<int>(FIXED) + entries_bytes(MOST_ENTRIES), seen);
   if (rc != 0) return rc;
-  rc = b200_launch(prefix_stream_kernel, dim3(sms), dim3(THREADS), SMEM, stream, 0, kmap, vmap, static_cast<const bf16*>(q), k, box_rows);
+  const int entries = entries_bytes(n_rows + n_groups);
+  rc = b200_launch(prefix_stream_kernel, dim3(sms), dim3(THREADS), FIXED + entries, stream, 0, kmap, vmap, static_cast<const bf16*>(q), k, box_rows);
   if (rc != 0) return rc;
-  const long long ctas = (static_cast<long long>(n_rows) * nh + JOIN_WARPS - 1) / JOIN_WARPS;
-  if (ctas > INT32_MAX / JOIN_WARPS) return B200_BAD_SIZE;
-  return b200_launch(prefix_join_kernel, dim3(static_cast<unsigned>(ctas)), dim3(JOIN_WARPS * 32), 0, stream, 0, static_cast<bf16*>(out), k);
+  return b200_launch(prefix_join_kernel, dim3(static_cast<unsigned>(n_rows) * nkv), dim3(JOIN_WARPS * 32), JOIN_WARPS * (D + 4) * 4 + entries, stream, 0,
+                     static_cast<bf16*>(out), k, sms * WARPS);
 }
