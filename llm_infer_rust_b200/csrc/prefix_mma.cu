@@ -39,10 +39,15 @@ __host__ __device__ constexpr int entries_bytes(int n_entries) { return (5 * n_e
 static_assert(WARPS <= 8, "a sum a warp");
 static_assert(FIXED + entries_bytes(MOST_ENTRIES) <= 227 * 1024, "shared memory of one CTA");
 
+// Which parts make up a row's vectors of one KV head: those of its own item, and of the tiles of its group that the vectors are in (at
+// most two, `first_vector` counted from the first vector behind those that the tcgen05 kernel serves).
+struct __align__(16) RowParts { int own, own_count, first_vector, tile[2], tile_count[2], grouped; };
+
 struct StreamCall {
   PrefixCall c;                                  // part_acc, part_ml: of the tcgen05 kernel, [n_rows * nh][splits_shared]
   float* acc;                                    // [parts][16][D]
   float2* ml;                                    // [parts][16]
+  RowParts* row_parts;                           // [n_rows][nkv]
   int covered;                                   // vectors of each group that the tcgen05 kernel serves
 };
 
@@ -417,141 +422,142 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       done = 0;
     }
   }
+  // what the joining kernel goes by
+  for (int x = static_cast<int>(threadIdx.x) * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x); x < c.n_rows * c.nkv; x += static_cast<int>(gridDim.x) * THREADS) {
+    const int i = x / c.nkv, kvh = x - i * c.nkv, e = c.n_groups + i;
+    auto parts_of_item = [&](int first, int blocks, int item, int& part) {      // of a run of blocks: the number of parts, the first
+      part = 0;
+      if (blocks <= 0) return 0;
+      const int s = kvh * at.blocks + first, w0 = stretches.of(s);
+      part = w0 + kvh * at.items + item;
+      return stretches.of(s + blocks - 1) - w0 + 1;
+    };
+    RowParts p = {};
+    p.own_count = parts_of_item(at.start[e], at.start[e + 1] - at.start[e], at.group_tiles + i, p.own);
+    int g = c.n_groups - 1;                        // the row's group (as lay_out has it)
+    while (g >= 0 && at.low[g] > i) --g;
+    p.grouped = g >= 0;
+    if (g >= 0) {
+      p.first_vector = (i - at.low[g]) * group - k.covered;
+      const int tiles_here = (g + 1 < c.n_groups ? at.where[g + 1] : at.group_tiles) - at.where[g];
+      const int blocks_here = tiles_here > 0 ? (at.start[g + 1] - at.start[g]) / tiles_here : 0, tile = max(p.first_vector, 0) / VT;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (tile + t < tiles_here) p.tile_count[t] = parts_of_item(at.start[g] + (tile + t) * blocks_here, blocks_here, at.where[g] + tile + t, p.tile[t]);
+    }
+    k.row_parts[x] = p;
+  }
   if (k.covered > 0) pdl_wait();
 }
 
-// A row's vectors of one KV head joined out of their parts: those of the row's item, of its group's tile, and of the tcgen05 kernel's
-// splits.  grid (n_rows * nkv).  The warps share a vector's parts, as many to a vector as there are.
-constexpr int JOIN_WARPS = 8;
+// A vector joined out of its parts: those of its group's tile, or of the tcgen05 kernel's splits, and those of its row's item.  grid (n_rows
+// * nh), the CTA's warps share the parts, up to eight of them a turn: maxima and sums are asked for together with the outputs that they
+// weight, for what this kernel takes is a few answers from the second-level cache one behind the other.  (A CTA four vectors, two
+// warps each, weights before outputs: eight rows behind 4,096 keys 12,800 cycles.)
+constexpr int JOIN_WARPS = 4, JOIN_BATCH = D <= 128 ? 8 : 4;
 __global__ void __launch_bounds__(JOIN_WARPS * 32)
-prefix_join_kernel(bf16* __restrict__ out, const StreamCall k, int most_workers) {
-  extern __shared__ int join_memory[];
+prefix_join_kernel(bf16* __restrict__ out, const StreamCall k) {
   const PrefixCall& c = k.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  constexpr int ROW = D + 4;                       // what a warp leaves of a vector: outputs, maximum, sum
-  float* left = reinterpret_cast<float*>(join_memory);               // [JOIN_WARPS][ROW]
-  // The stream kernel began when everything before the call had ended, so the call's index arrays may be read beside it.
-  Entries at;
-  lay_out<JOIN_WARPS>(k, at, join_memory + JOIN_WARPS * ROW);
+  constexpr int ROW = D + 4;                       // what a warp leaves: outputs, maximum, sum
+  constexpr int PER = (D + 127) / 128;
+  __shared__ __align__(16) float left[JOIN_WARPS * ROW];
   const int group = c.nh / c.nkv;
-  const int i = static_cast<int>(blockIdx.x) / c.nkv, kvh = static_cast<int>(blockIdx.x) - i * c.nkv;
-  const Stretches stretches(at.blocks * c.nkv, most_workers);
-  // the parts of a run of blocks of an item: first and number
-  auto parts_of_item = [&](int first, int blocks, int item, long long& part) {
-    if (blocks <= 0) return 0;
-    const int s = kvh * at.blocks + first;
-    const int w0 = stretches.of(s);
-    part = static_cast<long long>(w0) + kvh * at.items + item;
-    return stretches.of(s + blocks - 1) - w0 + 1;
-  };
-  const int e = c.n_groups + i;
-  long long own_part = 0;
-  const int own_count = parts_of_item(at.start[e], at.start[e + 1] - at.start[e], at.group_tiles + i, own_part);
-  const int g = group_of_row(c, i);
-  const int first_row = g >= 0 ? at.low[g] : 0;
-  const int tiles = g >= 0 ? (g + 1 < c.n_groups ? at.where[g + 1] : at.group_tiles) - at.where[g] : 0;
-  const int tile_blocks = tiles > 0 ? (at.start[g + 1] - at.start[g]) / tiles : 0;
-  bf16* dst = out + (static_cast<long long>(at.token[e]) * c.nh + kvh * group) * D;
+  const int i = static_cast<int>(blockIdx.x) / c.nh, head = static_cast<int>(blockIdx.x) - i * c.nh, kvh = head / group, r = head - kvh * group;
+  // (the stream kernel began when everything before the call had ended, so the call's index arrays may be read beside it)
+  bf16* dst = out + (static_cast<long long>(c.cu_q[c.rows[i]]) * c.nh + head) * D;
   pdl_launch_dependents();
   pdl_wait();
-
-  const int sharers = group >= JOIN_WARPS ? 1 : JOIN_WARPS / group;      // warps of a vector
-  constexpr int PER = (D + 127) / 128, BATCH = 8 / PER;
-  for (int r0 = 0; r0 < group; r0 += JOIN_WARPS / sharers) {
-    const int r = r0 + warp / sharers, share = warp % sharers;
-    float4 o[PER];
+  const RowParts* row = k.row_parts + static_cast<long long>(i) * c.nkv + kvh;
+  const int4 first = *reinterpret_cast<const int4*>(row), rest = *(reinterpret_cast<const int4*>(row) + 1);
+  const int own = first.x, own_count = first.y, v = first.z + r, grouped = rest.w;
+  const bool second = v / VT > max(first.z, 0) / VT, split = grouped != 0 && v < 0;
+  const int tile = second ? rest.x : first.w;
+  const int tile_count = grouped == 0 ? 0 : split ? c.splits_shared : second ? rest.z : rest.y;
+  // part p of tile_count + own_count: vector `at` of the stream's parts, or of the tcgen05 kernel's
+  const long long vec = static_cast<long long>(blockIdx.x) * c.splits_shared;
+  const int count = tile_count + own_count;
+  float4 o[PER];
 #pragma unroll
-    for (int n = 0; n < PER; ++n) o[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float m = -INFINITY, l = 0.0f;
-    // this warp's share of `count` parts, `step` vectors from one to the next
-    auto join = [&](const float* acc, const float2* ml, int count, int step) {
-      for (int p0 = share; p0 < count; p0 += 32 * sharers) {
-        const int p_mine = p0 + lane * sharers;
-        float2 mine = make_float2(-INFINITY, 0.0f);
-        if (p_mine < count) mine = __ldcg(ml + static_cast<long long>(p_mine) * step);
-        const float most = fmaxf(m, warp_max(mine.x));
-        if (most == -INFINITY) continue;
-        const float f = m == -INFINITY ? 0.0f : exp2f(m - most), w = mine.x == -INFINITY ? 0.0f : exp2f(mine.x - most);
-        m = most;
-        l = fmaf(l, f, warp_sum(mine.y * w));
+  for (int n = 0; n < PER; ++n) o[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float m = -INFINITY, l = 0.0f;
+  for (int p0 = warp * JOIN_BATCH; p0 < count; p0 += JOIN_WARPS * JOIN_BATCH) {
+    float4 a[JOIN_BATCH][PER];
+    float2 ml[JOIN_BATCH];
 #pragma unroll
-        for (int n = 0; n < PER; ++n) { o[n].x *= f; o[n].y *= f; o[n].z *= f; o[n].w *= f; }
-        const int some = min(32, (count - p0 + sharers - 1) / sharers);
-        // (all of a batch's loads before its sums: one after the other a part took 580 cycles)
-        for (int b0 = 0; b0 < some; b0 += BATCH) {
-          float4 a[BATCH][PER];
-#pragma unroll
-          for (int b = 0; b < BATCH; ++b)
-#pragma unroll
-            for (int n = 0; n < PER; ++n)
-              if (D % 128 == 0 || n * 128 + lane * 4 < D)
-                a[b][n] = __ldcg(reinterpret_cast<const float4*>(acc + static_cast<long long>(p0 + min(b0 + b, some - 1) * sharers) * step * D + n * 128 + lane * 4));
-#pragma unroll
-          for (int b = 0; b < BATCH; ++b) {
-            const float wp = __shfl_sync(0xffffffffu, w, (b0 + b) & 31);
-            if (b0 + b < some && wp > 0.0f) {      // (where a split saw no key nothing was written)
-#pragma unroll
-              for (int n = 0; n < PER; ++n) {
-                o[n].x = fmaf(wp, a[b][n].x, o[n].x);
-                o[n].y = fmaf(wp, a[b][n].y, o[n].y);
-                o[n].z = fmaf(wp, a[b][n].z, o[n].z);
-                o[n].w = fmaf(wp, a[b][n].w, o[n].w);
-              }
-            }
-          }
-        }
-      }
-    };
-    if (r < group) {
-      if (g >= 0) {
-        const int v = (i - first_row) * group + r;
-        if (v < k.covered) {
-          const long long place = (static_cast<long long>(i) * c.nh + kvh * group + r) * c.splits_shared;
-          join(c.part_acc + place * D, c.part_ml + place, c.splits_shared, 1);
-        } else {
-          long long part = 0;
-          const int tile = (v - k.covered) / VT, count = parts_of_item(at.start[g] + tile * tile_blocks, tile_blocks, at.where[g] + tile, part);
-          part = part * VT + (v - k.covered) % VT;
-          join(k.acc + part * D, k.ml + part, count, VT);
-        }
-      }
-      join(k.acc + (own_part * VT + r) * D, k.ml + own_part * VT + r, own_count, VT);
-    }
-    if (sharers > 1) {
-      __syncthreads();
+    for (int b = 0; b < JOIN_BATCH; ++b) {
+      const int p = min(p0 + b, count - 1);
+      const bool of_tc = split && p < tile_count;
+      const long long at = of_tc ? vec + p : p < tile_count ? static_cast<long long>(tile + p) * VT + v % VT : static_cast<long long>(own + p - tile_count) * VT + r;
+      ml[b] = __ldcg((of_tc ? c.part_ml : k.ml) + at);
+      const float* src = (of_tc ? c.part_acc : k.acc) + at * D;
 #pragma unroll
       for (int n = 0; n < PER; ++n)
-        if (D % 128 == 0 || n * 128 + lane * 4 < D) *reinterpret_cast<float4*>(left + warp * ROW + n * 128 + lane * 4) = o[n];
-      if (lane == 0) { left[warp * ROW + D] = m; left[warp * ROW + D + 1] = l; }
-      __syncthreads();
-      if (share == 0) {
-        for (int x = 1; x < sharers; ++x) {
-          const float* other = left + (warp + x) * ROW;
-          const float most = fmaxf(m, other[D]);
-          const float f = m == -INFINITY ? 0.0f : exp2f(m - most), w = other[D] == -INFINITY ? 0.0f : exp2f(other[D] - most);
-          m = most;
-          l = l * f + other[D + 1] * w;
-#pragma unroll
-          for (int n = 0; n < PER; ++n)
-            if (D % 128 == 0 || n * 128 + lane * 4 < D) {
-              const float4 a = *reinterpret_cast<const float4*>(other + n * 128 + lane * 4);
-              o[n].x = fmaf(w, a.x, o[n].x * f);
-              o[n].y = fmaf(w, a.y, o[n].y * f);
-              o[n].z = fmaf(w, a.z, o[n].z * f);
-              o[n].w = fmaf(w, a.w, o[n].w * f);
-            }
-        }
-      }
+        if (D % 128 == 0 || n * 128 + lane * 4 < D) a[b][n] = __ldcg(reinterpret_cast<const float4*>(src + n * 128 + lane * 4));
     }
-    if (share == 0 && r < group) {
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    float most = m;
+#pragma unroll
+    for (int b = 0; b < JOIN_BATCH; ++b) {
+      if (p0 + b >= count) ml[b] = make_float2(-INFINITY, 0.0f);
+      most = fmaxf(most, ml[b].x);
+    }
+    if (most == -INFINITY) continue;
+    const float f = fast_exp2(m - most);           // (0 on the first visible part)
+    m = most;
+    l *= f;
+#pragma unroll
+    for (int n = 0; n < PER; ++n) { o[n].x *= f; o[n].y *= f; o[n].z *= f; o[n].w *= f; }
+#pragma unroll
+    for (int b = 0; b < JOIN_BATCH; ++b) {
+      if (ml[b].x == -INFINITY) continue;          // (where a split saw no key nothing was written)
+      const float w = fast_exp2(ml[b].x - m);
+      l = fmaf(ml[b].y, w, l);
 #pragma unroll
       for (int n = 0; n < PER; ++n) {
-        const int dim = n * 128 + lane * 4;
-        if (D % 128 == 0 || dim < D)
-          *reinterpret_cast<uint2*>(dst + r * D + dim) = make_uint2(pack_bf16(o[n].x * inv, o[n].y * inv), pack_bf16(o[n].z * inv, o[n].w * inv));
+        o[n].x = fmaf(w, a[b][n].x, o[n].x);
+        o[n].y = fmaf(w, a[b][n].y, o[n].y);
+        o[n].z = fmaf(w, a[b][n].z, o[n].z);
+        o[n].w = fmaf(w, a[b][n].w, o[n].w);
       }
     }
+  }
+  if (count > JOIN_BATCH) {                        // (else all of it is the first warp's)
+#pragma unroll
+    for (int n = 0; n < PER; ++n)
+      if (D % 128 == 0 || n * 128 + lane * 4 < D) *reinterpret_cast<float4*>(left + warp * ROW + n * 128 + lane * 4) = o[n];
+    if (lane == 0) { left[warp * ROW + D] = m; left[warp * ROW + D + 1] = l; }
+    __syncthreads();
+  }
+  // columns are the threads' from here on, where the warps have shared; else the first warp's lanes'
+  if (count > JOIN_BATCH) {
+    float ms[JOIN_WARPS], most = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < JOIN_WARPS; ++w) {
+      ms[w] = left[w * ROW + D];
+      most = fmaxf(most, ms[w]);
+    }
+#pragma unroll
+    for (int w = 0; w < JOIN_WARPS; ++w) {
+      ms[w] = ms[w] == -INFINITY ? 0.0f : fast_exp2(ms[w] - most);
+      sum = fmaf(left[w * ROW + D + 1], ms[w], sum);
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    for (int dim = 2 * static_cast<int>(threadIdx.x); dim < D; dim += 2 * JOIN_WARPS * 32) {
+      float x = 0.0f, y = 0.0f;
+#pragma unroll
+      for (int w = 0; w < JOIN_WARPS; ++w) {
+        const float2 two = *reinterpret_cast<const float2*>(left + w * ROW + dim);
+        x = fmaf(two.x, ms[w], x);
+        y = fmaf(two.y, ms[w], y);
+      }
+      *reinterpret_cast<uint32_t*>(dst + dim) = pack_bf16(x * inv, y * inv);
+    }
+  } else if (warp == 0) {
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int n = 0; n < PER; ++n)
+      if (D % 128 == 0 || n * 128 + lane * 4 < D)
+        *reinterpret_cast<uint2*>(dst + n * 128 + lane * 4) = make_uint2(pack_bf16(o[n].x * inv, o[n].y * inv), pack_bf16(o[n].z * inv, o[n].w * inv));
   }
 }
 
@@ -567,7 +573,7 @@ B200_EXPORT int b200_prefix_most_entries() { return MOST_ENTRIES; }
 // Floats of scratch: the tcgen05 kernel's part first (splits_shared > 0).
 B200_EXPORT long long b200_prefix_scratch_floats(int n_rows, int n_groups, int nh, int nkv, int splits_shared, int sms) {
   const long long vectors = static_cast<long long>(n_rows) * nh * splits_shared, parts = parts_of(n_rows, n_groups, nh, nkv, sms) * VT;
-  return align4(vectors * (D + 2)) + parts * (D + 2);
+  return align4(vectors * (D + 2)) + parts * (D + 2) + static_cast<long long>(n_rows) * nkv * (sizeof(RowParts) / 4);
 }
 
 // q, out [tokens, nh * D]; k_cache, v_cache [pages, nkv, page_size, D]; `groups`: (first row, shared keys) each.  `scratch` holds
@@ -588,9 +594,11 @@ B200_EXPORT int b200_prefix_attention_mma(const void* q, const void* k_cache, co
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(scratch)) % 16 != 0) return B200_BAD_ALIGN;
   StreamCall k;
   const size_t vectors = static_cast<size_t>(n_rows) * nh * splits_shared, parts = static_cast<size_t>(parts_of(n_rows, n_groups, nh, nkv, sms)) * VT;
+  if (static_cast<long long>(n_rows) * nh > INT32_MAX) return B200_BAD_SIZE;
   float2* part_ml = reinterpret_cast<float2*>(scratch + vectors * D);
   k.acc = scratch + align4(vectors * (D + 2));
   k.ml = reinterpret_cast<float2*>(k.acc + parts * D);
+  k.row_parts = reinterpret_cast<RowParts*>(k.ml + parts);
   k.covered = covered;
   k.c = {block_table, cu_q, kv_len, rows, reinterpret_cast<const int2*>(groups), scratch, part_ml, err, table_stride, n_rows, n_groups, nh, nkv,
          page_size, pages, splits_shared, 0, 1, scale * 1.4426950408889634f};
@@ -606,6 +614,6 @@ B200_EXPORT int b200_prefix_attention_mma(const void* q, const void* k_cache, co
   const int entries = entries_bytes(n_rows + n_groups);
   rc = b200_launch(prefix_stream_kernel, dim3(sms), dim3(THREADS), FIXED + entries, stream, 0, kmap, vmap, static_cast<const bf16*>(q), k, box_rows);
   if (rc != 0) return rc;
-  return b200_launch(prefix_join_kernel, dim3(static_cast<unsigned>(n_rows) * nkv), dim3(JOIN_WARPS * 32), JOIN_WARPS * (D + 4) * 4 + entries, stream, 0,
-                     static_cast<bf16*>(out), k, sms * WARPS);
+  return b200_launch(prefix_join_kernel, dim3(static_cast<unsigned>(n_rows) * nh), dim3(JOIN_WARPS * 32), 0, stream, 0,
+                     static_cast<bf16*>(out), k);
 }

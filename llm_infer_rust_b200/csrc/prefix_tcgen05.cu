@@ -19,6 +19,8 @@ constexpr int THREADS = 320 + 32 * (COPY_WARPS - 1);      // warp 0 copies, 1 pr
 constexpr int V_STAGES = 2;
 constexpr int V_OFF = 0, Q_OFF = V_STAGES * TILE, K_OFF_TWO = Q_OFF + 2 * TILE, K_OFF_ONE = Q_OFF + TILE;
 constexpr int BAR_OFF = 6 * TILE;                         // V 2, Q 2 and K 2, or V 2, Q 1 and K 3
+constexpr int OUT_PITCH = D * 4 + 16;                      // of a row of outputs in shared memory
+static_assert(256 * OUT_PITCH <= BAR_OFF, "the outputs' rows fit where the tiles were");
 constexpr int N_BARS = 2 * 3 + 2 * V_STAGES + 4 * 2 + 1;
 constexpr int TBL_OFF = BAR_OFF + (N_BARS + 1) * 8;
 constexpr int SMEM = 1024 + TBL_OFF + TBL_ENTRIES * 4;
@@ -189,7 +191,19 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
       hi_key = min(k_end, keys_of_row(c, batch_row)) - 1;
     }
     if (count > 0 && (TWO || t == 0)) {
-      write_q_row<16>(sm + Q_OFF + t * TILE, q + (used ? (static_cast<long long>(c.cu_q[batch_row]) * c.nh + head) * D : 0), r, used, 0);
+      // The warp's 32 vectors, half a warp a vector, all on their way at once (zeros where there is none).  (Each lane its own vector,
+      // 32 lines an instruction: 5,700 cycles.)
+      const long long mine_at = used ? (static_cast<long long>(c.cu_q[batch_row]) * c.nh + head) * D : -1;
+      uint4 v[16];
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const long long at = __shfl_sync(0xffffffffu, mine_at, 2 * x + (lane >> 4));
+        v[x] = make_uint4(0u, 0u, 0u, 0u);
+        if (at >= 0) v[x] = *reinterpret_cast<const uint4*>(q + at + (lane & 15) * 8);
+      }
+#pragma unroll
+      for (int x = 0; x < 16; ++x) *reinterpret_cast<uint4*>(sm + Q_OFF + t * TILE + swz(quarter * 32 + 2 * x + (lane >> 4), lane & 15)) = v[x];
+      proxy_fence();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
     }
@@ -228,17 +242,25 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
     const long long place = (static_cast<long long>(row) * c.nh + head) * prefix_splits(c) + slot;
     const bool seen = ok && mine > 0 && st.m_ref > -INFINITY;
     if (used) c.part_ml[place] = seen ? make_float2(st.m_ref, st.l_run) : make_float2(-INFINITY, 0.0f);
+    // The outputs leave through shared memory, where both streams' products have been done: a thread puts its row there (rows 528
+    // bytes apart, so that eight threads' pieces lie in eight different groups of banks) and the copy engine takes it.  (Straight
+    // from the registers, 32 lines an instruction: 6,000 to 9,000 cycles.)
+    asm volatile("bar.sync 2, 256;\n" ::: "memory");             // (the softmax warps, whatever became of their waits)
     if (ok && mine > 0) {
       tc_fence_after();
+      unsigned char* line = sm + ((warp - 2) * 32 + lane) * OUT_PITCH;
 #pragma unroll 1
       for (int x = 0; x < 4; ++x) {
         float o[32];
         tmem_ld32(o_base + x * 32, o);
-        if (used && seen) {
-          float4* dst = reinterpret_cast<float4*>(c.part_acc + place * D + x * 32);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-        }
+        for (int e = 0; e < 8; ++e) *reinterpret_cast<float4*>(line + x * 128 + e * 16) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+      }
+      proxy_fence();
+      if (used && seen) {
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n" ::"l"(c.part_acc + place * D), "r"(smem_u32(line)), "n"(D * 4) : "memory");
+        asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+        asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
       }
       tc_fence_before();
     }
