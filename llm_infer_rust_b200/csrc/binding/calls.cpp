@@ -30,6 +30,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <initializer_list>
 #include <iterator>
 #include <vector>
 
@@ -306,6 +307,80 @@ PyObject* byte_product(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// prefix_attention(all sizes, tcgen05, mma, q, k, v, out, block table, cu_q, kv_len, rows, groups, heads, kv heads, head size, page size,
+//                  scale, plan, error word, stream) -> code
+// Decode attention behind shared prefixes (kernels/prefix.py) as one call: what the tensors must be, the memory between its kernels and
+// the launches.  The entry points are those of the plan, None where it has no use for one: the all-sizes kernel alone, or the
+// tensor-core kernels.  plan: (floats of scratch, splits of the shared keys, splits of the own keys, tiles, two tiles a CTA, vectors
+// that the tcgen05 kernel covers, CTAs).  None, and nothing done, where something is not as it should be (the wrapper then says what)
+// or this thread records its calls.  (Through Python the call took the host 17 us, of which 7 are three launches.)
+PyObject* prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 20 || !PyFloat_Check(args[16]) || !PyTuple_Check(args[17]) || PyTuple_GET_SIZE(args[17]) != 7) {
+    PyErr_SetString(PyExc_TypeError, "prefix_attention(all sizes, tcgen05, mma, q, k, v, out, block table, cu_q, kv_len, rows, groups, heads, kv heads, "
+                                     "head size, page size, scale, plan, error word, stream)");
+    return nullptr;
+  }
+  if (recording != nullptr) Py_RETURN_NONE;
+  void* entry[3] = {};
+  for (int i = 0; i < 3; ++i) {
+    if (args[i] == Py_None) continue;
+    if (Py_TYPE(args[i]) != &entry_type) Py_RETURN_NONE;
+    entry[i] = reinterpret_cast<Entry*>(args[i])->fn;
+  }
+  const at::Tensor* t[9];
+  for (int i = 0; i < 9; ++i) {
+    if (!THPVariable_Check(args[3 + i])) Py_RETURN_NONE;
+    t[i] = &THPVariable_Unpack(args[3 + i]);
+    if (!t[i]->is_cuda() || !t[i]->is_contiguous() || t[i]->device() != t[0]->device() ||
+        t[i]->scalar_type() != (i < 4 ? t[0]->scalar_type() : at::kInt))
+      Py_RETURN_NONE;
+  }
+  const at::Tensor &q = *t[0], &k = *t[1], &v = *t[2], &out = *t[3], &table = *t[4], &cu = *t[5], &lengths = *t[6], &rows = *t[7], &groups = *t[8];
+  I at[7], size[4];
+  for (int i = 0; i < 4; ++i) size[i] = PyLong_AsLongLong(args[12 + i]);
+  for (int i = 0; i < 7; ++i) at[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(args[17], i));
+  const I stream = PyLong_AsLongLong(args[19]);
+  if (PyErr_Occurred()) return nullptr;
+  const I heads = size[0], kv_heads = size[1], width = size[2], page = size[3];
+  const I code = q.scalar_type() == at::kBFloat16 ? 1 : q.scalar_type() == at::kFloat ? 0 : -1;
+  const double scale = PyFloat_AS_DOUBLE(args[16]);
+  if (code < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || width < 2 || page < 1 || !(scale > 0.0) || q.dim() != 2 ||
+      q.size(1) != heads * width || out.sizes() != q.sizes() || k.dim() != 4 || k.sizes() != v.sizes() || k.size(0) < 1 || k.size(0) > INT32_MAX ||
+      k.size(1) != kv_heads || k.size(2) != page || k.size(3) != width || table.dim() != 2 || table.size(1) < 1 || table.size(1) > INT32_MAX ||
+      cu.dim() != 1 || lengths.dim() != 1 || rows.dim() != 1 || rows.size(0) < 1 || groups.dim() != 2 || groups.size(1) != 2 ||
+      !THPVariable_Check(args[18]) || !THPVariable_Unpack(args[18]).is_cuda())
+    Py_RETURN_NONE;
+  const auto address = [](const at::Tensor& x) { return reinterpret_cast<I>(x.const_data_ptr()); };
+  if (entry[2] != nullptr && ((address(q) | address(out) | address(k) | address(v)) & 15) != 0) Py_RETURN_NONE;
+  I* const err = reinterpret_cast<I*>(THPVariable_Unpack(args[18]).mutable_data_ptr());
+  const float floats[MAX_FLOATS] = {static_cast<float>(scale)};
+  int rc = 0;
+  {
+    pybind11::gil_scoped_release free;
+    const at::Tensor scratch = at::empty({at[0]}, q.options().dtype(at::kFloat).requires_grad(false));
+    const auto call = [&](void* fn, std::initializer_list<I> ends) {
+      if (fn == nullptr || rc != 0) return;
+      I ints[MAX_INTS] = {};
+      int m = 0;
+      for (I x : {address(q), address(k), address(v)}) ints[m++] = x;
+      if (fn != entry[1]) ints[m++] = address(out);
+      for (I x : {address(scratch), address(table), table.size(1), address(cu), address(lengths), address(rows), rows.size(0), address(groups),
+                  groups.size(0), heads, kv_heads, page, k.size(0)})
+        ints[m++] = x;
+      for (I x : ends) ints[m++] = x;
+      ints[m++] = reinterpret_cast<I>(err);
+      ints[m++] = stream;
+      rc = invoke(fn, ints, m, floats);
+    };
+    call(entry[0], {at[1], at[2], at[3], code, width});
+    call(entry[1], {at[1], at[3], at[4]});
+    call(entry[2], {at[1], at[5], at[6]});
+  }
+  return PyLong_FromLong(rc);
+  END_HANDLE_TH_ERRORS
+}
+
 // ---- recordings
 struct RecordingObject {
   PyObject_HEAD
@@ -458,6 +533,7 @@ PyMethodDef methods[] = {
     {"all_contiguous", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(all_contiguous)), METH_FASTCALL, "whether every tensor (None counts as one) is contiguous"},
     {"empty", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(empty)), METH_FASTCALL, "empty(shape, dtype, device)"},
     {"byte_product", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(byte_product)), METH_FASTCALL, "a product in 8 bits: (out, code, kernels), or None"},
+    {"prefix_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prefix_attention)), METH_FASTCALL, "decode attention behind shared prefixes: a code, or None"},
     {"mm_t", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mm_t)), METH_FASTCALL, "mm_t(x, w): x . w^T"},
     {nullptr, nullptr, 0, nullptr}};
 

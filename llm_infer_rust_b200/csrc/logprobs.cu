@@ -22,9 +22,7 @@
 
 namespace cg = cooperative_groups;
 
-constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int CHUNKS = 4;                 // of a thread; its elements are dealt to them in turn of iterations
-constexpr int UNROLL = 4;                 // 16-byte loads of a thread on their way
 constexpr int MOST_TOP = 32;              // a list of the best is a register of a warp's lanes
 constexpr int MOST_CLUSTER = 8;
 typedef unsigned long long u64;
@@ -81,7 +79,7 @@ __device__ __forceinline__ void insert_all(K& list, K mine, bool have, int last)
   }
 }
 // The CTA's warps join their lists; all hold the result.  `sh`: [WARPS][32].
-template <typename K>
+template <int WARPS, typename K>
 __device__ K join_warps(K list, K* sh) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -133,11 +131,11 @@ __device__ __forceinline__ Sums sums_from(const Sums& a, int step) {
   return {__shfl_xor_sync(0xffffffffu, a.m, step), __shfl_xor_sync(0xffffffffu, a.s, step), __shfl_xor_sync(0xffffffffu, a.w, step)};
 }
 
+template <int THREADS>
 struct Shared {
-  union {
-    float maxima[WARPS * 32];
-    u64 keys[WARPS * 32];
-  };
+  static constexpr int WARPS = THREADS / 32;
+  float maxima[64];
+  u64 keys[WARPS * 32];
   int chunks[CHUNKS * THREADS];           // those whose maximum reaches the k-th largest
   int count;
   Sums sums[WARPS];
@@ -147,11 +145,14 @@ struct Shared {
 };
 
 // grid: rows x cluster.  A row's elements: up to three in front of the first 16-byte boundary, vectors of four, up to three behind.
-__global__ void __launch_bounds__(THREADS, 2)
+// UNROLL: 16-byte loads of a thread on their way.
+template <int THREADS, int UNROLL>
+__global__ void __launch_bounds__(THREADS)
 logprobs_kernel(const float* __restrict__ logits, long long row_stride, int vocab, const int* __restrict__ tokens, int top,
                 int cluster, float* __restrict__ logprobs, float* __restrict__ entropy, int* __restrict__ top_ids,
                 float* __restrict__ top_logprobs, int* err) {
-  __shared__ Shared sh;
+  constexpr int WARPS = THREADS / 32;
+  __shared__ Shared<THREADS> sh;
   const int rank = static_cast<int>(blockIdx.x % cluster);
   const long long row_index = blockIdx.x / cluster;
   const float* row = logits + row_index * row_stride;
@@ -221,11 +222,16 @@ logprobs_kernel(const float* __restrict__ logits, long long row_stride, int voca
 
   u64 best = 0;                                               // (0: nothing)
   if (top > 0) {
-    // the top-th largest of the chunks' maxima
-    float list = sort_lanes(maxima[0]);
+    // A value that at least `top` chunks reach, and as few others as can be: the top-th largest of 64 parts of the CTA's maxima.
+    float mx = maxima[0];
 #pragma unroll
-    for (int c = 1; c < CHUNKS; ++c) insert_all(list, maxima[c], true, top - 1);
-    list = join_warps(list, sh.maxima);
+    for (int c = 1; c < CHUNKS; ++c) mx = fmaxf(mx, maxima[c]);
+    constexpr int PARTS = 64 / WARPS;            // of a warp
+#pragma unroll
+    for (int step = 16 / PARTS; step > 0; step >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, step));
+    if (lane % (32 / PARTS) == 0) sh.maxima[warp * PARTS + lane / (32 / PARTS)] = mx;
+    __syncthreads();
+    const float list = join_lists(sort_lanes(sh.maxima[lane]), __shfl_xor_sync(0xffffffffu, sort_lanes(sh.maxima[32 + lane]), 31));
     const float reach = __shfl_sync(0xffffffffu, list, top - 1);
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c)
@@ -246,8 +252,7 @@ logprobs_kernel(const float* __restrict__ logits, long long row_stride, int voca
         insert_all(best, key_of(v, id), inside && v >= reach, top - 1);
       }
     }
-    __syncthreads();                                          // (the maxima's lists have been read)
-    best = join_warps(best, sh.keys);
+    best = join_warps<WARPS>(best, sh.keys);
   } else {
     __syncthreads();
   }
@@ -263,11 +268,10 @@ logprobs_kernel(const float* __restrict__ logits, long long row_stride, int voca
       *all.map_shared_rank(&sh.best[rank][lane], 0) = best;
     }
     all.sync();
-    if (rank != 0 || warp != 0) return;
+    if (rank != 0) return;
     a = {-INFINITY, 0.0f, 0.0f};
     for (int r = 0; r < cluster; ++r) add_to(a, sh.parts[r]);
-    best = sh.best[0][lane];
-    for (int r = 1; r < cluster; ++r) best = join_lists(best, sh.best[r][31 - lane]);
+    if (top > 0) best = join_warps<WARPS>(warp < cluster ? sh.best[warp][lane] : 0ull, sh.keys);
   }
   if (warp != 0) return;
   const float log_s = logf(a.s);
@@ -284,7 +288,7 @@ logprobs_kernel(const float* __restrict__ logits, long long row_stride, int voca
 // CTAs that share a row: clusters while rows are few, so that all SMs read.
 static int cluster_of(int rows, int vocab, int sms) {
   int cluster = 1;
-  while (cluster < MOST_CLUSTER && 2 * cluster * rows <= 2 * sms && vocab / (2 * cluster) >= 4 * THREADS) cluster *= 2;
+  while (cluster < MOST_CLUSTER && 2 * cluster * rows <= sms && vocab / (2 * cluster) >= 4096) cluster *= 2;
   return cluster;
 }
 
@@ -294,7 +298,7 @@ B200_EXPORT int b200_token_logprobs(const float* logits, long long row_stride, i
                                     cudaStream_t stream) {
   if (rows == 0) return 0;
   if (rows < 0 || vocab <= 0 || top < 0 || top > MOST_TOP || top > vocab || (rows > 1 && row_stride < vocab)) return B200_BAD_SIZE;
-  if (vocab > INT32_MAX - 4 * UNROLL * THREADS * MOST_CLUSTER || rows > INT32_MAX / MOST_CLUSTER) return B200_BAD_SIZE;
+  if (vocab > INT32_MAX - (1 << 20) || rows > INT32_MAX / MOST_CLUSTER) return B200_BAD_SIZE;
   if (logits == nullptr || entropy == nullptr || err == nullptr || (tokens != nullptr && logprobs == nullptr) ||
       (top > 0 && (top_ids == nullptr || top_logprobs == nullptr)))
     return B200_BAD_SIZE;
@@ -305,7 +309,10 @@ B200_EXPORT int b200_token_logprobs(const float* logits, long long row_stride, i
   const int cluster = cluster_of(rows, vocab, sms);
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(rows) * cluster);
-  config.blockDim = dim3(THREADS);
+  // Many rows: small CTAs, so that some read while others sort (the pass over a row is then four in five of a CTA's time).  Few: a
+  // thread has all of its elements on their way at once where it can.
+  const bool many = rows >= 2 * sms;
+  config.blockDim = dim3(many ? 256 : 512);
   config.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -314,6 +321,7 @@ B200_EXPORT int b200_token_logprobs(const float* logits, long long row_stride, i
   attr[0].val.clusterDim.z = 1;
   config.attrs = attr;
   config.numAttrs = cluster > 1 ? 1 : 0;
-  e = cudaLaunchKernelEx(&config, logprobs_kernel, logits, row_stride, vocab, tokens, top, cluster, logprobs, entropy, top_ids, top_logprobs, err);
+  e = cudaLaunchKernelEx(&config, many ? logprobs_kernel<256, 4> : logprobs_kernel<512, 8>, logits, row_stride, vocab, tokens, top, cluster, logprobs,
+                         entropy, top_ids, top_logprobs, err);
   return e == cudaSuccess ? b200_check_launch() : static_cast<int>(e);
 }
