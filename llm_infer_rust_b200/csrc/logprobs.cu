@@ -22,7 +22,7 @@
 
 namespace cg = cooperative_groups;
 
-constexpr int CHUNKS = 4;                 // of a thread; its elements are dealt to them in turn of iterations
+constexpr int CHUNKS = 8;                 // of a thread; its elements are dealt to them in turn of iterations
 constexpr int MOST_TOP = 32;              // a list of the best is a register of a warp's lanes
 constexpr int MOST_CLUSTER = 8;
 typedef unsigned long long u64;
@@ -146,8 +146,8 @@ struct Shared {
 
 // grid: rows x cluster.  A row's elements: up to three in front of the first 16-byte boundary, vectors of four, up to three behind.
 // UNROLL: 16-byte loads of a thread on their way.
-template <int THREADS, int UNROLL>
-__global__ void __launch_bounds__(THREADS)
+template <int THREADS, int UNROLL, int CTAS>
+__global__ void __launch_bounds__(THREADS, CTAS)
 logprobs_kernel(const float* __restrict__ logits, long long row_stride, int vocab, const int* __restrict__ tokens, int top,
                 int cluster, float* __restrict__ logprobs, float* __restrict__ entropy, int* __restrict__ top_ids,
                 float* __restrict__ top_logprobs, int* err) {
@@ -239,18 +239,27 @@ logprobs_kernel(const float* __restrict__ logits, long long row_stride, int voca
     __syncthreads();
     // the chunks' elements (in whatever order they stand there: a list of distinct keys does not depend on it)
     if (warp == 0) insert_all(best, has_loose ? key_of(loose_value, loose_id) : 0ull, has_loose && loose_value == loose_value, top - 1);
-    const int found = sh.count;
-    for (int i = warp; i < found; i += WARPS) {
-      const int c = sh.chunks[i] / THREADS, thread = sh.chunks[i] % THREADS;
-      const int first = c * turns_a_chunk, elements = (min(turns, first + turns_a_chunk) - first) * UNROLL * 4;
-      for (int e0 = 0; e0 < elements; e0 += 32) {
-        const int e = e0 + lane;
-        const int at = begin + (first + e / (UNROLL * 4)) * UNROLL * THREADS + e / 4 % UNROLL * THREADS + thread;
-        const bool inside = e < elements && at < end;
-        const int id = front + 4 * at + e % 4;
-        const float v = inside ? __ldg(row + id) : 0.0f;
-        insert_all(best, key_of(v, id), inside && v >= reach, top - 1);
+    // (all warps share all chunks' elements, AGAIN loads of a lane on their way: one chunk a warp, one load behind the other, were 30 us
+    // more for 2,048 rows of 151,936)
+    constexpr int AGAIN = 4;
+    const int elements = turns_a_chunk * UNROLL * 4, all = sh.count * elements;
+    for (int x0 = warp * 32; x0 < all; x0 += AGAIN * THREADS) {
+      float v[AGAIN];
+      int id[AGAIN];
+#pragma unroll
+      for (int y = 0; y < AGAIN; ++y) {
+        const int x = x0 + y * THREADS + lane;
+        id[y] = -1;
+        if (x < all) {
+          const int i = x / elements, e = x - i * elements, chunk = sh.chunks[i];
+          const int turn = chunk / THREADS * turns_a_chunk + e / (UNROLL * 4);
+          const int at = begin + turn * UNROLL * THREADS + e / 4 % UNROLL * THREADS + chunk % THREADS;
+          if (turn < turns && at < end) id[y] = front + 4 * at + e % 4;
+        }
+        if (id[y] >= 0) v[y] = __ldg(row + id[y]);
       }
+#pragma unroll
+      for (int y = 0; y < AGAIN; ++y) insert_all(best, id[y] >= 0 ? key_of(v[y], id[y]) : 0ull, id[y] >= 0 && v[y] >= reach, top - 1);
     }
     best = join_warps<WARPS>(best, sh.keys);
   } else {
@@ -309,10 +318,11 @@ B200_EXPORT int b200_token_logprobs(const float* logits, long long row_stride, i
   const int cluster = cluster_of(rows, vocab, sms);
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(rows) * cluster);
-  // Many rows: small CTAs, so that some read while others sort (the pass over a row is then four in five of a CTA's time).  Few: a
-  // thread has all of its elements on their way at once where it can.
-  const bool many = rows >= 2 * sms;
-  config.blockDim = dim3(many ? 256 : 512);
+  // Few rows: a thread has all of its elements on their way at once where it can.  Many: 1,536 threads an SM, so that some CTAs read
+  // while others sort; long rows in CTAs of 512 threads, short ones in 256 (2,048 rows of 151,936 with 20 alternatives: 212 us
+  // against 219, of 32,000 with 5: 72 against 63; without alternatives the first take 190, their bytes at the copy rate).
+  const bool many = rows >= 2 * sms, small = many && vocab < 65536;
+  config.blockDim = dim3(small ? 256 : 512);
   config.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -321,7 +331,7 @@ B200_EXPORT int b200_token_logprobs(const float* logits, long long row_stride, i
   attr[0].val.clusterDim.z = 1;
   config.attrs = attr;
   config.numAttrs = cluster > 1 ? 1 : 0;
-  e = cudaLaunchKernelEx(&config, many ? logprobs_kernel<256, 4> : logprobs_kernel<512, 8>, logits, row_stride, vocab, tokens, top, cluster, logprobs,
+  e = cudaLaunchKernelEx(&config, small ? logprobs_kernel<256, 4, 6> : many ? logprobs_kernel<512, 4, 3> : logprobs_kernel<512, 8, 1>, logits, row_stride, vocab, tokens, top, cluster, logprobs,
                          entropy, top_ids, top_logprobs, err);
   return e == cudaSuccess ? b200_check_launch() : static_cast<int>(e);
 }
