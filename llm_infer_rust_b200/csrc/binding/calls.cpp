@@ -381,6 +381,51 @@ PyObject* prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// token_logprobs(entry point, logits, tokens or None, top, device, error word, stream) -> (log probabilities or None, entropy, ids, log
+// probabilities of the ids, code)
+// Log probabilities (csrc/logprobs.cu) as one call: what the tensors must be, the outputs and the launch.  None, and nothing done, where
+// something is not as it should be (the wrapper then says what) or this thread records its calls.  (Through Python four outputs and the
+// call took the host 11 us.)
+PyObject* token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7 || Py_TYPE(args[0]) != &entry_type || !PyLong_Check(args[3]) || !PyLong_Check(args[4]) || !THPVariable_Check(args[5]) || !PyLong_Check(args[6])) {
+    PyErr_SetString(PyExc_TypeError, "token_logprobs(entry point, logits, tokens or None, top, device, error word, stream)");
+    return nullptr;
+  }
+  if (recording != nullptr || !THPVariable_Check(args[1]) || !(args[2] == Py_None || THPVariable_Check(args[2]))) Py_RETURN_NONE;
+  const at::Tensor& logits = THPVariable_Unpack(args[1]);
+  const at::Tensor* tokens = args[2] == Py_None ? nullptr : &THPVariable_Unpack(args[2]);
+  const I top = PyLong_AsLongLong(args[3]), device = PyLong_AsLongLong(args[4]), stream = PyLong_AsLongLong(args[6]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!logits.is_cuda() || logits.get_device() != device || logits.scalar_type() != at::kFloat || logits.dim() != 2) Py_RETURN_NONE;
+  const I rows = logits.size(0), vocab = logits.size(1), between = rows > 1 ? logits.stride(0) : vocab;
+  if (rows < 1 || rows > INT32_MAX || vocab < 1 || vocab > INT32_MAX || (vocab > 1 && logits.stride(1) != 1) || between < vocab || top < 0 ||
+      top > vocab || top > 32)
+    Py_RETURN_NONE;
+  if (tokens != nullptr && (!tokens->is_cuda() || tokens->get_device() != device || tokens->scalar_type() != at::kInt || tokens->dim() != 1 ||
+                            tokens->size(0) != rows || !tokens->is_contiguous()))
+    Py_RETURN_NONE;
+  I* const err = reinterpret_cast<I*>(THPVariable_Unpack(args[5]).mutable_data_ptr());
+  at::Tensor chosen, entropy, ids, best;
+  int rc;
+  {
+    pybind11::gil_scoped_release free;
+    const auto floats = logits.options().requires_grad(false);
+    if (tokens != nullptr) chosen = at::empty({rows}, floats);
+    entropy = at::empty({rows}, floats);
+    ids = at::empty({rows, top}, floats.dtype(at::kInt));
+    best = at::empty({rows, top}, floats);
+    const auto address = [](const at::Tensor& t) { return reinterpret_cast<I>(t.const_data_ptr()); };
+    I ints[MAX_INTS] = {address(logits), between, rows, vocab, tokens != nullptr ? address(*tokens) : 0, top, tokens != nullptr ? address(chosen) : 0,
+                        address(entropy), address(ids), address(best), reinterpret_cast<I>(err), stream};
+    const float none[MAX_FLOATS] = {};
+    rc = invoke(reinterpret_cast<Entry*>(args[0])->fn, ints, 12, none);
+  }
+  PyObject* first = tokens != nullptr ? THPVariable_Wrap(chosen) : Py_NewRef(Py_None);
+  return Py_BuildValue("NNNNi", first, THPVariable_Wrap(entropy), THPVariable_Wrap(ids), THPVariable_Wrap(best), rc);
+  END_HANDLE_TH_ERRORS
+}
+
 // ---- recordings
 struct RecordingObject {
   PyObject_HEAD
@@ -534,6 +579,7 @@ PyMethodDef methods[] = {
     {"empty", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(empty)), METH_FASTCALL, "empty(shape, dtype, device)"},
     {"byte_product", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(byte_product)), METH_FASTCALL, "a product in 8 bits: (out, code, kernels), or None"},
     {"prefix_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prefix_attention)), METH_FASTCALL, "decode attention behind shared prefixes: a code, or None"},
+    {"token_logprobs", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(token_logprobs)), METH_FASTCALL, "log probabilities: four tensors and a code, or None"},
     {"mm_t", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mm_t)), METH_FASTCALL, "mm_t(x, w): x . w^T"},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -1635,6 +1635,7 @@ class TokenLogprobs(NamedTuple):
 
 
 MAX_TOP_LOGPROBS = 32
+_logprobs_call = None            # of the compiled binding, which is loaded at the first call
 
 
 def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0) -> TokenLogprobs:
@@ -1644,8 +1645,20 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     -inf is a token that cannot come.  A row that holds a NaN or +inf, or -inf alone, has NaN for all its numbers (its ids still go
     by the logits that are no NaN; where those are too few they are -1).  A token outside the vocabulary has NaN and sets the
     error word (``check_errors``)."""
+    global _logprobs_call
+    if _held is not None or _chain is not None:
+        flush_chain()                            # (what waits in the chain may be what is read here)
+    entry = load_entry_points("logprobs.cu").b200_token_logprobs
+    if logits.is_cuda:
+        if _logprobs_call is None:
+            _logprobs_call = load_call_binding().token_logprobs
+        got = _logprobs_call(entry, logits, tokens, top, _current_device(), error_word(logits.device), _stream())
+        if got is not None:
+            _ok(got[4], "token_logprobs")
+            return TokenLogprobs(*got[:4])
+    # No rows, a layer's calls that are being kept, or something that is not as it should be.
     _cuda(logits, tokens)
-    if logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
+    if logits.dtype != torch.float32 or logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1) or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
         raise KernelError("token_logprobs takes float32 logits [rows, vocab] with unit inner stride")
     rows, vocab = logits.shape
     if not 0 <= top <= min(MAX_TOP_LOGPROBS, vocab):
@@ -1659,8 +1672,7 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     chosen = None if tokens is None else _empty((rows,), torch.float32, device)
     entropy = _empty((rows,), torch.float32, device)
     ids, best = _empty((rows, top), torch.int32, device), _empty((rows, top), torch.float32, device)
-    rc = load_entry_points("logprobs.cu").b200_token_logprobs(logits, logits.stride(0) if rows > 1 else vocab, rows, vocab, tokens, top, chosen,
-                                                              entropy, ids, best, error_word(device), _stream())
+    rc = entry(logits, logits.stride(0) if rows > 1 else vocab, rows, vocab, tokens, top, chosen, entropy, ids, best, error_word(device), _stream())
     _ok(rc, "token_logprobs", int(rows > 0))
     return TokenLogprobs(chosen, entropy, ids, best)
 
