@@ -3,8 +3,8 @@ parts so that another architecture is a registry entry.
 
 Public entry points:
 
-* ``Engine(model_path, ...)`` with ``generate(prompts, sampling_params)`` and the
-  step function ``step(entries)``;
+* ``Engine(model_path, ...)`` with ``generate(prompts, sampling_params)``, ``answers(prompt, n)``,
+  ``score(tokens)``, the step function ``step(entries)`` and ``fork_request(parent, children)``;
 * ``write_random_model(folder, config, seed)``: the random-weights mode;
 * ``python -m llm_infer_rust_b200 --model-path DIR ...``: the command line;
 * ``bin/trace_run``: trace replay.
@@ -15,7 +15,7 @@ when an engine first needs them.
 from .config import (Architecture, ConfigError, ModelSpec, PartSpec, LayerSpec, RunEntry, Qwen3Config,
                      register_architecture, registered_architectures, resolve_architecture)
 from . import architectures  # noqa: F401
-from .sampling import SamplingParams
+from .sampling import SamplingParams, TokenLogprob
 from .weights.random_init import random_tensors, write_random_model
 
 
@@ -29,4 +29,4 @@ def __getattr__(name):
 
 __all__ = ["Architecture", "ConfigError", "ModelSpec", "PartSpec", "LayerSpec", "RunEntry", "Qwen3Config",
            "register_architecture", "registered_architectures", "resolve_architecture", "SamplingParams",
-           "random_tensors", "write_random_model", "Engine", "StepEntry", "GenerationResult"]
+           "random_tensors", "write_random_model", "Engine", "StepEntry", "GenerationResult", "TokenLogprob"]

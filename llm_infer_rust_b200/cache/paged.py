@@ -27,6 +27,7 @@ from typing import Dict, List, Optional
 import torch
 
 from ..kernels.build import load_host_runtime
+from ..kernels.pages import PageCopier
 
 
 @dataclass
@@ -178,6 +179,27 @@ class PagedCache:
         self.embedding = LayerCache()
         for name, spec in plan.embedding_states.items():
             self.embedding.states[name] = torch.zeros((max_requests + 1,) + tuple(spec.shape), dtype=spec.dtype, device=device)
+
+        self._copiers: Optional[tuple] = None
+
+    def copy_fork(self, copies: List[tuple]) -> None:
+        """Copies on the device what forks have to (``CacheManager.fork``'s pages and state slots, one pair a fork), in all layers."""
+        if self._copiers is None:
+            of_group = []
+            for g in range(len(self.plan.groups)):
+                caches = [c for c in self.layer_caches if c.writes and c.k is not None and c.group == g]
+                of_group.append(PageCopier([t for c in caches for t in (c.k, c.v) if t is not None]))
+            states = [t for c in self.layer_caches + [self.embedding] for t in ([c.state] if c.state is not None else []) + list(c.states.values())]
+            # (a slot's state as one slot of a page of its own)
+            states = [t.view(t.shape[0], 1, 1, -1) for t in states if t.numel()]
+            self._copiers = (of_group, PageCopier(states) if states else None)
+        of_group, states = self._copiers
+        for g, copier in enumerate(of_group):
+            moves = [tuple(m) for pages, _ in copies for m in pages[g]]
+            if moves:
+                copier.copy(moves)
+        if states is not None:
+            states.copy([(source, target, 1) for _, (source, target) in copies])
 
     def bytes(self) -> int:
         total = 0

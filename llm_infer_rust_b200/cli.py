@@ -42,6 +42,8 @@ backend, one way of uploading a step's index arrays):
 Prompts and sampling (token ids in, token ids out):
   --prompt-ids IDS          comma-separated token ids; may be given several times (else JSON lists on stdin)
   --temperature T  --top-k K  --top-p P  --max-tokens N  --ignore-eos  --seed S
+  --answers N               N answers to each prompt, one line each: the prompt runs once and its cached pages are shared (1)
+  --logprobs K              with every output token its log probability, the entropy and the K most likely tokens, 0 to 32 (none)
 Random-weights mode (writes the model folder, then serves it if prompts are given):
   --random-weights          write config.json and model.safetensors into --model-path
   --config PATH             config.json to build the random model from
@@ -96,6 +98,8 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--max-tokens", type=int, default=1024)
     p.add_argument("--ignore-eos", action="store_true")
     p.add_argument("--seed", type=int, default=0)
+    p.add_argument("--answers", type=int, default=1)
+    p.add_argument("--logprobs", type=int, default=None)
     p.add_argument("--random-weights", action="store_true")
     p.add_argument("--config")
     p.add_argument("--init-std", type=float, default=0.02)
@@ -140,6 +144,12 @@ def main(argv: Optional[List[str]] = None) -> int:
             raw = json.load(fh)
         write_random_model(args.model_path, raw, args.seed, std=args.init_std, norm_std=args.norm_std)
         print(f"wrote {args.model_path}/config.json and model.safetensors", file=sys.stderr)
+    if args.answers < 1 or args.answers > args.max_running_req:
+        print("--answers: 1 to --max-running-req", file=sys.stderr)
+        return 2
+    if args.logprobs is not None and not 0 <= args.logprobs <= 32:
+        print("--logprobs: 0 to 32 alternatives", file=sys.stderr)
+        return 2
     prompts = read_prompts(args)
     if not prompts:
         return 0
@@ -155,8 +165,14 @@ def main(argv: Optional[List[str]] = None) -> int:
                     cpu_gpu_overlap=not args.disable_cpu_gpu_overlap, seed=args.seed, log_level=args.log_level,
                     int8_projections=args.int8_projections)
     params = SamplingParams(args.temperature, args.top_k, args.top_p, args.ignore_eos, args.max_tokens,
-                            args.seed if args.seed else None)
-    for prompt, result in zip(prompts, engine.generate(prompts, params)):
-        print(json.dumps({"prompt_ids": prompt, "output_ids": result.tokens,
-                          "finish_reason": result.finish_reason}), flush=True)
+                            args.seed if args.seed else None, args.logprobs)
+    if args.answers > 1:
+        results = ((prompt, result) for prompt in prompts for result in engine.answers(prompt, args.answers, params))
+    else:
+        results = zip(prompts, engine.generate(prompts, params))
+    for prompt, result in results:
+        line = {"prompt_ids": prompt, "output_ids": result.tokens, "finish_reason": result.finish_reason}
+        if result.logprobs is not None:
+            line["logprobs"] = [{"token": t.token, "logprob": t.logprob, "entropy": t.entropy, "top": t.top} for t in result.logprobs]
+        print(json.dumps(line), flush=True)
     return 0

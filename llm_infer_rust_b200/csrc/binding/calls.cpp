@@ -399,7 +399,7 @@ PyObject* token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (PyErr_Occurred()) return nullptr;
   if (!logits.is_cuda() || logits.get_device() != device || logits.scalar_type() != at::kFloat || logits.dim() != 2) Py_RETURN_NONE;
   const I rows = logits.size(0), vocab = logits.size(1), between = rows > 1 ? logits.stride(0) : vocab;
-  if (rows < 1 || rows > INT32_MAX || vocab < 1 || vocab > INT32_MAX || (vocab > 1 && logits.stride(1) != 1) || between < vocab || top < 0 ||
+  if (rows < 1 || rows > INT32_MAX || vocab < 1 || vocab > INT32_MAX || (vocab > 1 && logits.stride(1) != 1) || top < 0 ||
       top > vocab || top > 32)
     Py_RETURN_NONE;
   if (tokens != nullptr && (!tokens->is_cuda() || tokens->get_device() != device || tokens->scalar_type() != at::kInt || tokens->dim() != 1 ||

@@ -8,6 +8,50 @@ namespace b200 {
 
 static int align4(int n) { return (n + 3) & ~3; }
 
+namespace {
+struct Shared {
+  std::vector<int> rows;      // of the batch
+  int keys = 0;               // whole pages that all of them hold
+};
+// Decode rows whose first page is the same one, with at least two rows: each such set shares the pages that all of its rows hold.
+std::vector<Shared> shared_rows(const CacheManager& cache, const BatchRequest& req) {
+  std::vector<Shared> found;
+  const int g = req.prefix_group;
+  if (g < 0) return found;
+  if (g >= cache.num_groups() || cache.group(g).window != 0) throw std::invalid_argument("rows share pages of a group that keeps all keys");
+  if (cache.shared_pages(g) == 0) return found;
+  std::vector<std::pair<int, int>> first;      // (first page, row)
+  for (int r = 0; r < static_cast<int>(req.ids.size()); ++r) {
+    if (req.counts[r] != 1) continue;
+    const std::vector<int>& table = cache.block_table(req.ids[r], g);
+    if (!table.empty() && cache.length(req.ids[r]) >= cache.group(g).page_size) first.emplace_back(table[0], r);
+  }
+  std::stable_sort(first.begin(), first.end(), [](const std::pair<int, int>& a, const std::pair<int, int>& b) { return a.first < b.first; });
+  const int P = cache.group(g).page_size;
+  for (size_t i = 0, j; i < first.size(); i = j) {
+    Shared s;
+    const std::vector<int>& lead = cache.block_table(req.ids[first[i].second], g);
+    int pages = cache.length(req.ids[first[i].second]) / P;
+    for (j = i; j < first.size() && first[j].first == first[i].first; ++j) {
+      const std::vector<int>& table = cache.block_table(req.ids[first[j].second], g);
+      const int most = std::min(pages, cache.length(req.ids[first[j].second]) / P);
+      pages = static_cast<int>(std::mismatch(lead.begin(), lead.begin() + most, table.begin()).first - lead.begin());
+      s.rows.push_back(first[j].second);
+    }
+    s.keys = pages * P;
+    if (s.rows.size() > 1) found.push_back(std::move(s));
+  }
+  return found;
+}
+}  // namespace
+
+std::pair<int, int> count_prefix_groups(const CacheManager& cache, const BatchRequest& req) {
+  int saved = 0;
+  const std::vector<Shared> shared = shared_rows(cache, req);
+  for (const Shared& s : shared) saved += (static_cast<int>(s.rows.size()) - 1) * s.keys;
+  return {static_cast<int>(shared.size()), saved};
+}
+
 BatchLayout plan_batch(const CacheManager& cache, const BatchRequest& req) {
   const int real = static_cast<int>(req.ids.size());
   if (static_cast<int>(req.counts.size()) != real || static_cast<int>(req.want_counts.size()) != real)
@@ -63,6 +107,12 @@ BatchLayout plan_batch(const CacheManager& cache, const BatchRequest& req) {
     L.table_width.push_back(width);
     L.off_slots.push_back(take(L.num_tokens));
     L.off_table.push_back(take(L.num_rows * width));
+  }
+  const int found = req.prefix_group < 0 || L.num_decode == 0 ? 0 : req.prefix_groups > 0 ? req.prefix_groups : count_prefix_groups(cache, req).first;
+  if (found > 0) {
+    L.num_prefix_groups = req.prefix_groups > 0 ? found : found + 1;
+    L.off_prefix_rows = take(L.num_decode);
+    L.off_prefix_groups = take(2 * L.num_prefix_groups);
   }
   L.total_ints = off;
   return L;
@@ -126,6 +176,35 @@ BatchLayout build_batch(const CacheManager& cache, const BatchRequest& req, int3
   std::copy(out + L.off_decode_rows, out + L.off_decode_rows + n_dec, order);
   const int32_t* kv_len = out + L.off_kv_len;
   std::sort(order, order + n_dec, [kv_len](int32_t a, int32_t b) { return kv_len[a] != kv_len[b] ? kv_len[a] > kv_len[b] : a < b; });
+  if (L.num_prefix_groups > 0) {
+    const std::vector<Shared> shared = shared_rows(cache, req);
+    if (static_cast<int>(shared.size()) >= L.num_prefix_groups) throw std::length_error("more groups of rows share pages than the batch has places for");
+    std::vector<char> taken(L.num_rows, 0);
+    int32_t* rows = out + L.off_prefix_rows;
+    int32_t* groups = out + L.off_prefix_groups;
+    int at = 0, group = 0;
+    for (const Shared& s : shared) {
+      groups[2 * group] = at;
+      groups[2 * group++ + 1] = s.keys;
+      for (int r : s.rows) {
+        rows[at++] = r;
+        taken[r] = 1;
+        L.most_own_keys = std::max(L.most_own_keys, kv_len[r] - s.keys);
+      }
+      L.most_prefix_rows = std::max(L.most_prefix_rows, static_cast<int>(s.rows.size()));
+      L.most_prefix_keys = std::max(L.most_prefix_keys, s.keys);
+    }
+    for (int g = group; g < L.num_prefix_groups; ++g) {      // the other rows share nothing; places that are left hold no rows
+      groups[2 * g] = at;
+      groups[2 * g + 1] = 0;
+    }
+    for (int d = 0; d < n_dec; ++d) {
+      const int r = out[L.off_decode_rows + d];
+      if (taken[r]) continue;
+      rows[at++] = r;
+      L.most_own_keys = std::max(L.most_own_keys, kv_len[r]);
+    }
+  }
   return L;
 }
 

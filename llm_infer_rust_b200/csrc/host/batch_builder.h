@@ -10,6 +10,7 @@
 // block table per cache group.
 #pragma once
 #include <cstdint>
+#include <utility>
 #include <vector>
 
 #include "page_cache.h"
@@ -32,6 +33,12 @@ struct BatchLayout {
   std::vector<int> off_slots;     // per group: write slot of every token
   std::vector<int> off_table;     // per group: block table [num_rows, table_width]
   std::vector<int> table_width;   // per group
+  // Decode rows that hold the same first pages, for attention that reads them once (kernels/prefix.py); 0 groups: none was looked for
+  // or found.  The last group shares nothing and holds the other decode rows.
+  int num_prefix_groups = 0;
+  int off_prefix_rows = 0;        // the decode rows, group by group
+  int off_prefix_groups = 0;      // (index of the group's first row, shared keys) of each group
+  int most_prefix_rows = 0, most_prefix_keys = 0, most_own_keys = 0;      // of a group, of a group, of a row behind its group's
   int total_ints = 0;
 };
 
@@ -43,8 +50,13 @@ struct BatchRequest {
   std::vector<int> want_index;    // concatenated indices within the row's tokens
   int pad_rows_to = 0;            // > 0: add one-token padding rows (sink page, state slot 0) up to this many rows
   std::vector<int> fixed_table_width;   // per group; empty: as narrow as this batch allows
+  int prefix_group = -1;          // cache group whose pages decode rows may share (a group that keeps all keys); -1: not looked for
+  int prefix_groups = 0;          // > 0: places for exactly so many groups (a graph's), those that are not used hold no rows
 };
 
+// How many groups of decode rows of `req` share pages in its prefix_group (not counting the last one, of the other rows), and how many
+// keys their rows need not read again, summed over the rows.
+std::pair<int, int> count_prefix_groups(const CacheManager& cache, const BatchRequest& req);
 // Number of int32 the buffer must hold, without writing anything.
 BatchLayout plan_batch(const CacheManager& cache, const BatchRequest& req);
 // Fill `out` (capacity in int32).  Pages must already cover every row

@@ -28,7 +28,9 @@ PYBIND11_MODULE(_host_runtime, m) {
   py::class_<PagePool>(m, "PagePool")
       .def(py::init<int>())
       .def("alloc", &PagePool::alloc)
+      .def("share", &PagePool::share)
       .def("release", &PagePool::release)
+      .def("holders", &PagePool::holders)
       .def("free_count", &PagePool::free_count)
       .def("is_held", &PagePool::is_held)
       .def("free_list", &PagePool::free_list);
@@ -45,6 +47,12 @@ PYBIND11_MODULE(_host_runtime, m) {
       .def("pages_needed", &CacheManager::pages_needed)
       .def("acquire", &CacheManager::acquire, py::arg("id"), py::arg("capacity_tokens"), py::arg("max_step_tokens"))
       .def("open", &CacheManager::open)
+      .def("fork", [](CacheManager& c, int64_t parent, int64_t child) {
+             ForkCopies copies;
+             const Acquire got = c.fork(parent, child, copies);
+             return py::make_tuple(got, copies.pages, copies.state);
+           }, py::arg("parent"), py::arg("child"), "(result, pages to copy of each group: (source, target, slots), state slots: (source, target))")
+      .def("shared_pages", &CacheManager::shared_pages)
       .def("grow", &CacheManager::grow)
       .def("grow_all", &CacheManager::grow_all)
       .def("advance", &CacheManager::advance)
@@ -147,6 +155,12 @@ PYBIND11_MODULE(_host_runtime, m) {
       .def_readonly("off_slots", &BatchLayout::off_slots)
       .def_readonly("off_table", &BatchLayout::off_table)
       .def_readonly("table_width", &BatchLayout::table_width)
+      .def_readonly("num_prefix_groups", &BatchLayout::num_prefix_groups)
+      .def_readonly("off_prefix_rows", &BatchLayout::off_prefix_rows)
+      .def_readonly("off_prefix_groups", &BatchLayout::off_prefix_groups)
+      .def_readonly("most_prefix_rows", &BatchLayout::most_prefix_rows)
+      .def_readonly("most_prefix_keys", &BatchLayout::most_prefix_keys)
+      .def_readonly("most_own_keys", &BatchLayout::most_own_keys)
       .def_readonly("total_ints", &BatchLayout::total_ints);
 
   py::class_<BatchRequest>(m, "BatchRequest")
@@ -157,7 +171,11 @@ PYBIND11_MODULE(_host_runtime, m) {
       .def_readwrite("want_counts", &BatchRequest::want_counts)
       .def_readwrite("want_index", &BatchRequest::want_index)
       .def_readwrite("pad_rows_to", &BatchRequest::pad_rows_to)
-      .def_readwrite("fixed_table_width", &BatchRequest::fixed_table_width);
+      .def_readwrite("fixed_table_width", &BatchRequest::fixed_table_width)
+      .def_readwrite("prefix_group", &BatchRequest::prefix_group)
+      .def_readwrite("prefix_groups", &BatchRequest::prefix_groups);
+
+  m.def("count_prefix_groups", &count_prefix_groups);
 
   m.def("plan_batch", &plan_batch);
   m.def("build_batch", [](const CacheManager& cache, const BatchRequest& req,

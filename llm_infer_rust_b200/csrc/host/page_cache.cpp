@@ -22,10 +22,15 @@ int PagePool::alloc() {
   return page;
 }
 
+void PagePool::share(int page) {
+  if (!is_held(page)) throw std::logic_error("a page that nobody holds cannot be shared");
+  if (++held_[page] == 2) ++shared_;
+}
+
 bool PagePool::release(int page) {
   if (page < 1 || page > num_pages_ || !held_[page]) return false;
-  held_[page] = 0;
-  free_.push_back(page);
+  if (held_[page] == 2) --shared_;
+  if (--held_[page] == 0) free_.push_back(page);
   return true;
 }
 
@@ -80,6 +85,49 @@ Acquire CacheManager::acquire(int64_t id, int capacity_tokens, int max_step_toke
 }
 
 Acquire CacheManager::open(int64_t id) { return admit(id, std::vector<int>(specs_.size(), 0)); }
+
+Acquire CacheManager::fork(int64_t parent, int64_t child, ForkCopies& copies) {
+  copies = ForkCopies();
+  const RequestCache& from = requests_.at(parent);
+  for (size_t g = 0; g < specs_.size(); ++g)
+    if (from.groups[g].promise_cap != 0) throw std::invalid_argument("a request that was admitted with a promise of pages cannot be forked");
+  // the page that the parent has begun, where there is one: the child's copy of it has to be free
+  auto begun = [&](size_t g) {
+    const int P = specs_[g].page_size, lp = from.length / P;
+    return from.length % P != 0 && lp < static_cast<int>(from.groups[g].table.size()) && from.groups[g].table[lp] != 0 ? lp : -1;
+  };
+  if (requests_.count(child)) throw std::invalid_argument("request id is already live");
+  for (size_t g = 0; g < specs_.size(); ++g)
+    if (begun(g) >= 0 && unpromised_pages(static_cast<int>(g)) < 1) return Acquire::DeferredMemory;
+  const Acquire got = admit(child, std::vector<int>(specs_.size(), 0));
+  if (got != Acquire::Ready) return got;
+  const RequestCache& source = requests_.at(parent);          // (the table of requests may have moved)
+  RequestCache& to = requests_.at(child);
+  to.length = source.length;
+  copies.state = {source.state_slot, to.state_slot};
+  copies.pages.resize(specs_.size());
+  for (size_t g = 0; g < specs_.size(); ++g) {
+    const GroupPages& have = source.groups[g];
+    GroupPages& gp = to.groups[g];
+    const int P = specs_[g].page_size, whole = source.length / P;
+    const int pages = std::min(ceil_div(source.length, P), static_cast<int>(have.table.size()));
+    gp.first_live = have.first_live;
+    gp.table.assign(pages, 0);
+    for (int lp = 0; lp < pages; ++lp) {
+      if (have.table[lp] == 0) continue;
+      if (lp < whole) {
+        pools_[g].share(have.table[lp]);
+        gp.table[lp] = have.table[lp];
+      } else {
+        gp.table[lp] = pools_[g].alloc();
+        if (gp.table[lp] < 0) throw std::logic_error("page accounting is broken: pool empty after the check");
+        copies.pages[g].push_back({have.table[lp], gp.table[lp], source.length % P});
+      }
+      gp.held += 1;
+    }
+  }
+  return Acquire::Ready;
+}
 
 bool CacheManager::grow(int64_t id, int new_length) {
   RequestCache& rc = requests_.at(id);
@@ -211,7 +259,8 @@ std::string CacheManager::check() const {
     }
     for (int page = 1; page <= pool.num_pages(); ++page) {
       if (seen[page] == 0) err << "group " << g << ": page " << page << " is lost; ";
-      if (seen[page] > 1) err << "group " << g << ": page " << page << " is held " << seen[page] << " times; ";
+      const int times = std::max(1, pool.holders(page));
+      if (seen[page] > 0 && seen[page] != times) err << "group " << g << ": page " << page << " is held " << seen[page] << " times, counts " << times << "; ";
     }
     if (promised != promised_total_[g]) err << "group " << g << ": promises sum to " << promised << ", counter says " << promised_total_[g] << "; ";
     if (promised_total_[g] > pool.free_count()) err << "group " << g << ": more pages promised than free; ";

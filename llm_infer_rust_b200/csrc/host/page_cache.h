@@ -14,9 +14,13 @@
 // while the request still runs.  A request may hold a PROMISE of pages
 // (reserved at admission, taken later): a page that is promised to one request
 // is never handed to another, so a running request cannot run out of pages.
+// A request may be FORKED: its child shares the whole pages that the request holds (a page counts its holders and is free
+// again when the last one gives it up) and gets a copy of the page that the request has begun, so that both go on writing where
+// they are.  What has to be copied on the device is handed out as a list of moves.
 // Fixed-size state slots (one per live request, slot 0 is the sink for padding
 // rows) are handed out and taken back together with the pages.
 #pragma once
+#include <array>
 #include <cstdint>
 #include <string>
 #include <unordered_map>
@@ -35,17 +39,27 @@ enum class Acquire : int { Ready = 0, DeferredMemory = 1, Impossible = 2, Deferr
 class PagePool {
  public:
   explicit PagePool(int num_pages);
-  int alloc();                 // -1 when empty
-  bool release(int page);      // false: not held (freeing twice or a foreign id is refused)
+  int alloc();                 // -1 when empty; the page has one holder
+  void share(int page);        // one holder more
+  bool release(int page);      // one holder less, free with the last; false: not held (freeing twice or a foreign id is refused)
   int free_count() const { return static_cast<int>(free_.size()); }
   int num_pages() const { return num_pages_; }
-  bool is_held(int page) const { return page >= 1 && page <= num_pages_ && held_[page]; }
+  int holders(int page) const { return page >= 1 && page <= num_pages_ ? held_[page] : 0; }
+  bool is_held(int page) const { return holders(page) > 0; }
+  int shared_count() const { return shared_; }      // pages with more than one holder
   const std::vector<int>& free_list() const { return free_; }
 
  private:
   int num_pages_;
   std::vector<int> free_;
-  std::vector<uint8_t> held_;
+  std::vector<int> held_;      // holders of each page
+  int shared_ = 0;
+};
+
+// What a fork has to copy: of each cache group pages (source, target, slots) to copy, and the state slots (source, target).
+struct ForkCopies {
+  std::vector<std::vector<std::array<int, 3>>> pages;
+  std::array<int, 2> state = {0, 0};
 };
 
 struct GroupPages {
@@ -85,6 +99,13 @@ class CacheManager {
   // Admission without a promise: pages are taken as the request grows.
   Acquire open(int64_t id);
 
+  // Make `child` live as a copy of `parent` as it is now, without a promise: whole pages are shared, the begun one is copied (`copies`).
+  // Anything but Ready: nothing has changed.  A parent that was admitted with a promise is refused (invalid_argument): what it gives
+  // back to its promise as its window moves on would not be free while the child holds it.
+  Acquire fork(int64_t parent, int64_t child, ForkCopies& copies);
+  // Pages of group g with more than one holder.
+  int shared_pages(int g) const { return pools_.at(g).shared_count(); }
+
   // Make pages cover positions [0, new_length) (windowed groups: from the
   // first live page).  False, and nothing changed, if a group cannot give them.
   bool grow(int64_t id, int new_length);
@@ -105,8 +126,8 @@ class CacheManager {
   // Flat slot of `position`; -1 if the page is not held.
   int slot_of(int64_t id, int g, int position) const;
 
-  // Empty if every page is either free once or held once by one request, the
-  // sink is nowhere, and the counters agree; else what is wrong.
+  // Empty if every page is either free once or held once by each of as many requests as
+  // it counts, the sink is nowhere, and the counters agree; else what is wrong.
   std::string check() const;
 
  private:

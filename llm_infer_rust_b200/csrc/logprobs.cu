@@ -306,7 +306,7 @@ B200_EXPORT int b200_token_logprobs(const float* logits, long long row_stride, i
                                     float* logprobs, float* entropy, int* top_ids, float* top_logprobs, int* err,
                                     cudaStream_t stream) {
   if (rows == 0) return 0;
-  if (rows < 0 || vocab <= 0 || top < 0 || top > MOST_TOP || top > vocab || (rows > 1 && row_stride < vocab)) return B200_BAD_SIZE;
+  if (rows < 0 || vocab <= 0 || top < 0 || top > MOST_TOP || top > vocab || row_stride < 0) return B200_BAD_SIZE;
   if (vocab > INT32_MAX - (1 << 20) || rows > INT32_MAX / MOST_CLUSTER) return B200_BAD_SIZE;
   if (logits == nullptr || entropy == nullptr || err == nullptr || (tokens != nullptr && logprobs == nullptr) ||
       (top > 0 && (top_ids == nullptr || top_logprobs == nullptr)))

@@ -9,6 +9,18 @@ import torch
 
 
 @dataclass
+class SharedPrefixes:
+    """Decode rows that hold the same first pages of cache group ``cache_group`` (``kernels/prefix.py`` has what the fields mean)."""
+    cache_group: int
+    rows: torch.Tensor
+    groups: torch.Tensor
+    most_rows: int
+    most_shared: int
+    most_own: int
+    sharing_groups: int
+
+
+@dataclass
 class StepContext:
     """One step's batch, as device int32 arrays (views of one buffer) plus host numbers.
 
@@ -46,6 +58,7 @@ class StepContext:
     kv_len_bound: int = 0
     scratch: Optional[Callable[[int], torch.Tensor]] = None
     sm_count: int = 148
+    shared: Optional[SharedPrefixes] = None      # None: every decode row reads its own keys
     extras: dict = field(default_factory=dict)
 
 

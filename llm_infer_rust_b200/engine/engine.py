@@ -27,13 +27,15 @@ from ..config.spec import ConfigError
 from ..kernels import ops
 from ..kernels.build import load_host_runtime
 from ..parts import DecoderModel, int8_projections as with_int8_projections
-from ..sampling import Sampler, SamplingParams
+from ..sampling import PendingLogprobs, Sampler, SamplingParams, TokenLogprob
 from ..weights.loader import load_weights, read_model_config
 from ..weights.random_init import bind_random_weights
-from .context import StepContext, context_from_layout
+from .context import SharedPrefixes, StepContext, context_from_layout
 
 _DTYPES = {"bfloat16": torch.bfloat16, "float32": torch.float32}
 log = logging.getLogger("llm_infer_rust_b200")
+# Decode rows read the pages that they share once from so many keys on that they need not read again (summed over the rows).
+_SAVED_KEYS_AT_LEAST = 4096
 
 
 @dataclass
@@ -49,6 +51,7 @@ class StepEntry:
 class GenerationResult:
     tokens: List[int]
     finish_reason: str
+    logprobs: Optional[List[TokenLogprob]] = None      # one a token, where the request's SamplingParams ask for them
 
 
 def auto_chunked_prefill_size(memory_mib: int) -> int:
@@ -111,8 +114,9 @@ class _MetaBuffers:
 
 
 class _DecodeGraph:
-    def __init__(self, bucket: int):
+    def __init__(self, bucket: int, prefix_groups: int = 0):
         self.bucket = bucket
+        self.prefix_groups = prefix_groups      # > 0: for rows that share pages, with places for so many groups of them
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.meta: Optional[torch.Tensor] = None
         self.ctx: Optional[StepContext] = None
@@ -127,6 +131,7 @@ class _Flight:
     plan: object
     ids: Optional[torch.Tensor]
     read: Optional[object]
+    logprobs: Optional[PendingLogprobs] = None
 
 
 class Engine:
@@ -254,6 +259,12 @@ class Engine:
         self._shape_graphs: "OrderedDict[tuple, _DecodeGraph]" = OrderedDict()
         self._shape_seen: Dict[tuple, int] = {}
         self._shape_graph_limit = 6
+        # Requests that share pages (forks): which cache group they are looked for in, and the graphs of their decode steps, keyed by
+        # (rows, places for groups).
+        self._prefix_group = next((g for g, group in enumerate(self.cache_plan.groups) if not group.window), -1)
+        self._prefix_graphs: "OrderedDict[tuple, _DecodeGraph]" = OrderedDict()
+        self._logprobs: Dict[int, List[TokenLogprob]] = {}
+        self._own_ids = 1 << 62                          # ids of the requests that answers() opens
         # Decode graphs are captured now, while every page and state slot is free: a capture runs on throw-away
         # requests (see _capture), and a full engine has no room for those.  A bucket for which even the empty
         # pool is too small is tried again at its first use.
@@ -291,6 +302,29 @@ class Engine:
         """Give back everything ``request`` holds."""
         self.cache.manager.release(request)
 
+    def fork_request(self, parent: int, children: Sequence[int]) -> None:
+        """Make each of ``children`` live as a copy of ``parent`` as it is now: they hold its whole pages in common, and the page that it
+        has begun (and the states that layers keep) is copied.  From here on every one of them goes its own way.  All of them or none:
+        without room for one of them nothing changes and a MemoryError says so.  ``parent`` is a request that ``open_request`` or a
+        fork has made live; decode steps of requests that share pages read those once where that pays."""
+        mgr = self.cache.manager
+        if not mgr.has(parent):
+            raise ValueError(f"request {parent} is not live")
+        children = [int(c) for c in children]
+        if len(set(children)) != len(children) or any(mgr.has(c) for c in children):
+            raise ValueError("a fork's children are requests that are not live yet, each named once")
+        copies = []
+        for n, child in enumerate(children):
+            got, pages, states = mgr.fork(parent, child)
+            if got != self._rt.Acquire.Ready:
+                for c in children[:n]:
+                    mgr.release(c)
+                raise MemoryError(f"request {parent} cannot be forked into {len(children)}: {got.name} for the {n + 1}th; nothing has changed; free "
+                                  f"pages per group: {[mgr.free_pages(g) for g in range(mgr.num_groups())]}, free state slots: {mgr.free_state_slots()}")
+            copies.append((pages, states))
+        if copies:
+            self.cache.copy_fork(copies)
+
     def request_length(self, request: int) -> int:
         return self.cache.manager.length(request)
 
@@ -305,9 +339,19 @@ class Engine:
             self._scratch = torch.empty(max(floats, 1 << 16), dtype=torch.float32, device=self.device)
         return self._scratch
 
-    def _context(self, layout, dev: torch.Tensor, host: Optional[torch.Tensor], kv_len_bound: int) -> StepContext:
-        return context_from_layout(layout, dev, host, self.cache.page_sizes, self.device, self.dtype,
-                                   kv_len_bound, self._get_scratch, self.sm_count)
+    def _context(self, layout, dev: torch.Tensor, host: Optional[torch.Tensor], kv_len_bound: int, graph: Optional[_DecodeGraph] = None) -> StepContext:
+        ctx = context_from_layout(layout, dev, host, self.cache.page_sizes, self.device, self.dtype,
+                                  kv_len_bound, self._get_scratch, self.sm_count)
+        groups = layout.num_prefix_groups
+        if groups:
+            rows = dev[layout.off_prefix_rows:layout.off_prefix_rows + layout.num_decode]
+            places = dev[layout.off_prefix_groups:layout.off_prefix_groups + 2 * groups].view(groups, 2)
+            # (a graph is cut up for what may come, a step of its own for what is there)
+            most = (layout.num_decode, kv_len_bound, kv_len_bound) if graph is not None else \
+                (layout.most_prefix_rows, layout.most_prefix_keys, layout.most_own_keys)
+            most += (groups - 1,)
+            ctx.shared = SharedPrefixes(self._prefix_group, rows, places, *most)
+        return ctx
 
     def _batch_request(self, entries: Sequence[StepEntry]):
         req = self._rt.BatchRequest()
@@ -351,10 +395,11 @@ class Engine:
                                           or device_tokens.dtype != torch.int32 or not device_tokens.is_cuda):
             raise ValueError("device_tokens needs one int32 token on the device for each one-token entry")
         graph = None
+        groups = self._look_for_prefixes(req)
         if decode_only and self._graphs and all(len(e.want) == 1 for e in entries):
             bucket = next((b for b in sorted(self._graphs) if b >= len(entries)), None)
             if bucket is not None and max(mgr.length(e.request) for e in entries) < self.max_seq_len:
-                graph = self._graphs[bucket]
+                graph = self._prefix_graph(bucket, groups) if groups else self._graphs[bucket]
         if graph is None and not decode_only and 0 < len(req.tokens) <= self.prefill_graph_max_tokens \
                 and max(mgr.length(e.request) + len(e.tokens) for e in entries) <= self.max_seq_len:
             graph = self._shape_graph(tuple(req.counts) + (-1, len(req.want_index)))
@@ -365,6 +410,28 @@ class Engine:
         for e in entries:
             mgr.advance(e.request, mgr.length(e.request) + len(e.tokens))
         return logits
+
+    def _look_for_prefixes(self, req) -> int:
+        """Decide whether the step's decode rows read the pages that they share once; how many groups of rows do so (0: none)."""
+        mgr, g = self.cache.manager, self._prefix_group
+        if g < 0 or mgr.shared_pages(g) == 0:
+            return 0
+        req.prefix_group = g
+        groups, saved = self._rt.count_prefix_groups(mgr, req)
+        if saved < _SAVED_KEYS_AT_LEAST:
+            req.prefix_group, groups = -1, 0
+        return groups
+
+    def _prefix_graph(self, bucket: int, groups: int) -> _DecodeGraph:
+        places = 1 + (1 << (groups - 1).bit_length())            # (the last group is the other rows')
+        key = (bucket, places)
+        g = self._prefix_graphs.get(key)
+        if g is None:
+            g = self._prefix_graphs[key] = _DecodeGraph(bucket, places)
+            while len(self._prefix_graphs) > self._shape_graph_limit:
+                self._prefix_graphs.popitem(last=False)
+        self._prefix_graphs.move_to_end(key)
+        return g
 
     def _step_eager(self, req, device_tokens: Optional[torch.Tensor] = None) -> torch.Tensor:
         layout = self._rt.plan_batch(self.cache.manager, req)
@@ -398,6 +465,7 @@ class Engine:
     def _graph_request(self, req, g: _DecodeGraph):
         req.pad_rows_to = g.bucket
         req.fixed_table_width = list(self.table_width)
+        req.prefix_group, req.prefix_groups = (self._prefix_group if g.prefix_groups else -1), g.prefix_groups
         return req
 
     def _capture(self, g: _DecodeGraph, counts: Sequence[int], want_counts: Sequence[int],
@@ -426,7 +494,7 @@ class Engine:
             layout = rt.build_batch(mgr, req, host.numpy())
             g.meta = torch.empty(layout.total_ints, dtype=torch.int32, device=self.device)
             self._meta.upload(turn, layout.total_ints, g.meta)
-            g.ctx = self._context(layout, g.meta, None, self.max_seq_len)
+            g.ctx = self._context(layout, g.meta, None, self.max_seq_len, g)
             # Warm up outside the capture (sizes scratch, loads kernels), then capture.
             side = torch.cuda.Stream(self.device)
             side.wait_stream(torch.cuda.current_stream())
@@ -449,7 +517,8 @@ class Engine:
 
     def _step_graph(self, g: _DecodeGraph, req, real_rows: int,
                     device_tokens: Optional[torch.Tensor] = None) -> torch.Tensor:
-        if g.graph is None and not self._capture(g, req.counts, req.want_counts, req.want_index):
+        if g.graph is None and not (self._capture(g, [], [], []) if g.prefix_groups else      # (padding rows alone)
+                                    self._capture(g, req.counts, req.want_counts, req.want_index)):
             return self._step_eager(req, device_tokens)       # no room for the capture now: this step runs as it is
         self._graph_request(req, g)
         layout = self._rt.plan_batch(self.cache.manager, req)
@@ -514,7 +583,9 @@ class Engine:
         if not rows:
             return _Flight(plan, None, None)
         ids = self.sampler.sample_device(logits, rows)
-        return _Flight(plan, ids, ops.begin_read(ids))
+        wanted = [p.logprobs for p, _, _ in rows]
+        logprobs = PendingLogprobs(logits, ids, wanted) if any(w is not None for w in wanted) else None
+        return _Flight(plan, ids, ops.begin_read(ids), logprobs)
 
     def _forget_finished(self, out) -> None:
         for o in out:
@@ -569,9 +640,20 @@ class Engine:
             self.last_step_error = True
             self._forget_finished(out)
             raise
-        out += sched.commit_step(flight.plan, sampled)
+        committed = sched.commit_step(flight.plan, sampled)
+        if flight.logprobs is not None:
+            of_request = dict(zip((e.uid for e in flight.plan.entries if e.sample), flight.logprobs.finish()))
+            for o in committed:                               # (a request that had ended before has no token here)
+                if of_request.get(o.uid) is not None:
+                    self._logprobs.setdefault(o.uid, []).append(of_request[o.uid])
+        out += committed
         self._forget_finished(out)
         return out
+
+    def take_logprobs(self, uid: int) -> List[TokenLogprob]:
+        """The log probabilities of the tokens that request ``uid`` has put out since they were last taken, for a request whose
+        SamplingParams ask for them.  (They are kept until they are taken.)"""
+        return self._logprobs.pop(uid, [])
 
     def generate(self, prompts: Sequence[Sequence[int]],
                  sampling_params=None) -> List[GenerationResult]:
@@ -590,4 +672,88 @@ class Engine:
                     results[o.uid].tokens.append(o.token)
                 if o.finished:
                     results[o.uid].finish_reason = o.reason.name.lower()
+        for uid, sp in zip(uids, sampling_params):
+            if sp.logprobs is not None:
+                results[uid].logprobs = self.take_logprobs(uid)
         return [results[uid] for uid in uids]
+
+    # ------------------------------------------------------------------ several answers, scores
+    def answers(self, prompt: Sequence[int], n: int, params: Optional[SamplingParams] = None) -> List[GenerationResult]:
+        """``n`` answers to one prompt (host token ids in and out).  The prompt runs once; its request is then forked, so that the answers
+        hold its pages in common, and they decode side by side.  Answer i is sampled with seed ``params.seed`` + i (without a seed:
+        seeds of the engine's own), so answer 0 is what ``generate`` gives.  The requests live beside the scheduler's; a cache
+        without room for them raises MemoryError."""
+        params = (params or SamplingParams()).normalized()
+        prompt = [int(t) for t in prompt]
+        if n < 1 or n > self.max_running_req:
+            raise ValueError(f"{n} answers are refused: 1 to max_running_req ({self.max_running_req})")
+        if not 1 <= len(prompt) <= self.max_seq_len:
+            raise ValueError(f"a prompt of {len(prompt)} tokens is refused: 1 to {self.max_seq_len}")
+        first = self._own_ids
+        self._own_ids += n
+        seed = params.seed if params.seed is not None else (self.seed * 0x9E3779B97F4A7C15 + first * 0xD1B54A32D192ED03) & ((1 << 64) - 1)
+        results = [GenerationResult([], "", None if params.logprobs is None else []) for _ in range(n)]
+        request_of = {0: first}                              # of the answers that go on; the first of them has the prompt's own
+        self.open_request(first)
+        try:
+            portion = self.max_batch_tokens or len(prompt)
+            for at in range(0, len(prompt), portion):
+                tokens = prompt[at:at + portion]
+                want = [len(tokens) - 1] if at + len(tokens) == len(prompt) else []
+                logits = self.step([StepEntry(first, tokens, want)])
+            logits = logits.expand(n, -1)
+            live, length, forked = list(range(n)), len(prompt), False
+            while live:
+                sampled = self.sampler.sample_device(logits, [(params, seed + i, len(results[i].tokens)) for i in live])
+                logprobs = None if params.logprobs is None else PendingLogprobs(logits, sampled, [params.logprobs] * len(live))
+                tokens = dict(zip(live, ops.begin_read(sampled).finish()))
+                if any(t < 0 for t in tokens.values()):
+                    raise RuntimeError("sampling produced no valid token for a row (were the logits finite?)")
+                length += 1
+                for i, found in zip(live, [None] * len(live) if logprobs is None else logprobs.finish()):
+                    results[i].tokens.append(tokens[i])
+                    if found is not None:
+                        results[i].logprobs.append(found)
+                    if not params.ignore_eos and tokens[i] in self.eos_token_ids:
+                        results[i].finish_reason = "stop"
+                    elif len(results[i].tokens) >= params.max_tokens or length >= self.max_seq_len:
+                        results[i].finish_reason = "length"
+                live = [i for i in live if not results[i].finish_reason]
+                if not live:
+                    break
+                if not forked:
+                    self.fork_request(first, [first + x for x in range(1, len(live))])
+                    request_of = {i: first + x for x, i in enumerate(live)}
+                    forked = True
+                for i in [i for i in request_of if results[i].finish_reason]:
+                    self.close_request(request_of.pop(i))
+                logits = self.step([StepEntry(request_of[i], [tokens[i]], [0]) for i in live])
+        finally:
+            for request in request_of.values():
+                self.close_request(request)
+        return results
+
+    def score(self, tokens: Sequence[int], top: int = 0, portion: int = 1024) -> List[TokenLogprob]:
+        """The log probability of each of ``tokens`` behind the ones before it (none for the first one), with the entropy and the ``top``
+        most likely tokens of each place.  ``portion``: tokens of a step, whose logits are held at once."""
+        tokens = [int(t) for t in tokens]
+        if not 1 <= len(tokens) <= self.max_seq_len or portion < 1:
+            raise ValueError(f"{len(tokens)} tokens are refused: 1 to {self.max_seq_len}, in portions of at least 1")
+        if not 0 <= top <= ops.MAX_TOP_LOGPROBS:
+            raise ValueError(f"{top} alternatives are refused: 0 to {ops.MAX_TOP_LOGPROBS}")
+        if self.max_batch_tokens:
+            portion = min(portion, self.max_batch_tokens)
+        found: List[TokenLogprob] = []
+        request = self._own_ids
+        self._own_ids += 1
+        self.open_request(request)
+        try:
+            for at in range(0, len(tokens) - 1, portion):
+                here = tokens[at:min(at + portion, len(tokens) - 1)]
+                logits = self.step([StepEntry(request, here, range(len(here)))])
+                behind = torch.tensor(tokens[at + 1:at + 1 + len(here)], dtype=torch.int32).to(self.device)
+                found += PendingLogprobs(logits, behind, [top] * len(here)).finish()
+            self.check_kernel_errors()
+        finally:
+            self.close_request(request)
+        return found

@@ -1658,7 +1658,7 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
             return TokenLogprobs(*got[:4])
     # No rows, a layer's calls that are being kept, or something that is not as it should be.
     _cuda(logits, tokens)
-    if logits.dtype != torch.float32 or logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1) or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
+    if logits.dtype != torch.float32 or logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
         raise KernelError("token_logprobs takes float32 logits [rows, vocab] with unit inner stride")
     rows, vocab = logits.shape
     if not 0 <= top <= min(MAX_TOP_LOGPROBS, vocab):

@@ -37,17 +37,18 @@ def _splits(most_shared: int, most_own: int, shared_ctas: int, own_ctas: int, ro
 
 @functools.lru_cache(maxsize=4096)
 def _plan(dtype, heads: int, kv_heads: int, dim: int, page: int, n_rows: int, n_groups: int, most_rows: int, most_shared: int, most_own: int,
-          aligned: bool, sms: int) -> tuple:
+          sharing: int, aligned: bool, sms: int) -> tuple:
     """The entry points that a call goes to (all sizes, tcgen05, mma.sync; None: not this one), its sizes as the binding takes them, and
     its launches."""
     per = heads // kv_heads
     most_rows = max(1, min(most_rows, n_rows))
     vectors = most_rows * per
+    sharing = max(1, min(sharing, n_groups))
     if not aligned or not ops.decode_uses_tensor_cores(dtype, heads, kv_heads, dim, page) or n_rows + n_groups > _MOST_ENTRIES:
         lib = load_entry_points("prefix_attention.cu", {"HEAD_DIM": ops.padded_head_dim(dim)})
         tiles = -(-vectors // _TILE)
         per_sm = max(1, 227 * 1024 // (lib.b200_prefix_attention_smem() + 1024))
-        shared, own = _splits(most_shared, most_own, n_groups * kv_heads * tiles, n_rows * kv_heads * -(-per // _TILE), per_sm * sms)
+        shared, own = _splits(most_shared, most_own, sharing * kv_heads * tiles, n_rows * kv_heads * -(-per // _TILE), per_sm * sms)
         floats = n_rows * heads * (shared + own) * (ops.padded_head_dim(dim) + 2)
         return lib.b200_prefix_attention, None, None, (floats, shared, own, tiles, 0, 0, sms), 2
     tcgen05, tiles, two, shared, covered = None, 1, 0, 0, 0
@@ -56,7 +57,7 @@ def _plan(dtype, heads: int, kv_heads: int, dim: int, page: int, n_rows: int, n_
         two = int(vectors > _TC_VECTORS)
         a_cta = _TC_VECTORS << two
         tiles = -(-vectors // a_cta)
-        ctas = max(1, min(-(-most_shared // (256 >> two)), sms // (n_groups * kv_heads * tiles), _MOST_SPLITS))
+        ctas = max(1, min(-(-most_shared // (256 >> two)), sms // (sharing * kv_heads * tiles), _MOST_SPLITS))
         shared, covered = ctas << (1 - two), tiles * a_cta
         tcgen05 = load_entry_points("prefix_tcgen05.cu").b200_prefix_tcgen05
     lib = load_entry_points("prefix_mma.cu", {"HEAD_DIM": dim})
@@ -89,7 +90,7 @@ def _refuse(q, k_cache, v_cache, out, block_table, cu_q, kv_len, rows, groups, n
 
 
 def prefix_attention(q, k_cache, v_cache, out, block_table, cu_q, kv_len, rows, groups, num_heads, num_kv_heads, head_dim, page_size,
-                     scale, *, most_rows, most_shared, most_own) -> None:
+                     scale, *, most_rows, most_shared, most_own, sharing_groups=None) -> None:
     """Attention of single decoded tokens behind shared keys; operands as ``ops.decode_attention`` takes them.
 
     ``rows`` (int32) lists the batch rows to serve group by group; ``groups`` (int32 [groups, 2]) holds for each group the index
@@ -97,14 +98,14 @@ def prefix_attention(q, k_cache, v_cache, out, block_table, cu_q, kv_len, rows, 
     with a page; a row that sees fewer keys than its group shares sees those.  A row of no keys gets zeros.
 
     ``most_rows``, ``most_shared`` and ``most_own`` are about how many rows a group has, how many keys it shares and how many keys
-    a row has beyond them, at most: they decide how the work is cut up (and what a captured graph is cut up for), not the result's
-    meaning.  Page ids outside the pool and rows longer than their block table set the error word (``ops.check_errors``)."""
+    a row has beyond them, at most, ``sharing_groups`` about how many of the groups share keys (None: all): they decide how the work is
+    cut up (and what a captured graph is cut up for), not the result's meaning.  Page ids outside the pool and rows longer than their block table set the error word (``ops.check_errors``)."""
     if num_kv_heads <= 0 or num_heads <= 0 or num_heads % num_kv_heads:
         raise KernelError("num_heads must be a multiple of num_kv_heads")
     if head_dim % 2 or not 2 <= head_dim <= 512:
         raise KernelError(f"head size {head_dim} is refused: the attention kernels take even head sizes up to 512")
-    if most_rows < 0 or most_shared < 0 or most_own < 0:
-        raise KernelError("most_rows, most_shared and most_own must not be negative")
+    if most_rows < 0 or most_shared < 0 or most_own < 0 or (sharing_groups is not None and sharing_groups < 0):
+        raise KernelError("most_rows, most_shared, most_own and sharing_groups must not be negative")
     if ops._held is not None or ops._chain is not None:
         ops.flush_chain()                        # (what waits in the chain may be what is read here)
     operands = (q, k_cache, v_cache, out, block_table, cu_q, kv_len, rows, groups)
@@ -118,7 +119,8 @@ def prefix_attention(q, k_cache, v_cache, out, block_table, cu_q, kv_len, rows, 
     ops._on_current(rows.device)
     aligned = (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr() | out.data_ptr()) % 16 == 0
     all_sizes, tcgen05, mma, plan, kernels = _plan(q.dtype, num_heads, num_kv_heads, head_dim, page_size, n_rows, groups.shape[0], most_rows,
-                                                   most_shared, most_own, aligned, ops._sm_count(rows.device))
+                                                   most_shared, most_own, groups.shape[0] if sharing_groups is None else sharing_groups, aligned,
+                                                   ops._sm_count(rows.device))
     rc = _binding().prefix_attention(all_sizes, tcgen05, mma, *operands, *sizes, float(scale), plan, ops.error_word(rows.device), ops._stream())
     if rc is None:
         # something is not as it should be, or this thread keeps a layer's calls (ops.LayerCalls), which the entry points take part in

@@ -6,7 +6,7 @@ import math
 
 import torch
 
-from ..kernels import ops
+from ..kernels import ops, prefix
 from .base import PagedKVSpec, ParamDecl, Part, StateSpec
 from .registry import register_part
 
@@ -215,7 +215,12 @@ class GQAttention(Part):
             ops.prefill_attention(q, cache.k, cache.v, out, ctx.block_tables[g], ctx.cu_q, ctx.kv_len,
                                   ctx.prefix_len, ctx.prefill_rows, ctx.num_prefill, ctx.max_q_len,
                                   self.nh, self.nkv, self.d, page, self.window, self.scale)
-        if ctx.num_decode:
+        shared = ctx.shared
+        if shared is not None and shared.cache_group == g and not self.window:
+            prefix.prefix_attention(q, cache.k, cache.v, out, ctx.block_tables[g], ctx.cu_q, ctx.kv_len, shared.rows, shared.groups,
+                                    self.nh, self.nkv, self.d, page, self.scale, most_rows=shared.most_rows,
+                                    most_shared=shared.most_shared, most_own=shared.most_own, sharing_groups=shared.sharing_groups)
+        elif ctx.num_decode:
             bound = min(ctx.kv_len_bound, self.window) if self.window else ctx.kv_len_bound
             splits = attention_splits(q.dtype, ctx.num_decode, self.nh, self.nkv, self.d, page, bound, ctx.sm_count)
             need = ops.decode_scratch_floats(ctx.num_decode, self.nh, self.d, splits)

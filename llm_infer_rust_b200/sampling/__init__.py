@@ -1,3 +1,3 @@
-from .sampler import ROW_DTYPE, Sampler, SamplingParams, pack_rows
+from .sampler import ROW_DTYPE, PendingLogprobs, Sampler, SamplingParams, TokenLogprob, pack_rows
 
-__all__ = ["ROW_DTYPE", "Sampler", "SamplingParams", "pack_rows"]
+__all__ = ["ROW_DTYPE", "PendingLogprobs", "Sampler", "SamplingParams", "TokenLogprob", "pack_rows"]

@@ -2,8 +2,10 @@
 
 Options and their meaning follow the reference (src/engine/sampling.rs:9-48):
 ``temperature`` (<= 0: greedy), ``top_k`` (<= 0: off), ``top_p`` (0: greedy,
-outside [0, 1]: 1), ``ignore_eos``, ``max_tokens`` (at least 1).  ``seed`` is
-this engine's addition: the uniform number of a draw is a counter-based random
+outside [0, 1]: 1), ``ignore_eos``, ``max_tokens`` (at least 1).  ``logprobs`` is this engine's addition: how many of the
+most likely tokens are reported with their log probabilities beside each output token's
+own (None: no log probabilities at all); they are those of the model's distribution,
+before temperature and cut-offs.  So is ``seed``: the uniform number of a draw is a counter-based random
 number keyed by (seed, index of the output token), so a request samples the same
 tokens whatever else shares its batch.
 """
@@ -31,11 +33,14 @@ class SamplingParams:
     ignore_eos: bool = False
     max_tokens: int = 1024
     seed: Optional[int] = None
+    logprobs: Optional[int] = None
 
     def normalized(self) -> "SamplingParams":
         top_p = self.top_p if (math.isfinite(self.top_p) and 0.0 <= self.top_p <= 1.0) else 1.0
-        return SamplingParams(float(self.temperature), int(self.top_k), float(top_p),
-                              bool(self.ignore_eos), max(int(self.max_tokens), 1), self.seed)
+        if self.logprobs is not None and not 0 <= int(self.logprobs) <= ops.MAX_TOP_LOGPROBS:
+            raise ValueError(f"logprobs must be 0 to {ops.MAX_TOP_LOGPROBS} alternatives, or None")
+        return SamplingParams(float(self.temperature), int(self.top_k), float(top_p), bool(self.ignore_eos), max(int(self.max_tokens), 1),
+                              self.seed, None if self.logprobs is None else int(self.logprobs))
 
     @property
     def greedy(self) -> bool:
@@ -50,6 +55,36 @@ def pack_rows(rows: Sequence[Tuple[SamplingParams, int, int]]) -> np.ndarray:
         out[i] = (p.temperature, p.top_k, p.top_p, seed & 0xFFFFFFFF, seed >> 32,
                   counter & 0xFFFFFFFF, 0, 0)
     return out
+
+
+@dataclass(frozen=True)
+class TokenLogprob:
+    """A token's log probability, the entropy of the distribution that it came from (in nats) and that distribution's most likely
+    tokens, (id, log probability) each, most likely first."""
+    token: int
+    logprob: float
+    entropy: float
+    top: Tuple[Tuple[int, float], ...] = ()
+
+
+class PendingLogprobs:
+    """Log probabilities on their way to the host.  ``wanted``: of each row how many alternatives, None for a row that wants nothing."""
+
+    def __init__(self, logits: torch.Tensor, ids: torch.Tensor, wanted: Sequence[Optional[int]]):
+        most = max((w for w in wanted if w is not None), default=0)
+        found = ops.token_logprobs(logits, ids, top=min(most, logits.shape[1]))
+        self.wanted = list(wanted)
+        self._host = [torch.empty(t.shape, dtype=t.dtype, pin_memory=True) for t in (ids, *found)]
+        for host, t in zip(self._host, (ids, *found)):
+            host.copy_(t, non_blocking=True)
+        self._event = torch.cuda.Event()
+        self._event.record(torch.cuda.current_stream(logits.device))
+
+    def finish(self) -> List[Optional[TokenLogprob]]:
+        self._event.synchronize()
+        tokens, logprobs, entropy, top_ids, top_logprobs = (t.tolist() for t in self._host)
+        return [None if w is None else TokenLogprob(tokens[r], logprobs[r], entropy[r], tuple(zip(top_ids[r][:w], top_logprobs[r][:w])))
+                for r, w in enumerate(self.wanted)]
 
 
 class Sampler:

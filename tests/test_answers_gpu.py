@@ -1,0 +1,322 @@
+"""Forks, several answers to one prompt and scores through the engine, against the plain implementation."""
+import json
+import os
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+import kefetar_kit as K
+import plain_qwen3 as P
+
+pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+TOL = {"float32": 1e-5, "bfloat16": 2.0 ** -5}      # of the logits' scale (those of long decoding in test_engine_gpu.py)
+
+
+def tokens(vocab, n, seed):
+    return torch.randint(0, vocab, (n,), generator=torch.Generator().manual_seed(seed)).tolist()
+
+
+def engine(folder, **kw):
+    from llm_infer_rust_b200.engine import Engine
+    kw.setdefault("cuda_graph_bs", 0)
+    kw.setdefault("max_running_req", 12)
+    kw.setdefault("max_total_tokens", 2048)
+    return Engine(folder, **kw)
+
+
+@pytest.fixture(autouse=True)
+def always_shared(monkeypatch):
+    """Small steps take the shared kernels too."""
+    from llm_infer_rust_b200.engine import engine as module
+    monkeypatch.setattr(module, "_SAVED_KEYS_AT_LEAST", 1)
+
+
+@pytest.fixture(scope="module")
+def folders(tiny, tiny_dirs, tmp_path_factory):
+    """(folder, weights) of a configuration, stored in 32 or in 16 bits."""
+    from llm_infer_rust_b200 import random_tensors, write_random_model
+    made = {}
+
+    def of(name, dtype):
+        if (name, dtype) not in made:
+            v = tiny[name]
+            w = random_tensors(v["raw"], v["seed"], norm_std=v["norm_std"])
+            folder = tiny_dirs[name]
+            if dtype == "bfloat16":
+                folder = write_random_model(str(tmp_path_factory.mktemp("answers")), v["raw"], v["seed"], norm_std=v["norm_std"], dtype="bfloat16")
+                w = {n: t.to(torch.bfloat16) for n, t in w.items()}
+            made[name, dtype] = folder, w
+        return made[name, dtype]
+    return of
+
+
+def near(got, want, dtype):
+    assert np.abs(got - want).max() <= TOL[dtype] * max(1.0, np.abs(want).max()), np.abs(got - want).max()
+
+
+@pytest.mark.parametrize("graphs", [0, 12])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name", ["A", "B", "C", "D", "E"])
+def test_forked_requests_go_their_own_ways(name, dtype, graphs, tiny, folders):
+    """A prompt, forks of it and of one of them, other requests beside them, prompts while they decode, ends: every row's logits are
+    those of its own tokens."""
+    from llm_infer_rust_b200.engine import StepEntry
+    if graphs and dtype == "float32":
+        pytest.skip("float32 engines have no graphs")
+    raw = tiny[name]["raw"]
+    vocab, page = raw["vocab_size"], tiny[name]["page_size"]
+    folder, w = folders(name, dtype)
+    eng = engine(folder, dtype=dtype, page_size=page, cuda_graph_bs=graphs)
+    mgr = eng.cache.manager
+    seq = {1: tokens(vocab, 5 * page + 3, 11), 2: tokens(vocab, 7, 12)}
+    for r in (1, 2):
+        eng.open_request(r)
+        eng.step([StepEntry(r, seq[r], [])])
+
+    def fork(parent, children):
+        eng.fork_request(parent, children)
+        for c in children:
+            seq[c] = list(seq[parent])
+
+    def decode(rows, seed, more=()):
+        entries = []
+        for i, r in enumerate(rows):
+            new = tokens(vocab, 1, 100 * seed + i)
+            seq[r] = seq.get(r, []) + new
+            entries.append(StepEntry(r, new, [0]))
+        for r, n in more:
+            new = tokens(vocab, n, 7000 + seed)
+            seq[r] = seq.get(r, []) + new
+            entries.append(StepEntry(r, new, [n - 1]))
+        got = eng.step(entries).float().cpu().numpy()
+        for row, e in zip(got, entries):
+            near(row, P.plain_forward(w, raw, seq[e.request]).numpy()[-1], dtype)
+        eng.check_kernel_errors()
+        assert mgr.check() == ""
+    fork(1, [3, 4, 5, 6])
+    assert mgr.shared_pages(eng._prefix_group) == 5
+    for step in range(3):
+        decode([2, 3, 1, 4, 6, 5], step)
+    fork(4, [7])                                             # shares the first prompt's pages and none beyond them, or its own too
+    fork(2, [8])
+    for step in range(3, 3 + page):
+        decode([7, 2, 5, 8, 4, 1], step)
+    eng.open_request(9)
+    decode([3, 4, 7], 90, more=[(9, page + 1)])              # a prompt beside decoded tokens
+    eng.close_request(1)                                     # the parent ends first
+    decode([7, 4, 3, 9], 91)
+    decode([6], 92)
+    if graphs:
+        assert eng._prefix_graphs and all(g.graph is not None for g in eng._prefix_graphs.values())
+    for r in (2, 3, 4, 5, 6, 7, 8, 9):
+        eng.close_request(r)
+    assert mgr.check() == "" and mgr.live_requests() == 0 and all(mgr.shared_pages(g) == 0 for g in range(mgr.num_groups()))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name", ["K1", "K3", "K4"])
+def test_states_of_layers_are_copied(name, dtype, tmp_path):
+    """Convolutions and retention keep states beside the pages: a fork's go on from its parent's."""
+    from llm_infer_rust_b200.engine import StepEntry
+    raw = K.CONFIGS[name]
+    w = K.random_weights(raw, 3)
+    eng = K.make_engine(K.write_model(str(tmp_path / "m"), raw, w), dtype, max_requests=6)
+    prompt = K.tokens(raw["vocab"], 41, 5)
+    eng.open_request(1)
+    eng.step([StepEntry(1, prompt, [])])
+    eng.fork_request(1, [2, 3])
+    seq = {r: list(prompt) for r in (1, 2, 3)}
+    for step in range(6):
+        entries = []
+        for r in seq:
+            new = K.tokens(raw["vocab"], 1, 50 * step + r)
+            seq[r] += new
+            entries.append(StepEntry(r, new, [0]))
+        got = eng.step(entries).float().cpu().numpy()
+        for row, r in zip(got, seq):
+            want = K.oracle(raw, w, seq[r])[-1]
+            tol = 2e-5 if dtype == "float32" else 8e-2
+            assert np.abs(row - want).max() <= tol * max(1.0, np.abs(want).max())
+    eng.check_kernel_errors()
+
+
+def test_a_fork_without_room_and_forks_that_make_no_sense(folders):
+    from llm_infer_rust_b200.engine import StepEntry
+    folder, _ = folders("A", "float32")
+    eng = engine(folder, dtype="float32", page_size=4, max_running_req=3, max_total_tokens=32)
+    eng.open_request(1)
+    eng.step([StepEntry(1, tokens(256, 27, 1), [])])           # seven of eight pages
+    free = eng.cache.manager.free_pages(0)
+    with pytest.raises(MemoryError, match="nothing has changed"):
+        eng.fork_request(1, [2, 3])
+    assert eng.cache.manager.free_pages(0) == free and eng.cache.manager.live_requests() == 1 and eng.cache.manager.check() == ""
+    for parent, children in ((9, [2]), (1, [1]), (1, [2, 2])):
+        with pytest.raises(ValueError):
+            eng.fork_request(parent, children)
+    eng.fork_request(1, [])
+    eng.fork_request(1, [2])
+    assert eng.request_length(2) == 27
+
+
+@pytest.mark.parametrize("graphs", [0, 8])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_answers_are_what_generate_gives_with_their_seeds(dtype, graphs, folders):
+    from llm_infer_rust_b200 import SamplingParams
+    if graphs and dtype == "float32":
+        pytest.skip("float32 engines have no graphs")
+    folder, w = folders("E", dtype)
+    eng = engine(folder, dtype=dtype, cuda_graph_bs=graphs)
+    prompt = tokens(307, 70, 3)
+    sp = SamplingParams(temperature=0.9, top_k=40, max_tokens=12, ignore_eos=True, seed=21, logprobs=3)
+    got = eng.answers(prompt, 6, sp)
+    assert eng.cache.manager.live_requests() == 0 and eng.cache.manager.check() == ""
+    assert len({tuple(r.tokens) for r in got}) > 1
+    for i, r in enumerate(got):
+        assert r.finish_reason == "length" and len(r.tokens) == len(r.logprobs) == 12
+        alone = eng.generate([prompt], SamplingParams(temperature=0.9, top_k=40, max_tokens=12, ignore_eos=True, seed=21 + i, logprobs=3))[0]
+        # 32-bit logits leave a drawn token no choice; in bfloat16 another batch's products may move one that lies at a border
+        same = next((n for n, (a, b) in enumerate(zip(r.tokens, alone.tokens)) if a != b), 12)
+        assert same == 12 or dtype == "bfloat16"
+        for a, b in zip(r.logprobs[:same], alone.logprobs[:same]):
+            assert a.token == b.token and abs(a.logprob - b.logprob) <= 2 * TOL[dtype] * 10 and abs(a.entropy - b.entropy) <= 2 * TOL[dtype] * 10
+    # what is reported is the model's own distribution
+    for r in got:
+        logits = P.plain_forward(w, json.load(open(os.path.join(folder, "config.json"))), prompt + r.tokens).double()
+        lp = torch.log_softmax(logits, -1)[len(prompt) - 1:-1]
+        scale = float(logits.abs().max())
+        for t, (token, found) in enumerate(zip(r.tokens, r.logprobs)):
+            assert found.token == token and len(found.top) == 3
+            assert abs(found.logprob - float(lp[t, token])) <= 2 * TOL[dtype] * max(1.0, scale)
+            assert all(abs(v - float(lp[t, i])) <= 2 * TOL[dtype] * max(1.0, scale) for i, v in found.top)
+            assert found.top[0][1] >= found.top[1][1] >= found.top[2][1]
+
+
+def test_answers_that_end_at_unlike_places(folders):
+    from llm_infer_rust_b200 import SamplingParams
+    folder, _ = folders("A", "float32")
+    prompt = tokens(256, 30, 8)
+    sp = SamplingParams(temperature=1.5, max_tokens=20, seed=4)
+    stops = list(range(0, 256, 5))                              # an answer ends after five tokens or so, some at once
+    eng = engine(folder, dtype="float32", page_size=4, eos_token_ids=stops)
+    got = eng.answers(prompt, 12, sp)
+    reasons = {r.finish_reason for r in got}
+    assert "stop" in reasons and len({len(r.tokens) for r in got}) > 3 and any(len(r.tokens) == 1 for r in got)
+    for i, r in enumerate(got):
+        alone = eng.generate([prompt], SamplingParams(temperature=1.5, max_tokens=20, seed=4 + i))[0]
+        assert (r.tokens, r.finish_reason) == (alone.tokens, alone.finish_reason) and r.logprobs is None
+    assert eng.cache.manager.live_requests() == 0 and eng.cache.manager.check() == ""
+
+
+def test_answers_at_their_limits(folders):
+    from llm_infer_rust_b200 import SamplingParams
+    folder, _ = folders("A", "float32")
+    eng = engine(folder, dtype="float32", page_size=4, max_running_req=3, max_total_tokens=60, max_seq_len=40)
+    one = eng.answers(tokens(256, 5, 1), 1, SamplingParams(max_tokens=6, ignore_eos=True))[0]
+    assert one.tokens == eng.generate([tokens(256, 5, 1)], SamplingParams(max_tokens=6, ignore_eos=True))[0].tokens
+    full = eng.answers(tokens(256, 40, 2), 2, SamplingParams(max_tokens=6, ignore_eos=True))
+    assert [(len(r.tokens), r.finish_reason) for r in full] == [(1, "length")] * 2
+    near_end = eng.answers(tokens(256, 38, 2), 2, SamplingParams(max_tokens=6, ignore_eos=True))
+    alone = eng.generate([tokens(256, 38, 2)], SamplingParams(max_tokens=6, ignore_eos=True))[0]
+    assert [r.tokens for r in near_end] == [alone.tokens] * 2 and near_end[0].finish_reason == alone.finish_reason == "length"
+    for n, prompt in ((0, [1]), (4, [1]), (2, []), (2, [1] * 41)):
+        with pytest.raises(ValueError):
+            eng.answers(prompt, n)
+    with pytest.raises(MemoryError):
+        eng.answers(tokens(256, 30, 2), 3, SamplingParams(max_tokens=30, ignore_eos=True))      # 7 pages in common and 3 of each answer's own: 16, and there are 15
+    assert eng.cache.manager.live_requests() == 0 and eng.cache.manager.check() == ""
+
+
+@pytest.mark.parametrize("overlap", [False, True])
+def test_logprobs_of_the_scheduler(overlap, folders):
+    """Requests with and without log probabilities side by side, some ending before others."""
+    from llm_infer_rust_b200 import SamplingParams
+    folder, w = folders("B", "float32")
+    raw = json.load(open(os.path.join(folder, "config.json")))
+    eng = engine(folder, dtype="float32", cpu_gpu_overlap=overlap, max_running_req=3)
+    prompts = [tokens(509, n, n) for n in (4, 33, 17, 9)]
+    params = [SamplingParams(max_tokens=5, ignore_eos=True, logprobs=2), SamplingParams(max_tokens=9, ignore_eos=True),
+              SamplingParams(max_tokens=7, ignore_eos=True, logprobs=0), SamplingParams(max_tokens=3, ignore_eos=True, logprobs=32)]
+    plain = [SamplingParams(max_tokens=p.max_tokens, ignore_eos=True) for p in params]
+    without = eng.generate(prompts, plain)
+    got = eng.generate(prompts, params)
+    assert [r.tokens for r in got] == [r.tokens for r in without] and all(r.logprobs is None for r in without)
+    assert got[1].logprobs is None and not eng._logprobs
+    for r, p, prompt in zip(got, params, prompts):
+        if p.logprobs is None:
+            continue
+        lp = torch.log_softmax(P.plain_forward(w, raw, prompt + r.tokens).double(), -1)[len(prompt) - 1:-1]
+        assert [t.token for t in r.logprobs] == r.tokens and all(len(t.top) == p.logprobs for t in r.logprobs)
+        for t, found in enumerate(r.logprobs):
+            assert abs(found.logprob - float(lp[t, found.token])) <= 4e-5
+            assert abs(found.entropy + float((lp[t].exp() * lp[t]).sum())) <= 4e-4
+            if found.top:
+                assert found.top[0][0] == found.token                     # (greedy)
+    uid = eng.add_request(prompts[0], params[0])
+    while not eng.is_idle():
+        eng.schedule_step()
+    assert [t.token for t in eng.take_logprobs(uid)] == got[0].tokens and eng.take_logprobs(uid) == []
+
+
+@pytest.mark.parametrize("portion", [1, 7, 1024])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_scores(dtype, portion, folders):
+    folder, w = folders("E", dtype)
+    raw = json.load(open(os.path.join(folder, "config.json")))
+    eng = engine(folder, dtype=dtype)
+    ids = tokens(307, 90, 2)
+    found = eng.score(ids, top=4, portion=portion)
+    logits = P.plain_forward(w, raw, ids).double()
+    lp = torch.log_softmax(logits, -1)
+    assert [f.token for f in found] == ids[1:]
+    for t, f in enumerate(found):
+        assert abs(f.logprob - float(lp[t, ids[t + 1]])) <= 2 * TOL[dtype] * max(1.0, float(logits.abs().max())) and len(f.top) == 4
+    assert eng.score([5]) == [] and eng.cache.manager.live_requests() == 0
+    for bad in (dict(tokens=[]), dict(tokens=[1, 2], top=33), dict(tokens=[1, 2], portion=0)):
+        with pytest.raises(ValueError):
+            eng.score(**bad)
+    with pytest.raises(Exception, match="token id"):
+        eng.score([1, 400, 2])
+    assert eng.cache.manager.live_requests() == 0
+
+
+def test_command_line(folders):
+    folder, _ = folders("A", "float32")
+    run = subprocess.run([sys.executable, "-m", "llm_infer_rust_b200", "--model-path", folder, "--prompt-ids", "1,2,3,4,5", "--max-tokens", "4",
+                          "--ignore-eos", "--answers", "3", "--logprobs", "2", "--temperature", "1.0", "--seed", "3", "--max-total-tokens", "256",
+                          "--max-running-req", "4", "--cuda-graph-bs", "0", "--log-level", "error"], cwd=ROOT, capture_output=True, text=True)
+    assert run.returncode == 0, run.stderr
+    lines = [json.loads(line) for line in run.stdout.splitlines()]
+    assert len(lines) == 3 and all(len(l["output_ids"]) == len(l["logprobs"]) == 4 and len(l["logprobs"][0]["top"]) == 2 for l in lines)
+
+
+def test_large_groups_through_the_tcgen05_kernel(folders):
+    """Head size 128, 48 answers of two query heads a KV head behind 300 tokens: the engine's own step against decode attention's."""
+    from llm_infer_rust_b200.engine import StepEntry
+    from llm_infer_rust_b200.engine import engine as module
+    folder, _ = folders("E", "bfloat16")
+    eng = engine(folder, dtype="bfloat16", max_running_req=50, max_total_tokens=4096)
+    eng.open_request(1)
+    eng.step([StepEntry(1, tokens(307, 300, 4), [])])
+    eng.fork_request(1, list(range(2, 49)))
+    ids = list(range(1, 49))
+    for step in range(3):
+        logits = []
+        eng.step([StepEntry(r, tokens(307, 1, 60 * step + r), [0]) for r in ids])
+    # one more token, by both ways on the same cache: forks of every request take it without sharing
+    new = [tokens(307, 1, 999 + r)[0] for r in ids]
+    twin = engine(folder, dtype="bfloat16", max_running_req=50, max_total_tokens=4096)
+    twin.open_request(1)
+    twin.step([StepEntry(1, tokens(307, 300, 4), [])])
+    twin.fork_request(1, list(range(2, 49)))
+    for least, e in ((1, eng), (1 << 30, twin)):
+        module._SAVED_KEYS_AT_LEAST = least
+        if e is twin:
+            for step in range(3):
+                e.step([StepEntry(r, tokens(307, 1, 60 * step + r), [0]) for r in ids])
+        logits.append(e.step([StepEntry(r, [t], [0]) for r, t in zip(ids, new)]).float().cpu().numpy().copy())
+        e.check_kernel_errors()
+    near(logits[0], logits[1], "bfloat16")

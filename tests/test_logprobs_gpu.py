@@ -193,3 +193,12 @@ def test_rows_beyond_2_31_elements():
 def test_no_rows():
     f = ops().token_logprobs(torch.zeros(0, 100, device=DEV), torch.zeros(0, dtype=torch.int32, device=DEV), top=4)
     assert f.logprobs.shape == (0,) and f.top_ids.shape == (0, 4)
+
+
+def test_one_row_for_many_tokens():
+    """Rows that are one row again and again, and rows that overlap."""
+    x, t = logits_of(1, 5000).expand(7, -1), given(7, 5000)
+    check(x, t, 4, ops().token_logprobs(x, t, top=4))
+    x = logits_of(1, 5000)[0].as_strided((7, 4000), (130, 1))
+    t = given(7, 4000)
+    check(x, t, 4, ops().token_logprobs(x, t, top=4))

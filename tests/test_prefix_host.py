@@ -1,0 +1,118 @@
+"""What attention behind shared prefixes, page copies and log probabilities refuse, where no GPU is needed to say so."""
+import ctypes
+
+import pytest
+import torch
+
+from llm_infer_rust_b200 import SamplingParams
+from llm_infer_rust_b200.kernels import ops, pages, prefix
+from llm_infer_rust_b200.kernels.build import load_cuda_library
+from llm_infer_rust_b200.kernels.ops import KernelError
+
+I32 = dict(dtype=torch.int32)
+
+
+def operands(dtype=torch.float32, heads=4, kv_heads=2, dim=16, page=8, n=3):
+    cache = torch.zeros(9, kv_heads, page, dim, dtype=dtype)
+    return dict(q=torch.zeros(n, heads * dim, dtype=dtype), k_cache=cache, v_cache=cache.clone(), out=torch.zeros(n, heads * dim, dtype=dtype),
+                block_table=torch.zeros(n, 4, **I32), cu_q=torch.arange(n + 1, **I32), kv_len=torch.ones(n, **I32), rows=torch.arange(n, **I32),
+                groups=torch.zeros(1, 2, **I32), num_heads=heads, num_kv_heads=kv_heads, head_dim=dim, page_size=page, scale=0.25,
+                most_rows=n, most_shared=8, most_own=8)
+
+
+def test_no_path_on_the_cpu():
+    with pytest.raises(KernelError, match="CUDA"):
+        prefix.prefix_attention(**operands())
+    with pytest.raises(KernelError, match="CUDA"):
+        ops.token_logprobs(torch.zeros(2, 8))
+    with pytest.raises(KernelError, match="CUDA"):
+        pages.PageCopier([torch.zeros(4, 2, 8, 16)])
+
+
+@pytest.mark.parametrize("change,what", [
+    (dict(num_heads=3), "multiple of num_kv_heads"), (dict(num_kv_heads=0), "multiple of num_kv_heads"), (dict(head_dim=15), "even head sizes"),
+    (dict(head_dim=514), "even head sizes"), (dict(most_rows=-1), "negative"), (dict(most_own=-1), "negative"), (dict(sharing_groups=-1), "negative")])
+def test_sizes_that_are_refused(change, what):
+    with pytest.raises(KernelError, match=what):
+        prefix.prefix_attention(**{**operands(), **change})
+
+
+@pytest.mark.parametrize("change,what", [
+    (dict(k_cache=torch.zeros(9, 2, 8, 16, dtype=torch.bfloat16)), "share a dtype"), (dict(out=torch.zeros(3, 64, dtype=torch.bfloat16)), "share a dtype"),
+    (dict(q=torch.zeros(3, 64, dtype=torch.float16)), "not supported"), (dict(rows=torch.arange(3)), "are int32"),
+    (dict(groups=torch.zeros(1, 2)), "are int32"), (dict(v_cache=torch.zeros(8, 2, 8, 16)), "as many pages"),
+    (dict(k_cache=torch.zeros(9, 2, 4, 16)), "cache must be"), (dict(q=torch.zeros(3, 32)), "num_heads"), (dict(out=torch.zeros(2, 64)), "num_heads"),
+    (dict(block_table=torch.zeros(3, 0, **I32)), "block_table is"), (dict(groups=torch.zeros(2, **I32)), "block_table is"),
+    (dict(groups=torch.zeros(1, 3, **I32)), "block_table is"), (dict(rows=torch.zeros(3, 1, **I32)), "block_table is"),
+    (dict(q=torch.zeros(64, 3).t()), "non-contiguous"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale")])
+def test_operands_that_are_refused(monkeypatch, change, what):
+    monkeypatch.setattr(ops, "_cuda", lambda *tensors: None)
+    o = {**operands(), **change}
+    for name in ("most_rows", "most_shared", "most_own"):
+        o.pop(name)
+    with pytest.raises(KernelError, match=what):
+        prefix._refuse(**o)
+    prefix._refuse(**{k: v for k, v in operands().items() if not k.startswith("most")})      # (and nothing else is)
+
+
+def test_calls_go_where_they_are_served():
+    def plan(dtype=torch.bfloat16, heads=32, kv_heads=8, dim=128, page=16, n_rows=64, n_groups=1, most_rows=64, shared=4096, own=100, sharing=1, aligned=True):
+        got = prefix._plan(dtype, heads, kv_heads, dim, page, n_rows, n_groups, most_rows, shared, own, sharing, aligned, 148)
+        return ["all sizes", "tcgen05", "mma"][0 if got[0] is not None else 1 if got[1] is not None else 2], got[3]
+    assert plan()[0] == "tcgen05"
+    floats, splits, _, tiles, two, covered, ctas = plan()[1]
+    assert (tiles, two, covered, splits, ctas) == (1, 1, 256, 18, 148)
+    assert plan(most_rows=32)[1][1:6] == (32, 0, 1, 0, 128)                # one tile: a CTA leaves two parts; 4,096 keys are 16 pairs of blocks
+    assert plan(most_rows=8, n_rows=8)[0] == "mma" and plan(shared=200)[0] == "mma" and plan(dim=64)[0] == "mma"
+    for other in (dict(dtype=torch.float32), dict(page=24), dict(dim=72), dict(heads=17, kv_heads=1), dict(n_rows=400), dict(aligned=False)):
+        assert plan(**other)[0] == "all sizes", other
+    assert plan(n_rows=399)[0] == "tcgen05"
+    # groups that share nothing are no reason to cut the others into fewer splits
+    assert plan(n_groups=3)[1][1] == plan(n_groups=3, sharing=1)[1][1] > plan(n_groups=3, sharing=3)[1][1]
+
+
+@pytest.mark.parametrize("moves,rc", [
+    ([(0, 1, 4)], None), ([(0, 1, 4), (2, 1, 4)], -11), ([(0, 1, 4), (1, 2, 4)], -11), ([(3, 3, 4)], -11), ([(0, 9, 4)], -10), ([(9, 1, 4)], -10),
+    ([(-1, 2, 4)], -10), ([(0, 2, 5)], -10), ([(0, 2, -1)], -10), ([(0, 2 ** 31 - 1, 1)], -10)])
+@pytest.mark.parametrize("before", [0, 20])
+def test_moves_are_checked_before_anything_runs(moves, rc, before):
+    """``before``: so many good moves in front (the two ways of comparing pages)."""
+    if rc is None:
+        return                                                     # (a good call would launch)
+    entry = load_cuda_library("pages.cu").b200_copy_pages
+    entry.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_int, ctypes.c_int, ctypes.c_longlong,
+                      ctypes.c_void_p]
+    pages_there = 9 + 2 * before
+    table = torch.zeros(4, dtype=torch.int64)
+    all_moves = [(9 + i, 9 + before + i, 4) for i in range(before)] + [tuple(pages_there if x == 9 and i < 2 else x for i, x in enumerate(m)) for m in moves]
+    m = torch.tensor(all_moves, dtype=torch.int32)
+    assert entry(m.data_ptr(), len(all_moves), table.data_ptr(), 1, pages_there, 4, 16, 256, None) == rc
+
+
+def test_c_entry_points_refuse_what_they_cannot_serve():
+    lib = load_cuda_library("logprobs.cu")
+    none = ctypes.c_void_p()
+    some = ctypes.c_void_p(1 << 20)                                # (never followed)
+
+    def logprobs(rows=1, vocab=100, top=0, stride=100, logits=some, tokens=none, chosen=none, entropy=some, ids=none, best=none, err=some):
+        return lib.b200_token_logprobs(logits, ctypes.c_longlong(stride), rows, vocab, tokens, top, chosen, entropy, ids, best, err, none)
+    assert logprobs(rows=0) == 0
+    for bad in (dict(rows=-1), dict(vocab=0), dict(top=-1), dict(top=33), dict(vocab=3, top=4), dict(stride=-1), dict(logits=none),
+                dict(entropy=none), dict(err=none), dict(tokens=some), dict(top=1), dict(top=1, ids=some), dict(vocab=2 ** 31 - 1), dict(rows=2 ** 30)):
+        assert logprobs(**bad) == -2, bad
+
+
+@pytest.mark.parametrize("logprobs", [-1, 33])
+def test_sampling_params_refuse(logprobs):
+    with pytest.raises(ValueError, match="0 to 32"):
+        SamplingParams(logprobs=logprobs).normalized()
+    assert SamplingParams(logprobs=5).normalized().logprobs == 5 and SamplingParams().normalized().logprobs is None
+
+
+def test_options_of_the_command_line(capsys):
+    from llm_infer_rust_b200 import cli
+    args = cli.parse_args(["--model-path", "x", "--answers", "4", "--logprobs", "3"])
+    assert (args.answers, args.logprobs) == (4, 3)
+    for bad in (["--answers", "0"], ["--answers", "9", "--max-running-req", "8"], ["--logprobs", "33"], ["--logprobs", "-1"]):
+        assert cli.main(["--model-path", "x", "--prompt-ids", "1"] + bad) == 2
+    assert "--answers" in cli.USAGE and "--logprobs" in cli.USAGE
