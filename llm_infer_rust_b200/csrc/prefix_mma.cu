@@ -454,7 +454,8 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
 // * nh), the CTA's warps share the parts, up to eight of them a turn: maxima and sums are asked for together with the outputs that they
 // weight, for what this kernel takes is a few answers from the second-level cache one behind the other.  (A CTA four vectors, two
 // warps each, weights before outputs: eight rows behind 4,096 keys 12,800 cycles.)
-constexpr int JOIN_WARPS = 4, JOIN_BATCH = D <= 128 ? 8 : 4;
+constexpr int JOIN_BATCH = D <= 128 ? 8 : 4;
+template <int JOIN_WARPS>
 __global__ void __launch_bounds__(JOIN_WARPS * 32)
 prefix_join_kernel(bf16* __restrict__ out, const StreamCall k) {
   const PrefixCall& c = k.c;
@@ -542,7 +543,7 @@ prefix_join_kernel(bf16* __restrict__ out, const StreamCall k) {
       sum = fmaf(left[w * ROW + D + 1], ms[w], sum);
     }
     const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-    for (int dim = 2 * static_cast<int>(threadIdx.x); dim < D; dim += 2 * JOIN_WARPS * 32) {
+    for (int dim = 2 * static_cast<int>(threadIdx.x); dim < D; dim += 2 * JOIN_WARPS * 32) {      // (of 16 warps some have none)
       float x = 0.0f, y = 0.0f;
 #pragma unroll
       for (int w = 0; w < JOIN_WARPS; ++w) {
@@ -614,6 +615,10 @@ B200_EXPORT int b200_prefix_attention_mma(const void* q, const void* k_cache, co
   const int entries = entries_bytes(n_rows + n_groups);
   rc = b200_launch(prefix_stream_kernel, dim3(sms), dim3(THREADS), FIXED + entries, stream, 0, kmap, vmap, static_cast<const bf16*>(q), k, box_rows);
   if (rc != 0) return rc;
-  return b200_launch(prefix_join_kernel, dim3(static_cast<unsigned>(n_rows) * nh), dim3(JOIN_WARPS * 32), 0, stream, 0,
-                     static_cast<bf16*>(out), k);
+  // Few vectors have many parts each, a hundred and more where one prompt's keys are all there is: then all of them at once, while an SM has a
+  // CTA.  (4 / 16 warps: two rows of 16 heads behind 4,096 keys 18.6 / 13.4 us in all, 32 rows behind 512 keys 15.0 / 19.0.)
+  const long long vectors_here = static_cast<long long>(n_rows) * nh;
+  const int warps = vectors_here <= sms ? 16 : vectors_here <= 2 * sms ? 8 : 4;
+  return b200_launch(warps == 16 ? prefix_join_kernel<16> : warps == 8 ? prefix_join_kernel<8> : prefix_join_kernel<4>, dim3(static_cast<unsigned>(n_rows) * nh),
+                     dim3(warps * 32), 0, stream, 0, static_cast<bf16*>(out), k);
 }

@@ -34,8 +34,11 @@ from .context import SharedPrefixes, StepContext, context_from_layout
 
 _DTYPES = {"bfloat16": torch.bfloat16, "float32": torch.float32}
 log = logging.getLogger("llm_infer_rust_b200")
-# Decode rows read the pages that they share once from so many keys on that they need not read again (summed over the rows).
-_SAVED_KEYS_AT_LEAST = 4096
+# Decode rows read the pages that they share once where that saves so many bytes of a layer's keys and values, summed over the rows.
+# (Decode attention / shared, us, at 8 KV heads of 128 in bfloat16, 4 KiB a key: 2 rows behind 16,384 keys, 64 MiB saved, 21.7 / 24.6; 4
+# behind 4,096, 48 MiB, 14.5 / 14.0; 8 behind 2,048, 56 MiB, 14.3 / 12.3; 16 behind 1,024, 60 MiB, 12.4 / 12.0; 48 behind 512, 94 MiB,
+# 23.4 / 15.0; 48 behind 16,384 438 / 33.)
+_SAVED_BYTES_AT_LEAST = 48 << 20
 
 
 @dataclass
@@ -262,6 +265,8 @@ class Engine:
         # Requests that share pages (forks): which cache group they are looked for in, and the graphs of their decode steps, keyed by
         # (rows, places for groups).
         self._prefix_group = next((g for g, group in enumerate(self.cache_plan.groups) if not group.window), -1)
+        group = self.cache_plan.groups[self._prefix_group] if self._prefix_group >= 0 else None
+        self._key_bytes = max(1, group.bytes_per_page // (group.page_size * max(1, len(group.entries)))) if group is not None else 1
         self._prefix_graphs: "OrderedDict[tuple, _DecodeGraph]" = OrderedDict()
         self._logprobs: Dict[int, List[TokenLogprob]] = {}
         self._own_ids = 1 << 62                          # ids of the requests that answers() opens
@@ -418,7 +423,7 @@ class Engine:
             return 0
         req.prefix_group = g
         groups, saved = self._rt.count_prefix_groups(mgr, req)
-        if saved < _SAVED_KEYS_AT_LEAST:
+        if saved * self._key_bytes < _SAVED_BYTES_AT_LEAST:
             req.prefix_group, groups = -1, 0
         return groups
 

@@ -24,8 +24,14 @@ _TC_VECTORS = 128             # of a tile of the tcgen05 kernel; a CTA takes one
 _KEYS_PER_CTA_AT_LEAST = 64
 _MOST_SPLITS = 64
 _MOST_ENTRIES = 400           # rows and groups of a call that the tensor-core kernels take
-_TENSOR_CORE_KEYS = 256       # shared keys from which on, and query vectors of a KV head beyond which, the tcgen05 kernel takes a group
-_TENSOR_CORE_VECTORS = 32
+# The tcgen05 kernel takes the shared keys of more vectors of a KV head than the mma.sync kernel has in a tile, from so many blocks on (32 keys
+# of a KV head against 16 vectors each).  (mma.sync / tcgen05, us, 8 KV heads of 128: 32 vectors, 4,096 keys 19.0 / 20.6, 8,192 keys 22.8 /
+# 23.6, 32,768 keys 58.9 / 43.8; 64 vectors, 2,048 keys 23.4 / 25.6, 4,096 keys 29.3 / 26.4; 128 vectors, 1,024 keys 17.6 / 19.9, 2,048 keys
+# 23.6 / 20.7; 256 vectors, 512 keys 22.6 / 23.3, 1,024 keys 29.4 / 24.4.  One KV head: 128 vectors, 8,192 keys 15.8 / 15.8; 512 vectors,
+# 4,096 keys 27.6 / 27.4.  Two tiles of vectors leave three quarters of its rows empty: six groups of 4 to 24 vectors behind 500 to 3,001 keys
+# 29.7 / 40.0.)
+_TENSOR_CORE_BLOCKS, _TENSOR_CORE_BLOCKS_OF_TWO_TILES = 2560, 12288
+_MMA_VECTORS = 16
 
 
 def _splits(most_shared: int, most_own: int, shared_ctas: int, own_ctas: int, room: int) -> tuple:
@@ -52,7 +58,9 @@ def _plan(dtype, heads: int, kv_heads: int, dim: int, page: int, n_rows: int, n_
         floats = n_rows * heads * (shared + own) * (ops.padded_head_dim(dim) + 2)
         return lib.b200_prefix_attention, None, None, (floats, shared, own, tiles, 0, 0, sms), 2
     tcgen05, tiles, two, shared, covered = None, 1, 0, 0, 0
-    if n_groups and dim == 128 and vectors > _TENSOR_CORE_VECTORS and most_shared >= _TENSOR_CORE_KEYS:
+    blocks = -(-vectors // _MMA_VECTORS) * -(-most_shared // 32) * kv_heads * sharing
+    least = _TENSOR_CORE_BLOCKS if vectors > 2 * _MMA_VECTORS else _TENSOR_CORE_BLOCKS_OF_TWO_TILES
+    if n_groups and dim == 128 and vectors > _MMA_VECTORS and blocks >= least:
         # one or two tiles a CTA; as many CTAs a tile as the SMs hold, none without a block of keys for each of its streams
         two = int(vectors > _TC_VECTORS)
         a_cta = _TC_VECTORS << two

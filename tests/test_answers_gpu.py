@@ -32,7 +32,7 @@ def engine(folder, **kw):
 def always_shared(monkeypatch):
     """Small steps take the shared kernels too."""
     from llm_infer_rust_b200.engine import engine as module
-    monkeypatch.setattr(module, "_SAVED_KEYS_AT_LEAST", 1)
+    monkeypatch.setattr(module, "_SAVED_BYTES_AT_LEAST", 1)
 
 
 @pytest.fixture(scope="module")
@@ -312,8 +312,8 @@ def test_large_groups_through_the_tcgen05_kernel(folders):
     twin.open_request(1)
     twin.step([StepEntry(1, tokens(307, 300, 4), [])])
     twin.fork_request(1, list(range(2, 49)))
-    for least, e in ((1, eng), (1 << 30, twin)):
-        module._SAVED_KEYS_AT_LEAST = least
+    for least, e in ((1, eng), (1 << 60, twin)):
+        module._SAVED_BYTES_AT_LEAST = least
         if e is twin:
             for step in range(3):
                 e.step([StepEntry(r, tokens(307, 1, 60 * step + r), [0]) for r in ids])

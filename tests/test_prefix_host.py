@@ -63,7 +63,8 @@ def test_calls_go_where_they_are_served():
     floats, splits, _, tiles, two, covered, ctas = plan()[1]
     assert (tiles, two, covered, splits, ctas) == (1, 1, 256, 18, 148)
     assert plan(most_rows=32)[1][1:6] == (32, 0, 1, 0, 128)                # one tile: a CTA leaves two parts; 4,096 keys are 16 pairs of blocks
-    assert plan(most_rows=8, n_rows=8)[0] == "mma" and plan(shared=200)[0] == "mma" and plan(dim=64)[0] == "mma"
+    assert plan(most_rows=4)[0] == "mma" and plan(shared=600)[0] == "mma" and plan(dim=64)[0] == "mma"
+    assert plan(shared=640)[0] == "tcgen05" and plan(most_rows=8, shared=24576)[0] == "tcgen05" and plan(most_rows=8, shared=24544)[0] == "mma"
     for other in (dict(dtype=torch.float32), dict(page=24), dict(dim=72), dict(heads=17, kv_heads=1), dict(n_rows=400), dict(aligned=False)):
         assert plan(**other)[0] == "all sizes", other
     assert plan(n_rows=399)[0] == "tcgen05"
