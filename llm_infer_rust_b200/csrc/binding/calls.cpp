@@ -373,7 +373,7 @@ PyObject* prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       ints[m++] = stream;
       rc = invoke(fn, ints, m, floats);
     };
-    call(entry[0], {at[1], at[2], at[3], code, width});
+    call(entry[0], {at[1], at[2], at[3], code, width, at[6]});
     call(entry[1], {at[1], at[3], at[4]});
     call(entry[2], {at[1], at[5], at[6]});
   }

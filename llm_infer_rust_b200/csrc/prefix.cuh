@@ -83,80 +83,89 @@ struct PrefixItem {
   bool shared;
 };
 
-// A vector's splits joined, a warp a vector: grid (vectors / MERGE_WARPS), blocks of MERGE_WARPS warps.  The splits' weights
-// 2^(m - max) stand in the lanes; a lane owns groups of four dims.  `pitch`: floats of a split's output (a multiple of 4).
-constexpr int MERGE_WARPS = 4;
-template <typename T, int PITCH>
-__global__ void __launch_bounds__(MERGE_WARPS * 32)
-prefix_merge_kernel(T* __restrict__ out, const PrefixCall c, int hd) {
-  constexpr int MOST = 128;                     // splits in all
-  const int lane = threadIdx.x & 31;
-  pdl_launch_dependents();
-  pdl_wait();
-  const long long vec = static_cast<long long>(blockIdx.x) * MERGE_WARPS + (threadIdx.x >> 5);
-  if (vec >= static_cast<long long>(c.n_rows) * c.nh) return;
-  const int splits = prefix_splits(c);
-  const float2* ml = c.part_ml + vec * splits;
-  const float* acc = c.part_acc + vec * splits * PITCH;
-  float2 mine[MOST / 32];
-  float m = -INFINITY;
-#pragma unroll
-  for (int k = 0; k < MOST / 32; ++k) {
-    mine[k] = make_float2(-INFINITY, 0.0f);
-    if (k * 32 + lane < splits) mine[k] = ml[k * 32 + lane];
-    m = fmaxf(m, mine[k].x);
-  }
-  m = warp_max(m);
-  float l = 0.0f, f[MOST / 32];
-#pragma unroll
-  for (int k = 0; k < MOST / 32; ++k) {
-    f[k] = mine[k].x == -INFINITY ? 0.0f : exp2f(mine[k].x - m);
-    l = fmaf(mine[k].y, f[k], l);
-  }
-  l = warp_sum(l);
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-  const int row = static_cast<int>(vec / c.nh), head = static_cast<int>(vec % c.nh);
-  T* dst = out + (static_cast<long long>(c.cu_q[c.rows[row]]) * c.nh + head) * hd;
-  constexpr int PER = (PITCH + 127) / 128;
+__device__ __forceinline__ float prefix_exp2(float x) {      // 2^x, one special-function instruction (-inf gives 0)
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// One vector out of its `count` parts, rows of PITCH floats of which `hd` are the head's: the CTA's warps share the parts, up to BATCH of them a
+// turn, maxima and sums asked for together with the outputs that they weight, for what this takes is a few answers from the
+// second-level cache one behind the other.  `where`: the place of part p's maximum and sum, and of its outputs.  `left`: shared memory.
+template <int PITCH, int WARPS>
+struct JoinShared { float row[WARPS][PITCH + 4]; };
+template <int PITCH, int WARPS, typename T, typename Where>
+__device__ __forceinline__ void join_parts(T* __restrict__ dst, int hd, int count, const Where& where, JoinShared<PITCH, WARPS>& left) {
+  constexpr int PER = (PITCH + 127) / 128, BATCH = PER == 1 ? 8 : PER == 2 ? 4 : 2;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float4 o[PER];
 #pragma unroll
   for (int n = 0; n < PER; ++n) o[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float m = -INFINITY, l = 0.0f;
+  for (int p0 = warp * BATCH; p0 < count; p0 += WARPS * BATCH) {
+    float4 a[BATCH][PER];
+    float2 ml[BATCH];
 #pragma unroll
-  for (int k = 0; k < MOST / 32; ++k) {
-    const int some = min(32, splits - 32 * k);
-#pragma unroll 4
-    for (int s = 0; s < some; ++s) {
-      const float w = __shfl_sync(0xffffffffu, f[k], s);
-      if (w == 0.0f) continue;                  // (nothing was written where a split saw no key)
-      const float* src = acc + static_cast<long long>(32 * k + s) * PITCH;
+    for (int b = 0; b < BATCH; ++b) {
+      const float2* of_part;
+      const float* src;
+      where(min(p0 + b, count - 1), of_part, src);
+      ml[b] = __ldcg(of_part);
+#pragma unroll
+      for (int n = 0; n < PER; ++n)
+        if (PITCH % 128 == 0 || n * 128 + lane * 4 < PITCH) a[b][n] = __ldcg(reinterpret_cast<const float4*>(src + n * 128 + lane * 4));
+    }
+    float most = m;
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      if (p0 + b >= count) ml[b] = make_float2(-INFINITY, 0.0f);
+      most = fmaxf(most, ml[b].x);
+    }
+    if (most == -INFINITY) continue;
+    const float f = prefix_exp2(m - most);         // (0 on the first visible part)
+    m = most;
+    l *= f;
+#pragma unroll
+    for (int n = 0; n < PER; ++n) { o[n].x *= f; o[n].y *= f; o[n].z *= f; o[n].w *= f; }
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      if (ml[b].x == -INFINITY) continue;          // (where a split saw no key nothing was written)
+      const float w = prefix_exp2(ml[b].x - m);
+      l = fmaf(ml[b].y, w, l);
 #pragma unroll
       for (int n = 0; n < PER; ++n) {
-        const int dim = n * 128 + lane * 4;
-        if (PITCH % 128 == 0 || dim < PITCH) {
-          const float4 a = __ldcg(reinterpret_cast<const float4*>(src + dim));
-          o[n].x = fmaf(w, a.x, o[n].x);
-          o[n].y = fmaf(w, a.y, o[n].y);
-          o[n].z = fmaf(w, a.z, o[n].z);
-          o[n].w = fmaf(w, a.w, o[n].w);
-        }
+        o[n].x = fmaf(w, a[b][n].x, o[n].x);
+        o[n].y = fmaf(w, a[b][n].y, o[n].y);
+        o[n].z = fmaf(w, a[b][n].z, o[n].z);
+        o[n].w = fmaf(w, a[b][n].w, o[n].w);
       }
     }
   }
+  // the warps' parts: columns are the threads' from here on (some have none)
 #pragma unroll
-  for (int n = 0; n < PER; ++n) {
-    const int dim = n * 128 + lane * 4;
-    const float y[4] = {o[n].x * inv, o[n].y * inv, o[n].z * inv, o[n].w * inv};
-#pragma unroll
-    for (int e = 0; e < 4; e += 2)              // (head sizes are even)
-      if (dim + e < hd) {
-        dst[dim + e] = from_f32<T>(y[e]);
-        dst[dim + e + 1] = from_f32<T>(y[e + 1]);
-      }
+  for (int n = 0; n < PER; ++n)
+    if (PITCH % 128 == 0 || n * 128 + lane * 4 < PITCH) *reinterpret_cast<float4*>(left.row[warp] + n * 128 + lane * 4) = o[n];
+  if (lane == 0) { left.row[warp][PITCH] = m; left.row[warp][PITCH + 1] = l; }
+  __syncthreads();
+  const int warps = min(WARPS, (count + BATCH - 1) / BATCH);      // that had parts
+  float most = -INFINITY, sum = 0.0f;
+  for (int w = 0; w < warps; ++w) most = fmaxf(most, left.row[w][PITCH]);
+  const float base = most == -INFINITY ? 0.0f : most;
+  for (int w = 0; w < warps; ++w) sum = fmaf(left.row[w][PITCH + 1], prefix_exp2(left.row[w][PITCH] - base), sum);
+  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  for (int dim = 2 * static_cast<int>(threadIdx.x); dim < hd; dim += 2 * WARPS * 32) {      // (head sizes are even)
+    float x = 0.0f, y = 0.0f;
+    for (int w = 0; w < warps; ++w) {
+      const float2 two = *reinterpret_cast<const float2*>(left.row[w] + dim);
+      const float f = prefix_exp2(left.row[w][PITCH] - base);
+      x = fmaf(two.x, f, x);
+      y = fmaf(two.y, f, y);
+    }
+    dst[dim] = from_f32<T>(x * inv);
+    dst[dim + 1] = from_f32<T>(y * inv);
   }
 }
-template <typename T, int PITCH>
-static inline int prefix_merge(void* out, const PrefixCall& c, int hd, cudaStream_t stream) {
-  const long long vectors = static_cast<long long>(c.n_rows) * c.nh;
-  return b200_launch(prefix_merge_kernel<T, PITCH>, dim3(static_cast<unsigned>((vectors + MERGE_WARPS - 1) / MERGE_WARPS)), dim3(MERGE_WARPS * 32), 0,
-                     stream, 0, static_cast<T*>(out), c, hd);
-}
+// Warps of a CTA that joins one of `vectors` vectors.  Few vectors have many parts each, a hundred and more where one prompt's keys are all there
+// is: then all of them at once, while an SM has a CTA.  (4 / 16 warps: two rows of 16 heads behind 4,096 keys 18.6 / 13.4 us in all, 32
+// rows behind 512 keys 15.0 / 19.0.)
+static inline int join_warps_of(long long vectors, int sms) { return vectors <= sms ? 16 : vectors <= 2 * sms ? 8 : 4; }

@@ -451,18 +451,12 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
 }
 
 // A vector joined out of its parts: those of its group's tile, or of the tcgen05 kernel's splits, and those of its row's item.  grid (n_rows
-// * nh), the CTA's warps share the parts, up to eight of them a turn: maxima and sums are asked for together with the outputs that they
-// weight, for what this kernel takes is a few answers from the second-level cache one behind the other.  (A CTA four vectors, two
-// warps each, weights before outputs: eight rows behind 4,096 keys 12,800 cycles.)
-constexpr int JOIN_BATCH = D <= 128 ? 8 : 4;
+// * nh).  (A CTA four vectors, two warps each, weights before outputs: eight rows behind 4,096 keys 12,800 cycles.)
 template <int JOIN_WARPS>
 __global__ void __launch_bounds__(JOIN_WARPS * 32)
 prefix_join_kernel(bf16* __restrict__ out, const StreamCall k) {
+  __shared__ __align__(16) JoinShared<D, JOIN_WARPS> left;
   const PrefixCall& c = k.c;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  constexpr int ROW = D + 4;                       // what a warp leaves: outputs, maximum, sum
-  constexpr int PER = (D + 127) / 128;
-  __shared__ __align__(16) float left[JOIN_WARPS * ROW];
   const int group = c.nh / c.nkv;
   const int i = static_cast<int>(blockIdx.x) / c.nh, head = static_cast<int>(blockIdx.x) - i * c.nh, kvh = head / group, r = head - kvh * group;
   // (the stream kernel began when everything before the call had ended, so the call's index arrays may be read beside it)
@@ -475,91 +469,13 @@ prefix_join_kernel(bf16* __restrict__ out, const StreamCall k) {
   const bool second = v / VT > max(first.z, 0) / VT, split = grouped != 0 && v < 0;
   const int tile = second ? rest.x : first.w;
   const int tile_count = grouped == 0 ? 0 : split ? c.splits_shared : second ? rest.z : rest.y;
-  // part p of tile_count + own_count: vector `at` of the stream's parts, or of the tcgen05 kernel's
   const long long vec = static_cast<long long>(blockIdx.x) * c.splits_shared;
-  const int count = tile_count + own_count;
-  float4 o[PER];
-#pragma unroll
-  for (int n = 0; n < PER; ++n) o[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float m = -INFINITY, l = 0.0f;
-  for (int p0 = warp * JOIN_BATCH; p0 < count; p0 += JOIN_WARPS * JOIN_BATCH) {
-    float4 a[JOIN_BATCH][PER];
-    float2 ml[JOIN_BATCH];
-#pragma unroll
-    for (int b = 0; b < JOIN_BATCH; ++b) {
-      const int p = min(p0 + b, count - 1);
-      const bool of_tc = split && p < tile_count;
-      const long long at = of_tc ? vec + p : p < tile_count ? static_cast<long long>(tile + p) * VT + v % VT : static_cast<long long>(own + p - tile_count) * VT + r;
-      ml[b] = __ldcg((of_tc ? c.part_ml : k.ml) + at);
-      const float* src = (of_tc ? c.part_acc : k.acc) + at * D;
-#pragma unroll
-      for (int n = 0; n < PER; ++n)
-        if (D % 128 == 0 || n * 128 + lane * 4 < D) a[b][n] = __ldcg(reinterpret_cast<const float4*>(src + n * 128 + lane * 4));
-    }
-    float most = m;
-#pragma unroll
-    for (int b = 0; b < JOIN_BATCH; ++b) {
-      if (p0 + b >= count) ml[b] = make_float2(-INFINITY, 0.0f);
-      most = fmaxf(most, ml[b].x);
-    }
-    if (most == -INFINITY) continue;
-    const float f = fast_exp2(m - most);           // (0 on the first visible part)
-    m = most;
-    l *= f;
-#pragma unroll
-    for (int n = 0; n < PER; ++n) { o[n].x *= f; o[n].y *= f; o[n].z *= f; o[n].w *= f; }
-#pragma unroll
-    for (int b = 0; b < JOIN_BATCH; ++b) {
-      if (ml[b].x == -INFINITY) continue;          // (where a split saw no key nothing was written)
-      const float w = fast_exp2(ml[b].x - m);
-      l = fmaf(ml[b].y, w, l);
-#pragma unroll
-      for (int n = 0; n < PER; ++n) {
-        o[n].x = fmaf(w, a[b][n].x, o[n].x);
-        o[n].y = fmaf(w, a[b][n].y, o[n].y);
-        o[n].z = fmaf(w, a[b][n].z, o[n].z);
-        o[n].w = fmaf(w, a[b][n].w, o[n].w);
-      }
-    }
-  }
-  if (count > JOIN_BATCH) {                        // (else all of it is the first warp's)
-#pragma unroll
-    for (int n = 0; n < PER; ++n)
-      if (D % 128 == 0 || n * 128 + lane * 4 < D) *reinterpret_cast<float4*>(left + warp * ROW + n * 128 + lane * 4) = o[n];
-    if (lane == 0) { left[warp * ROW + D] = m; left[warp * ROW + D + 1] = l; }
-    __syncthreads();
-  }
-  // columns are the threads' from here on, where the warps have shared; else the first warp's lanes'
-  if (count > JOIN_BATCH) {
-    float ms[JOIN_WARPS], most = -INFINITY, sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < JOIN_WARPS; ++w) {
-      ms[w] = left[w * ROW + D];
-      most = fmaxf(most, ms[w]);
-    }
-#pragma unroll
-    for (int w = 0; w < JOIN_WARPS; ++w) {
-      ms[w] = ms[w] == -INFINITY ? 0.0f : fast_exp2(ms[w] - most);
-      sum = fmaf(left[w * ROW + D + 1], ms[w], sum);
-    }
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-    for (int dim = 2 * static_cast<int>(threadIdx.x); dim < D; dim += 2 * JOIN_WARPS * 32) {      // (of 16 warps some have none)
-      float x = 0.0f, y = 0.0f;
-#pragma unroll
-      for (int w = 0; w < JOIN_WARPS; ++w) {
-        const float2 two = *reinterpret_cast<const float2*>(left + w * ROW + dim);
-        x = fmaf(two.x, ms[w], x);
-        y = fmaf(two.y, ms[w], y);
-      }
-      *reinterpret_cast<uint32_t*>(dst + dim) = pack_bf16(x * inv, y * inv);
-    }
-  } else if (warp == 0) {
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-#pragma unroll
-    for (int n = 0; n < PER; ++n)
-      if (D % 128 == 0 || n * 128 + lane * 4 < D)
-        *reinterpret_cast<uint2*>(dst + n * 128 + lane * 4) = make_uint2(pack_bf16(o[n].x * inv, o[n].y * inv), pack_bf16(o[n].z * inv, o[n].w * inv));
-  }
+  join_parts<D, JOIN_WARPS>(dst, D, tile_count + own_count, [&](int p, const float2*& ml, const float*& acc) {
+    const bool of_tc = split && p < tile_count;
+    const long long at = of_tc ? vec + p : p < tile_count ? static_cast<long long>(tile + p) * VT + v % VT : static_cast<long long>(own + p - tile_count) * VT + r;
+    ml = (of_tc ? c.part_ml : k.ml) + at;
+    acc = (of_tc ? c.part_acc : k.acc) + at * D;
+  }, left);
 }
 
 // Parts that the kernel may leave: one for every stretch and item.
@@ -615,10 +531,7 @@ B200_EXPORT int b200_prefix_attention_mma(const void* q, const void* k_cache, co
   const int entries = entries_bytes(n_rows + n_groups);
   rc = b200_launch(prefix_stream_kernel, dim3(sms), dim3(THREADS), FIXED + entries, stream, 0, kmap, vmap, static_cast<const bf16*>(q), k, box_rows);
   if (rc != 0) return rc;
-  // Few vectors have many parts each, a hundred and more where one prompt's keys are all there is: then all of them at once, while an SM has a
-  // CTA.  (4 / 16 warps: two rows of 16 heads behind 4,096 keys 18.6 / 13.4 us in all, 32 rows behind 512 keys 15.0 / 19.0.)
-  const long long vectors_here = static_cast<long long>(n_rows) * nh;
-  const int warps = vectors_here <= sms ? 16 : vectors_here <= 2 * sms ? 8 : 4;
+  const int warps = join_warps_of(static_cast<long long>(n_rows) * nh, sms);
   return b200_launch(warps == 16 ? prefix_join_kernel<16> : warps == 8 ? prefix_join_kernel<8> : prefix_join_kernel<4>, dim3(static_cast<unsigned>(n_rows) * nh),
                      dim3(warps * 32), 0, stream, 0, static_cast<bf16*>(out), k);
 }

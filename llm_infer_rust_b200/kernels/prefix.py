@@ -21,7 +21,7 @@ from .ops import KernelError
 
 _TILE = 32                    # query vectors of a CTA of the all-sizes kernel
 _TC_VECTORS = 128             # of a tile of the tcgen05 kernel; a CTA takes one or two
-_KEYS_PER_CTA_AT_LEAST = 64
+_KEYS_PER_CTA_AT_LEAST = 32
 _MOST_SPLITS = 64
 _MOST_ENTRIES = 400           # rows and groups of a call that the tensor-core kernels take
 # The tcgen05 kernel takes the shared keys of more vectors of a KV head than the mma.sync kernel has in a tile, from so many blocks on (32 keys
@@ -36,8 +36,9 @@ _MMA_VECTORS = 16
 
 def _splits(most_shared: int, most_own: int, shared_ctas: int, own_ctas: int, room: int) -> tuple:
     """Into how many splits the all-sizes kernel cuts the shared and the own keys, ``shared_ctas`` and ``own_ctas`` CTAs for each split:
-    about as many keys a CTA on both sides, and about ``room`` CTAs in all."""
-    a_cta = max(_KEYS_PER_CTA_AT_LEAST, -(-(most_shared * shared_ctas + most_own * own_ctas) // max(1, room)))
+    about as many keys a CTA on both sides, and about twice ``room`` CTAs in all (a CTA is a chain of waits; groups and rows are often
+    smaller than the largest)."""
+    a_cta = max(_KEYS_PER_CTA_AT_LEAST, -(-(most_shared * shared_ctas + most_own * own_ctas) // max(1, 2 * room)))
     return max(1, min(_MOST_SPLITS, -(-most_shared // a_cta))), max(1, min(_MOST_SPLITS, -(-most_own // a_cta)))
 
 
@@ -139,7 +140,7 @@ def prefix_attention(q, k_cache, v_cache, out, block_table, cu_q, kv_len, rows, 
                   k_cache.shape[0], float(scale))
         ends = (ops.error_word(rows.device), ops._stream())
         if all_sizes is not None:
-            rc = all_sizes(q, k_cache, v_cache, out, *common, shared, own, tiles, ops._code(q), head_dim, *ends)
+            rc = all_sizes(q, k_cache, v_cache, out, *common, shared, own, tiles, ops._code(q), head_dim, sms, *ends)
         else:
             rc = tcgen05(q, k_cache, v_cache, *common, shared, tiles, two, *ends) if tcgen05 is not None else 0
             rc = rc or mma(q, k_cache, v_cache, out, *common, shared, covered, sms, *ends)
