@@ -312,11 +312,11 @@ PyObject* byte_product(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // Decode attention behind shared prefixes (kernels/prefix.py) as one call: what the tensors must be, the memory between its kernels and
 // the launches.  The entry points are those of the plan, None where it has no use for one: the all-sizes kernel alone, or the
 // tensor-core kernels.  plan: (floats of scratch, splits of the shared keys, splits of the own keys, tiles, two tiles a CTA, vectors
-// that the tcgen05 kernel covers, CTAs).  None, and nothing done, where something is not as it should be (the wrapper then says what)
+// that the tcgen05 kernel covers, CTAs of the stream kernel, multiprocessors).  None, and nothing done, where something is not as it should be (the wrapper then says what)
 // or this thread records its calls.  (Through Python the call took the host 17 us, of which 7 are three launches.)
 PyObject* prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 20 || !PyFloat_Check(args[16]) || !PyTuple_Check(args[17]) || PyTuple_GET_SIZE(args[17]) != 7) {
+  if (n != 20 || !PyFloat_Check(args[16]) || !PyTuple_Check(args[17]) || PyTuple_GET_SIZE(args[17]) != 8) {
     PyErr_SetString(PyExc_TypeError, "prefix_attention(all sizes, tcgen05, mma, q, k, v, out, block table, cu_q, kv_len, rows, groups, heads, kv heads, "
                                      "head size, page size, scale, plan, error word, stream)");
     return nullptr;
@@ -337,9 +337,9 @@ PyObject* prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       Py_RETURN_NONE;
   }
   const at::Tensor &q = *t[0], &k = *t[1], &v = *t[2], &out = *t[3], &table = *t[4], &cu = *t[5], &lengths = *t[6], &rows = *t[7], &groups = *t[8];
-  I at[7], size[4];
+  I at[8], size[4];
   for (int i = 0; i < 4; ++i) size[i] = PyLong_AsLongLong(args[12 + i]);
-  for (int i = 0; i < 7; ++i) at[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(args[17], i));
+  for (int i = 0; i < 8; ++i) at[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(args[17], i));
   const I stream = PyLong_AsLongLong(args[19]);
   if (PyErr_Occurred()) return nullptr;
   const I heads = size[0], kv_heads = size[1], width = size[2], page = size[3];
@@ -373,9 +373,9 @@ PyObject* prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       ints[m++] = stream;
       rc = invoke(fn, ints, m, floats);
     };
-    call(entry[0], {at[1], at[2], at[3], code, width, at[6]});
+    call(entry[0], {at[1], at[2], at[3], code, width, at[7]});
     call(entry[1], {at[1], at[3], at[4]});
-    call(entry[2], {at[1], at[5], at[6]});
+    call(entry[2], {at[1], at[5], at[6], at[7]});
   }
   return PyLong_FromLong(rc);
   END_HANDLE_TH_ERRORS

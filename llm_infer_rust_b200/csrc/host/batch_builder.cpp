@@ -45,11 +45,18 @@ std::vector<Shared> shared_rows(const CacheManager& cache, const BatchRequest& r
 }
 }  // namespace
 
-std::pair<int, int> count_prefix_groups(const CacheManager& cache, const BatchRequest& req) {
-  int saved = 0;
-  const std::vector<Shared> shared = shared_rows(cache, req);
-  for (const Shared& s : shared) saved += (static_cast<int>(s.rows.size()) - 1) * s.keys;
-  return {static_cast<int>(shared.size()), saved};
+PrefixCount count_prefix_groups(const CacheManager& cache, const BatchRequest& req) {
+  PrefixCount found;
+  std::vector<int> of(req.ids.size(), 0);
+  for (const Shared& s : shared_rows(cache, req)) {
+    found.groups += 1;
+    found.saved_keys += static_cast<int64_t>(s.rows.size() - 1) * s.keys;
+    found.most_shared = std::max(found.most_shared, s.keys);
+    for (int r : s.rows) of[r] = s.keys;
+  }
+  for (size_t r = 0; r < req.ids.size(); ++r)
+    if (req.counts[r] == 1) found.most_own = std::max(found.most_own, cache.length(req.ids[r]) + 1 - of[r]);
+  return found;
 }
 
 BatchLayout plan_batch(const CacheManager& cache, const BatchRequest& req) {
@@ -108,7 +115,7 @@ BatchLayout plan_batch(const CacheManager& cache, const BatchRequest& req) {
     L.off_slots.push_back(take(L.num_tokens));
     L.off_table.push_back(take(L.num_rows * width));
   }
-  const int found = req.prefix_group < 0 || L.num_decode == 0 ? 0 : req.prefix_groups > 0 ? req.prefix_groups : count_prefix_groups(cache, req).first;
+  const int found = req.prefix_group < 0 || L.num_decode == 0 ? 0 : req.prefix_groups > 0 ? req.prefix_groups : count_prefix_groups(cache, req).groups;
   if (found > 0) {
     L.num_prefix_groups = req.prefix_groups > 0 ? found : found + 1;
     L.off_prefix_rows = take(L.num_decode);

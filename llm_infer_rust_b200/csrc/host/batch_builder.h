@@ -10,7 +10,6 @@
 // block table per cache group.
 #pragma once
 #include <cstdint>
-#include <utility>
 #include <vector>
 
 #include "page_cache.h"
@@ -54,9 +53,14 @@ struct BatchRequest {
   int prefix_groups = 0;          // > 0: places for exactly so many groups (a graph's), those that are not used hold no rows
 };
 
-// How many groups of decode rows of `req` share pages in its prefix_group (not counting the last one, of the other rows), and how many
-// keys their rows need not read again, summed over the rows.
-std::pair<int, int> count_prefix_groups(const CacheManager& cache, const BatchRequest& req);
+// Groups of decode rows of `req` that share pages in its prefix_group (not counting the last one, of the other rows), the keys that their
+// rows need not read again, summed over the rows, the most keys that a group shares and the most that a row has beyond its group's.
+struct PrefixCount {
+  int groups = 0;
+  int64_t saved_keys = 0;
+  int most_shared = 0, most_own = 0;
+};
+PrefixCount count_prefix_groups(const CacheManager& cache, const BatchRequest& req);
 // Number of int32 the buffer must hold, without writing anything.
 BatchLayout plan_batch(const CacheManager& cache, const BatchRequest& req);
 // Fill `out` (capacity in int32).  Pages must already cover every row

@@ -175,7 +175,10 @@ PYBIND11_MODULE(_host_runtime, m) {
       .def_readwrite("prefix_group", &BatchRequest::prefix_group)
       .def_readwrite("prefix_groups", &BatchRequest::prefix_groups);
 
-  m.def("count_prefix_groups", &count_prefix_groups);
+  m.def("count_prefix_groups", [](const CacheManager& cache, const BatchRequest& req) {
+    const PrefixCount found = count_prefix_groups(cache, req);
+    return py::make_tuple(found.groups, found.saved_keys, found.most_shared, found.most_own);
+  }, "(groups of decode rows that share pages, keys that need not be read again, most shared keys, most own keys)");
 
   m.def("plan_batch", &plan_batch);
   m.def("build_batch", [](const CacheManager& cache, const BatchRequest& req,

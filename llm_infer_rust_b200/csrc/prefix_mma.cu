@@ -479,27 +479,28 @@ prefix_join_kernel(bf16* __restrict__ out, const StreamCall k) {
 }
 
 // Parts that the kernel may leave: one for every stretch and item.
-static long long parts_of(int n_rows, int n_groups, int nh, int nkv, int sms) {
+static long long parts_of(int n_rows, int n_groups, int nh, int nkv, int ctas) {
   const long long group = nh / nkv;
-  return static_cast<long long>(sms) * WARPS + nkv * ((n_rows * group + VT - 1) / VT + n_groups + n_rows) + 1;
+  return static_cast<long long>(ctas) * WARPS + nkv * ((n_rows * group + VT - 1) / VT + n_groups + n_rows) + 1;
 }
 static long long align4(long long n) { return (n + 3) / 4 * 4; }
 
 // Rows and groups of a call, in all.
 B200_EXPORT int b200_prefix_most_entries() { return MOST_ENTRIES; }
 // Floats of scratch: the tcgen05 kernel's part first (splits_shared > 0).
-B200_EXPORT long long b200_prefix_scratch_floats(int n_rows, int n_groups, int nh, int nkv, int splits_shared, int sms) {
-  const long long vectors = static_cast<long long>(n_rows) * nh * splits_shared, parts = parts_of(n_rows, n_groups, nh, nkv, sms) * VT;
+B200_EXPORT long long b200_prefix_scratch_floats(int n_rows, int n_groups, int nh, int nkv, int splits_shared, int ctas) {
+  const long long vectors = static_cast<long long>(n_rows) * nh * splits_shared, parts = parts_of(n_rows, n_groups, nh, nkv, ctas) * VT;
   return align4(vectors * (D + 2)) + parts * (D + 2) + static_cast<long long>(n_rows) * nkv * (sizeof(RowParts) / 4);
 }
 
 // q, out [tokens, nh * D]; k_cache, v_cache [pages, nkv, page_size, D]; `groups`: (first row, shared keys) each.  `scratch` holds
-// b200_prefix_scratch_floats(...) floats on a 16-byte boundary.  `covered` > 0: b200_prefix_tcgen05 has just been launched with the
-// same scratch for the first `covered` vectors of every group, in splits_shared splits (else 0 of both).  `sms`: CTAs.
+// b200_prefix_scratch_floats(...) floats on a 16-byte boundary (of as many `ctas`).  `covered` > 0: b200_prefix_tcgen05 has just been launched with the
+// same scratch for the first `covered` vectors of every group, in splits_shared splits (else 0 of both).  `ctas`: of the stream kernel, at
+// most one for each of the device's `sms`.
 B200_EXPORT int b200_prefix_attention_mma(const void* q, const void* k_cache, const void* v_cache, void* out, float* scratch, const int* block_table,
                                           int table_stride, const int* cu_q, const int* kv_len, const int* rows, int n_rows, const int* groups,
                                           int n_groups, int nh, int nkv, int page_size, int pages, float scale, int splits_shared, int covered,
-                                          int sms, int* err, cudaStream_t stream) {
+                                          int ctas, int sms, int* err, cudaStream_t stream) {
   if (n_rows <= 0) return 0;
   if (nh <= 0 || nkv <= 0 || nh % nkv != 0 || nh / nkv > 16 || page_size <= 0 || (page_size & (page_size - 1)) != 0 || pages <= 0 || table_stride <= 0 || n_groups < 0)
     return B200_BAD_SIZE;
@@ -507,10 +508,10 @@ B200_EXPORT int b200_prefix_attention_mma(const void* q, const void* k_cache, co
   const long long most_blocks = (static_cast<long long>(table_stride) * page_size / KB + 2) * nkv *
                                 ((static_cast<long long>(n_rows) * (nh / nkv) + VT - 1) / VT + n_groups + n_rows);
   if (most_blocks > INT32_MAX / 2) return B200_BAD_SIZE;
-  if (splits_shared < 0 || covered < 0 || (covered > 0) != (splits_shared > 0) || sms < 1 || n_rows + n_groups > MOST_ENTRIES) return B200_BAD_SIZE;
+  if (splits_shared < 0 || covered < 0 || (covered > 0) != (splits_shared > 0) || ctas < 1 || ctas > sms || n_rows + n_groups > MOST_ENTRIES) return B200_BAD_SIZE;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(scratch)) % 16 != 0) return B200_BAD_ALIGN;
   StreamCall k;
-  const size_t vectors = static_cast<size_t>(n_rows) * nh * splits_shared, parts = static_cast<size_t>(parts_of(n_rows, n_groups, nh, nkv, sms)) * VT;
+  const size_t vectors = static_cast<size_t>(n_rows) * nh * splits_shared, parts = static_cast<size_t>(parts_of(n_rows, n_groups, nh, nkv, ctas)) * VT;
   if (static_cast<long long>(n_rows) * nh > INT32_MAX) return B200_BAD_SIZE;
   float2* part_ml = reinterpret_cast<float2*>(scratch + vectors * D);
   k.acc = scratch + align4(vectors * (D + 2));
@@ -529,7 +530,7 @@ B200_EXPORT int b200_prefix_attention_mma(const void* q, const void* k_cache, co
   rc = prefix_smem_limit(prefix_stream_kernel, static_cast<int>(FIXED) + entries_bytes(MOST_ENTRIES), seen);
   if (rc != 0) return rc;
   const int entries = entries_bytes(n_rows + n_groups);
-  rc = b200_launch(prefix_stream_kernel, dim3(sms), dim3(THREADS), FIXED + entries, stream, 0, kmap, vmap, static_cast<const bf16*>(q), k, box_rows);
+  rc = b200_launch(prefix_stream_kernel, dim3(ctas), dim3(THREADS), FIXED + entries, stream, 0, kmap, vmap, static_cast<const bf16*>(q), k, box_rows);
   if (rc != 0) return rc;
   const int warps = join_warps_of(static_cast<long long>(n_rows) * nh, sms);
   return b200_launch(warps == 16 ? prefix_join_kernel<16> : warps == 8 ? prefix_join_kernel<8> : prefix_join_kernel<4>, dim3(static_cast<unsigned>(n_rows) * nh),

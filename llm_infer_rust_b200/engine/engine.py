@@ -117,9 +117,10 @@ class _MetaBuffers:
 
 
 class _DecodeGraph:
-    def __init__(self, bucket: int, prefix_groups: int = 0):
+    def __init__(self, bucket: int, prefix_groups: int = 0, prefix_keys: Tuple[int, int] = (0, 0)):
         self.bucket = bucket
         self.prefix_groups = prefix_groups      # > 0: for rows that share pages, with places for so many groups of them
+        self.prefix_keys = prefix_keys          # and what it is cut up for: shared keys of a group, own keys of a row
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.meta: Optional[torch.Tensor] = None
         self.ctx: Optional[StepContext] = None
@@ -263,7 +264,7 @@ class Engine:
         self._shape_seen: Dict[tuple, int] = {}
         self._shape_graph_limit = 6
         # Requests that share pages (forks): which cache group they are looked for in, and the graphs of their decode steps, keyed by
-        # (rows, places for groups).
+        # (rows, places for groups, shared keys, own keys), the keys rounded up to powers of two and of four.
         self._prefix_group = next((g for g, group in enumerate(self.cache_plan.groups) if not group.window), -1)
         group = self.cache_plan.groups[self._prefix_group] if self._prefix_group >= 0 else None
         self._key_bytes = max(1, group.bytes_per_page // (group.page_size * max(1, len(group.entries)))) if group is not None else 1
@@ -352,7 +353,7 @@ class Engine:
             rows = dev[layout.off_prefix_rows:layout.off_prefix_rows + layout.num_decode]
             places = dev[layout.off_prefix_groups:layout.off_prefix_groups + 2 * groups].view(groups, 2)
             # (a graph is cut up for what may come, a step of its own for what is there)
-            most = (layout.num_decode, kv_len_bound, kv_len_bound) if graph is not None else \
+            most = (layout.num_decode,) + graph.prefix_keys if graph is not None else \
                 (layout.most_prefix_rows, layout.most_prefix_keys, layout.most_own_keys)
             most += (groups - 1,)
             ctx.shared = SharedPrefixes(self._prefix_group, rows, places, *most)
@@ -404,7 +405,7 @@ class Engine:
         if decode_only and self._graphs and all(len(e.want) == 1 for e in entries):
             bucket = next((b for b in sorted(self._graphs) if b >= len(entries)), None)
             if bucket is not None and max(mgr.length(e.request) for e in entries) < self.max_seq_len:
-                graph = self._prefix_graph(bucket, groups) if groups else self._graphs[bucket]
+                graph = self._prefix_graph(bucket, *groups) if groups else self._graphs[bucket]
         if graph is None and not decode_only and 0 < len(req.tokens) <= self.prefill_graph_max_tokens \
                 and max(mgr.length(e.request) + len(e.tokens) for e in entries) <= self.max_seq_len:
             graph = self._shape_graph(tuple(req.counts) + (-1, len(req.want_index)))
@@ -416,23 +417,26 @@ class Engine:
             mgr.advance(e.request, mgr.length(e.request) + len(e.tokens))
         return logits
 
-    def _look_for_prefixes(self, req) -> int:
-        """Decide whether the step's decode rows read the pages that they share once; how many groups of rows do so (0: none)."""
+    def _look_for_prefixes(self, req) -> Optional[Tuple[int, int, int]]:
+        """Decide whether the step's decode rows read the pages that they share once: how many groups of rows do so, the most keys that one
+        shares and the most that a row has beyond them (None: none does)."""
         mgr, g = self.cache.manager, self._prefix_group
         if g < 0 or mgr.shared_pages(g) == 0:
-            return 0
+            return None
         req.prefix_group = g
-        groups, saved = self._rt.count_prefix_groups(mgr, req)
-        if saved * self._key_bytes < _SAVED_BYTES_AT_LEAST:
-            req.prefix_group, groups = -1, 0
-        return groups
+        groups, saved, shared, own = self._rt.count_prefix_groups(mgr, req)
+        if not groups or saved * self._key_bytes < _SAVED_BYTES_AT_LEAST:
+            req.prefix_group = -1
+            return None
+        return groups, shared, own
 
-    def _prefix_graph(self, bucket: int, groups: int) -> _DecodeGraph:
+    def _prefix_graph(self, bucket: int, groups: int, shared: int, own: int) -> _DecodeGraph:
         places = 1 + (1 << (groups - 1).bit_length())            # (the last group is the other rows')
-        key = (bucket, places)
+        keys = 1 << (shared - 1).bit_length(), 1 << (max(own, 64) - 1).bit_length() // 2 * 2 + 2
+        key = (bucket, places) + keys
         g = self._prefix_graphs.get(key)
         if g is None:
-            g = self._prefix_graphs[key] = _DecodeGraph(bucket, places)
+            g = self._prefix_graphs[key] = _DecodeGraph(bucket, places, keys)
             while len(self._prefix_graphs) > self._shape_graph_limit:
                 self._prefix_graphs.popitem(last=False)
         self._prefix_graphs.move_to_end(key)

@@ -42,6 +42,27 @@ def _splits(most_shared: int, most_own: int, shared_ctas: int, own_ctas: int, ro
     return max(1, min(_MOST_SPLITS, -(-most_shared // a_cta))), max(1, min(_MOST_SPLITS, -(-most_own // a_cta)))
 
 
+# What the tcgen05 kernel takes beside its steps (a block of keys, or one for each stream), and a step; what the stream kernel takes beside
+# its bytes, bytes that one of few SMs and all of them together take in, and the keys that an item costs beside its own (us, bytes a us).
+_TC_FIXED, _TC_STEP = 9.6, 2.25
+_OWN_FIXED, _OWN_BYTES, _OWN_BYTES_ALL, _OWN_KEYS = 9.0, 58000.0, 4.5e6, 64
+
+
+def _share_sms(steps: int, tiles: int, items: int, most_own: int, key_bytes: int, sms: int) -> tuple:
+    """How many CTAs cut each of ``tiles`` tiles' ``steps``, and the CTAs of the stream kernel for ``items`` of own keys (half of ``most_own``
+    each): side by side on SMs of their own, as the registers and shared memory of either leave no room for the other, or one behind the
+    other on all.  (64 rows of 32 heads behind 32,768 keys, own keys of 1 to 1,024: 12 or 13 CTAs a tile beside 52 or 44 SMs 72.6 us, 10
+    beside 68 80.8, 15 beside 28 105, one behind the other 84; 24 rows of 64 heads behind 8,000 keys, 1 to 200: 27.4 and 31.1.)"""
+    own_bytes = items * (most_own / 2 + _OWN_KEYS) * key_bytes
+    most = max(1, min(steps, sms // tiles, _MOST_SPLITS))
+    best = _TC_FIXED + _TC_STEP * -(-steps // most) + _OWN_FIXED + own_bytes / _OWN_BYTES_ALL, most, sms
+    for ctas in range(1, most + 1):
+        left = sms - ctas * tiles
+        if left >= 1:
+            best = min(best, (max(_TC_FIXED + _TC_STEP * -(-steps // ctas), _OWN_FIXED + own_bytes / min(left * _OWN_BYTES, _OWN_BYTES_ALL)), ctas, left))
+    return best[1:]
+
+
 @functools.lru_cache(maxsize=4096)
 def _plan(dtype, heads: int, kv_heads: int, dim: int, page: int, n_rows: int, n_groups: int, most_rows: int, most_shared: int, most_own: int,
           sharing: int, aligned: bool, sms: int) -> tuple:
@@ -57,23 +78,23 @@ def _plan(dtype, heads: int, kv_heads: int, dim: int, page: int, n_rows: int, n_
         per_sm = max(1, 227 * 1024 // (lib.b200_prefix_attention_smem() + 1024))
         shared, own = _splits(most_shared, most_own, sharing * kv_heads * tiles, n_rows * kv_heads * -(-per // _TILE), per_sm * sms)
         floats = n_rows * heads * (shared + own) * (ops.padded_head_dim(dim) + 2)
-        return lib.b200_prefix_attention, None, None, (floats, shared, own, tiles, 0, 0, sms), 2
-    tcgen05, tiles, two, shared, covered = None, 1, 0, 0, 0
+        return lib.b200_prefix_attention, None, None, (floats, shared, own, tiles, 0, 0, 0, sms), 2
+    tcgen05, tiles, two, shared, covered, stream = None, 1, 0, 0, 0, sms
     blocks = -(-vectors // _MMA_VECTORS) * -(-most_shared // 32) * kv_heads * sharing
     least = _TENSOR_CORE_BLOCKS if vectors > 2 * _MMA_VECTORS else _TENSOR_CORE_BLOCKS_OF_TWO_TILES
     if n_groups and dim == 128 and vectors > _MMA_VECTORS and blocks >= least:
-        # one or two tiles a CTA; as many CTAs a tile as the SMs hold, none without a block of keys for each of its streams
+        # one or two tiles a CTA, none without a block of keys for each of its streams
         two = int(vectors > _TC_VECTORS)
         a_cta = _TC_VECTORS << two
         tiles = -(-vectors // a_cta)
-        ctas = max(1, min(-(-most_shared // (256 >> two)), sms // (sharing * kv_heads * tiles), _MOST_SPLITS))
+        ctas, stream = _share_sms(-(-most_shared // (256 >> two)), sharing * kv_heads * tiles, n_rows * kv_heads, most_own, 4 * dim, sms)
         shared, covered = ctas << (1 - two), tiles * a_cta
         tcgen05 = load_entry_points("prefix_tcgen05.cu").b200_prefix_tcgen05
     lib = load_entry_points("prefix_mma.cu", {"HEAD_DIM": dim})
     count = lib.library.b200_prefix_scratch_floats
     count.restype = ctypes.c_longlong
-    floats = count(n_rows, n_groups, heads, kv_heads, shared, sms)
-    return None, tcgen05, lib.b200_prefix_attention_mma, (floats, shared, 0, tiles, two, covered, sms), 2 + (tcgen05 is not None)
+    floats = count(n_rows, n_groups, heads, kv_heads, shared, stream)
+    return None, tcgen05, lib.b200_prefix_attention_mma, (floats, shared, 0, tiles, two, covered, stream, sms), 2 + (tcgen05 is not None)
 
 
 def _refuse(q, k_cache, v_cache, out, block_table, cu_q, kv_len, rows, groups, num_heads, num_kv_heads, head_dim, page_size, scale) -> None:
@@ -134,7 +155,7 @@ def prefix_attention(q, k_cache, v_cache, out, block_table, cu_q, kv_len, rows, 
     if rc is None:
         # something is not as it should be, or this thread keeps a layer's calls (ops.LayerCalls), which the entry points take part in
         _refuse(*operands, *sizes, scale)
-        floats, shared, own, tiles, two, covered, sms = plan
+        floats, shared, own, tiles, two, covered, stream, sms = plan
         scratch = ops._empty((floats,), torch.float32, rows.device)
         common = (scratch, block_table, block_table.shape[1], cu_q, kv_len, rows, n_rows, groups, groups.shape[0], num_heads, num_kv_heads, page_size,
                   k_cache.shape[0], float(scale))
@@ -143,7 +164,7 @@ def prefix_attention(q, k_cache, v_cache, out, block_table, cu_q, kv_len, rows, 
             rc = all_sizes(q, k_cache, v_cache, out, *common, shared, own, tiles, ops._code(q), head_dim, sms, *ends)
         else:
             rc = tcgen05(q, k_cache, v_cache, *common, shared, tiles, two, *ends) if tcgen05 is not None else 0
-            rc = rc or mma(q, k_cache, v_cache, out, *common, shared, covered, sms, *ends)
+            rc = rc or mma(q, k_cache, v_cache, out, *common, shared, covered, stream, sms, *ends)
     ops._ok(rc, "prefix_attention", kernels)
 
 

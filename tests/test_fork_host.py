@@ -177,7 +177,7 @@ def test_rows_that_share_pages_are_found():
     plain, _, req = batch(m, ids)
     assert plain.num_prefix_groups == 0
     req.prefix_group = 0
-    assert rt.count_prefix_groups(m, req) == (2, 2 * 12 + 1 * 8)
+    assert rt.count_prefix_groups(m, req) == (2, 2 * 12 + 1 * 8, 12, 31)
     layout, out, _ = batch(m, ids, prefix_group=0)
     assert layout.num_prefix_groups == 3
     found = groups_of(layout, out)

@@ -60,14 +60,17 @@ def test_calls_go_where_they_are_served():
         got = prefix._plan(dtype, heads, kv_heads, dim, page, n_rows, n_groups, most_rows, shared, own, sharing, aligned, 148)
         return ["all sizes", "tcgen05", "mma"][0 if got[0] is not None else 1 if got[1] is not None else 2], got[3]
     assert plan()[0] == "tcgen05"
-    floats, splits, _, tiles, two, covered, ctas = plan()[1]
-    assert (tiles, two, covered, splits, ctas) == (1, 1, 256, 18, 148)
-    assert plan(most_rows=32)[1][1:6] == (32, 0, 1, 0, 128)                # one tile: a CTA leaves two parts; 4,096 keys are 16 pairs of blocks
+    floats, splits, _, tiles, two, covered, ctas, sms = plan()[1]
+    assert (tiles, two, covered, sms) == (1, 1, 256, 148) and 8 * splits + ctas <= 148      # (side by side)
+    floats, splits, _, tiles, two, covered, ctas, sms = plan(most_rows=32, n_rows=32)[1]
+    assert (tiles, two, covered) == (1, 0, 128) and splits % 2 == 0 and 8 * splits // 2 + ctas <= 148      # one tile: a CTA leaves two parts
     assert plan(most_rows=4)[0] == "mma" and plan(shared=600)[0] == "mma" and plan(dim=64)[0] == "mma"
     assert plan(shared=640)[0] == "tcgen05" and plan(most_rows=8, shared=24576)[0] == "tcgen05" and plan(most_rows=8, shared=24544)[0] == "mma"
     for other in (dict(dtype=torch.float32), dict(page=24), dict(dim=72), dict(heads=17, kv_heads=1), dict(n_rows=400), dict(aligned=False)):
         assert plan(**other)[0] == "all sizes", other
     assert plan(n_rows=399)[0] == "tcgen05"
+    # own keys that outweigh the shared ones come behind them, on all SMs or on most
+    assert plan(own=1)[1][6] < plan(own=4000)[1][6]
     # groups that share nothing are no reason to cut the others into fewer splits
     assert plan(n_groups=3)[1][1] == plan(n_groups=3, sharing=1)[1][1] > plan(n_groups=3, sharing=3)[1][1]
 
