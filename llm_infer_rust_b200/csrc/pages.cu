@@ -108,9 +108,6 @@ static int launch_all(const PageMove* moves, int n, const PageTensor* tensors, i
   return 0;
 }
 
-// How many launches a copy of n moves takes.
-B200_EXPORT int b200_copy_pages_launches(int n) { return (n + MOST_MOVES - 1) / MOST_MOVES; }
-
 // `moves`: host memory, n times (source, target, slots); `tensors`: device memory, `count` PageTensors of `pages` pages each;
 // `vector`: 16, 4 or 2, which divides every base, row and page; `page_bytes`: of the largest page.  Moves of no slots do nothing.
 B200_EXPORT int b200_copy_pages(const void* moves, int n, const void* tensors, int count, long long pages, int page_size, int vector,

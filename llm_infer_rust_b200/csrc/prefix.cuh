@@ -8,6 +8,8 @@
 #pragma once
 #include <math.h>
 
+#include <initializer_list>
+
 #include "common.cuh"
 
 struct PrefixCall {
@@ -63,6 +65,13 @@ __device__ __forceinline__ int group_of_row(const PrefixCall& c, int i) {
   return before - 1;
 }
 
+// Whether a call's operands are there, and its keys, blocks and splits can be counted in 32 bits.
+static inline bool prefix_can_be_served(std::initializer_list<const void*> operands, const int* groups, int n_groups, int table_stride, int page_size) {
+  for (const void* p : operands)
+    if (p == nullptr) return false;
+  return (groups != nullptr || n_groups == 0) && static_cast<long long>(table_stride) * page_size <= (1 << 30);
+}
+
 // Sets a kernel's limit of shared memory, once a device (`seen`: the kernel's own, one for each of the first 16 devices).
 template <typename Kernel>
 static inline int prefix_smem_limit(Kernel kernel, int bytes, bool (&seen)[16]) {
@@ -80,8 +89,11 @@ struct PrefixItem {
   const int* table;
   int i0, vector0, vectors;    // vector v: row i0 + (vector0 + v) / group of `rows`, query head kvh * group + (vector0 + v) % group
   int begin, end, kvh, slot;
-  bool shared;
 };
+
+// A part's maximum and sum as they are stored.  Scores that are all NaN leave no maximum; the sum, NaN too, must not be taken for that of a
+// part without keys.
+__device__ __forceinline__ float2 part_of(float m, float l) { return make_float2(l != l && m == -INFINITY ? 0.0f : m, l); }
 
 __device__ __forceinline__ float prefix_exp2(float x) {      // 2^x, one special-function instruction (-inf gives 0)
   float y;
@@ -152,7 +164,7 @@ __device__ __forceinline__ void join_parts(T* __restrict__ dst, int hd, int coun
   for (int w = 0; w < warps; ++w) most = fmaxf(most, left.row[w][PITCH]);
   const float base = most == -INFINITY ? 0.0f : most;
   for (int w = 0; w < warps; ++w) sum = fmaf(left.row[w][PITCH + 1], prefix_exp2(left.row[w][PITCH] - base), sum);
-  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;             // (a row of no keys gets zeros, a NaN stays one)
   for (int dim = 2 * static_cast<int>(threadIdx.x); dim < hd; dim += 2 * WARPS * 32) {      // (head sizes are even)
     float x = 0.0f, y = 0.0f;
     for (int w = 0; w < warps; ++w) {

@@ -27,12 +27,6 @@ constexpr int STAGES = (FIXED + 2 * TILE) * 4 <= 220 * 1024 ? 2 : 1;
 constexpr int SMEM = (FIXED + STAGES * TILE) * 4;
 static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
 
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // Rows first_key .. first_key + 31 of one KV head into `k` and `v` (zeros from `end` on).  Four threads a key.
 template <typename T>
 __device__ __forceinline__ void load_block(float* k, float* v, const T* __restrict__ kc, const T* __restrict__ vc, const PrefixCall& c,
@@ -241,9 +235,9 @@ __device__ __forceinline__ void attend(const T* __restrict__ q, const T* __restr
     for (int x = 0; x < 2 * MT; ++x) {
       const int r = 8 * x + g;
       const float m_new = fmaxf(m[x], fmaxf(fmaxf(tops[r], tops[VT + r]), fmaxf(tops[2 * VT + r], tops[3 * VT + r])));
-      const float base = m_new == -INFINITY ? 0.0f : m_new, f = fast_exp2(m[x] - base);      // (0 on the first visible block)
+      const float base = m_new == -INFINITY ? 0.0f : m_new, f = prefix_exp2(m[x] - base);      // (0 on the first visible block)
       const float* two = s[x >> 1] + 2 * (x & 1);
-      const float p0 = fast_exp2(two[0] - base), p1 = fast_exp2(two[1] - base);
+      const float p0 = prefix_exp2(two[0] - base), p1 = prefix_exp2(two[1] - base);
       *reinterpret_cast<float2*>(ps + r * LDP + warp * 8 + 2 * t) = make_float2(p0, p1);
       l[x] = l[x] * f + (p0 + p1);
       m[x] = m_new;
@@ -294,7 +288,7 @@ __device__ __forceinline__ void attend(const T* __restrict__ q, const T* __restr
     const int r = 8 * x + g;
     if (r >= it.vectors) continue;
     const long long place = place_of(c, it, r);
-    if (warp == 0 && t == 0) c.part_ml[place] = make_float2(m[x], (tops[r] + tops[VT + r]) + (tops[2 * VT + r] + tops[3 * VT + r]));
+    if (warp == 0 && t == 0) c.part_ml[place] = part_of(m[x], (tops[r] + tops[VT + r]) + (tops[2 * VT + r] + tops[3 * VT + r]));
     if (blocks > 0)
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -418,6 +412,8 @@ B200_EXPORT int b200_prefix_attention(const void* q, const void* k_cache, const 
   if (n_rows <= 0) return 0;
   if (nh <= 0 || nkv <= 0 || nh % nkv != 0 || page_size <= 0 || pages <= 0 || table_stride <= 0 || n_groups < 0) return B200_BAD_SIZE;
   if (splits_shared < 1 || splits_own < 1 || tiles < 1 || head_dim <= 0 || head_dim > D || (head_dim & 1) || sms < 1) return B200_BAD_SIZE;
+  if (!prefix_can_be_served({q, k_cache, v_cache, out, scratch, block_table, cu_q, kv_len, rows, err}, groups, n_groups, table_stride, page_size))
+    return B200_BAD_SIZE;
   const PrefixCall c = {block_table, cu_q, kv_len, rows, reinterpret_cast<const int2*>(groups), scratch,
                         reinterpret_cast<float2*>(scratch + static_cast<size_t>(n_rows) * nh * (splits_shared + splits_own) * D), err, table_stride, n_rows,
                         n_groups, nh, nkv, page_size, pages, splits_shared, splits_own, tiles, scale * 1.4426950408889634f};

@@ -76,6 +76,16 @@ __device__ __forceinline__ int sums_before(int v, int& sum, int* sh) {
   return before + upto - v;
 }
 
+// The group of the i-th row, the last one that begins at or before it (-1: none does).
+__device__ __forceinline__ int group_of(const Entries& at, int n_groups, int i) {
+  int lo = 0, hi = n_groups;
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (at.low[mid] <= i) lo = mid + 1; else hi = mid;
+  }
+  return lo - 1;
+}
+
 // Fills in `at` (a whole CTA).  What the kernels wait for here is two loads one behind the other, a row's number and its length.
 template <int WARPS_HERE>
 __device__ __forceinline__ void lay_out(const StreamCall& k, Entries& at, int* memory) {
@@ -120,12 +130,8 @@ __device__ __forceinline__ void lay_out(const StreamCall& k, Entries& at, int* m
       tiles = at.where[e];
       v = tiles * ((at.keys[e] + KB - 1) / KB);
     } else if (e < n_entries) {
-      int lo = 0, hi = c.n_groups;                 // the groups that begin at or before the row: it is the last one's
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (at.low[mid] <= e - c.n_groups) lo = mid + 1; else hi = mid;
-      }
-      const int keys = at.keys[e], low = lo == 0 ? 0 : min(keys, at.keys[lo - 1]);
+      const int g = group_of(at, c.n_groups, e - c.n_groups);
+      const int keys = at.keys[e], low = g < 0 ? 0 : min(keys, at.keys[g]);
       at.low[e] = low;
       v = keys > low ? (keys + KB - 1) / KB - low / KB : 0;
     }
@@ -410,7 +416,7 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
           float* dst = k.acc + (part * VT + r) * D + (lane & 3) * 2;
 #pragma unroll
           for (int dn = 0; dn < D / 8; ++dn) *reinterpret_cast<float2*>(dst + dn * 8) = make_float2(st.o[dn][2 * half], st.o[dn][2 * half + 1]);
-          if ((lane & 3) == 0) k.ml[part * VT + r] = make_float2(st.m[half], l);
+          if ((lane & 3) == 0) k.ml[part * VT + r] = part_of(st.m[half], l);
         }
       }
       if (now.s + now.left >= s_end) break;
@@ -434,8 +440,7 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     };
     RowParts p = {};
     p.own_count = parts_of_item(at.start[e], at.start[e + 1] - at.start[e], at.group_tiles + i, p.own);
-    int g = c.n_groups - 1;                        // the row's group (as lay_out has it)
-    while (g >= 0 && at.low[g] > i) --g;
+    const int g = group_of(at, c.n_groups, i);
     p.grouped = g >= 0;
     if (g >= 0) {
       p.first_vector = (i - at.low[g]) * group - k.covered;
@@ -485,8 +490,6 @@ static long long parts_of(int n_rows, int n_groups, int nh, int nkv, int ctas) {
 }
 static long long align4(long long n) { return (n + 3) / 4 * 4; }
 
-// Rows and groups of a call, in all.
-B200_EXPORT int b200_prefix_most_entries() { return MOST_ENTRIES; }
 // Floats of scratch: the tcgen05 kernel's part first (splits_shared > 0).
 B200_EXPORT long long b200_prefix_scratch_floats(int n_rows, int n_groups, int nh, int nkv, int splits_shared, int ctas) {
   const long long vectors = static_cast<long long>(n_rows) * nh * splits_shared, parts = parts_of(n_rows, n_groups, nh, nkv, ctas) * VT;
@@ -509,6 +512,9 @@ B200_EXPORT int b200_prefix_attention_mma(const void* q, const void* k_cache, co
                                 ((static_cast<long long>(n_rows) * (nh / nkv) + VT - 1) / VT + n_groups + n_rows);
   if (most_blocks > INT32_MAX / 2) return B200_BAD_SIZE;
   if (splits_shared < 0 || covered < 0 || (covered > 0) != (splits_shared > 0) || ctas < 1 || ctas > sms || n_rows + n_groups > MOST_ENTRIES) return B200_BAD_SIZE;
+  if (!prefix_can_be_served({q, k_cache, v_cache, out, scratch, block_table, cu_q, kv_len, rows, err}, groups, n_groups, table_stride, page_size))
+    return B200_BAD_SIZE;
+  if (static_cast<long long>(pages) * nkv * page_size > INT32_MAX) return B200_BAD_SIZE;      // (a copy's row is counted in 32 bits)
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(scratch)) % 16 != 0) return B200_BAD_ALIGN;
   StreamCall k;
   const size_t vectors = static_cast<size_t>(n_rows) * nh * splits_shared, parts = static_cast<size_t>(parts_of(n_rows, n_groups, nh, nkv, ctas)) * VT;

@@ -240,8 +240,8 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
     if (ok && mine > 0) ok = mbar_wait_warp(pv_done + t, (mine - 1) & 1, c.err);
     const int slot = TWO ? static_cast<int>(blockIdx.x) : 2 * static_cast<int>(blockIdx.x) + t;
     const long long place = (static_cast<long long>(row) * c.nh + head) * prefix_splits(c) + slot;
-    const bool seen = ok && mine > 0 && st.m_ref > -INFINITY;
-    if (used) c.part_ml[place] = seen ? make_float2(st.m_ref, st.l_run) : make_float2(-INFINITY, 0.0f);
+    const bool seen = ok && mine > 0 && (st.m_ref > -INFINITY || st.l_run != st.l_run);
+    if (used) c.part_ml[place] = seen ? part_of(st.m_ref, st.l_run) : make_float2(-INFINITY, 0.0f);
     // The outputs leave through shared memory, where both streams' products have been done: a thread puts its row there (rows 528
     // bytes apart, so that eight threads' pieces lie in eight different groups of banks) and the copy engine takes it.  (Straight
     // from the registers, 32 lines an instruction: 6,000 to 9,000 cycles.)
@@ -273,9 +273,6 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
   }
 }
 
-// Vectors of a group that a CTA takes: `two` tiles or one.
-B200_EXPORT int b200_prefix_tcgen05_vectors(int two) { return two != 0 ? 2 * BQ : BQ; }
-
 // The first `tiles` tiles (of one or `two` times 128) of every group's vectors against its shared keys, whose parts go to slots
 // 0 .. splits_shared - 1 of [n_rows * nh][splits_shared], at the start of `scratch` (splits_shared is the number of CTAs, or with one
 // tile a CTA twice that).  The kernels of b200_prefix_attention_mma follow.  Other arguments as there.
@@ -288,6 +285,9 @@ B200_EXPORT int b200_prefix_tcgen05(const void* q, const void* k_cache, const vo
   if (splits_shared < 1 || tiles < 1 || (two == 0 && splits_shared % 2 != 0) ||
       static_cast<long long>(n_groups) * tiles > 65535)
     return B200_BAD_SIZE;
+  if (!prefix_can_be_served({q, k_cache, v_cache, scratch, block_table, cu_q, kv_len, rows, err}, groups, n_groups, table_stride, page_size))
+    return B200_BAD_SIZE;
+  if (static_cast<long long>(pages) * nkv * page_size > INT32_MAX) return B200_BAD_SIZE;      // (a copy's row is counted in 32 bits)
   if (!(scale > 0.0f)) return B200_BAD_SIZE;                         // maxima and masks are taken of the unscaled scores
   if (reinterpret_cast<uintptr_t>(q) % 16 != 0) return B200_BAD_ALIGN;
   const PrefixCall c = {block_table, cu_q, kv_len, rows, reinterpret_cast<const int2*>(groups), scratch,

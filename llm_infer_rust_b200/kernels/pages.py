@@ -15,6 +15,7 @@ from . import ops
 from .build import load_entry_points
 from .ops import KernelError
 
+_MOVES_OF_A_LAUNCH = 2048
 _REFUSED = {-10: "a move names a page outside the pool, or more slots than a page has",
             -11: "a page is the target of two moves, or of one and the source of another",
             -12: "no memory on the host to check the moves"}
@@ -72,4 +73,4 @@ class PageCopier:
         rc = self._entry(moves, n, self._table, len(self._tensors), self.pages, self.page_size, self._vector, self._page_bytes, ops._stream())
         if rc in _REFUSED:
             raise KernelError(_REFUSED[rc])
-        ops._ok(rc, "copy_pages", 0 if n == 0 else -(-n // 2048))
+        ops._ok(rc, "copy_pages", -(-n // _MOVES_OF_A_LAUNCH))

@@ -125,11 +125,13 @@ def prefix_attention(q, k_cache, v_cache, out, block_table, cu_q, kv_len, rows, 
 
     ``rows`` (int32) lists the batch rows to serve group by group; ``groups`` (int32 [groups, 2]) holds for each group the index
     of its first row in ``rows`` (0 for the first group, rising) and how many keys its rows share.  The shared keys need not end
-    with a page; a row that sees fewer keys than its group shares sees those.  A row of no keys gets zeros.
+    with a page; a row that sees fewer keys than its group shares sees those (the others, which its group's longer rows see, have to be
+    finite: they are multiplied by weights of zero).  A row of no keys gets zeros.  Each row stands in ``rows`` once; ``out`` may be ``q``.
 
     ``most_rows``, ``most_shared`` and ``most_own`` are about how many rows a group has, how many keys it shares and how many keys
     a row has beyond them, at most, ``sharing_groups`` about how many of the groups share keys (None: all): they decide how the work is
-    cut up (and what a captured graph is cut up for), not the result's meaning.  Page ids outside the pool and rows longer than their block table set the error word (``ops.check_errors``)."""
+    cut up (and what a captured graph is cut up for), not the result's meaning.  Page ids outside the pool and rows longer than
+    their block table (of at most 2^30 places) set the error word (``ops.check_errors``); the other index arrays are taken at their word, as ``ops.decode_attention`` takes them."""
     if num_kv_heads <= 0 or num_heads <= 0 or num_heads % num_kv_heads:
         raise KernelError("num_heads must be a multiple of num_kv_heads")
     if head_dim % 2 or not 2 <= head_dim <= 512:

@@ -320,3 +320,42 @@ def test_large_groups_through_the_tcgen05_kernel(folders):
         logits.append(e.step([StepEntry(r, [t], [0]) for r, t in zip(ids, new)]).float().cpu().numpy().copy())
         e.check_kernel_errors()
     near(logits[0], logits[1], "bfloat16")
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_layers_whose_calls_are_made_again(head_dim, dtype):
+    """Many rows without a graph: the first layer, which finds no residual yet, and the second go through Python, the third's and the
+    fourth's calls are those that the second made."""
+    from llm_infer_rust_b200 import Engine
+    from llm_infer_rust_b200.engine import StepEntry
+    from llm_infer_rust_b200.kernels import ops, prefix
+    config = {"model_type": "qwen3", "architectures": ["Qwen3ForCausalLM"], "num_hidden_layers": 4, "hidden_size": 256,
+              "num_attention_heads": 4, "num_key_value_heads": 2, "head_dim": head_dim, "intermediate_size": 512, "vocab_size": 300,
+              "rope_theta": 10000.0, "rms_norm_eps": 1e-6, "tie_word_embeddings": True, "max_position_embeddings": 4096, "eos_token_id": None}
+    eng = Engine(None, random_weights_config=config, random_weights_seed=3, dtype=dtype, max_running_req=160, max_seq_len=3000,
+                 max_total_tokens=8000, cuda_graph_bs=0, log_level="warn")
+    ids = list(range(1, 151))
+    eng.open_request(1)
+    eng.step([StepEntry(1, tokens(300, 2200, 5), [])])
+    eng.fork_request(1, ids[1:])
+    twins = [tokens(300, 1, r)[0] for r in ids]
+    called, again = [], []
+    inner, inner_again = prefix.prefix_attention, ops.LayerCalls.again
+    prefix.prefix_attention = lambda *a, **kw: called.append(1) or inner(*a, **kw)
+    ops.LayerCalls.again = lambda self, values: again.append(inner_again(self, values)) or again[-1]
+    try:
+        got = eng.step([StepEntry(r, [t], [0]) for r, t in zip(ids, twins)]).clone()
+        assert len(called) == 2 and again == [True] * 2
+        for r in ids:                                            # the same step again, every layer through Python
+            eng.close_request(r)
+        eng.open_request(1)
+        eng.step([StepEntry(1, tokens(300, 2200, 5), [])])
+        eng.fork_request(1, ids[1:])
+        eng.model.repeats_layers = False
+        want = eng.step([StepEntry(r, [t], [0]) for r, t in zip(ids, twins)]).clone()
+        assert len(called) == 6
+    finally:
+        prefix.prefix_attention, ops.LayerCalls.again = inner, inner_again
+    assert torch.equal(got, want)
+    eng.check_kernel_errors()

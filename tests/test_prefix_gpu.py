@@ -270,3 +270,54 @@ def test_nothing_to_do():
     out = torch.full_like(c.q, 7.0)
     c.run(out)
     assert (out == 7.0).all()
+
+
+NAN_CASES = {"mma": ([(3, 200, [5, 1, 40]), (1, 10, [3])], 8, 2, 64, 16), "tcgen05": ([(40, 2600, [1 + i for i in range(40)])], 32, 8, 128, 16),
+             "tcgen05, two tiles": ([(80, 1100, [1 + i for i in range(80)])], 32, 8, 128, 16)}
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("name", list(NAN_CASES))
+def test_a_nan_stays_with_its_row(name, dtype):
+    c = Case(*NAN_CASES[name], dtype)
+    q = c.q.clone()
+    want = c.run()
+    bad = [1, 2]
+    c.q[1] = float("nan")
+    c.q[2, 0] = float("nan")                        # (of one head)
+    got = c.run()
+    assert got[1].isnan().all() and got[2, :c.d].isnan().all() and not got[2, c.d:].isnan().any()
+    c.q.copy_(q)
+    got[1], got[2, :c.d] = want[1], want[2, :c.d]
+    c.check(got)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("name", ["mma", "tcgen05"])
+def test_the_output_may_be_where_the_queries_are(name, dtype):
+    c = Case(*NAN_CASES[name], dtype, other_tokens=1)
+    q, want = c.q.clone(), c.run()
+    got = c.run(out=c.q)
+    tokens = c.cu_q[:-1].long()
+    rest = torch.ones(len(q), dtype=torch.bool, device=DEV)
+    rest[tokens] = False
+    assert torch.equal(got[tokens], want[tokens]) and torch.equal(got[rest], q[rest])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("name", ["mma", "tcgen05"])
+def test_calls_on_two_streams_at_once(name, dtype):
+    """Every call has memory of its own between its kernels."""
+    cases = [Case(*NAN_CASES[name], dtype, seed=s) for s in (0, 1)]
+    want = [c.run() for c in cases]
+    outs = [[torch.full_like(c.q, 7.0) for _ in range(6)] for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for x in range(6):
+        for c, out, stream in zip(cases, outs, streams):
+            with torch.cuda.stream(stream):
+                c.run(out=out[x])
+    torch.cuda.synchronize()
+    for w, of in zip(want, outs):
+        for got in of:
+            assert torch.equal(got, w)

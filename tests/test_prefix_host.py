@@ -106,6 +106,36 @@ def test_c_entry_points_refuse_what_they_cannot_serve():
         assert logprobs(**bad) == -2, bad
 
 
+def test_entry_points_of_the_attention_refuse_what_they_cannot_serve():
+    none, some = ctypes.c_void_p(), ctypes.c_void_p(1 << 20)       # (never followed)
+    names = ("q", "k", "v", "out", "scratch", "table", "cu", "lengths", "rows", "groups", "err")
+    mma = load_cuda_library("prefix_mma.cu", {"HEAD_DIM": 128})
+    tc = load_cuda_library("prefix_tcgen05.cu")
+    every = load_cuda_library("prefix_attention.cu", {"HEAD_DIM": 128})
+
+    def call(kind, n_rows=2, n_groups=1, nh=8, nkv=2, page=16, pages=9, scale=0.1, stride=4, last=None, **change):
+        p = {**{x: some for x in names}, **change}
+        args = [p["q"], p["k"], p["v"]] + ([p["out"]] if kind != "tc" else [])
+        args += [p["scratch"], p["table"], stride, p["cu"], p["lengths"], p["rows"], n_rows, p["groups"], n_groups, nh, nkv, page, pages, ctypes.c_float(scale)]
+        tail = {"mma": [0, 0, 148, 148], "tc": [2, 1, 0], "every": [1, 1, 1, 1, 128, 148]}[kind] if last is None else last
+        entry = {"mma": mma.b200_prefix_attention_mma, "tc": tc.b200_prefix_tcgen05, "every": every.b200_prefix_attention}[kind]
+        return entry(*args, *tail, p["err"], none)
+
+    for kind in ("mma", "tc", "every"):
+        assert call(kind, n_rows=0) == 0 and call(kind, n_rows=-1) == 0
+        for name in names:
+            if kind != "tc" or name != "out":
+                assert call(kind, **{name: none}) == -2, (kind, name)
+        # sizes; tables of more than 2^30 places
+        for bad in (dict(nh=0), dict(nkv=0), dict(nh=7), dict(page=0), dict(pages=0), dict(stride=0), dict(stride=2 ** 27), dict(n_groups=-1)):
+            assert call(kind, **bad) == (0 if kind == "tc" and "n_groups" in bad else -2), (kind, bad)
+    for kind in ("mma", "tc"):
+        assert call(kind, page=24) == -2 and call(kind, pages=2 ** 27) == -2 and call(kind, q=ctypes.c_void_p((1 << 20) + 8)) == -3
+    assert call("mma", nh=34) == -2 and call("mma", n_rows=400) == -2 and call("mma", last=[2, 0, 148, 148]) == -2 and call("mma", last=[0, 0, 149, 148]) == -2
+    assert call("tc", scale=0.0) == -2 and call("tc", last=[3, 1, 0]) == -2 and call("tc", last=[0, 1, 1]) == -2
+    assert call("every", last=[1, 1, 1, 1, 130, 148]) == -2 and call("every", last=[1, 1, 1, 1, 127, 148]) == -2 and call("every", last=[0, 1, 1, 1, 128, 148]) == -2
+
+
 @pytest.mark.parametrize("logprobs", [-1, 33])
 def test_sampling_params_refuse(logprobs):
     with pytest.raises(ValueError, match="0 to 32"):
