@@ -3,17 +3,20 @@
 //
 // Work comes in items: up to 16 query vectors of one KV head (a tile of a group's against its shared keys, or one row's against its
 // own), an item in blocks of 32 keys.  All items' blocks stand in one sequence, and every warp of a persistent grid takes an equal
-// stretch of it, whatever the rows' lengths.  A warp works alone: it fetches blocks by TMA into a ring of its own, across the
+// stretch of it, whatever the rows' lengths.  A warp works alone: it fetches blocks by cp.async into a ring of its own, across the
 // borders of items, multiplies them (as attention_mma.cu does) with an item's queries, which stay in registers up to 128 dims and come
 // while the item before is worked on, and leaves for each item that it touches one part: float outputs, maximum, sum.  Stretch w
 // and item x meet in part w + x, which rises along the sequence, so no two meet in one place and none needs to be asked for.
 // A kernel behind this one joins a vector's parts.
 //
-// Bound by the keys' and values' bytes.  (A CTA an item with a split, warps joined in shared memory: 64 rows of 1 to 1,024 own keys, 8 KV
-// heads, took 52 us, 2.6 TB/s, most of it the CTAs' beginnings and ends.)  A group of more than 16 vectors reads its shared keys
-// once for each 16 (from the second-level cache), which prefix_tcgen05.cu does not.
+// Bound, where there are many keys, by their bytes (six groups of 104 MB: 28.5 us, of which 19 at 5.5 TB/s, the rest the beginning and
+// the join), else by what a warp waits for: of 2,700 cycles a block of 128 dims the products take 900, the softmax 430, asking for the next
+// block 800.  (That by the copy engine, a box of 64 dims of a page a copy: 900, with a wait for the page's number in front 1,400, and the
+// calls 1 to 2.5 us slower; a box of all dims a copy: 500, with a longer way until the first one is there, 8.5 us for 8.3 at two rows
+// behind 300 keys, 21.3 for 19.9 at four groups of eight behind 1,000, 73.9 for 75.3 at 64 behind 32,768.  A CTA an item with a split,
+// warps joined in shared memory: 64 rows of 1 to 1,024 own keys, 8 KV heads, 52 us, most of it the CTAs' beginnings and ends.)  A group
+// of more than 16 vectors reads its shared keys once for each 16 (from the second-level cache), which prefix_tcgen05.cu does not.
 #include "attention_mma.cuh"
-#include "kv_map.cuh"
 #include "prefix.cuh"
 
 constexpr bool kQueriesInRegisters = D <= 128;
@@ -24,7 +27,7 @@ constexpr int THREADS = WARPS * 32;
 constexpr int MOST_ENTRIES = 400;                // rows and groups of a call, whose places in the sequence stand in shared memory
 constexpr size_t RING = static_cast<size_t>(WARPS) * STAGES * TILE_BYTES;
 constexpr size_t QUERIES = static_cast<size_t>(WARPS) * VT * LD * sizeof(bf16);
-constexpr size_t FIXED = 1024 + RING + QUERIES + WARPS * STAGES * 8;
+constexpr size_t FIXED = 128 + RING + QUERIES;
 
 // The places of a call's groups, then rows, in the sequence of blocks (of one KV head), in shared memory.
 struct Entries {
@@ -149,19 +152,15 @@ __device__ __forceinline__ void lay_out(const StreamCall& k, Entries& at, int* m
   __syncthreads();
 }
 
-// The sequence of all KV heads' blocks in equal stretches, the first `longer` of them one block longer.
+// The sequence of all KV heads' blocks in equal stretches, the last one what is left: as many blocks as the longest has to have anyway, for
+// every stretch costs a part more.  (Stretches that differ by a block, on all workers: eight rows behind 4,096 keys 16.1 us, 15.0 so.)
 struct Stretches {
-  int workers, blocks, longer;
-  __device__ __forceinline__ Stretches(int total, int most) {
-    workers = max(1, min(total, most));
-    blocks = total / workers;
-    longer = total - blocks * workers;
-  }
-  __device__ __forceinline__ int begin(int w) const { return w * blocks + min(w, longer); }
-  __device__ __forceinline__ int of(int s) const {
-    const int edge = longer * (blocks + 1);
-    return s < edge ? s / (blocks + 1) : longer + (s - edge) / blocks;
-  }
+  int blocks, workers;
+  __device__ __forceinline__ Stretches(int total, int most) : blocks(max(1, (total + most - 1) / most)), workers((total + blocks - 1) / blocks), total_(total) {}
+  __device__ __forceinline__ int begin(int w) const { return min(w * blocks, total_); }
+  __device__ __forceinline__ int of(int s) const { return s / blocks; }
+ private:
+  int total_;
 };
 
 // Where a worker stands: `left` blocks of an item from key first_key on.
@@ -208,15 +207,51 @@ __device__ __noinline__ Place locate(const Entries& at, int s, int s_end, int n_
   return p;
 }
 
-// The page of this lane's sub-block, inside the pool (the sink's where the table names none that is, or where the sub-block ends
-// below `lowest`: those keys are another table's).
-__device__ __forceinline__ int lane_page_checked(const PrefixCall& c, const Place& p, int box_rows, int lane) {
-  const int key0 = p.first_key + lane * box_rows;
-  if (lane * box_rows >= KB || key0 >= p.end || key0 + box_rows <= p.lowest) return 0;
-  const int page = c.block_table[static_cast<long long>(p.table_row) * c.table_stride + key0 / c.page_size];
-  if (page >= 0 && page < c.pages) return page;
-  atomicOr(c.err, B200_ERR_SLOT_RANGE);
-  return 0;
+// What the block table says of the page of this lane's keys, asked for a block before it is used: a block is cut into boxes, the keys of
+// one page each, and lane j has the j-th.  A box that ends below `lowest` is another table's: the sink's page, 0, and so is what a
+// lane without a box gets.
+struct Boxes { int log2_rows, log2_page; };
+__device__ __forceinline__ int lane_page(const PrefixCall& c, const Boxes& boxes, const Place& p, int lane) {
+  const int key0 = p.first_key + (lane << boxes.log2_rows);
+  if ((lane << boxes.log2_rows) >= KB || key0 >= p.end || key0 + (1 << boxes.log2_rows) <= p.lowest) return 0;
+  return __ldg(c.block_table + static_cast<long long>(p.table_row) * c.table_stride + (key0 >> boxes.log2_page));
+}
+// The warp asks for the block at p.first_key, its boxes on the lanes' pages (the sink's for one outside the pool); rows that are not the
+// item's become zeros, so that whatever a page holds there does not reach P V.
+__device__ __forceinline__ void fetch_block_of(const PrefixCall& c, const Boxes& boxes, const Place& p, int page, const bf16* __restrict__ kc,
+                                               const bf16* __restrict__ vc, unsigned char* tile, int lane) {
+  constexpr int CHUNKS = D / 8, TURNS = KB * CHUNKS / 32, ROWS = 32 / CHUNKS;      // of 16 bytes in a row; rows a turn of the warp's lanes
+  if (page < 0 || page >= c.pages) {
+    atomicOr(c.err, B200_ERR_SLOT_RANGE);
+    page = 0;
+  }
+  const int y = (page * c.nkv + p.kvh) * c.page_size + ((p.first_key + (lane << boxes.log2_rows)) & (c.page_size - 1));
+  const int from = p.lowest - p.first_key, to = p.end - p.first_key;
+  if (32 % CHUNKS == 0 && ROWS <= 8 && boxes.log2_rows >= 3) {      // eight keys behind one another at a time
+#pragma unroll
+    for (int r8 = 0; r8 < KB; r8 += 8) {
+      const int mine = lane / CHUNKS, chunk = lane % CHUNKS;
+      const int line = __shfl_sync(0xffffffffu, y, r8 >> boxes.log2_rows) + (r8 & ((1 << boxes.log2_rows) - 1)) + mine;
+      const long long at = static_cast<long long>(line) * D + chunk * 8;
+#pragma unroll
+      for (int r = 0; r < 8; r += ROWS <= 8 && ROWS > 0 ? ROWS : 8) {
+        const int row = r8 + r + mine;
+        unsigned char* dst = tile + swz(row, chunk);
+        cp_async16(dst, kc + at + r * D, row >= from && row < to);
+        cp_async16(dst + V_OFFSET, vc + at + r * D, row >= from && row < to);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int x = 0; x < TURNS; ++x) {
+    const int row = (x * 32 + lane) / CHUNKS, chunk = (x * 32 + lane) % CHUNKS;
+    const int line = __shfl_sync(0xffffffffu, y, row >> boxes.log2_rows) + (row & ((1 << boxes.log2_rows) - 1));
+    const long long at = static_cast<long long>(line) * D + chunk * 8;
+    unsigned char* dst = tile + swz(row, chunk);
+    cp_async16(dst, kc + at, row >= from && row < to);
+    cp_async16(dst + V_OFFSET, vc + at, row >= from && row < to);
+  }
 }
 
 // One block of 32 keys against the 16 vectors whose queries are `qa` (or stand at `qs`): as block_mma of attention_mma.cuh, with the
@@ -304,23 +339,20 @@ __device__ __forceinline__ void item_block(const uint32_t (&qa)[kQueriesInRegist
 }
 
 __global__ void __launch_bounds__(THREADS, 1)
-prefix_stream_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const bf16* __restrict__ q,
-                     const StreamCall k, int box_rows) {
+prefix_stream_kernel(const bf16* __restrict__ kc, const bf16* __restrict__ vc, const bf16* __restrict__ q,
+                     const StreamCall k, const Boxes boxes) {
   extern __shared__ unsigned char smem_raw[];
-  unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
   bf16* queries = reinterpret_cast<bf16*>(tiles + RING);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<unsigned char*>(queries) + QUERIES);      // [WARPS][STAGES]
   const PrefixCall& c = k.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (threadIdx.x < WARPS * STAGES) mbar_init(bars + threadIdx.x, 1);
-  asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   // Behind the tcgen05 kernel of the same call, which has waited for the kernels before it, this one begins beside it, and waits
   // for its end at its own: whoever waits for this kernel then waits for both.  The joining kernel may come as soon as what was
   // launched before the call has ended.
   if (k.covered == 0) pdl_wait();
   pdl_launch_dependents();
   Entries at;
-  lay_out<WARPS>(k, at, reinterpret_cast<int*>(bars + WARPS * STAGES));
+  lay_out<WARPS>(k, at, reinterpret_cast<int*>(reinterpret_cast<unsigned char*>(queries) + QUERIES));
 
   const int group = c.nh / c.nkv;
   const Stretches stretches(at.blocks * c.nkv, static_cast<int>(gridDim.x) * WARPS);
@@ -328,7 +360,6 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   const int s_begin = worker < stretches.workers ? stretches.begin(worker) : 0, s_end = worker < stretches.workers ? stretches.begin(worker + 1) : 0;
   if (s_begin < s_end) {
     unsigned char* ring = tiles + static_cast<size_t>(warp) * STAGES * TILE_BYTES;
-    uint64_t* full = bars + warp * STAGES;
     bf16* qs = queries + warp * VT * LD;
     // the queries of an item into shared memory: two lanes a vector
     auto fetch_queries = [&](const Place& p) {
@@ -339,27 +370,26 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       cp_async_commit();
     };
     Place now = locate(at, s_begin, s_end, c.n_groups, c.n_rows, group, k.covered), ahead = now, next = now;
-    int page = lane_page_checked(c, ahead, box_rows, lane);
+    int page = lane_page(c, boxes, ahead, lane);
     fetch_queries(now);
     uint32_t qa[kQueriesInRegisters ? D / 16 : 1][4];
     WarpAcc st;
     int last[2], all_see = 0, done = 0;            // `done`: blocks of the item behind us
     int fetch_stage = 0, stage = 0;
-    uint32_t parity = 0;
     for (int tick = 1 - STAGES;; ++tick) {
       // the next block of the stretch on its way, whatever item it is of; the page numbers of the one behind it are asked for
       if (ahead.s < s_end) {
-        fetch_block(ring + fetch_stage * TILE_BYTES, &kmap, &vmap, page, c.page_size, c.nkv, ahead.kvh, box_rows, ahead.first_key, ahead.end,
-                    full + fetch_stage, lane);
+        fetch_block_of(c, boxes, ahead, page, kc, vc, ring + fetch_stage * TILE_BYTES, lane);
         fetch_stage = fetch_stage + 1 == STAGES ? 0 : fetch_stage + 1;
         ++ahead.s;
         ahead.first_key += KB;
         if (--ahead.left == 0 && ahead.s < s_end) ahead = locate(at, ahead.s, s_end, c.n_groups, c.n_rows, group, k.covered);
-        if (ahead.s < s_end) page = lane_page_checked(c, ahead, box_rows, lane);
+        if (ahead.s < s_end) page = lane_page(c, boxes, ahead, lane);
       }
+      cp_async_commit();                           // (one a tick; an item's queries are one more, behind that of a tick)
       if (tick < 0) continue;
       if (done == 0) {                             // an item begins
-        cp_async_wait<0>();
+        cp_async_wait<1>();
         __syncwarp();
         if constexpr (kQueriesInRegisters) {
 #pragma unroll
@@ -384,25 +414,13 @@ prefix_stream_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         all_see = __reduce_min_sync(0xffffffffu, all_see);
         st.init();
       }
-      if (!mbar_wait(full + stage, parity, c.err)) {
-        // Give the copies that are still in flight a bounded time to land before the warp leaves; the error word is flagged.
-        for (int t = 0; t < STAGES; ++t) mbar_wait(full + t, t < stage ? parity ^ 1u : parity, c.err);
-        break;
-      }
+      cp_async_wait<STAGES - 1>();
+      __syncwarp();
       unsigned char* t = ring + stage * TILE_BYTES;
       const int first_key = now.first_key + done * KB;
-      if (first_key + KB > now.end || first_key < now.lowest) {
-        // Value rows that are not the item's: whatever the page holds there must not reach P V.
-        if (first_key + lane >= now.end || first_key + lane < now.lowest) {
-          const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll 1
-          for (int v = 0; v < VALUE_CHUNKS; ++v) *reinterpret_cast<uint4*>(t + V_OFFSET + (v >> 3) * HALF_BYTES + lane * 128 + (v & 7) * 16) = zero;
-        }
-      }
-      __syncwarp();
       item_block(qa, qs, t, t + V_OFFSET, first_key + KB - 1 > all_see || first_key < now.lowest, first_key, now.lowest, last[0], last[1], c.scale_log2, st);
       __syncwarp();                                // every lane is done reading before the stage is refilled
-      if (++stage == STAGES) { stage = 0; parity ^= 1u; }
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
       if (++done < now.left) continue;
       // the item ends here, or the stretch: its part
       const long long part = static_cast<long long>(worker) + now.item;
@@ -515,7 +533,7 @@ B200_EXPORT int b200_prefix_attention_mma(const void* q, const void* k_cache, co
   if (!prefix_can_be_served({q, k_cache, v_cache, out, scratch, block_table, cu_q, kv_len, rows, err}, groups, n_groups, table_stride, page_size))
     return B200_BAD_SIZE;
   if (static_cast<long long>(pages) * nkv * page_size > INT32_MAX) return B200_BAD_SIZE;      // (a copy's row is counted in 32 bits)
-  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(scratch)) % 16 != 0) return B200_BAD_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(scratch)) % 16 != 0) return B200_BAD_ALIGN;
   StreamCall k;
   const size_t vectors = static_cast<size_t>(n_rows) * nh * splits_shared, parts = static_cast<size_t>(parts_of(n_rows, n_groups, nh, nkv, ctas)) * VT;
   if (static_cast<long long>(n_rows) * nh > INT32_MAX) return B200_BAD_SIZE;
@@ -526,17 +544,14 @@ B200_EXPORT int b200_prefix_attention_mma(const void* q, const void* k_cache, co
   k.covered = covered;
   k.c = {block_table, cu_q, kv_len, rows, reinterpret_cast<const int2*>(groups), scratch, part_ml, err, table_stride, n_rows, n_groups, nh, nkv,
          page_size, pages, splits_shared, 0, 1, scale * 1.4426950408889634f};
-  CUtensorMap kmap, vmap;
-  const int box_rows = page_size < KB ? page_size : KB;
-  const long long lines = static_cast<long long>(pages) * nkv * page_size;
-  int rc = make_kv_tensor_map(&kmap, k_cache, lines, D, box_rows);
-  if (rc == 0) rc = make_kv_tensor_map(&vmap, v_cache, lines, D, box_rows);
-  if (rc != 0) return rc;
+  Boxes boxes;
+  boxes.log2_page = __builtin_ctz(page_size);
+  boxes.log2_rows = page_size < KB ? boxes.log2_page : __builtin_ctz(KB);
   static bool seen[16];
-  rc = prefix_smem_limit(prefix_stream_kernel, static_cast<int>(FIXED) + entries_bytes(MOST_ENTRIES), seen);
+  int rc = prefix_smem_limit(prefix_stream_kernel, static_cast<int>(FIXED) + entries_bytes(MOST_ENTRIES), seen);
   if (rc != 0) return rc;
   const int entries = entries_bytes(n_rows + n_groups);
-  rc = b200_launch(prefix_stream_kernel, dim3(ctas), dim3(THREADS), FIXED + entries, stream, 0, kmap, vmap, static_cast<const bf16*>(q), k, box_rows);
+  rc = b200_launch(prefix_stream_kernel, dim3(ctas), dim3(THREADS), FIXED + entries, stream, 0, static_cast<const bf16*>(k_cache), static_cast<const bf16*>(v_cache), static_cast<const bf16*>(q), k, boxes);
   if (rc != 0) return rc;
   const int warps = join_warps_of(static_cast<long long>(n_rows) * nh, sms);
   return b200_launch(warps == 16 ? prefix_join_kernel<16> : warps == 8 ? prefix_join_kernel<8> : prefix_join_kernel<4>, dim3(static_cast<unsigned>(n_rows) * nh),
