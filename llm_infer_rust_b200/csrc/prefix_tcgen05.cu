@@ -14,8 +14,10 @@
 #include "kv_map.cuh"
 #include "prefix.cuh"
 
-constexpr int COPY_WARPS = 2;
-constexpr int THREADS = 320 + 32 * (COPY_WARPS - 1);      // warp 0 copies, 1 products, 2-5 and 6-9 the streams' softmax, 10.. copy
+constexpr int COPY_WARPS = 3;
+constexpr int THREADS = 288 + 32 * COPY_WARPS;            // warps 0-3 and 4-7 the streams' softmax, 8 products, 9-11 copies
+constexpr int SOFTMAX_REGISTERS = 208, OTHER_REGISTERS = 88;      // of a thread, out of the 168 that 384 threads are launched with
+static_assert(256 * SOFTMAX_REGISTERS + (THREADS - 256) * OTHER_REGISTERS <= THREADS * 168, "the split is of what the launch has");
 constexpr int V_STAGES = 2;
 constexpr int V_OFF = 0, Q_OFF = V_STAGES * TILE, K_OFF_TWO = Q_OFF + 2 * TILE, K_OFF_ONE = Q_OFF + TILE;
 constexpr int BAR_OFF = 6 * TILE;                         // V 2, Q 2 and K 2, or V 2, Q 1 and K 3
@@ -53,7 +55,7 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
     mbar_init(q_full, TWO ? 8 : 4);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  if (warp == 1) {
+  if (warp == 8) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
@@ -82,9 +84,11 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
   const int nblk[2] = {TWO ? count : (count + 1) / 2, TWO ? (vectors > BQ ? count : 0) : count / 2};
   const int* table = c.block_table + static_cast<long long>(rows.y > 0 ? c.rows[rows.x] : 0) * c.table_stride;
 
-  if (warp == 0 || warp >= 10) {
+  if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(OTHER_REGISTERS));
+  else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(SOFTMAX_REGISTERS));
+  if (warp > 8) {
     // ---- copies, as in the prompt kernels: the page numbers first, then the blocks' boxes, COPY_WARPS warps in turn
-    const int cw = warp == 0 ? 0 : warp - 9;
+    const int cw = warp - 9;
     bool ok = true;
     int* tbl = reinterpret_cast<int*>(sm + TBL_OFF);
     const int first_page = k_begin / c.page_size;
@@ -122,7 +126,7 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
       if (use > 0) ok = mbar_wait_warp(v_empty + s, (use - 1) & 1, c.err);
       if (ok) fetch(&vmap, sm + V_OFF + s * TILE, v_full + s, k_begin + i * BKV);
     }
-  } else if (warp == 1) {
+  } else if (warp == 8) {
     // ---- products: P V of a stream's block, then S of its next one, the streams in turn
     if (count > 0) {
       bool ok = mbar_wait_warp(q_full, 0, c.err);
@@ -180,7 +184,7 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
     }
   } else {
     // ---- softmax: thread (stream t, row r) owns one query vector (tensor-memory lane r of the stream's columns)
-    const int t = (warp - 2) >> 2, quarter = warp & 3;
+    const int t = warp >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const int vec = vector0 + (TWO ? t * BQ : 0) + r;
     const bool used = vec - vector0 < vectors;
@@ -248,7 +252,7 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
     asm volatile("bar.sync 2, 256;\n" ::: "memory");             // (the softmax warps, whatever became of their waits)
     if (ok && mine > 0) {
       tc_fence_after();
-      unsigned char* line = sm + ((warp - 2) * 32 + lane) * OUT_PITCH;
+      unsigned char* line = sm + threadIdx.x * OUT_PITCH;
 #pragma unroll 1
       for (int x = 0; x < 4; ++x) {
         float o[32];
@@ -267,7 +271,7 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
+  if (warp == 8) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
   }
