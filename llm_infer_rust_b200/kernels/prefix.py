@@ -25,12 +25,14 @@ _KEYS_PER_CTA_AT_LEAST = 32
 _MOST_SPLITS = 64
 _MOST_ENTRIES = 400           # rows and groups of a call that the tensor-core kernels take
 # The tcgen05 kernel takes the shared keys of more vectors of a KV head than the mma.sync kernel has in a tile, from so many blocks on (32 keys
-# of a KV head against 16 vectors each).  (mma.sync / tcgen05, us, 8 KV heads of 128: 32 vectors, 4,096 keys 19.0 / 20.6, 8,192 keys 22.8 /
-# 23.6, 32,768 keys 58.9 / 43.8; 64 vectors, 2,048 keys 23.4 / 25.6, 4,096 keys 29.3 / 26.4; 128 vectors, 1,024 keys 17.6 / 19.9, 2,048 keys
-# 23.6 / 20.7; 256 vectors, 512 keys 22.6 / 23.3, 1,024 keys 29.4 / 24.4.  One KV head: 128 vectors, 8,192 keys 15.8 / 15.8; 512 vectors,
-# 4,096 keys 27.6 / 27.4.  Two tiles of vectors leave three quarters of its rows empty: six groups of 4 to 24 vectors behind 500 to 3,001 keys
-# 29.7 / 40.0.)
-_TENSOR_CORE_BLOCKS, _TENSOR_CORE_BLOCKS_OF_TWO_TILES = 2560, 12288
+# of a KV head against 16 vectors each).  (mma.sync / tcgen05, us, 8 KV heads of 128: 32 vectors, 2,048 keys 12.4 / 12.9, 4,096 keys 15.5 /
+# 14.3; 64 vectors, 1,024 keys 12.9 / 12.9, 2,048 keys 15.7 / 13.6; 128 vectors, 512 keys 13.4 / 14.6, 1,024 keys 16.4 / 15.0; 256 vectors, 512
+# keys 19.5 / 18.9; 256 behind 32,768 keys 307 / 55.  One KV head: 128 vectors, 4,096 keys 11.5 / 13.4, 8,192 keys 15.4 / 13.9; 512 vectors,
+# 2,048 keys 15.8 / 16.2, 4,096 keys 20.8 / 17.3.)  Several groups are as a rule unlike in their rows and keys, and `blocks` counts
+# each as the largest, so it has to be more then: of up to 24 vectors six behind up to 3,001 keys (9,024 blocks) 20.8 / 28.8, of up to 80
+# three behind 500 (1,920) 14.7 / 15.6 and behind 1,500 (5,640) 19.2 / 18.5, of up to 48 six behind 700 (3,168) 15.4 / 18.0, of up to 64
+# twelve behind 1,000 (12,288) 31.0 / 29.4.
+_TENSOR_CORE_BLOCKS, _TENSOR_CORE_BLOCKS_OF_TWO_TILES, _TENSOR_CORE_BLOCKS_OF_GROUPS = 1536, 2048, 12288
 _MMA_VECTORS = 16
 
 
@@ -42,24 +44,26 @@ def _splits(most_shared: int, most_own: int, shared_ctas: int, own_ctas: int, ro
     return max(1, min(_MOST_SPLITS, -(-most_shared // a_cta))), max(1, min(_MOST_SPLITS, -(-most_own // a_cta)))
 
 
-# What the tcgen05 kernel takes beside its steps (a block of keys, or one for each stream), and a step; what the stream kernel takes beside
-# its bytes, bytes that one of few SMs and all of them together take in, and the keys that an item costs beside its own (us, bytes a us).
-_TC_FIXED, _TC_STEP = 9.6, 2.25
-_OWN_FIXED, _OWN_BYTES, _OWN_BYTES_ALL, _OWN_KEYS = 9.0, 58000.0, 4.5e6, 64
+# What the tcgen05 kernel takes beside its steps, and a step: one tile of vectors (a block of keys for each of two streams), two tiles (a
+# block for both).  What the stream kernel takes beside its bytes, bytes that one of few SMs and all of them together take in, and the
+# keys that an item costs beside its own (us, bytes a us).
+_TC_FIXED, _TC_STEP = (5.0, 12.0), (2.9, 1.8)
+_OWN_FIXED, _OWN_BYTES, _OWN_BYTES_ALL, _OWN_KEYS = 5.0, 78000.0, 6.5e6, 64
 
 
-def _share_sms(steps: int, tiles: int, items: int, most_own: int, key_bytes: int, sms: int) -> tuple:
+def _share_sms(steps: int, two: int, tiles: int, items: int, most_own: int, key_bytes: int, sms: int) -> tuple:
     """How many CTAs cut each of ``tiles`` tiles' ``steps``, and the CTAs of the stream kernel for ``items`` of own keys (half of ``most_own``
     each): side by side on SMs of their own, as the registers and shared memory of either leave no room for the other, or one behind the
-    other on all.  (64 rows of 32 heads behind 32,768 keys, own keys of 1 to 1,024: 12 or 13 CTAs a tile beside 52 or 44 SMs 72.6 us, 10
-    beside 68 80.8, 15 beside 28 105, one behind the other 84; 24 rows of 64 heads behind 8,000 keys, 1 to 200: 27.4 and 31.1.)"""
+    other on all.  (64 rows of 32 heads behind 32,768 keys, own keys of 1 to 1,024: 13 CTAs a tile beside 44 SMs 66.6 us, 10 beside 68
+    77.2, 15 beside 28 90.8, one behind the other 79.5; 24 rows of 64 heads behind 8,000 keys, 1 to 200: 26.0 and 29.3.)"""
     own_bytes = items * (most_own / 2 + _OWN_KEYS) * key_bytes
+    of_tc = lambda ctas: _TC_FIXED[two] + _TC_STEP[two] * -(-steps // ctas)
     most = max(1, min(steps, sms // tiles, _MOST_SPLITS))
-    best = _TC_FIXED + _TC_STEP * -(-steps // most) + _OWN_FIXED + own_bytes / _OWN_BYTES_ALL, most, sms
+    best = of_tc(most) + _OWN_FIXED + own_bytes / _OWN_BYTES_ALL, most, sms
     for ctas in range(1, most + 1):
         left = sms - ctas * tiles
         if left >= 1:
-            best = min(best, (max(_TC_FIXED + _TC_STEP * -(-steps // ctas), _OWN_FIXED + own_bytes / min(left * _OWN_BYTES, _OWN_BYTES_ALL)), ctas, left))
+            best = min(best, (max(of_tc(ctas), _OWN_FIXED + own_bytes / min(left * _OWN_BYTES, _OWN_BYTES_ALL)), ctas, left))
     return best[1:]
 
 
@@ -81,13 +85,13 @@ def _plan(dtype, heads: int, kv_heads: int, dim: int, page: int, n_rows: int, n_
         return lib.b200_prefix_attention, None, None, (floats, shared, own, tiles, 0, 0, 0, sms), 2
     tcgen05, tiles, two, shared, covered, stream = None, 1, 0, 0, 0, sms
     blocks = -(-vectors // _MMA_VECTORS) * -(-most_shared // 32) * kv_heads * sharing
-    least = _TENSOR_CORE_BLOCKS if vectors > 2 * _MMA_VECTORS else _TENSOR_CORE_BLOCKS_OF_TWO_TILES
+    least = _TENSOR_CORE_BLOCKS_OF_GROUPS if sharing > 1 else _TENSOR_CORE_BLOCKS if vectors > 2 * _MMA_VECTORS else _TENSOR_CORE_BLOCKS_OF_TWO_TILES
     if n_groups and dim == 128 and vectors > _MMA_VECTORS and blocks >= least:
         # one or two tiles a CTA, none without a block of keys for each of its streams
         two = int(vectors > _TC_VECTORS)
         a_cta = _TC_VECTORS << two
         tiles = -(-vectors // a_cta)
-        ctas, stream = _share_sms(-(-most_shared // (256 >> two)), sharing * kv_heads * tiles, n_rows * kv_heads, most_own, 4 * dim, sms)
+        ctas, stream = _share_sms(-(-most_shared // (256 >> two)), two, sharing * kv_heads * tiles, n_rows * kv_heads, most_own, 4 * dim, sms)
         shared, covered = ctas << (1 - two), tiles * a_cta
         tcgen05 = load_entry_points("prefix_tcgen05.cu").b200_prefix_tcgen05
     lib = load_entry_points("prefix_mma.cu", {"HEAD_DIM": dim})

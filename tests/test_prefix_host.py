@@ -64,13 +64,14 @@ def test_calls_go_where_they_are_served():
     assert (tiles, two, covered, sms) == (1, 1, 256, 148) and 8 * splits + ctas <= 148      # (side by side)
     floats, splits, _, tiles, two, covered, ctas, sms = plan(most_rows=32, n_rows=32)[1]
     assert (tiles, two, covered) == (1, 0, 128) and splits % 2 == 0 and 8 * splits // 2 + ctas <= 148      # one tile: a CTA leaves two parts
-    assert plan(most_rows=4)[0] == "mma" and plan(shared=600)[0] == "mma" and plan(dim=64)[0] == "mma"
-    assert plan(shared=640)[0] == "tcgen05" and plan(most_rows=8, shared=24576)[0] == "tcgen05" and plan(most_rows=8, shared=24544)[0] == "mma"
+    assert plan(most_rows=4)[0] == "mma" and plan(shared=352)[0] == "mma" and plan(dim=64)[0] == "mma"
+    assert plan(shared=353)[0] == "tcgen05" and plan(most_rows=8, shared=4065)[0] == "tcgen05" and plan(most_rows=8, shared=4064)[0] == "mma"
     for other in (dict(dtype=torch.float32), dict(page=24), dict(dim=72), dict(heads=17, kv_heads=1), dict(n_rows=400), dict(aligned=False)):
         assert plan(**other)[0] == "all sizes", other
     assert plan(n_rows=399)[0] == "tcgen05"
     # own keys that outweigh the shared ones come behind them, on all SMs or on most
     assert plan(own=1)[1][6] < plan(own=4000)[1][6]
+    assert plan(n_groups=4, sharing=3, most_rows=16, shared=4064)[0] == "mma" and plan(n_groups=4, sharing=3, most_rows=16, shared=4097)[0] == "tcgen05"
     # groups that share nothing are no reason to cut the others into fewer splits
     assert plan(n_groups=3)[1][1] == plan(n_groups=3, sharing=1)[1][1] > plan(n_groups=3, sharing=3)[1][1]
 
