@@ -1,5 +1,5 @@
 // Decode attention behind shared prefixes (prefix.cuh) for float32, and for what the bfloat16 kernels do not take (head sizes that are
-// no multiple of 16, pages of no power of two, more than 16 query heads a KV head, very many rows).  Compile with -DHEAD_DIM=<multiple
+// no multiple of 16 or above 256, more than 16 query heads a KV head, very many rows).  Compile with -DHEAD_DIM=<multiple
 // of 16, at most 512>; the real head size may be smaller.
 //
 // A CTA has a tile of up to 32 query vectors and walks its split of the keys in blocks of 32, two blocks of keys and values on their

@@ -1,5 +1,5 @@
 // Decode attention behind shared prefixes (prefix.cuh) over the bfloat16 cache, on mma.sync.  Compile with -DHEAD_DIM=<multiple of
-// 16, at most 256>; pages of a power of two, at most 16 query heads a KV head.
+// 16, at most 256>; at most 16 query heads a KV head.
 //
 // Work comes in items: up to 16 query vectors of one KV head (a tile of a group's against its shared keys, or one row's against its
 // own), an item in blocks of 32 keys.  All items' blocks stand in one sequence, and every warp of a persistent grid takes an equal
@@ -208,13 +208,16 @@ __device__ __noinline__ Place locate(const Entries& at, int s, int s_end, int n_
 }
 
 // What the block table says of the page of this lane's keys, asked for a block before it is used: a block is cut into boxes, the keys of
-// one page each, and lane j has the j-th.  A box that ends below `lowest` is another table's: the sink's page, 0, and so is what a
-// lane without a box gets.
+// one page each, and lane j has the j-th; pages of no power of two end anywhere in a block, and a box is a key then (log2_page -1).  A
+// box that ends below `lowest` is another table's: the sink's page, 0, and so is what a lane without a box gets.
 struct Boxes { int log2_rows, log2_page; };
+__device__ __forceinline__ int page_of_key(const PrefixCall& c, const Boxes& boxes, int key) {
+  return boxes.log2_page >= 0 ? key >> boxes.log2_page : key / c.page_size;
+}
 __device__ __forceinline__ int lane_page(const PrefixCall& c, const Boxes& boxes, const Place& p, int lane) {
   const int key0 = p.first_key + (lane << boxes.log2_rows);
   if ((lane << boxes.log2_rows) >= KB || key0 >= p.end || key0 + (1 << boxes.log2_rows) <= p.lowest) return 0;
-  return __ldg(c.block_table + static_cast<long long>(p.table_row) * c.table_stride + (key0 >> boxes.log2_page));
+  return __ldg(c.block_table + static_cast<long long>(p.table_row) * c.table_stride + page_of_key(c, boxes, key0));
 }
 // The warp asks for the block at p.first_key, its boxes on the lanes' pages (the sink's for one outside the pool); rows that are not the
 // item's become zeros, so that whatever a page holds there does not reach P V.
@@ -225,7 +228,8 @@ __device__ __forceinline__ void fetch_block_of(const PrefixCall& c, const Boxes&
     atomicOr(c.err, B200_ERR_SLOT_RANGE);
     page = 0;
   }
-  const int y = (page * c.nkv + p.kvh) * c.page_size + ((p.first_key + (lane << boxes.log2_rows)) & (c.page_size - 1));
+  const int key0 = p.first_key + (lane << boxes.log2_rows);
+  const int y = (page * c.nkv + p.kvh) * c.page_size + key0 - page_of_key(c, boxes, key0) * c.page_size;
   const int from = p.lowest - p.first_key, to = p.end - p.first_key;
   if (32 % CHUNKS == 0 && ROWS <= 8 && boxes.log2_rows >= 3) {      // eight keys behind one another at a time
 #pragma unroll
@@ -523,7 +527,7 @@ B200_EXPORT int b200_prefix_attention_mma(const void* q, const void* k_cache, co
                                           int n_groups, int nh, int nkv, int page_size, int pages, float scale, int splits_shared, int covered,
                                           int ctas, int sms, int* err, cudaStream_t stream) {
   if (n_rows <= 0) return 0;
-  if (nh <= 0 || nkv <= 0 || nh % nkv != 0 || nh / nkv > 16 || page_size <= 0 || (page_size & (page_size - 1)) != 0 || pages <= 0 || table_stride <= 0 || n_groups < 0)
+  if (nh <= 0 || nkv <= 0 || nh % nkv != 0 || nh / nkv > 16 || page_size <= 0 || pages <= 0 || table_stride <= 0 || n_groups < 0)
     return B200_BAD_SIZE;
   // (blocks are counted in 32 bits)
   const long long most_blocks = (static_cast<long long>(table_stride) * page_size / KB + 2) * nkv *
@@ -545,8 +549,8 @@ B200_EXPORT int b200_prefix_attention_mma(const void* q, const void* k_cache, co
   k.c = {block_table, cu_q, kv_len, rows, reinterpret_cast<const int2*>(groups), scratch, part_ml, err, table_stride, n_rows, n_groups, nh, nkv,
          page_size, pages, splits_shared, 0, 1, scale * 1.4426950408889634f};
   Boxes boxes;
-  boxes.log2_page = __builtin_ctz(page_size);
-  boxes.log2_rows = page_size < KB ? boxes.log2_page : __builtin_ctz(KB);
+  boxes.log2_page = (page_size & (page_size - 1)) != 0 ? -1 : __builtin_ctz(page_size);
+  boxes.log2_rows = boxes.log2_page < 0 ? 0 : page_size < KB ? boxes.log2_page : __builtin_ctz(KB);
   static bool seen[16];
   int rc = prefix_smem_limit(prefix_stream_kernel, static_cast<int>(FIXED) + entries_bytes(MOST_ENTRIES), seen);
   if (rc != 0) return rc;

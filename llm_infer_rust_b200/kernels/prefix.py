@@ -76,7 +76,8 @@ def _plan(dtype, heads: int, kv_heads: int, dim: int, page: int, n_rows: int, n_
     most_rows = max(1, min(most_rows, n_rows))
     vectors = most_rows * per
     sharing = max(1, min(sharing, n_groups))
-    if not aligned or not ops.decode_uses_tensor_cores(dtype, heads, kv_heads, dim, page) or n_rows + n_groups > _MOST_ENTRIES:
+    # (pages of any size: powers of two in what decode attention asks for and the tcgen05 kernel fetches, not here)
+    if not aligned or not ops.decode_uses_tensor_cores(dtype, heads, kv_heads, dim, 1) or n_rows + n_groups > _MOST_ENTRIES:
         lib = load_entry_points("prefix_attention.cu", {"HEAD_DIM": ops.padded_head_dim(dim)})
         tiles = -(-vectors // _TILE)
         per_sm = max(1, 227 * 1024 // (lib.b200_prefix_attention_smem() + 1024))
@@ -86,7 +87,7 @@ def _plan(dtype, heads: int, kv_heads: int, dim: int, page: int, n_rows: int, n_
     tcgen05, tiles, two, shared, covered, stream = None, 1, 0, 0, 0, sms
     blocks = -(-vectors // _MMA_VECTORS) * -(-most_shared // 32) * kv_heads * sharing
     least = _TENSOR_CORE_BLOCKS_OF_GROUPS if sharing > 1 else _TENSOR_CORE_BLOCKS if vectors > 2 * _MMA_VECTORS else _TENSOR_CORE_BLOCKS_OF_TWO_TILES
-    if n_groups and dim == 128 and vectors > _MMA_VECTORS and blocks >= least:
+    if n_groups and dim == 128 and page & (page - 1) == 0 and vectors > _MMA_VECTORS and blocks >= least:
         # one or two tiles a CTA, none without a block of keys for each of its streams
         two = int(vectors > _TC_VECTORS)
         a_cta = _TC_VECTORS << two

@@ -132,6 +132,8 @@ CASES = {
     "a long prompt": ([(3, 5000, [100, 1, 33])], 8, 2, 128, 16),
     "long answers": ([(2, 31, [1500, 700])], 8, 2, 128, 16),
     "pages of 24": ([(4, 130, [1, 25, 24, 50])], 6, 2, 96, 24),
+    "pages of 7": ([(6, 200, [1, 8, 30, 60, 3, 100]), (2, 13, [1, 40])], 8, 2, 128, 7),
+    "pages of 40": ([(3, 333, [1, 8, 130])], 8, 2, 64, 40),
     "pages of one": ([(3, 37, [1, 2, 3])], 4, 2, 48, 1),
     "pages of two": ([(3, 75, [1, 2, 30])], 4, 2, 128, 2),
     "pages of 128": ([(3, 300, [1, 2, 130])], 4, 2, 64, 128),

@@ -66,7 +66,8 @@ def test_calls_go_where_they_are_served():
     assert (tiles, two, covered) == (1, 0, 128) and splits % 2 == 0 and 8 * splits // 2 + ctas <= 148      # one tile: a CTA leaves two parts
     assert plan(most_rows=4)[0] == "mma" and plan(shared=352)[0] == "mma" and plan(dim=64)[0] == "mma"
     assert plan(shared=353)[0] == "tcgen05" and plan(most_rows=8, shared=4065)[0] == "tcgen05" and plan(most_rows=8, shared=4064)[0] == "mma"
-    for other in (dict(dtype=torch.float32), dict(page=24), dict(dim=72), dict(heads=17, kv_heads=1), dict(n_rows=400), dict(aligned=False)):
+    assert plan(page=24)[0] == "mma"
+    for other in (dict(dtype=torch.float32), dict(dim=72), dict(heads=17, kv_heads=1), dict(n_rows=400), dict(aligned=False)):
         assert plan(**other)[0] == "all sizes", other
     assert plan(n_rows=399)[0] == "tcgen05"
     # own keys that outweigh the shared ones come behind them, on all SMs or on most
@@ -130,8 +131,9 @@ def test_entry_points_of_the_attention_refuse_what_they_cannot_serve():
         # sizes; tables of more than 2^30 places
         for bad in (dict(nh=0), dict(nkv=0), dict(nh=7), dict(page=0), dict(pages=0), dict(stride=0), dict(stride=2 ** 27), dict(n_groups=-1)):
             assert call(kind, **bad) == (0 if kind == "tc" and "n_groups" in bad else -2), (kind, bad)
+    assert call("tc", page=24) == -2
     for kind in ("mma", "tc"):
-        assert call(kind, page=24) == -2 and call(kind, pages=2 ** 27) == -2 and call(kind, q=ctypes.c_void_p((1 << 20) + 8)) == -3
+        assert call(kind, pages=2 ** 27) == -2 and call(kind, q=ctypes.c_void_p((1 << 20) + 8)) == -3
     assert call("mma", nh=34) == -2 and call("mma", n_rows=400) == -2 and call("mma", last=[2, 0, 148, 148]) == -2 and call("mma", last=[0, 0, 149, 148]) == -2
     assert call("tc", scale=0.0) == -2 and call("tc", last=[3, 1, 0]) == -2 and call("tc", last=[0, 1, 1]) == -2
     assert call("every", last=[1, 1, 1, 1, 130, 148]) == -2 and call("every", last=[1, 1, 1, 1, 127, 148]) == -2 and call("every", last=[0, 1, 1, 1, 128, 148]) == -2
