@@ -313,7 +313,8 @@ PyObject* byte_product(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // the launches.  The entry points are those of the plan, None where it has no use for one: the all-sizes kernel alone, or the
 // tensor-core kernels.  plan: (floats of scratch, splits of the shared keys, splits of the own keys, tiles, two tiles a CTA, vectors
 // that the tcgen05 kernel covers, CTAs of the stream kernel, multiprocessors).  None, and nothing done, where something is not as it should be (the wrapper then says what)
-// or this thread records its calls.  (Through Python the call took the host 17 us, of which 7 are three launches.)
+// or this thread records its calls.  (Through Python the call took the host 17 us, as one 9 to 10,
+// of which 5 to 7 are two or three launches.)
 PyObject* prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 20 || !PyFloat_Check(args[16]) || !PyTuple_Check(args[17]) || PyTuple_GET_SIZE(args[17]) != 8) {

@@ -9,7 +9,11 @@
 //   two tiles (more than 128 vectors)   each stream has 128 vectors of its own, both walk the same keys, fetched once;
 //   one tile                            both streams have the same vectors and take every other block of keys; each leaves a part
 //                                       of its own, and the rings are a stage of keys deeper.
-// Bound by the special-function unit and the products from about 128 vectors on, by the copies below.
+// Bound, two tiles, by the products: a pair of blocks takes 3,360 cycles, 2,050 of them products, which wait for shared memory where the
+// copies write it (2,560 together); one tile by the copies' instructions, 64 of some 130 cycles a pair of blocks.  (256 vectors of 8 KV
+// heads behind 32,768 keys, 13 CTAs a head: 60.7 us; with two copy warps and no more than 168 registers for the softmax, which spilled, 65.9;
+// 64 vectors behind 16,384 keys 27.5 and 30.0.  Four copy warps leave 128 registers a thread: 115.5.  Scores in buffers of 64 keys, two a
+// stream, ready before the softmax wants them: 65.1, for a product of 64 columns reads as many queries as one of 128.)
 #include "attention_tcgen05.cuh"
 #include "kv_map.cuh"
 #include "prefix.cuh"
