@@ -29,6 +29,17 @@ struct PrefixCall {
 
 __device__ __forceinline__ int prefix_splits(const PrefixCall& c) { return c.splits_shared + c.splits_own; }
 
+// Asks for the call's index arrays, into the second-level cache, before the kernel may read them (a warp; what is written there after this
+// arrives there too): a chain of them, group, row, length, stands in front of the first key.  Of the rows' lengths and tokens the lines that
+// they begin in, for which rows there are is not known yet.  (Six groups of 42 rows 28.5 -> 28.2 us, 64 rows behind 32,768 keys 67.9 -> 67.5.)
+__device__ __forceinline__ void prefetch_indices(const PrefixCall& c) {
+  const int lane = threadIdx.x & 31;
+  auto ask = [](const void* p) { asm volatile("prefetch.global.L2 [%0];\n" ::"l"(p)); };
+  if (lane * 8 < c.n_rows) ask(c.rows + lane * 8);
+  if (lane * 4 < c.n_groups) ask(c.groups + lane * 4);
+  if (lane < 8) ask(reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(lane < 4 ? c.kv_len : c.cu_q) & ~uintptr_t(127)) + (lane & 3) * 32);
+}
+
 // (first row, rows) of group g, inside the call's rows whatever the array says.
 __device__ __forceinline__ int2 rows_of_group(const PrefixCall& c, int g) {
   const int first = min(max(c.groups[g].x, 0), c.n_rows);

@@ -309,6 +309,7 @@ template <typename T>
 __global__ void __launch_bounds__(THREADS)
 prefix_any_kernel(const T* __restrict__ q, const T* __restrict__ kc, const T* __restrict__ vc, const PrefixCall c, int hd, bool wide) {
   extern __shared__ __align__(16) float sm[];
+  if (threadIdx.x < 32) prefetch_indices(c);
   pdl_wait();
   pdl_launch_dependents();
   const int group = c.nh / c.nkv;

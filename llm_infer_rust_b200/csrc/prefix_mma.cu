@@ -353,6 +353,7 @@ prefix_stream_kernel(const bf16* __restrict__ kc, const bf16* __restrict__ vc, c
   // Behind the tcgen05 kernel of the same call, which has waited for the kernels before it, this one begins beside it, and waits
   // for its end at its own: whoever waits for this kernel then waits for both.  The joining kernel may come as soon as what was
   // launched before the call has ended.
+  if (threadIdx.x < 32) prefetch_indices(c);
   if (k.covered == 0) pdl_wait();
   pdl_launch_dependents();
   Entries at;

@@ -52,6 +52,7 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
 
   const int warp = same_in_warp(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (threadIdx.x < 32) prefetch_indices(c);
   if (threadIdx.x == 0) {
     for (int s = 0; s < 3; ++s) { mbar_init(k_full + s, 1); mbar_init(k_empty + s, 1); }
     for (int s = 0; s < VS; ++s) { mbar_init(v_full + s, 1); mbar_init(v_empty + s, 1); }
