@@ -189,6 +189,7 @@ __device__ __forceinline__ void join_parts(T* __restrict__ dst, int hd, int coun
   }
 }
 // Warps of a CTA that joins one of `vectors` vectors.  Few vectors have many parts each, a hundred and more where one prompt's keys are all there
-// is: then all of them at once, while an SM has a CTA.  (4 / 16 warps: two rows of 16 heads behind 4,096 keys 18.6 / 13.4 us in all, 32
-// rows behind 512 keys 15.0 / 19.0.)
-static inline int join_warps_of(long long vectors, int sms) { return vectors <= sms ? 16 : vectors <= 2 * sms ? 8 : 4; }
+// is: then all of them at once, while an SM has a CTA.  Many have a dozen, and all vectors are to be on the SMs at once.  (4 / 16 warps: two
+// rows of 16 heads behind 4,096 keys 18.6 / 13.4 us in all, 32 rows behind 512 keys 15.0 / 19.0; 2 / 4 warps: 768 vectors 22.6 / 22.0, 1,536
+// 27.2 / 27.5, 2,048 65.2 / 67.8 and 92.7 / 96.4.)
+static inline int join_warps_of(long long vectors, int sms) { return vectors <= sms ? 16 : vectors <= 2 * sms ? 8 : vectors <= 10 * sms ? 4 : 2; }

@@ -399,7 +399,7 @@ static int launch(const void* q, const void* kc, const void* vc, void* out, cons
   if (rc != 0) return rc;
   // (16 warps' rows of 512 floats: 33 KB)
   const int warps = join_warps_of(vectors, sms);
-  return b200_launch(warps == 16 ? prefix_any_join_kernel<T, 16> : warps == 8 ? prefix_any_join_kernel<T, 8> : prefix_any_join_kernel<T, 4>,
+  return b200_launch(warps == 16 ? prefix_any_join_kernel<T, 16> : warps == 8 ? prefix_any_join_kernel<T, 8> : warps == 4 ? prefix_any_join_kernel<T, 4> : prefix_any_join_kernel<T, 2>,
                      dim3(static_cast<unsigned>(vectors)), dim3(warps * 32), 0, stream, 0, static_cast<T*>(out), c, hd);
 }
 

@@ -559,6 +559,6 @@ B200_EXPORT int b200_prefix_attention_mma(const void* q, const void* k_cache, co
   rc = b200_launch(prefix_stream_kernel, dim3(ctas), dim3(THREADS), FIXED + entries, stream, 0, static_cast<const bf16*>(k_cache), static_cast<const bf16*>(v_cache), static_cast<const bf16*>(q), k, boxes);
   if (rc != 0) return rc;
   const int warps = join_warps_of(static_cast<long long>(n_rows) * nh, sms);
-  return b200_launch(warps == 16 ? prefix_join_kernel<16> : warps == 8 ? prefix_join_kernel<8> : prefix_join_kernel<4>, dim3(static_cast<unsigned>(n_rows) * nh),
+  return b200_launch(warps == 16 ? prefix_join_kernel<16> : warps == 8 ? prefix_join_kernel<8> : warps == 4 ? prefix_join_kernel<4> : prefix_join_kernel<2>, dim3(static_cast<unsigned>(n_rows) * nh),
                      dim3(warps * 32), 0, stream, 0, static_cast<bf16*>(out), k);
 }
