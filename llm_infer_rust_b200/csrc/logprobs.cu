@@ -78,13 +78,13 @@ __device__ __forceinline__ void insert_all(K& list, K mine, bool have, int last)
     list = lane < place ? list : lane == place ? next : up;
   }
 }
-// The CTA's warps join their lists; all hold the result.  `sh`: [WARPS][32].
+// The lists of the CTA's first `some` warps joined; all warps hold the result.  `sh`: [WARPS][32].
 template <int WARPS, typename K>
-__device__ K join_warps(K list, K* sh) {
+__device__ K join_warps(K list, int some, K* sh) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int half = WARPS / 2; half > 0; half >>= 1) {
-    if (warp >= half && warp < 2 * half) sh[warp * 32 + lane] = list;
+  some = min(some, WARPS);
+  for (int half = some > 1 ? 1 << (31 - __clz(some - 1)) : 0; half > 0; half >>= 1) {
+    if (warp >= half && warp < 2 * half) sh[warp * 32 + lane] = list;      // (a warp beyond `some` has nothing)
     __syncthreads();
     if (warp < half) list = join_lists(list, sh[(warp + half) * 32 + 31 - lane]);
   }
@@ -148,7 +148,7 @@ struct Shared {
 // UNROLL: 16-byte loads of a thread on their way.
 template <int THREADS, int UNROLL, int CTAS>
 __global__ void __launch_bounds__(THREADS, CTAS)
-logprobs_kernel(const float* __restrict__ logits, long long row_stride, int vocab, const int* __restrict__ tokens, int top,
+logprobs_kernel(const float* logits, long long row_stride, int vocab, const int* tokens, int top,
                 int cluster, float* __restrict__ logprobs, float* __restrict__ entropy, int* __restrict__ top_ids,
                 float* __restrict__ top_logprobs, int* err) {
   constexpr int WARPS = THREADS / 32;
@@ -157,6 +157,8 @@ logprobs_kernel(const float* __restrict__ logits, long long row_stride, int voca
   const long long row_index = blockIdx.x / cluster;
   const float* row = logits + row_index * row_stride;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_wait();
+  pdl_launch_dependents();
   float given = 0.0f;
   if (rank == 0 && threadIdx.x == 0 && tokens != nullptr) {
     const int token = tokens[row_index];
@@ -199,7 +201,7 @@ logprobs_kernel(const float* __restrict__ logits, long long row_stride, int voca
 #pragma unroll
       for (int u = 0; u < UNROLL; ++u) {
         v[u] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        if (at + u * THREADS < end) v[u] = __ldg(body + at + u * THREADS);
+        if (at + u * THREADS < end) v[u] = __ldcg(body + at + u * THREADS);
       }
       float mx = -INFINITY;
 #pragma unroll
@@ -240,15 +242,17 @@ logprobs_kernel(const float* __restrict__ logits, long long row_stride, int voca
     // the chunks' elements (in whatever order they stand there: a list of distinct keys does not depend on it)
     if (warp == 0) insert_all(best, has_loose ? key_of(loose_value, loose_id) : 0ull, has_loose && loose_value == loose_value, top - 1);
     // (all warps share all chunks' elements, AGAIN loads of a lane on their way: one chunk a warp, one load behind the other, were 30 us
-    // more for 2,048 rows of 151,936)
+    // more for 2,048 rows of 151,936.  In the kernel of few rows few elements are a few warps', whose lists take fewer steps to join: one
+    // row with 5 alternatives 8.9 -> 8.7 us, 45 masked rows 9.6 -> 9.4; in that of many 205.3 -> 207.3.)
     constexpr int AGAIN = 4;
     const int elements = turns_a_chunk * UNROLL * 4, all = sh.count * elements;
-    for (int x0 = warp * 32; x0 < all; x0 += AGAIN * THREADS) {
+    const int some = CTAS == 1 && all <= 4 * 32 * AGAIN ? max(1, (all + 32 * AGAIN - 1) / (32 * AGAIN)) : WARPS;
+    for (int x0 = warp < some ? warp * 32 : all; x0 < all; x0 += AGAIN * 32 * some) {
       float v[AGAIN];
       int id[AGAIN];
 #pragma unroll
       for (int y = 0; y < AGAIN; ++y) {
-        const int x = x0 + y * THREADS + lane;
+        const int x = x0 + y * 32 * some + lane;
         id[y] = -1;
         if (x < all) {
           const int i = x / elements, e = x - i * elements, chunk = sh.chunks[i];
@@ -256,12 +260,12 @@ logprobs_kernel(const float* __restrict__ logits, long long row_stride, int voca
           const int at = begin + turn * UNROLL * THREADS + e / 4 % UNROLL * THREADS + chunk % THREADS;
           if (turn < turns && at < end) id[y] = front + 4 * at + e % 4;
         }
-        if (id[y] >= 0) v[y] = __ldg(row + id[y]);
+        if (id[y] >= 0) v[y] = __ldcg(row + id[y]);
       }
 #pragma unroll
       for (int y = 0; y < AGAIN; ++y) insert_all(best, id[y] >= 0 ? key_of(v[y], id[y]) : 0ull, id[y] >= 0 && v[y] >= reach, top - 1);
     }
-    best = join_warps<WARPS>(best, sh.keys);
+    best = join_warps<WARPS>(best, some, sh.keys);
   } else {
     __syncthreads();
   }
@@ -280,7 +284,7 @@ logprobs_kernel(const float* __restrict__ logits, long long row_stride, int voca
     if (rank != 0) return;
     a = {-INFINITY, 0.0f, 0.0f};
     for (int r = 0; r < cluster; ++r) add_to(a, sh.parts[r]);
-    if (top > 0) best = join_warps<WARPS>(warp < cluster ? sh.best[warp][lane] : 0ull, sh.keys);
+    if (top > 0) best = join_warps<WARPS>(warp < cluster ? sh.best[warp][lane] : 0ull, cluster, sh.keys);
   }
   if (warp != 0) return;
   const float log_s = logf(a.s);
@@ -317,22 +321,11 @@ B200_EXPORT int b200_token_logprobs(const float* logits, long long row_stride, i
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
   if (e != cudaSuccess) return static_cast<int>(e);
   const int cluster = cluster_of(rows, vocab, sms);
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(rows) * cluster);
   // Few rows: a thread has all of its elements on their way at once where it can.  Many: 1,536 threads an SM, so that some CTAs read
   // while others sort; long rows in CTAs of 512 threads, short ones in 256 (2,048 rows of 151,936 with 20 alternatives: 212 us
   // against 219, of 32,000 with 5: 72 against 63; without alternatives the first take 190, their bytes at the copy rate).
   const bool many = rows >= 2 * sms, small = many && vocab < 65536;
-  config.blockDim = dim3(small ? 256 : 512);
-  config.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  config.attrs = attr;
-  config.numAttrs = cluster > 1 ? 1 : 0;
-  e = cudaLaunchKernelEx(&config, small ? logprobs_kernel<256, 4, 6> : many ? logprobs_kernel<512, 4, 3> : logprobs_kernel<512, 10, 1>, logits, row_stride, vocab, tokens, top, cluster, logprobs,
-                         entropy, top_ids, top_logprobs, err);
-  return e == cudaSuccess ? b200_check_launch() : static_cast<int>(e);
+  return b200_launch(small ? logprobs_kernel<256, 4, 6> : many ? logprobs_kernel<512, 4, 3> : logprobs_kernel<512, 10, 1>,
+                     dim3(static_cast<unsigned>(rows) * cluster), dim3(small ? 256 : 512), 0, stream, cluster > 1 ? cluster : 0, logits, row_stride, vocab, tokens, top, cluster, logprobs,
+                     entropy, top_ids, top_logprobs, err);
 }
