@@ -25,15 +25,16 @@ _KEYS_PER_CTA_AT_LEAST = 32
 _MOST_SPLITS = 64
 _MOST_ENTRIES = 400           # rows and groups of a call that the tensor-core kernels take
 # The tcgen05 kernel takes the shared keys of more vectors of a KV head than the mma.sync kernel has in a tile, from so many blocks on (32 keys
-# of a KV head against 16 vectors each).  (mma.sync / tcgen05, us, 8 KV heads of 128: 32 vectors, 2,048 keys 12.4 / 12.9, 4,096 keys 15.5 /
-# 14.3; 64 vectors, 1,024 keys 12.9 / 12.9, 2,048 keys 15.7 / 13.6; 128 vectors, 512 keys 13.4 / 14.6, 1,024 keys 16.4 / 15.0; 256 vectors, 512
-# keys 19.5 / 18.9; 256 behind 32,768 keys 307 / 55.  One KV head: 128 vectors, 4,096 keys 11.5 / 13.4, 8,192 keys 15.4 / 13.9; 512 vectors,
-# 2,048 keys 15.8 / 16.2, 4,096 keys 20.8 / 17.3.)  Several groups are as a rule unlike in their rows and keys, and `blocks` counts
+# of a KV head against 16 vectors each), which goes by the steps that a CTA would have.  (mma.sync / tcgen05, us, 8 KV heads of 128, a step: 32
+# vectors, 3,000 keys 13.7 / 14.3, 4,096 keys 15.9 / 12.9; 64 vectors, 1,000 keys 12.8 / 14.0, 1,500 keys 14.3 / 14.2, 2,000 keys 16.3 / 14.7; 128
+# vectors, 512 keys 13.4 / 14.6, 1,024 keys 16.4 / 15.0; 256 vectors, 512 keys 19.5 / 18.9.  Two: 32 vectors, 5,000 keys 16.7 / 17.9, 6,500 keys 20.2 / 16.4;
+# 256 vectors, 8,192 keys 99 / 28.  One KV head, a step: 128 vectors, 4,096 keys 11.5 / 13.4, 8,192 keys 15.4 / 13.9; 512 vectors, 2,048 keys 15.8 /
+# 16.2, 4,096 keys 20.8 / 17.3.)  Several groups are as a rule unlike in their rows and keys, and `blocks` counts
 # each as the largest, so it has to be more then: of up to 24 vectors six behind up to 3,001 keys (9,024 blocks) 20.8 / 28.8, of up to 80
 # three behind 500 (1,920) 14.7 / 15.6 and behind 1,500 (5,640) 19.2 / 18.5, of up to 48 six behind 700 (3,168) 15.4 / 18.0, of up to 64
 # twelve behind 1,000 (12,288) 31.0 / 29.4.
-_TENSOR_CORE_BLOCKS, _TENSOR_CORE_BLOCKS_OF_TWO_TILES, _TENSOR_CORE_BLOCKS_OF_GROUPS = 1536, 2048, 12288
-_MMA_VECTORS = 16
+_TENSOR_CORE_BLOCKS, _TENSOR_CORE_BLOCKS_A_STEP, _TENSOR_CORE_BLOCKS_OF_GROUPS = 600, 1150, 12288
+_MMA_VECTORS = _TENSOR_CORE_VECTORS = 16      # of a tile of the mma.sync kernel; more than which the other takes
 
 
 def _splits(most_shared: int, most_own: int, shared_ctas: int, own_ctas: int, room: int) -> tuple:
@@ -51,6 +52,10 @@ _TC_FIXED, _TC_STEP = (5.0, 12.0), (2.9, 1.8)
 _OWN_FIXED, _OWN_BYTES, _OWN_BYTES_ALL, _OWN_KEYS = 5.0, 78000.0, 6.5e6, 64
 
 
+def _most_ctas(steps: int, tiles: int, sms: int) -> int:
+    return max(1, min(steps, sms // tiles, _MOST_SPLITS))
+
+
 def _share_sms(steps: int, two: int, tiles: int, items: int, most_own: int, key_bytes: int, sms: int) -> tuple:
     """How many CTAs cut each of ``tiles`` tiles' ``steps``, and the CTAs of the stream kernel for ``items`` of own keys (half of ``most_own``
     each): side by side on SMs of their own, as the registers and shared memory of either leave no room for the other, or one behind the
@@ -58,7 +63,7 @@ def _share_sms(steps: int, two: int, tiles: int, items: int, most_own: int, key_
     77.2, 15 beside 28 90.8, one behind the other 79.5; 24 rows of 64 heads behind 8,000 keys, 1 to 200: 26.0 and 29.3.)"""
     own_bytes = items * (most_own / 2 + _OWN_KEYS) * key_bytes
     of_tc = lambda ctas: _TC_FIXED[two] + _TC_STEP[two] * -(-steps // ctas)
-    most = max(1, min(steps, sms // tiles, _MOST_SPLITS))
+    most = _most_ctas(steps, tiles, sms)
     best = of_tc(most) + _OWN_FIXED + own_bytes / _OWN_BYTES_ALL, most, sms
     for ctas in range(1, most + 1):
         left = sms - ctas * tiles
@@ -86,15 +91,17 @@ def _plan(dtype, heads: int, kv_heads: int, dim: int, page: int, n_rows: int, n_
         return lib.b200_prefix_attention, None, None, (floats, shared, own, tiles, 0, 0, 0, sms), 2
     tcgen05, tiles, two, shared, covered, stream = None, 1, 0, 0, 0, sms
     blocks = -(-vectors // _MMA_VECTORS) * -(-most_shared // 32) * kv_heads * sharing
-    least = _TENSOR_CORE_BLOCKS_OF_GROUPS if sharing > 1 else _TENSOR_CORE_BLOCKS if vectors > 2 * _MMA_VECTORS else _TENSOR_CORE_BLOCKS_OF_TWO_TILES
-    if n_groups and dim == 128 and page & (page - 1) == 0 and vectors > _MMA_VECTORS and blocks >= least:
+    if n_groups and dim == 128 and page & (page - 1) == 0 and vectors > _TENSOR_CORE_VECTORS:
         # one or two tiles a CTA, none without a block of keys for each of its streams
         two = int(vectors > _TC_VECTORS)
-        a_cta = _TC_VECTORS << two
-        tiles = -(-vectors // a_cta)
-        ctas, stream = _share_sms(-(-most_shared // (256 >> two)), two, sharing * kv_heads * tiles, n_rows * kv_heads, most_own, 4 * dim, sms)
-        shared, covered = ctas << (1 - two), tiles * a_cta
-        tcgen05 = load_entry_points("prefix_tcgen05.cu").b200_prefix_tcgen05
+        tiles = -(-vectors // (_TC_VECTORS << two))
+        steps, all_tiles = max(1, -(-most_shared // (256 >> two))), sharing * kv_heads * tiles
+        least = _TENSOR_CORE_BLOCKS_OF_GROUPS if sharing > 1 else \
+            _TENSOR_CORE_BLOCKS + _TENSOR_CORE_BLOCKS_A_STEP * -(-steps // _most_ctas(steps, all_tiles, sms))
+        if blocks >= least:
+            ctas, stream = _share_sms(steps, two, all_tiles, n_rows * kv_heads, most_own, 4 * dim, sms)
+            shared, covered = ctas << (1 - two), tiles * (_TC_VECTORS << two)
+            tcgen05 = load_entry_points("prefix_tcgen05.cu").b200_prefix_tcgen05
     lib = load_entry_points("prefix_mma.cu", {"HEAD_DIM": dim})
     count = lib.library.b200_prefix_scratch_floats
     count.restype = ctypes.c_longlong

@@ -293,10 +293,16 @@ def test_command_line(folders):
     assert len(lines) == 3 and all(len(l["output_ids"]) == len(l["logprobs"]) == 4 and len(l["logprobs"][0]["top"]) == 2 for l in lines)
 
 
-def test_large_groups_through_the_tcgen05_kernel(folders):
+def test_large_groups_through_the_tcgen05_kernel(folders, monkeypatch):
     """Head size 128, 48 answers of two query heads a KV head behind 300 tokens: the engine's own step against decode attention's."""
     from llm_infer_rust_b200.engine import StepEntry
     from llm_infer_rust_b200.engine import engine as module
+    from llm_infer_rust_b200.kernels import prefix
+    for name in ("_TENSOR_CORE_BLOCKS", "_TENSOR_CORE_BLOCKS_A_STEP", "_TENSOR_CORE_BLOCKS_OF_GROUPS"):
+        monkeypatch.setattr(prefix, name, 0)
+    asked, load = [], prefix.load_entry_points
+    monkeypatch.setattr(prefix, "load_entry_points", lambda source, *a: asked.append(source) or load(source, *a))
+    prefix._plan.cache_clear()
     folder, _ = folders("E", "bfloat16")
     eng = engine(folder, dtype="bfloat16", max_running_req=50, max_total_tokens=4096)
     eng.open_request(1)
@@ -319,6 +325,8 @@ def test_large_groups_through_the_tcgen05_kernel(folders):
                 e.step([StepEntry(r, tokens(307, 1, 60 * step + r), [0]) for r in ids])
         logits.append(e.step([StepEntry(r, [t], [0]) for r, t in zip(ids, new)]).float().cpu().numpy().copy())
         e.check_kernel_errors()
+    prefix._plan.cache_clear()
+    assert "prefix_tcgen05.cu" in asked
     near(logits[0], logits[1], "bfloat16")
 
 

@@ -323,3 +323,102 @@ def test_calls_on_two_streams_at_once(name, dtype):
     for w, of in zip(want, outs):
         for got in of:
             assert torch.equal(got, w)
+
+
+# What the tcgen05 kernel is given when it is given everything: (groups, nh, nkv, page), heads of 128 in bfloat16
+TCGEN05_CASES = {
+    "one key": ([(3, 1, [0, 0, 0])], 8, 8, 16),
+    "one row": ([(1, 300, [5])], 4, 2, 16),
+    "a block less a key": ([(3, 127, [1, 0, 20])], 8, 2, 16),
+    "a block": ([(3, 128, [1, 0, 20])], 8, 2, 16),
+    "a block and a key": ([(3, 129, [1, 0, 20])], 8, 2, 16),
+    "two blocks and a key": ([(3, 257, [1, 0, 20])], 8, 2, 16),
+    "five blocks": ([(12, 640, [1 + i for i in range(12)])], 8, 2, 16),
+    "rows that see less than is shared, and nothing": ([(6, 700, [4, -40, 0, -700, -699, -300])], 8, 2, 16),
+    "a tile and a row of vectors": ([(33, 400, [1 + i % 5 for i in range(33)])], 8, 2, 16),
+    "two tiles": ([(64, 1000, [1 + i % 50 for i in range(64)])], 8, 2, 16),
+    "three tiles of two": ([(70, 300, [1 + i % 3 for i in range(70)])], 16, 2, 16),
+    "groups of all sizes": ([(1, 17, [3]), (7, 129, [1, 2, 3, 40, 5, 6, 70]), (2, 0, [5, 80]), (40, 640, list(range(1, 41)))], 8, 2, 16),
+    "sixteen query heads": ([(9, 500, [1 + i for i in range(9)])], 16, 1, 16),
+    "pages of one": ([(4, 150, [1, 2, 3, 4])], 4, 2, 1),
+    "pages of four": ([(20, 333, [1 + i for i in range(20)])], 8, 2, 4),
+    "pages of 64": ([(20, 333, [1 + i for i in range(20)])], 8, 2, 64),
+    "a long prompt": ([(5, 20000, [100, 1, 33, 7, 2])], 8, 1, 16),
+}
+
+
+@pytest.fixture
+def always_tcgen05(monkeypatch):
+    m = prefix()
+    asked = []
+    load = m.load_entry_points
+    monkeypatch.setattr(m, "load_entry_points", lambda source, *a: asked.append(source) or load(source, *a))
+    for name in ("_TENSOR_CORE_BLOCKS", "_TENSOR_CORE_BLOCKS_A_STEP", "_TENSOR_CORE_BLOCKS_OF_GROUPS"):
+        monkeypatch.setattr(m, name, 0)
+    # (it is asked for from the first vector on; what an item of the other kernel takes stays)
+    monkeypatch.setattr(m, "_TENSOR_CORE_VECTORS", 0)
+    m._plan.cache_clear()
+    yield asked
+    m._plan.cache_clear()
+    assert "prefix_tcgen05.cu" in asked
+
+
+@pytest.mark.parametrize("name", list(TCGEN05_CASES))
+def test_tcgen05_against_64_bits(name, always_tcgen05):
+    groups, nh, nkv, page = TCGEN05_CASES[name]
+    c = Case(groups, nh, nkv, 128, page, BF16)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("hints", [dict(most_rows=1, most_shared=0, most_own=0), dict(most_rows=0, most_shared=1 << 20, most_own=1),
+                                   dict(most_rows=1000, most_shared=10, most_own=1 << 20), dict(sharing_groups=1), dict(sharing_groups=0)])
+def test_tcgen05_with_other_hints(hints, always_tcgen05):
+    c = Case([(3, 40, [1, 9, 30]), (50, 300, [2 + i for i in range(50)]), (7, 1300, [5] * 7)], 8, 2, 128, 16, BF16, other_tokens=1, scramble=True)
+    c.check(c.run(**hints))
+
+
+def test_tcgen05_large_scores(always_tcgen05):
+    """Scores in the hundreds, rising along the keys: the reference maximum moves again and again."""
+    c = Case([(20, 1500, [1 + i for i in range(20)])], 8, 2, 128, 16, BF16)
+    c.q.mul_(24.0)
+    c.v.mul_(64.0)
+    rise = torch.linspace(0.1, 4.0, c.k.shape[0], device=DEV).to(BF16)
+    order = torch.tensor(c.tables[0][:1500 // 16], device=DEV)
+    c.k[order] *= rise[:len(order), None, None, None]
+    for t in c.tables[1:]:                          # (the begun page is in every row's table)
+        assert t[:1500 // 16] == c.tables[0][:1500 // 16]
+    c.check(c.run())
+
+
+def test_tcgen05_the_same_bits_on_other_streams_and_in_a_graph(always_tcgen05):
+    c = Case([(20, 600, [1 + i for i in range(20)]), (30, 900, [1 + i for i in range(30)])], 8, 2, 128, 16, BF16)
+    first = c.run()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    outs = [torch.full_like(c.q, 7.0) for _ in range(8)]
+    for i, o in enumerate(outs[:6]):
+        with torch.cuda.stream(side if i % 2 else torch.cuda.current_stream()):
+            c.run(o)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.run(outs[6])
+        c.run(outs[7])
+    for _ in range(3):
+        outs[6].fill_(7.0)
+        outs[7].fill_(7.0)
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, first) for o in outs)
+    # the captured call on other lengths and groups: rows move to the first group, lengths shrink
+    c.groups.copy_(torch.tensor([[0, 600], [35, 333]], dtype=torch.int32))
+    lengths = c.kv_len.tolist()
+    c.kv_len[20:35] = torch.tensor([590] * 15, dtype=torch.int32)
+    c.kv_len[35:] -= 100
+    graph.replay()
+    torch.cuda.synchronize()
+    got = outs[6].clone()
+    # (rows 20 to 34 now read the first group's keys, no further than 590; the others their own from 333 on)
+    c.lengths = [lengths[i] if i < 20 else 590 if i < 35 else lengths[i] - 100 for i in range(50)]
+    c.tables = [t if i < 20 or i >= 35 else c.tables[0] for i, t in enumerate(c.tables)]
+    c.check(got)

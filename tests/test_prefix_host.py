@@ -64,8 +64,9 @@ def test_calls_go_where_they_are_served():
     assert (tiles, two, covered, sms) == (1, 1, 256, 148) and 8 * splits + ctas <= 148      # (side by side)
     floats, splits, _, tiles, two, covered, ctas, sms = plan(most_rows=32, n_rows=32)[1]
     assert (tiles, two, covered) == (1, 0, 128) and splits % 2 == 0 and 8 * splits // 2 + ctas <= 148      # one tile: a CTA leaves two parts
-    assert plan(most_rows=4)[0] == "mma" and plan(shared=352)[0] == "mma" and plan(dim=64)[0] == "mma"
-    assert plan(shared=353)[0] == "tcgen05" and plan(most_rows=8, shared=4065)[0] == "tcgen05" and plan(most_rows=8, shared=4064)[0] == "mma"
+    assert plan(most_rows=4)[0] == "mma" and plan(shared=416)[0] == "mma" and plan(dim=64)[0] == "mma"
+    assert plan(shared=417)[0] == "tcgen05" and plan(most_rows=8, shared=3489)[0] == "tcgen05" and plan(most_rows=8, shared=3488)[0] == "mma"
+    assert plan(most_rows=8, shared=4609)[0] == "mma" and plan(most_rows=8, shared=5793)[0] == "tcgen05"      # (a second step)
     assert plan(page=24)[0] == "mma"
     for other in (dict(dtype=torch.float32), dict(dim=72), dict(heads=17, kv_heads=1), dict(n_rows=400), dict(aligned=False)):
         assert plan(**other)[0] == "all sizes", other
