@@ -35,10 +35,10 @@ from .context import SharedPrefixes, StepContext, context_from_layout
 _DTYPES = {"bfloat16": torch.bfloat16, "float32": torch.float32}
 log = logging.getLogger("llm_infer_rust_b200")
 # Decode rows read the pages that they share once where that saves so many bytes of a layer's keys and values, summed over the rows.
-# (Decode attention / shared, us, at 8 KV heads of 128 in bfloat16, 4 KiB a key: 2 rows behind 16,384 keys, 64 MiB saved, 21.7 / 24.6; 4
-# behind 4,096, 48 MiB, 14.5 / 14.0; 8 behind 2,048, 56 MiB, 14.3 / 12.3; 16 behind 1,024, 60 MiB, 12.4 / 12.0; 48 behind 512, 94 MiB,
-# 23.4 / 15.0; 48 behind 16,384 438 / 33.)
-_SAVED_BYTES_AT_LEAST = 48 << 20
+# (Decode attention / shared, us, 16 heads on 8 KV heads of 128 in bfloat16, 4 KiB a key: 16 rows behind 512 keys, 30 MiB saved, 8.3 / 9.5; 2 rows
+# behind 8,192, 32 MiB, 14.7 / 14.9; 32 behind 300, 36 MiB, 12.0 / 10.3; 6 behind 2,048, 40 MiB, 14.2 / 10.0; 4 behind 4,096, 48 MiB, 14.6 /
+# 11.3; 16 behind 1,024, 60 MiB, 12.6 / 10.9; 2 behind 16,384, 64 MiB, 22.9 / 21.7; 48 behind 512, 94 MiB, 23.7 / 13.1; 48 behind 16,384 438 / 33.)
+_SAVED_BYTES_AT_LEAST = 32 << 20
 
 
 @dataclass
