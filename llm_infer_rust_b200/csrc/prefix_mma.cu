@@ -238,7 +238,7 @@ __device__ __forceinline__ void fetch_block_of(const PrefixCall& c, const Boxes&
       const int line = __shfl_sync(0xffffffffu, y, r8 >> boxes.log2_rows) + (r8 & ((1 << boxes.log2_rows) - 1)) + mine;
       const long long at = static_cast<long long>(line) * D + chunk * 8;
 #pragma unroll
-      for (int r = 0; r < 8; r += ROWS <= 8 && ROWS > 0 ? ROWS : 8) {
+      for (int r = 0; r < 8; r += ROWS <= 8 ? ROWS : 8) {
         const int row = r8 + r + mine;
         unsigned char* dst = tile + swz(row, chunk);
         cp_async16(dst, kc + at + r * D, row >= from && row < to);
