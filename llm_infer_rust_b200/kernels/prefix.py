@@ -160,20 +160,24 @@ def prefix_attention(q, k_cache, v_cache, out, block_table, cu_q, kv_len, rows, 
     if n_rows == 0:
         _refuse(*operands, *sizes, scale)
         return
-    ops._on_current(rows.device)
-    aligned = (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr() | out.data_ptr()) % 16 == 0
-    all_sizes, tcgen05, mma, plan, kernels = _plan(q.dtype, num_heads, num_kv_heads, head_dim, page_size, n_rows, groups.shape[0], most_rows,
-                                                   most_shared, most_own, groups.shape[0] if sharing_groups is None else sharing_groups, aligned,
-                                                   ops._sm_count(rows.device))
-    rc = _binding().prefix_attention(all_sizes, tcgen05, mma, *operands, *sizes, float(scale), plan, ops.error_word(rows.device), ops._stream())
+    device = rows.device
+    ops._on_current(device)
+    ends = (ops.error_word(device), ops._stream())
+    chosen = (q.dtype, num_heads, num_kv_heads, head_dim, page_size, n_rows, groups.shape[0], most_rows, most_shared, most_own,
+              groups.shape[0] if sharing_groups is None else sharing_groups)
+    sms, scale = ops._sm_count(device), float(scale)
+    all_sizes, tcgen05, mma, plan, kernels = _plan(*chosen, True, sms)
+    rc = _binding().prefix_attention(all_sizes, tcgen05, mma, *operands, *sizes, scale, plan, *ends)
     if rc is None:
-        # something is not as it should be, or this thread keeps a layer's calls (ops.LayerCalls), which the entry points take part in
+        # something is not as it should be, tensors are not aligned, or this thread keeps a layer's calls (ops.LayerCalls), which the entry
+        # points take part in
         _refuse(*operands, *sizes, scale)
-        floats, shared, own, tiles, two, covered, stream, sms = plan
-        scratch = ops._empty((floats,), torch.float32, rows.device)
+        aligned = (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr() | out.data_ptr()) % 16 == 0
+        all_sizes, tcgen05, mma, plan, kernels = _plan(*chosen, aligned, sms)
+        floats, shared, own, tiles, two, covered, stream, _ = plan
+        scratch = ops._empty((floats,), torch.float32, device)
         common = (scratch, block_table, block_table.shape[1], cu_q, kv_len, rows, n_rows, groups, groups.shape[0], num_heads, num_kv_heads, page_size,
-                  k_cache.shape[0], float(scale))
-        ends = (ops.error_word(rows.device), ops._stream())
+                  k_cache.shape[0], scale)
         if all_sizes is not None:
             rc = all_sizes(q, k_cache, v_cache, out, *common, shared, own, tiles, ops._code(q), head_dim, sms, *ends)
         else:

@@ -422,3 +422,19 @@ def test_tcgen05_the_same_bits_on_other_streams_and_in_a_graph(always_tcgen05):
     c.lengths = [lengths[i] if i < 20 else 590 if i < 35 else lengths[i] - 100 for i in range(50)]
     c.tables = [t if i < 20 or i >= 35 else c.tables[0] for i, t in enumerate(c.tables)]
     c.check(got)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("which", ["q", "k", "v", "out"])
+def test_tensors_off_16_bytes(which, dtype):
+    c = Case([(5, 100, [4, -40, 0, -100, 33]), (2, 13, [1, 2])], 8, 2, 128, 16, dtype)
+
+    def off(t):
+        there = torch.empty(t.numel() + 1, dtype=t.dtype, device=DEV)[1:].view(t.shape)
+        return there.copy_(t)
+    out = torch.full_like(c.q, 7.0)
+    if which == "out":
+        out = off(out)
+    else:
+        setattr(c, which, off(getattr(c, which)))
+    c.check(c.run(out))
