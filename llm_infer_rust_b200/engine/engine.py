@@ -311,7 +311,7 @@ class Engine:
     def fork_request(self, parent: int, children: Sequence[int]) -> None:
         """Make each of ``children`` live as a copy of ``parent`` as it is now: they hold its whole pages in common, and the page that it
         has begun (and the states that layers keep) is copied.  From here on every one of them goes its own way.  All of them or none:
-        without room for one of them nothing changes and a MemoryError says so.  ``parent`` is a request that ``open_request`` or a
+        without room for one of them nothing changes and a MemoryError says so, and where the copies fail no child is left either.  ``parent`` is a request that ``open_request`` or a
         fork has made live; decode steps of requests that share pages read those once where that pays."""
         mgr = self.cache.manager
         if not mgr.has(parent):
@@ -319,17 +319,22 @@ class Engine:
         children = [int(c) for c in children]
         if len(set(children)) != len(children) or any(mgr.has(c) for c in children):
             raise ValueError("a fork's children are requests that are not live yet, each named once")
-        copies = []
-        for n, child in enumerate(children):
-            got, pages, states = mgr.fork(parent, child)
-            if got != self._rt.Acquire.Ready:
-                for c in children[:n]:
-                    mgr.release(c)
-                raise MemoryError(f"request {parent} cannot be forked into {len(children)}: {got.name} for the {n + 1}th; nothing has changed; free "
-                                  f"pages per group: {[mgr.free_pages(g) for g in range(mgr.num_groups())]}, free state slots: {mgr.free_state_slots()}")
-            copies.append((pages, states))
-        if copies:
-            self.cache.copy_fork(copies)
+        copies: List[tuple] = []
+        try:
+            for child in children:
+                got, pages, states = mgr.fork(parent, child)
+                if got != self._rt.Acquire.Ready:
+                    raise MemoryError(f"request {parent} cannot be forked into {len(children)}: {got.name} for the {len(copies) + 1}th")
+                copies.append((pages, states))
+            if copies:
+                self.cache.copy_fork(copies)
+        except BaseException as e:
+            for child in children[:len(copies)]:
+                mgr.release(child)
+            if isinstance(e, MemoryError):
+                raise MemoryError(f"{e}; nothing has changed; free pages per group: {[mgr.free_pages(g) for g in range(mgr.num_groups())]}, "
+                                  f"free state slots: {mgr.free_state_slots()}") from None
+            raise
 
     def request_length(self, request: int) -> int:
         return self.cache.manager.length(request)

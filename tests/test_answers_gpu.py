@@ -367,3 +367,20 @@ def test_layers_whose_calls_are_made_again(head_dim, dtype):
         prefix.prefix_attention, ops.LayerCalls.again = inner, inner_again
     assert torch.equal(got, want)
     eng.check_kernel_errors()
+
+
+def test_answers_whose_copies_fail_leave_nothing(folders, monkeypatch):
+    from llm_infer_rust_b200 import SamplingParams
+    folder, _ = folders("A", "float32")
+    eng = engine(folder, dtype="float32", page_size=4)
+    free = eng.cache.manager.free_pages(0)
+
+    def fails(copies):
+        raise RuntimeError("the copies fail")
+    with monkeypatch.context() as m:
+        m.setattr(eng.cache, "copy_fork", fails)
+        with pytest.raises(RuntimeError, match="the copies fail"):
+            eng.answers(tokens(256, 30, 2), 4, SamplingParams(max_tokens=5, ignore_eos=True))
+    mgr = eng.cache.manager
+    assert mgr.live_requests() == 0 and mgr.free_pages(0) == free and mgr.shared_pages(0) == 0 and mgr.check() == ""
+    assert len(eng.answers(tokens(256, 30, 2), 4, SamplingParams(max_tokens=5, ignore_eos=True))) == 4

@@ -232,3 +232,30 @@ def test_groups_with_a_window_are_not_looked_in():
     m.fork(1, 2)
     with pytest.raises(Exception, match="keeps all keys"):
         batch(m, [1, 2], prefix_group=1)
+
+
+@pytest.mark.parametrize("error", [RuntimeError("the copies fail"), KeyboardInterrupt(), MemoryError("no room for a table")])
+def test_no_child_is_left_where_the_copies_fail(error):
+    from types import SimpleNamespace
+    from llm_infer_rust_b200.engine import Engine
+    m = manager([30, 20], window=[0, 9], slots=6)
+    m.open(1)
+    hold(m, 1, 14)
+    free = [m.free_pages(g) for g in range(2)], m.free_state_slots()
+
+    def fails(copies):
+        assert len(copies) == 3
+        raise error
+    engine = SimpleNamespace(cache=SimpleNamespace(manager=m, copy_fork=fails), _rt=rt)
+    with pytest.raises(type(error)):
+        Engine.fork_request(engine, 1, [2, 3, 4])
+    assert m.live_requests() == 1 and ([m.free_pages(g) for g in range(2)], m.free_state_slots()) == free
+    assert m.shared_pages(0) == m.shared_pages(1) == 0 and m.check() == ""
+    # too few slots for all of them: none is made, and nothing is copied
+    engine.cache.copy_fork = lambda copies: pytest.fail("copied")
+    with pytest.raises(MemoryError, match="for the 6th; nothing has changed"):
+        Engine.fork_request(engine, 1, list(range(2, 9)))
+    assert m.live_requests() == 1 and m.shared_pages(0) == 0 and m.check() == ""
+    engine.cache.copy_fork = lambda copies: None
+    Engine.fork_request(engine, 1, [2, 3, 4])
+    assert m.live_requests() == 4 and m.check() == ""
