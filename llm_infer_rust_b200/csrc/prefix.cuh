@@ -115,10 +115,12 @@ __device__ __forceinline__ float prefix_exp2(float x) {      // 2^x, one special
 // One vector out of its `count` parts, rows of PITCH floats of which `hd` are the head's: the CTA's warps share the parts, up to BATCH of them a
 // turn, maxima and sums asked for together with the outputs that they weight, for what this takes is a few answers from the
 // second-level cache one behind the other.  `where`: the place of part p's maximum and sum, and of its outputs.  `left`: shared memory.
+// CHECKED: false, and nothing written, where an output or a sum is no number or an infinity, or an output is below 2^-80 and not zero (the
+// largest weight behind each is 1).
 template <int PITCH, int WARPS>
 struct JoinShared { float row[WARPS][PITCH + 4]; };
-template <int PITCH, int WARPS, typename T, typename Where>
-__device__ __forceinline__ void join_parts(T* __restrict__ dst, int hd, int count, const Where& where, JoinShared<PITCH, WARPS>& left) {
+template <int PITCH, int WARPS, bool CHECKED = false, typename T, typename Where>
+__device__ __forceinline__ bool join_parts(T* __restrict__ dst, int hd, int count, const Where& where, JoinShared<PITCH, WARPS>& left) {
   constexpr int PER = (PITCH + 127) / 128, BATCH = PER == 1 ? 8 : PER == 2 ? 4 : 2;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float4 o[PER];
@@ -169,7 +171,16 @@ __device__ __forceinline__ void join_parts(T* __restrict__ dst, int hd, int coun
   for (int n = 0; n < PER; ++n)
     if (PITCH % 128 == 0 || n * 128 + lane * 4 < PITCH) *reinterpret_cast<float4*>(left.row[warp] + n * 128 + lane * 4) = o[n];
   if (lane == 0) { left.row[warp][PITCH] = m; left.row[warp][PITCH + 1] = l; }
-  __syncthreads();
+  if constexpr (CHECKED) {
+    bool settled = fabsf(l) < INFINITY;
+    const auto look = [&](float x) { settled = settled && fabsf(x) < INFINITY && (fabsf(x) >= 8.2718061e-25f || x == 0.0f); };
+#pragma unroll
+    for (int n = 0; n < PER; ++n)
+      if (PITCH % 128 == 0 || n * 128 + lane * 4 < PITCH) { look(o[n].x); look(o[n].y); look(o[n].z); look(o[n].w); }
+    if (__syncthreads_or(!settled)) return false;
+  } else {
+    __syncthreads();
+  }
   const int warps = min(WARPS, (count + BATCH - 1) / BATCH);      // that had parts
   float most = -INFINITY, sum = 0.0f;
   for (int w = 0; w < warps; ++w) most = fmaxf(most, left.row[w][PITCH]);
@@ -187,6 +198,7 @@ __device__ __forceinline__ void join_parts(T* __restrict__ dst, int hd, int coun
     dst[dim] = from_f32<T>(x * inv);
     dst[dim + 1] = from_f32<T>(y * inv);
   }
+  return true;
 }
 // Warps of a CTA that joins one of `vectors` vectors.  Few vectors have many parts each, a hundred and more where one prompt's keys are all there
 // is: then all of them at once, while an SM has a CTA.  Many have a dozen, and all vectors are to be on the SMs at once.  (4 / 16 warps: two

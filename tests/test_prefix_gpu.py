@@ -438,3 +438,83 @@ def test_tensors_off_16_bytes(which, dtype):
     else:
         setattr(c, which, off(getattr(c, which)))
     c.check(c.run(out))
+
+
+def by_definition(c):
+    """Every row's outputs in 64 bits, NaN and infinities as the definition has them, and how far they may be off: as at the top of this
+    file, with the largest value of each dim that is no infinity."""
+    q, k, v = c.q.double().cpu(), c.k.double().cpu(), c.v.double().cpu()
+    per, found = c.nh // c.nkv, []
+    for i, (t, length) in enumerate(zip(c.tables, c.lengths)):
+        token = c.cu_q.tolist()[c.batch[i]]
+        at = torch.arange(length)
+        pages = torch.tensor(t)[at // c.page]
+        kk, vv = k[pages, :, at % c.page], v[pages, :, at % c.page]
+        s = torch.einsum("hqd,lhd->hql", q[token].view(c.nkv, per, c.d), kk) * c.scale
+        want = torch.einsum("hql,lhd->hqd", torch.softmax(s, -1), vv)
+        sizes = torch.einsum("hqd,lhd->hql", q[token].view(c.nkv, per, c.d).abs(), kk.abs())
+        e = (c.d + 4) * 2.0 ** -24 * float(sizes[sizes.isfinite()].max()) * c.scale
+        most = vv.abs().masked_fill(vv.isinf(), 0.0).amax(0)[:, None]                   # [nkv, 1, d]
+        bound = 2 * (math.exp(e) - 1 + 2.0 ** -21 + (length + 64) * 2.0 ** -24) * most
+        if c.dtype == BF16:
+            bound = bound + 2.0 ** -8 * most + 2.0 ** -8 * want.abs()
+        # (a result below the smallest normal number has the last place of those)
+        found.append((token, want, bound + length * torch.finfo(c.dtype).smallest_normal * torch.finfo(c.dtype).eps))
+    return found
+
+
+def agrees(c, out):
+    for token, want, bound in by_definition(c):
+        got = out[token].double().cpu().view(want.shape)
+        assert torch.equal(got.isnan(), want.isnan()), token
+        assert torch.equal(got.isposinf(), want.isposinf()) and torch.equal(got.isneginf(), want.isneginf()), token
+        some = want.isfinite()
+        assert ((got - want).abs() <= bound)[some].all(), (token, float(((got - want).abs() / bound)[some].max()))
+
+
+# (groups, nh, nkv, d, page, dtype): every kernel
+ODD_VALUES = {
+    "float32": ([(6, 200, [1, 5, 9, 2, 2, 40])], 8, 2, 64, 16, F32),
+    "float32, two tiles of vectors": ([(20, 200, [1 + i for i in range(20)])], 8, 2, 128, 16, F32),
+    "float32, heads of 30": ([(6, 200, [1, 5, 9, 2, 2, 40])], 8, 2, 30, 16, F32),
+    "float32, heads of 512": ([(6, 200, [1, 5, 9, 2, 2, 40])], 4, 2, 512, 16, F32),
+    "bfloat16, all sizes": ([(6, 200, [1, 5, 9, 2, 2, 40])], 34, 2, 64, 16, BF16),
+    "mma": ([(6, 200, [1, 5, 9, 2, 2, 40])], 8, 2, 64, 16, BF16),
+    "tcgen05": ([(40, 2600, [1 + i for i in range(40)])], 32, 8, 128, 16, BF16),
+    "tcgen05, two tiles": ([(80, 1100, [1 + i for i in range(80)])], 32, 8, 128, 16, BF16),
+}
+
+
+@pytest.mark.parametrize("name", list(ODD_VALUES))
+def test_infinities_among_keys_and_values(name):
+    c = Case(*ODD_VALUES[name])
+    inf = float("inf")
+
+    def put(cache, row, key, head, dim, value):
+        cache[c.tables[row][key // c.page], head, key % c.page, dim] = value
+    c.q.view(len(c.q), c.nh, c.d)[..., 3] = c.q.view(len(c.q), c.nh, c.d)[..., 3].abs() + 0.5
+    put(c.k, 0, 17, 0, 3, -inf)                      # a shared key that no row's weight falls on
+    put(c.k, 5, c.lengths[5] - 2, 0, 3, -inf)        # an own one
+    put(c.k, 4, c.lengths[4] - 1, 1, 3, inf)         # one that takes all of the weight: no distribution
+    put(c.v, 0, 40, 0, 5, inf)
+    put(c.v, 0, 41, 0, 7, -inf)
+    put(c.v, 0, 42, 0, 9, inf)
+    put(c.v, 0, 43, 0, 9, -inf)                      # (the sum of both is none)
+    put(c.v, 3, c.lengths[3] - 1, 1, 0, -inf)
+    want = by_definition(c)
+    assert want[4][1][1].isnan().all() and want[3][1][1, :, 0].isneginf().all() and want[0][1][0, :, 9].isnan().all() and want[0][1][1].isfinite().all()
+    agrees(c, c.run())
+
+
+@pytest.mark.parametrize("name", [n for n in ODD_VALUES if "mma" not in n and "tcgen05" not in n])
+def test_the_largest_and_the_smallest_floats(name):
+    """Floats that rounding to 11 bits would carry beyond the largest one, and those whose rest would be lost below the smallest."""
+    c = Case(*ODD_VALUES[name])
+    largest = torch.finfo(c.dtype).max
+    key = (c.tables[0][2], 1, 5)
+    c.q.view(len(c.q), c.nh, c.d)[..., 4] = 2.0 ** -124
+    c.k[key][4] = largest
+    c.v[key][6] = largest
+    c.v[key][8] = -largest
+    c.v[..., 11] *= 2.0 ** -122
+    agrees(c, c.run())
