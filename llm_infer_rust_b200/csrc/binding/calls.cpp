@@ -353,7 +353,13 @@ PyObject* prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       !THPVariable_Check(args[18]) || !THPVariable_Unpack(args[18]).is_cuda())
     Py_RETURN_NONE;
   const auto address = [](const at::Tensor& x) { return reinterpret_cast<I>(x.const_data_ptr()); };
-  if (entry[2] != nullptr && ((address(q) | address(out) | address(k) | address(v)) & 15) != 0) Py_RETURN_NONE;
+  if (entry[2] != nullptr) {
+    // (what the tensor-core kernels cannot take is the all-sizes kernel's: the wrapper sends it there)
+    const I places = table.size(1) * page, items = (rows.size(0) * (heads / kv_heads) + 15) / 16 + groups.size(0) + rows.size(0);
+    if (((address(q) | address(out) | address(k) | address(v)) & 15) != 0 || k.size(0) * kv_heads * page > INT32_MAX ||
+        places > (1 << 30) || (places / 32 + 2) * kv_heads * items > INT32_MAX / 2)
+      Py_RETURN_NONE;
+  }
   I* const err = reinterpret_cast<I*>(THPVariable_Unpack(args[18]).mutable_data_ptr());
   const float floats[MAX_FLOATS] = {static_cast<float>(scale)};
   int rc = 0;

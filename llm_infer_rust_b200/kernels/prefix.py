@@ -74,15 +74,15 @@ def _share_sms(steps: int, two: int, tiles: int, items: int, most_own: int, key_
 
 @functools.lru_cache(maxsize=4096)
 def _plan(dtype, heads: int, kv_heads: int, dim: int, page: int, n_rows: int, n_groups: int, most_rows: int, most_shared: int, most_own: int,
-          sharing: int, aligned: bool, sms: int) -> tuple:
+          sharing: int, taken: bool, sms: int) -> tuple:
     """The entry points that a call goes to (all sizes, tcgen05, mma.sync; None: not this one), its sizes as the binding takes them, and
-    its launches."""
+    its launches.  ``taken``: its tensors are aligned and counted as the tensor-core kernels take them."""
     per = heads // kv_heads
     most_rows = max(1, min(most_rows, n_rows))
     vectors = most_rows * per
     sharing = max(1, min(sharing, n_groups))
     # (pages of any size: powers of two in what decode attention asks for and the tcgen05 kernel fetches, not here)
-    if not aligned or not ops.decode_uses_tensor_cores(dtype, heads, kv_heads, dim, 1) or n_rows + n_groups > _MOST_ENTRIES:
+    if not taken or not ops.decode_uses_tensor_cores(dtype, heads, kv_heads, dim, 1) or n_rows + n_groups > _MOST_ENTRIES:
         lib = load_entry_points("prefix_attention.cu", {"HEAD_DIM": ops.padded_head_dim(dim)})
         tiles = -(-vectors // _TILE)
         per_sm = max(1, 227 * 1024 // (lib.b200_prefix_attention_smem() + 1024))
@@ -107,6 +107,14 @@ def _plan(dtype, heads: int, kv_heads: int, dim: int, page: int, n_rows: int, n_
     count.restype = ctypes.c_longlong
     floats = count(n_rows, n_groups, heads, kv_heads, shared, stream)
     return None, tcgen05, lib.b200_prefix_attention_mma, (floats, shared, 0, tiles, two, covered, stream, sms), 2 + (tcgen05 is not None)
+
+
+def _counts(k_cache, block_table, n_rows: int, n_groups: int, num_heads: int, num_kv_heads: int, page_size: int) -> bool:
+    """Whether the tensor-core kernels, which count a cache's rows and a call's blocks of keys in 32 bits, can count a call's (as
+    ``prefix_attention`` of csrc/binding/calls.cpp asks)."""
+    places = block_table.shape[1] * page_size
+    items = -(-n_rows * (num_heads // num_kv_heads) // 16) + n_groups + n_rows
+    return k_cache.shape[0] * num_kv_heads * page_size < 1 << 31 and (places // 32 + 2) * num_kv_heads * items < 1 << 30
 
 
 def _refuse(q, k_cache, v_cache, out, block_table, cu_q, kv_len, rows, groups, num_heads, num_kv_heads, head_dim, page_size, scale) -> None:
@@ -169,11 +177,12 @@ def prefix_attention(q, k_cache, v_cache, out, block_table, cu_q, kv_len, rows, 
     all_sizes, tcgen05, mma, plan, kernels = _plan(*chosen, True, sms)
     rc = _binding().prefix_attention(all_sizes, tcgen05, mma, *operands, *sizes, scale, plan, *ends)
     if rc is None:
-        # something is not as it should be, tensors are not aligned, or this thread keeps a layer's calls (ops.LayerCalls), which the entry
-        # points take part in
+        # something is not as it should be, the tensor-core kernels cannot take the call, or this thread keeps a layer's calls
+        # (ops.LayerCalls), which the entry points take part in
         _refuse(*operands, *sizes, scale)
-        aligned = (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr() | out.data_ptr()) % 16 == 0
-        all_sizes, tcgen05, mma, plan, kernels = _plan(*chosen, aligned, sms)
+        taken = (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr() | out.data_ptr()) % 16 == 0 and \
+            _counts(k_cache, block_table, n_rows, groups.shape[0], num_heads, num_kv_heads, page_size)
+        all_sizes, tcgen05, mma, plan, kernels = _plan(*chosen, taken, sms)
         floats, shared, own, tiles, two, covered, stream, _ = plan
         scratch = ops._empty((floats,), torch.float32, device)
         common = (scratch, block_table, block_table.shape[1], cu_q, kv_len, rows, n_rows, groups, groups.shape[0], num_heads, num_kv_heads, page_size,

@@ -518,3 +518,26 @@ def test_the_largest_and_the_smallest_floats(name):
     c.v[key][8] = -largest
     c.v[..., 11] *= 2.0 ** -122
     agrees(c, c.run())
+
+
+def test_tables_and_caches_beyond_what_the_tensor_core_kernels_count():
+    """They count in 32 bits; the all-sizes kernel takes the rest."""
+    c = Case([(2, 300, [5, 130])], 16, 8, 64, 128, BF16)
+    small = c.table
+    c.table = torch.zeros(2, 1 << 23, dtype=torch.int32, device=DEV)          # 2^30 places
+    c.table[:, :small.shape[1]] = small
+    c.check(c.run())
+    # 2^31 rows of keys, the call's pages the last ones
+    c = Case([(3, 300, [5, 130, 0])], 16, 8, 16, 128, BF16)
+    c.v = c.k
+    pages = (1 << 21) + 5
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("64 GiB of keys")
+    small, first = c.k, pages - c.k.shape[0]
+    c.k = c.v = torch.empty((pages,) + tuple(small.shape[1:]), dtype=BF16, device=DEV)
+    c.k[first:] = small
+    c.table += first
+    out = c.run()
+    c.k = c.v = small
+    torch.cuda.empty_cache()
+    c.check(out)

@@ -154,3 +154,13 @@ def test_options_of_the_command_line(capsys):
     for bad in (["--answers", "0"], ["--answers", "9", "--max-running-req", "8"], ["--logprobs", "33"], ["--logprobs", "-1"]):
         assert cli.main(["--model-path", "x", "--prompt-ids", "1"] + bad) == 2
     assert "--answers" in cli.USAGE and "--logprobs" in cli.USAGE
+
+
+def test_calls_that_the_tensor_core_kernels_cannot_count():
+    def counts(pages=1000, kv_heads=8, page=16, width=100, n_rows=4, n_groups=1, heads=32):
+        return prefix._counts(torch.empty(pages, kv_heads, page, 1, device="meta"), torch.empty(n_rows, width, device="meta"), n_rows, n_groups, heads,
+                              kv_heads, page)
+    assert counts() and counts(pages=2 ** 24 - 1) and not counts(pages=2 ** 24)
+    items = 1 + 1 + 4                                          # tiles of 16 vectors, groups, rows
+    most = (2 ** 30 - 1) // (8 * items) - 2                    # blocks of a row
+    assert counts(width=2 * most) and not counts(width=2 * (most + 1))
