@@ -1,6 +1,8 @@
 #include "batch_builder.h"
 
 #include <algorithm>
+#include <cstring>
+#include <iterator>
 #include <stdexcept>
 #include <string>
 
@@ -11,36 +13,93 @@ static int align4(int n) { return (n + 3) & ~3; }
 namespace {
 struct Shared {
   std::vector<int> rows;      // of the batch
-  int keys = 0;               // whole pages that all of them hold
+  int keys = 0;               // that all of them hold in whole pages (of a division: those pages)
 };
-// Decode rows whose first page is the same one, with at least two rows: each such set shares the pages that all of its rows hold.
+struct Held { int row, pages; const std::vector<int>* table; };      // a decode row, its whole pages
+
+// Rows divided into sets that share pages, and those left over.
+struct Division {
+  std::vector<Shared> sets;
+  std::vector<int> loose;
+  int64_t saved = 0;          // pages that the sets' rows need not read again
+};
+// Rows [begin, end), which hold the same first `depth` pages.  Where they part, those of a branch form sets by themselves if that saves more
+// than sharing what all have in common, which the others do; so no row takes from the others what they share, and what is saved is
+// no less than in one set.
+Division divide(std::vector<Held>::iterator begin, std::vector<Held>::iterator end, int depth) {
+  Division d;
+  if (end - begin < 2) {
+    for (auto i = begin; i != end; ++i) d.loose.push_back(i->row);
+    return d;
+  }
+  const int* lead = begin->table->data();
+  int common = begin->pages;
+  for (auto i = begin + 1; i != end; ++i) {
+    const int* pages = i->table->data();
+    common = std::min(common, i->pages);
+    if (std::memcmp(lead + depth, pages + depth, sizeof(int) * (common - depth)) != 0)      // (as a rule they are the same, and this is quicker)
+      common = static_cast<int>(std::mismatch(lead + depth, lead + common, pages + depth).first - lead);
+  }
+  depth = common;
+  // the branches: rows that end here are one each
+  const auto page_of = [&](const Held& h) { return h.pages > depth ? (*h.table)[depth] : 0; };
+  std::stable_sort(begin, end, [&](const Held& a, const Held& b) { return page_of(a) < page_of(b); });
+  std::vector<Division> branches;
+  std::vector<char> apart;                       // whether a branch forms sets by itself
+  std::vector<int> staying;
+  int64_t saved = 0, saved_apart = 0;
+  for (auto i = begin, j = i; i != end; i = j) {
+    for (j = i + 1; j != end && page_of(*i) != 0 && page_of(*j) == page_of(*i); ++j) {}
+    branches.push_back(divide(i, j, std::min(depth + 1, i->pages)));
+    const Division& b = branches.back();
+    apart.push_back(b.saved + static_cast<int64_t>(b.loose.size()) * depth > static_cast<int64_t>(j - i) * depth);
+    saved_apart += b.saved;
+    if (apart.back()) {
+      saved += b.saved;
+      staying.insert(staying.end(), b.loose.begin(), b.loose.end());
+    } else {
+      for (auto x = i; x != j; ++x) staying.push_back(x->row);
+    }
+  }
+  saved += (static_cast<int64_t>(staying.size()) - 1) * depth;
+  const bool set_here = staying.size() > 1 && saved >= saved_apart;
+  for (size_t x = 0; x < branches.size(); ++x) {
+    Division& b = branches[x];
+    if (set_here && !apart[x]) continue;
+    std::move(b.sets.begin(), b.sets.end(), std::back_inserter(d.sets));
+    if (!set_here) d.loose.insert(d.loose.end(), b.loose.begin(), b.loose.end());
+  }
+  if (set_here) {
+    std::sort(staying.begin(), staying.end());
+    d.sets.push_back({std::move(staying), depth});
+  }
+  d.saved = set_here ? saved : saved_apart;
+  return d;
+}
+
+// Sets of decode rows that hold the same first pages, at least two rows each.
 std::vector<Shared> shared_rows(const CacheManager& cache, const BatchRequest& req) {
   std::vector<Shared> found;
   const int g = req.prefix_group;
   if (g < 0) return found;
   if (g >= cache.num_groups() || cache.group(g).window != 0) throw std::invalid_argument("rows share pages of a group that keeps all keys");
   if (cache.shared_pages(g) == 0) return found;
-  std::vector<std::pair<int, int>> first;      // (first page, row)
+  const int P = cache.group(g).page_size;
+  std::vector<Held> held;
   for (int r = 0; r < static_cast<int>(req.ids.size()); ++r) {
     if (req.counts[r] != 1) continue;
     const std::vector<int>& table = cache.block_table(req.ids[r], g);
-    if (!table.empty() && cache.length(req.ids[r]) >= cache.group(g).page_size) first.emplace_back(table[0], r);
+    const int pages = std::min(cache.length(req.ids[r]) / P, static_cast<int>(table.size()));
+    if (pages > 0) held.push_back({r, pages, &table});
   }
-  std::stable_sort(first.begin(), first.end(), [](const std::pair<int, int>& a, const std::pair<int, int>& b) { return a.first < b.first; });
-  const int P = cache.group(g).page_size;
-  for (size_t i = 0, j; i < first.size(); i = j) {
-    Shared s;
-    const std::vector<int>& lead = cache.block_table(req.ids[first[i].second], g);
-    int pages = cache.length(req.ids[first[i].second]) / P;
-    for (j = i; j < first.size() && first[j].first == first[i].first; ++j) {
-      const std::vector<int>& table = cache.block_table(req.ids[first[j].second], g);
-      const int most = std::min(pages, cache.length(req.ids[first[j].second]) / P);
-      pages = static_cast<int>(std::mismatch(lead.begin(), lead.begin() + most, table.begin()).first - lead.begin());
-      s.rows.push_back(first[j].second);
-    }
-    s.keys = pages * P;
-    if (s.rows.size() > 1) found.push_back(std::move(s));
+  const auto first = [](const Held& h) { return h.table->front(); };
+  std::stable_sort(held.begin(), held.end(), [&](const Held& a, const Held& b) { return first(a) < first(b); });
+  for (auto i = held.begin(), j = i; i != held.end(); i = j) {
+    for (j = i + 1; j != held.end() && first(*j) == first(*i); ++j) {}
+    std::vector<Shared> sets = divide(i, j, 1).sets;
+    std::move(sets.begin(), sets.end(), std::back_inserter(found));
   }
+  for (Shared& s : found) s.keys *= P;
   return found;
 }
 }  // namespace

@@ -33,7 +33,8 @@ struct BatchLayout {
   std::vector<int> off_table;     // per group: block table [num_rows, table_width]
   std::vector<int> table_width;   // per group
   // Decode rows that hold the same first pages, for attention that reads them once (kernels/prefix.py); 0 groups: none was looked for
-  // or found.  The last group shares nothing and holds the other decode rows.
+  // or found.  Rows that share some pages and part further on are divided so that the most keys are saved.  The last group shares nothing and
+  // holds the other decode rows.
   int num_prefix_groups = 0;
   int off_prefix_rows = 0;        // the decode rows, group by group
   int off_prefix_groups = 0;      // (index of the group's first row, shared keys) of each group

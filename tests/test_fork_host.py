@@ -259,3 +259,80 @@ def test_no_child_is_left_where_the_copies_fail(error):
     engine.cache.copy_fork = lambda copies: None
     Engine.fork_request(engine, 1, [2, 3, 4])
     assert m.live_requests() == 4 and m.check() == ""
+
+
+def test_a_row_that_parted_early_takes_the_sharing_from_no_one():
+    """Many answers behind a long prompt, and one conversation more that left it after its first page."""
+    m = manager(400, slots=20)
+    m.open(1)
+    hold(m, 1, 5)
+    m.fork(1, 2)                                              # one page in common
+    hold(m, 1, 103)
+    for c in range(3, 13):
+        m.fork(1, c)                                          # 25
+    layout, out, _ = batch(m, [2, 1] + list(range(3, 13)), prefix_group=0)
+    assert groups_of(layout, out) == [(list(range(1, 12)), 100), ([0], 0)]
+    req = rt.BatchRequest()
+    req.ids, req.counts, req.tokens, req.want_counts, req.want_index = [2, 1, 3], [1] * 3, [0] * 3, [1] * 3, [0] * 3
+    req.prefix_group = 0
+    assert rt.count_prefix_groups(m, req) == (1, 100, 100, 6)
+
+
+def test_several_that_parted_early_share_what_they_have():
+    m = manager(400, slots=20)
+    m.open(1)
+    hold(m, 1, 41)
+    for c in (2, 3, 4):
+        m.fork(1, c)                                          # ten pages
+        hold(m, c, 45)                                        # (and a page of its own)
+    hold(m, 1, 85)
+    for c in range(5, 10):
+        m.fork(1, c)                                          # 21
+    layout, out, _ = batch(m, list(range(1, 10)), prefix_group=0)
+    assert sorted(groups_of(layout, out)) == sorted([([0, 4, 5, 6, 7, 8], 84), ([1, 2, 3], 40), ([], 0)])
+
+
+def test_random_trees_of_forks_against_all_ways_of_dividing_their_rows():
+    from functools import lru_cache
+    rng, optimal = random.Random(11), 0
+    for turn in range(40):
+        m = manager(2000, slots=10)
+        m.open(1)
+        hold(m, 1, rng.randint(1, 30))
+        live = [1]
+        while len(live) < 6:
+            if rng.random() < 0.5:
+                m.fork(rng.choice(live), len(live) + 1)
+                live.append(len(live) + 1)
+            else:
+                r = rng.choice(live)
+                hold(m, r, m.length(r) + rng.randint(1, 14))
+        tables = [m.block_table(r, 0)[:m.length(r) // 4] for r in live]
+        layout, out, _ = batch(m, live, prefix_group=0)
+        found = groups_of(layout, out)[:-1] if layout.num_prefix_groups else []
+
+        @lru_cache(None)
+        def shared(rows):
+            n = 0
+            while all(len(tables[r]) > n for r in rows) and len({tables[r][n] for r in rows}) == 1:
+                n += 1
+            return n
+
+        @lru_cache(None)
+        def best(rows):                                       # (all divisions of a set)
+            if len(rows) < 2:
+                return 0
+            lead, rest = rows[0], rows[1:]
+            most = 0
+            for pick in range(1 << len(rest)):
+                mine = (lead,) + tuple(r for i, r in enumerate(rest) if pick >> i & 1)
+                most = max(most, (len(mine) - 1) * shared(mine) + best(tuple(r for i, r in enumerate(rest) if not pick >> i & 1)))
+            return most
+        for rows, keys in found:
+            assert len(rows) > 1 and keys == 4 * shared(tuple(rows)) > 0
+        assert sorted(r for rows, _ in groups_of(layout, out) for r in rows) == list(range(6)) if found else True
+        saved, most = sum((len(rows) - 1) * keys for rows, keys in found) // 4, best(tuple(range(6)))
+        assert saved >= 5 * shared(tuple(range(6))) and saved >= 0.8 * most, (turn, saved, most)
+        optimal += saved == most
+        assert m.check() == ""
+    assert optimal >= 35
