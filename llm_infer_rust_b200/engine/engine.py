@@ -77,6 +77,14 @@ def graph_batch_sizes(limit: int) -> List[int]:
     return sorted(sizes)
 
 
+def prefix_group(model, plan) -> int:
+    """The cache group in which rows that share pages are looked for: one that keeps all keys, and with a mixer that reads shared keys once
+    (-1: there is none)."""
+    readers = {g for e, g in plan.group_of_entry.items()
+               if getattr(model.blocks[model.run_list[e].layer].mixer, "reads_shared_prefixes", False)}
+    return min((g for g in readers if not plan.groups[g].window), default=-1)
+
+
 class _MetaBuffers:
     """Pinned staging buffers (a small ring) and the device copy of a step's index arrays."""
 
@@ -265,7 +273,7 @@ class Engine:
         self._shape_graph_limit = 6
         # Requests that share pages (forks): which cache group they are looked for in, and the graphs of their decode steps, keyed by
         # (rows, places for groups, shared keys, own keys), the keys rounded up to powers of two and of four.
-        self._prefix_group = next((g for g, group in enumerate(self.cache_plan.groups) if not group.window), -1)
+        self._prefix_group = prefix_group(self.model, self.cache_plan)
         group = self.cache_plan.groups[self._prefix_group] if self._prefix_group >= 0 else None
         self._key_bytes = max(1, group.bytes_per_page // (group.page_size * max(1, len(group.entries)))) if group is not None else 1
         self._prefix_graphs: "OrderedDict[tuple, _DecodeGraph]" = OrderedDict()

@@ -138,6 +138,7 @@ class GQAttention(Part):
     """
     category = "mixer"
     chainable = True          # reads its input through ops.* only, and may return a product that still waits (ops.few_row_linear)
+    reads_shared_prefixes = True
 
     def __init__(self, spec, env):
         super().__init__(spec, env)

@@ -14,8 +14,9 @@ Categories and the interface each must have:
 ``mixer``             ``forward(x, ctx, cache) -> y``; ``cache_spec()`` (paged keys and
                       values it needs, or None); ``state_spec()`` (fixed-size
                       per-request state it needs, or None); optionally ``state_specs()`` (several, by name:
-                      ``mixer_state(cache, name)`` gives the tensor) and ``children()`` (parts inside the part, by
-                      name: their parameters' paths continue the part's own)
+                      ``mixer_state(cache, name)`` gives the tensor), ``children()`` (parts inside the part, by
+                      name: their parameters' paths continue the part's own) and ``reads_shared_prefixes = True`` (decode rows
+                      that share pages read those once, by ``ctx.shared``: nobody looks for such rows without a mixer that does)
 ``feed_forward``      ``forward(x) -> y``
 ``token_conv``        ``forward(x, scale, ctx, state, out_dtype) -> y`` (a convolution over time whose last
                       inputs are per-request state); ``state_spec()``

@@ -29,6 +29,7 @@ class ParallelMixers(Part):
         if any(m.state_spec() is not None for m in (self.left, self.right)):
             raise ValueError("mixers side by side name their states (state_specs)")
         self.paged = paged[0] if paged else None
+        self.reads_shared_prefixes = getattr(self.paged, "reads_shared_prefixes", False)
         self.joint = None              # (packed weights of both branches, first row of the right one)
 
     def children(self):

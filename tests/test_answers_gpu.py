@@ -384,3 +384,32 @@ def test_answers_whose_copies_fail_leave_nothing(folders, monkeypatch):
     mgr = eng.cache.manager
     assert mgr.live_requests() == 0 and mgr.free_pages(0) == free and mgr.shared_pages(0) == 0 and mgr.check() == ""
     assert len(eng.answers(tokens(256, 30, 2), 4, SamplingParams(max_tokens=5, ignore_eos=True))) == 4
+
+
+@pytest.mark.parametrize("name", ["K1", "K4"])
+def test_layers_that_read_every_row_by_itself_have_no_graphs_of_shared_pages(name, tmp_path):
+    """Their forks decode in the graphs that are there."""
+    from llm_infer_rust_b200.engine import StepEntry
+    raw = K.CONFIGS[name]
+    w = K.random_weights(raw, 3)
+    eng = K.make_engine(K.write_model(str(tmp_path / "m"), raw, w), "bfloat16", max_requests=4, cuda_graph_bs=4)
+    captures = []
+    capture = eng._capture
+    eng._capture = lambda *a: captures.append(a) or capture(*a)
+    prompt = K.tokens(raw["vocab"], 41, 5)
+    eng.open_request(1)
+    eng.step([StepEntry(1, prompt, [])])
+    eng.fork_request(1, [2, 3])
+    seq = {r: list(prompt) for r in (1, 2, 3)}
+    for step in range(4):
+        entries = []
+        for r in seq:
+            new = K.tokens(raw["vocab"], 1, 50 * step + r)
+            seq[r] += new
+            entries.append(StepEntry(r, new, [0]))
+        got = eng.step(entries).float().cpu().numpy()
+        for row, r in zip(got, seq):
+            want = K.oracle(raw, w, seq[r])[-1]
+            assert np.abs(row - want).max() <= 8e-2 * max(1.0, np.abs(want).max())
+    eng.check_kernel_errors()
+    assert not captures and not eng._prefix_graphs

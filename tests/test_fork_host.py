@@ -336,3 +336,29 @@ def test_random_trees_of_forks_against_all_ways_of_dividing_their_rows():
         optimal += saved == most
         assert m.check() == ""
     assert optimal >= 35
+
+
+def test_shared_pages_are_looked_for_where_a_mixer_reads_them_once(tiny):
+    import importlib
+
+    import torch
+
+    from llm_infer_rust_b200.cache import plan_cache
+    from llm_infer_rust_b200.config import resolve_architecture
+    from llm_infer_rust_b200.engine.engine import prefix_group
+    from llm_infer_rust_b200.parts import DecoderModel, int8_projections
+
+    def group_of(raw, change=lambda spec: spec):
+        arch = resolve_architecture(raw)
+        model = DecoderModel(change(arch.model_spec(arch.parse_config(raw))), torch.float32, torch.device("cpu"))
+        plan = plan_cache(model, 8, 4)
+        found = prefix_group(model, plan)
+        assert found < 0 or plan.groups[found].window is None
+        return found
+    for name in "ABCDE":
+        assert group_of(tiny[name]["raw"]) >= 0 and group_of(tiny[name]["raw"], int8_projections) >= 0
+    for kit in ("bevuvik", "kefetar", "lufizen", "mukenex", "sigudra", "torinex"):
+        configs = importlib.import_module(f"{kit}_kit").CONFIGS
+        assert configs
+        for raw in configs.values():
+            assert group_of(raw) == -1, kit
