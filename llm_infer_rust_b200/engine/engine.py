@@ -24,7 +24,7 @@ from .. import architectures  # noqa: F401  (registers the shipped architectures
 from ..cache import PagedCache, cache_budget_bytes, plan_cache, size_groups
 from ..config.registry import resolve_architecture
 from ..config.spec import ConfigError
-from ..kernels import ops
+from ..kernels import ops, prefix
 from ..kernels.build import load_host_runtime
 from ..parts import DecoderModel, int8_projections as with_int8_projections
 from ..sampling import PendingLogprobs, Sampler, SamplingParams, TokenLogprob
@@ -34,11 +34,9 @@ from .context import SharedPrefixes, StepContext, context_from_layout
 
 _DTYPES = {"bfloat16": torch.bfloat16, "float32": torch.float32}
 log = logging.getLogger("llm_infer_rust_b200")
-# Decode rows read the pages that they share once where that saves so many bytes of a layer's keys and values, summed over the rows.
-# (Decode attention / shared, us, 16 heads on 8 KV heads of 128 in bfloat16, 4 KiB a key: 16 rows behind 512 keys, 30 MiB saved, 8.3 / 9.5; 2 rows
-# behind 8,192, 32 MiB, 14.7 / 14.9; 32 behind 300, 36 MiB, 12.0 / 10.3; 6 behind 2,048, 40 MiB, 14.2 / 10.0; 4 behind 4,096, 48 MiB, 14.6 /
-# 11.3; 16 behind 1,024, 60 MiB, 12.6 / 10.9; 2 behind 16,384, 64 MiB, 22.9 / 21.7; 48 behind 512, 94 MiB, 23.7 / 13.1; 48 behind 16,384 438 / 33.)
-_SAVED_BYTES_AT_LEAST = 32 << 20
+# Decode rows read the pages that they share once where that saves so many bytes of a layer's keys and values, summed over the rows
+# (prefix.pays has what is asked beside it, and what was measured).
+_SAVED_BYTES_AT_LEAST = 48 << 20
 
 
 @dataclass
@@ -77,12 +75,16 @@ def graph_batch_sizes(limit: int) -> List[int]:
     return sorted(sizes)
 
 
-def prefix_group(model, plan) -> int:
-    """The cache group in which rows that share pages are looked for: one that keeps all keys, and with a mixer that reads shared keys once
-    (-1: there is none)."""
-    readers = {g for e, g in plan.group_of_entry.items()
-               if getattr(model.blocks[model.run_list[e].layer].mixer, "reads_shared_prefixes", False)}
-    return min((g for g in readers if not plan.groups[g].window), default=-1)
+def prefix_group(model, plan) -> Tuple[int, List[Tuple[int, int, int]]]:
+    """The cache group in which rows that share pages are looked for, one that keeps all keys and has mixers that read shared keys once (-1:
+    there is none), and the (query heads, KV heads, head size) of those."""
+    heads: Dict[int, set] = {}
+    for e, g in plan.group_of_entry.items():
+        of = getattr(model.blocks[model.run_list[e].layer].mixer, "shared_prefix_heads", None)
+        if of is not None and of() is not None and not plan.groups[g].window:
+            heads.setdefault(g, set()).add(of())
+    found = min(heads, default=-1)
+    return found, sorted(heads.get(found, ()))
 
 
 class _MetaBuffers:
@@ -273,9 +275,7 @@ class Engine:
         self._shape_graph_limit = 6
         # Requests that share pages (forks): which cache group they are looked for in, and the graphs of their decode steps, keyed by
         # (rows, places for groups, shared keys, own keys), the keys rounded up to powers of two and of four.
-        self._prefix_group = prefix_group(self.model, self.cache_plan)
-        group = self.cache_plan.groups[self._prefix_group] if self._prefix_group >= 0 else None
-        self._key_bytes = max(1, group.bytes_per_page // (group.page_size * max(1, len(group.entries)))) if group is not None else 1
+        self._prefix_group, self._prefix_heads = prefix_group(self.model, self.cache_plan)
         self._prefix_graphs: "OrderedDict[tuple, _DecodeGraph]" = OrderedDict()
         self._logprobs: Dict[int, List[TokenLogprob]] = {}
         self._own_ids = 1 << 62                          # ids of the requests that answers() opens
@@ -413,12 +413,12 @@ class Engine:
         if device_tokens is not None and (not decode_only or device_tokens.numel() != len(entries)
                                           or device_tokens.dtype != torch.int32 or not device_tokens.is_cuda):
             raise ValueError("device_tokens needs one int32 token on the device for each one-token entry")
-        graph = None
-        groups = self._look_for_prefixes(req)
-        if decode_only and self._graphs and all(len(e.want) == 1 for e in entries):
+        graph = bucket = None
+        if decode_only and self._graphs and all(len(e.want) == 1 for e in entries) and max(new_lengths) <= self.max_seq_len:
             bucket = next((b for b in sorted(self._graphs) if b >= len(entries)), None)
-            if bucket is not None and max(mgr.length(e.request) for e in entries) < self.max_seq_len:
-                graph = self._prefix_graph(bucket, *groups) if groups else self._graphs[bucket]
+        groups = self._look_for_prefixes(req, bucket, new_lengths)
+        if bucket is not None:
+            graph = self._prefix_graph(bucket, *groups) if groups else self._graphs[bucket]
         if graph is None and not decode_only and 0 < len(req.tokens) <= self.prefill_graph_max_tokens \
                 and max(mgr.length(e.request) + len(e.tokens) for e in entries) <= self.max_seq_len:
             graph = self._shape_graph(tuple(req.counts) + (-1, len(req.want_index)))
@@ -430,21 +430,29 @@ class Engine:
             mgr.advance(e.request, mgr.length(e.request) + len(e.tokens))
         return logits
 
-    def _look_for_prefixes(self, req) -> Optional[Tuple[int, int, int]]:
+    def _look_for_prefixes(self, req, bucket: Optional[int], lengths: Sequence[int]) -> Optional[Tuple[int, int, int]]:
         """Decide whether the step's decode rows read the pages that they share once: how many groups of rows do so, the most keys that one
-        shares and the most that a row has beyond them (None: none does)."""
+        shares and the most that a row has beyond them (None: none does).  ``bucket``: rows of the step's graph (None: it has none);
+        ``lengths``: the rows' keys."""
         mgr, g = self.cache.manager, self._prefix_group
         if g < 0 or mgr.shared_pages(g) == 0:
             return None
         req.prefix_group = g
         groups, saved, shared, own = self._rt.count_prefix_groups(mgr, req)
-        if not groups or saved * self._key_bytes < _SAVED_BYTES_AT_LEAST:
+        decoded = [n for n, count in zip(lengths, req.counts) if count == 1]
+        rows, places = (len(decoded), groups + 1) if bucket is None else (bucket, self._prefix_places(groups))
+        if not groups or not all(prefix.pays(self.dtype, *heads, self.cache.page_sizes[g], rows, places, saved, sum(decoded) - saved, _SAVED_BYTES_AT_LEAST)
+                                 for heads in self._prefix_heads):
             req.prefix_group = -1
             return None
         return groups, shared, own
 
+    @staticmethod
+    def _prefix_places(groups: int) -> int:
+        return 1 + (1 << (groups - 1).bit_length())              # (the last group is the other rows')
+
     def _prefix_graph(self, bucket: int, groups: int, shared: int, own: int) -> _DecodeGraph:
-        places = 1 + (1 << (groups - 1).bit_length())            # (the last group is the other rows')
+        places = self._prefix_places(groups)
         keys = 1 << (shared - 1).bit_length(), 1 << (max(own, 64) - 1).bit_length() // 2 * 2 + 2
         key = (bucket, places) + keys
         g = self._prefix_graphs.get(key)

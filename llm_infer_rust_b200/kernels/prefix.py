@@ -109,6 +109,33 @@ def _plan(dtype, heads: int, kv_heads: int, dim: int, page: int, n_rows: int, n_
     return None, tcgen05, lib.b200_prefix_attention_mma, (floats, shared, 0, tiles, two, covered, stream, sms), 2 + (tcgen05 is not None)
 
 
+def pays(dtype, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, n_rows: int, n_groups: int, saved_keys: int, read_keys: int,
+         least: int) -> bool:
+    """Whether ``prefix_attention`` of ``n_rows`` rows in ``n_groups`` groups is quicker than ``ops.decode_attention`` of the same rows, where it
+    reads ``read_keys`` keys in all and ``saved_keys`` less than that.  ``least``: bytes that are to be saved in the usual case.
+
+    On the tensor cores (decode attention / shared, us): what a call takes beside its bytes is made up for by 48 MiB, and by 64 MiB where
+    more than two query heads share a KV head and their parts are joined (16 heads on 8 KV heads of 128: 16 rows 39 MiB 10.0 / 10.5, 48 MiB
+    11.1 / 10.8; 32 on 8: 16 rows 55 MiB 13.5 / 13.8; 64 on 8: 16 rows 55 MiB 14.6 / 16.2, 64 MiB 15.0 / 14.7; 16 on 1: 16 rows 48 MiB 16.4 / 17.4, 64
+    MiB 18.9 / 17.9).  Keys that a row has to itself are read up to a twelfth slower, so a sixth of what is read has to be saved (128 rows
+    with 600 of their own, 300 MiB: 32 MiB saved 69.3 / 72.4, 64 74.1 / 62.5; 384 rows, 900 MiB: 48 203 / 221, 120 204 / 180; eight rows beside 60
+    of 2,000 that share nothing, 470 MiB: 64 91.6 / 93.5, 128 110 / 96).
+    float32 gains from the smallest (two rows 16 MiB 39.2 / 19.9, 450 rows 28 MiB of 2.3 GiB 561 / 353), and so do more than 16 query heads
+    on a KV head (32 on 1: 450 rows 14 MiB 200 / 76): two thirds.
+    Other bfloat16 calls go to the all-sizes kernel, element by element: never where decode attention has its tensor-core kernel (more rows
+    and groups than the others take: 450 rows of 64 keys, 505 MiB saved, 154 / 230), else where eight times as much is saved as
+    read (heads of 72: 64 rows of 600 keys, 1.5 times, 136 / 143, 16 of 64, 11 times, 94 / 24; heads of 320: 64 rows, 3 times, 111 / 145, 12
+    times, 244 / 210)."""
+    saved = 2 * saved_keys * num_kv_heads * head_dim * dtype.itemsize
+    group = num_heads // num_kv_heads
+    if dtype == torch.bfloat16 and group <= ops.MMA_MAX_GROUP:
+        if ops.decode_uses_tensor_cores(dtype, num_heads, num_kv_heads, head_dim, 1) and n_rows + n_groups <= _MOST_ENTRIES:
+            return saved >= (least if group <= 2 else least * 4 // 3) and 6 * saved_keys >= read_keys
+        if ops.decode_uses_tensor_cores(dtype, num_heads, num_kv_heads, head_dim, page_size) or saved_keys < 8 * read_keys:
+            return False
+    return saved >= least * 2 // 3
+
+
 def _counts(k_cache, block_table, n_rows: int, n_groups: int, num_heads: int, num_kv_heads: int, page_size: int) -> bool:
     """Whether the tensor-core kernels, which count a cache's rows and a call's blocks of keys in 32 bits, can count a call's (as
     ``prefix_attention`` of csrc/binding/calls.cpp asks)."""

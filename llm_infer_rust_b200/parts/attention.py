@@ -138,7 +138,6 @@ class GQAttention(Part):
     """
     category = "mixer"
     chainable = True          # reads its input through ops.* only, and may return a product that still waits (ops.few_row_linear)
-    reads_shared_prefixes = True
 
     def __init__(self, spec, env):
         super().__init__(spec, env)
@@ -166,6 +165,9 @@ class GQAttention(Part):
 
     def cache_spec(self):
         return PagedKVSpec(self.nkv, self.d, self.window)
+
+    def shared_prefix_heads(self):
+        return None if self.window else (self.nh, self.nkv, self.d)
 
     def state_spec(self):
         return None

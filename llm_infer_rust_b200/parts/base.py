@@ -15,8 +15,9 @@ Categories and the interface each must have:
                       values it needs, or None); ``state_spec()`` (fixed-size
                       per-request state it needs, or None); optionally ``state_specs()`` (several, by name:
                       ``mixer_state(cache, name)`` gives the tensor), ``children()`` (parts inside the part, by
-                      name: their parameters' paths continue the part's own) and ``reads_shared_prefixes = True`` (decode rows
-                      that share pages read those once, by ``ctx.shared``: nobody looks for such rows without a mixer that does)
+                      name: their parameters' paths continue the part's own) and ``shared_prefix_heads()``, (query heads, KV
+                      heads, head size) of a mixer whose decode rows read the pages that they share once, by ``ctx.shared``
+                      (nobody looks for such rows where no mixer has it, or it says None)
 ``feed_forward``      ``forward(x) -> y``
 ``token_conv``        ``forward(x, scale, ctx, state, out_dtype) -> y`` (a convolution over time whose last
                       inputs are per-request state); ``state_spec()``

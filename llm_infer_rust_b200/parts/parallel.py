@@ -29,7 +29,6 @@ class ParallelMixers(Part):
         if any(m.state_spec() is not None for m in (self.left, self.right)):
             raise ValueError("mixers side by side name their states (state_specs)")
         self.paged = paged[0] if paged else None
-        self.reads_shared_prefixes = getattr(self.paged, "reads_shared_prefixes", False)
         self.joint = None              # (packed weights of both branches, first row of the right one)
 
     def children(self):
@@ -44,6 +43,10 @@ class ParallelMixers(Part):
 
     def cache_spec(self):
         return self.paged.cache_spec() if self.paged is not None else None
+
+    def shared_prefix_heads(self):
+        of_paged = getattr(self.paged, "shared_prefix_heads", None)
+        return of_paged() if of_paged is not None else None
 
     def state_spec(self):
         return None

@@ -413,3 +413,35 @@ def test_layers_that_read_every_row_by_itself_have_no_graphs_of_shared_pages(nam
             assert np.abs(row - want).max() <= 8e-2 * max(1.0, np.abs(want).max())
     eng.check_kernel_errors()
     assert not captures and not eng._prefix_graphs
+
+
+@pytest.mark.parametrize("graphs", [0, 8])
+def test_steps_of_more_rows_than_the_tensor_core_kernels_take_read_by_themselves(graphs, folders, monkeypatch):
+    """The limit is lowered: six rows in three groups, a graph of eight rows in as many, are beyond it."""
+    from llm_infer_rust_b200.engine import StepEntry
+    from llm_infer_rust_b200.kernels import prefix
+    folder, w = folders("E", "bfloat16")
+    raw = json.load(open(os.path.join(folder, "config.json")))
+    calls = []
+    inner = prefix.prefix_attention
+    monkeypatch.setattr(prefix, "prefix_attention", lambda *a, **k: calls.append(k) or inner(*a, **k))
+    found = {}
+    for limit in (8, 400):
+        monkeypatch.setattr(prefix, "_MOST_ENTRIES", limit)
+        prefix._plan.cache_clear()
+        eng = engine(folder, dtype="bfloat16", cuda_graph_bs=graphs)
+        prompts = {1: tokens(307, 70, 3), 2: tokens(307, 90, 4)}
+        for r, prompt in prompts.items():
+            eng.open_request(r)
+            eng.step([StepEntry(r, prompt, [])])
+        eng.fork_request(1, [3, 4])
+        eng.fork_request(2, [5, 6])
+        calls.clear()
+        for step in range(3):
+            rows = {r: tokens(307, 1, 60 * step + r) for r in range(1, 7)}
+            logits = eng.step([StepEntry(r, t, [0]) for r, t in rows.items()]).float().cpu().numpy().copy()
+        eng.check_kernel_errors()
+        found[limit] = logits
+        assert bool(calls) == (limit == 400)
+    prefix._plan.cache_clear()
+    near(found[8], found[400], "bfloat16")

@@ -352,8 +352,8 @@ def test_shared_pages_are_looked_for_where_a_mixer_reads_them_once(tiny):
         arch = resolve_architecture(raw)
         model = DecoderModel(change(arch.model_spec(arch.parse_config(raw))), torch.float32, torch.device("cpu"))
         plan = plan_cache(model, 8, 4)
-        found = prefix_group(model, plan)
-        assert found < 0 or plan.groups[found].window is None
+        found, heads = prefix_group(model, plan)
+        assert not heads if found < 0 else plan.groups[found].window is None and heads == [tuple(model.blocks[0].mixer.spec[n] for n in ("num_heads", "num_kv_heads", "head_dim"))]
         return found
     for name in "ABCDE":
         assert group_of(tiny[name]["raw"]) >= 0 and group_of(tiny[name]["raw"], int8_projections) >= 0

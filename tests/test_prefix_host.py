@@ -164,3 +164,28 @@ def test_calls_that_the_tensor_core_kernels_cannot_count():
     items = 1 + 1 + 4                                          # tiles of 16 vectors, groups, rows
     most = (2 ** 30 - 1) // (8 * items) - 2                    # blocks of a row
     assert counts(width=2 * most) and not counts(width=2 * (most + 1))
+
+
+def test_shared_keys_are_read_once_where_that_was_measured_to_pay():
+    BF16, F32, MiB = torch.bfloat16, torch.float32, 1 << 20
+
+    def pays(mib, rows, groups=2, heads=16, kv_heads=8, dim=128, dtype=BF16, page=16, own=64, least=48 * MiB):
+        a_key = 2 * kv_heads * dim * dtype.itemsize
+        saved = int(mib * MiB) // a_key
+        return prefix.pays(dtype, heads, kv_heads, dim, page, rows, groups, saved, saved // (rows - 1) + rows * own, least)
+    assert pays(48, 16) and not pays(47, 16) and pays(48, 2) and pays(512, 48) and not pays(30, 48)
+    assert pays(64, 16, heads=64) and not pays(63, 16, heads=64) and pays(64, 16, heads=16, kv_heads=1) and not pays(56, 16, heads=16, kv_heads=1)
+    # rows with many keys of their own
+    assert not pays(48, 128, own=600) and pays(64, 128, own=600) and not pays(64, 384, own=600) and pays(160, 384, own=600)
+    # more rows and groups than the tensor-core kernels take, where decode attention has its own
+    for mib in (28, 128, 512, 4096, 1 << 20):
+        for own in (1, 64, 600):
+            assert not pays(mib, 450, own=own) and not pays(mib, 512, own=own) and not pays(mib, 399, own=own)
+    assert pays(512, 398, groups=2) and not pays(512, 398, groups=3)
+    # the all-sizes kernel against decode attention's
+    assert not pays(128, 64, heads=8, dim=72, own=600) and pays(128, 16, heads=8, dim=72) and not pays(512, 4, dim=320) and pays(512, 64, dim=320, own=16)
+    assert pays(32, 450, heads=32, kv_heads=1) and pays(32, 2, dtype=F32) and pays(32, 450, dtype=F32, own=600) and not pays(31, 8, dtype=F32)
+    # (pages of no power of two are the all-sizes kernel's in decode attention)
+    assert pays(48, 16, page=24) and not pays(512, 450, page=24, own=600)
+    # nothing saved, and nothing asked for
+    assert not pays(0, 16) and pays(1, 16, least=1, own=1)
