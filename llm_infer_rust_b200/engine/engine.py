@@ -274,9 +274,14 @@ class Engine:
         self._shape_seen: Dict[tuple, int] = {}
         self._shape_graph_limit = 6
         # Requests that share pages (forks): which cache group they are looked for in, and the graphs of their decode steps, keyed by
-        # (rows, places for groups, shared keys, own keys), the keys rounded up to powers of two and of four.
+        # (rows, places for groups, shared keys, own keys); shared keys are rounded up to a power of two, own keys to a power of four that
+        # is at least twice as many, from 256 on (a call that is cut up for more own keys than there are loses less than the other way round:
+        # 48 rows of 32 heads behind 16,384 keys and 250 of their own, cut up for 250 53 us, for 1,024 42).  As the prompts' shapes, one is
+        # captured when it comes a second time.  As many are kept as answers that end one after the other pass on their way through all
+        # buckets, with one change of own keys in each.
         self._prefix_group, self._prefix_heads = prefix_group(self.model, self.cache_plan)
         self._prefix_graphs: "OrderedDict[tuple, _DecodeGraph]" = OrderedDict()
+        self._prefix_graph_limit = max(6, 2 * len(self._graphs))
         self._logprobs: Dict[int, List[TokenLogprob]] = {}
         self._own_ids = 1 << 62                          # ids of the requests that answers() opens
         # Decode graphs are captured now, while every page and state slot is free: a capture runs on throw-away
@@ -418,7 +423,7 @@ class Engine:
             bucket = next((b for b in sorted(self._graphs) if b >= len(entries)), None)
         groups = self._look_for_prefixes(req, bucket, new_lengths)
         if bucket is not None:
-            graph = self._prefix_graph(bucket, *groups) if groups else self._graphs[bucket]
+            graph = (self._prefix_graph(bucket, *groups) if groups else None) or self._graphs[bucket]
         if graph is None and not decode_only and 0 < len(req.tokens) <= self.prefill_graph_max_tokens \
                 and max(mgr.length(e.request) + len(e.tokens) for e in entries) <= self.max_seq_len:
             graph = self._shape_graph(tuple(req.counts) + (-1, len(req.want_index)))
@@ -451,14 +456,23 @@ class Engine:
     def _prefix_places(groups: int) -> int:
         return 1 + (1 << (groups - 1).bit_length())              # (the last group is the other rows')
 
-    def _prefix_graph(self, bucket: int, groups: int, shared: int, own: int) -> _DecodeGraph:
+    def _comes_again(self, key: tuple) -> bool:
+        seen = self._shape_seen.get(key, 0) + 1
+        if len(self._shape_seen) > 4096:
+            self._shape_seen.clear()
+        self._shape_seen[key] = seen
+        return seen >= 2                     # (what comes once is not worth a capture)
+
+    def _prefix_graph(self, bucket: int, groups: int, shared: int, own: int) -> Optional[_DecodeGraph]:
         places = self._prefix_places(groups)
         keys = 1 << (shared - 1).bit_length(), 1 << (max(own, 64) - 1).bit_length() // 2 * 2 + 2
         key = (bucket, places) + keys
         g = self._prefix_graphs.get(key)
         if g is None:
+            if not self._comes_again(("shared",) + key):
+                return None
             g = self._prefix_graphs[key] = _DecodeGraph(bucket, places, keys)
-            while len(self._prefix_graphs) > self._shape_graph_limit:
+            while len(self._prefix_graphs) > self._prefix_graph_limit:
                 self._prefix_graphs.popitem(last=False)
         self._prefix_graphs.move_to_end(key)
         return g
@@ -480,12 +494,8 @@ class Engine:
         if g is not None:
             self._shape_graphs.move_to_end(key)
             return g
-        seen = self._shape_seen.get(key, 0) + 1
-        if len(self._shape_seen) > 4096:
-            self._shape_seen.clear()
-        self._shape_seen[key] = seen
-        if seen < 2:
-            return None                      # a shape that comes once is not worth a capture
+        if not self._comes_again(key):
+            return None
         g = _DecodeGraph(0)
         self._shape_graphs[key] = g
         while len(self._shape_graphs) > self._shape_graph_limit:

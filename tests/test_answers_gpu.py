@@ -445,3 +445,38 @@ def test_steps_of_more_rows_than_the_tensor_core_kernels_take_read_by_themselves
         assert bool(calls) == (limit == 400)
     prefix._plan.cache_clear()
     near(found[8], found[400], "bfloat16")
+
+
+def test_graphs_of_shared_pages_are_captured_when_they_come_again_and_kept(folders):
+    from llm_infer_rust_b200 import SamplingParams
+    from llm_infer_rust_b200.engine import StepEntry
+    folder, _ = folders("A", "bfloat16")
+    eng = engine(folder, dtype="bfloat16", cuda_graph_bs=12, eos_token_ids=list(range(0, 256, 11)))
+    captures = []
+    capture = eng._capture
+    eng._capture = lambda g, *a: captures.append(g.bucket) or capture(g, *a)
+    eng.open_request(1)
+    eng.step([StepEntry(1, tokens(256, 40, 1), [])])
+    eng.fork_request(1, [2, 3])
+    counts = []
+    for step in range(4):
+        eng.step([StepEntry(r, tokens(256, 1, 10 * step + r), [0]) for r in (1, 2, 3)])
+        counts.append(len(captures))
+    assert counts == [0, 1, 1, 1]                             # (the first step went through the graph that was there)
+    for r in (1, 2, 3):
+        eng.close_request(r)
+    # answers that end at unlike places pass through all buckets, with few and with many keys of their own
+    sp = SamplingParams(temperature=1.5, max_tokens=200, seed=4)
+    first = eng.answers(tokens(256, 30, 8), 12, sp)
+    assert max(len(r.tokens) for r in first) > 1
+    for _ in range(2):
+        last = eng.answers(tokens(256, 30, 8), 12, sp)
+    known = len(captures)
+    assert 3 <= len(eng._prefix_graphs) <= eng._prefix_graph_limit == 10
+    again = eng.answers(tokens(256, 30, 8), 12, sp)
+    assert len(captures) == known and [r.tokens for r in again] == [r.tokens for r in last]
+    # what is not asked for goes first
+    eng._prefix_graph_limit = 2
+    for bucket in (1, 2, 4):
+        assert eng._prefix_graph(bucket, 1, 1 << 12, 7) is None and eng._prefix_graph(bucket, 1, 1 << 12, 7).bucket == bucket
+    assert [key[0] for key in eng._prefix_graphs] == [2, 4]
