@@ -311,9 +311,9 @@ PyObject* byte_product(PyObject*, PyObject* const* args, Py_ssize_t n) {
 //                  scale, plan, error word, stream) -> code
 // Decode attention behind shared prefixes (kernels/prefix.py) as one call: what the tensors must be, the memory between its kernels and
 // the launches.  The entry points are those of the plan, None where it has no use for one: the all-sizes kernel alone, or the
-// tensor-core kernels.  plan: (floats of scratch, splits of the shared keys, splits of the own keys, tiles, two tiles a CTA, vectors
-// that the tcgen05 kernel covers, CTAs of the stream kernel, multiprocessors).  None, and nothing done, where something is not as it should be (the wrapper then says what)
-// or this thread records its calls.  (Through Python the call took the host 17 us, as one 9 to 10,
+// tensor-core kernels.  plan: (floats of scratch, splits of the shared keys, splits of the own keys or groups that the tcgen05 kernel
+// serves, tiles, two tiles a CTA, vectors that the tcgen05 kernel covers, CTAs of the stream kernel, multiprocessors).  None, and nothing
+// done, where something is not as it should be (the wrapper then says what) or this thread records its calls.  (Through Python the call took the host 17 us, as one 9 to 10,
 // of which 5 to 7 are two or three launches.)
 PyObject* prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -381,8 +381,8 @@ PyObject* prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       rc = invoke(fn, ints, m, floats);
     };
     call(entry[0], {at[1], at[2], at[3], code, width, at[7]});
-    call(entry[1], {at[1], at[3], at[4]});
-    call(entry[2], {at[1], at[5], at[6], at[7]});
+    call(entry[1], {at[1], at[3] | at[2] << 16, at[4]});
+    call(entry[2], {at[1], at[5] | at[2] << 16, at[6], at[7]});
   }
   return PyLong_FromLong(rc);
   END_HANDLE_TH_ERRORS

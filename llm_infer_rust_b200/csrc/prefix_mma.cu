@@ -51,10 +51,11 @@ struct StreamCall {
   float* acc;                                    // [parts][16][D]
   float2* ml;                                    // [parts][16]
   RowParts* row_parts;                           // [n_rows][nkv]
-  int covered;                                   // vectors of each group that the tcgen05 kernel serves
+  int covered, covered_groups;                   // vectors of each of the first groups that the tcgen05 kernel serves, and how many groups
+  __device__ __forceinline__ int covered_of(int g) const { return g < covered_groups ? covered : 0; }
 };
 
-__device__ __forceinline__ int tiles_of(const StreamCall& k, int rows, int group) { return (max(0, rows * group - k.covered) + VT - 1) / VT; }
+__device__ __forceinline__ int tiles_of(const StreamCall& k, int g, int rows, int group) { return (max(0, rows * group - k.covered_of(g)) + VT - 1) / VT; }
 
 // Sums of `v` over the CTA's threads before this one; `sum` becomes that of all.  `sh`: one int a warp.
 template <int WARPS_HERE>
@@ -116,7 +117,7 @@ __device__ __forceinline__ void lay_out(const StreamCall& k, Entries& at, int* m
       const int first = min(max(here.x, 0), c.n_rows), rows = min(max(behind, first), c.n_rows) - first;
       at.keys[x] = rows > 0 ? checked(here.y) : 0;
       at.low[x] = first;
-      at.where[x] = tiles_of(k, rows, group);
+      at.where[x] = tiles_of(k, x, rows, group);
     }
     if (is_row) {
       at.where[c.n_groups + x] = row;
@@ -168,7 +169,7 @@ struct Place {
   int s, kvh, first_key, end, lowest, left, item, i0, vector0, vectors, table_row;
 };
 // (not inlined: it is asked in three places, and a kernel this short waits for its instructions)
-__device__ __noinline__ Place locate(const Entries& at, int s, int s_end, int n_groups, int n_rows, int group, int covered) {
+__device__ __noinline__ Place locate(const Entries& at, int s, int s_end, int n_groups, int n_rows, int group, int covered, int covered_groups) {
   Place p;
   p.s = s;
   p.kvh = s / at.blocks;
@@ -189,7 +190,7 @@ __device__ __noinline__ Place locate(const Entries& at, int s, int s_end, int n_
     p.lowest = 0;
     p.i0 = at.low[e];
     const int next = e + 1 < n_groups ? max(at.low[e + 1], p.i0) : n_rows;
-    p.vector0 = covered + tile * VT;
+    p.vector0 = (e < covered_groups ? covered : 0) + tile * VT;
     p.vectors = min(VT, (next - p.i0) * group - p.vector0);
     p.table_row = at.where[n_groups + p.i0];
     p.first_key = block * KB;
@@ -374,7 +375,7 @@ prefix_stream_kernel(const bf16* __restrict__ kc, const bf16* __restrict__ vc, c
       for (int part = lane & 1; part < D / 8; part += 2) cp_async16(qs + r * LD + part * 8, src + part * 8, r < p.vectors);
       cp_async_commit();
     };
-    Place now = locate(at, s_begin, s_end, c.n_groups, c.n_rows, group, k.covered), ahead = now, next = now;
+    Place now = locate(at, s_begin, s_end, c.n_groups, c.n_rows, group, k.covered, k.covered_groups), ahead = now, next = now;
     int page = lane_page(c, boxes, ahead, lane);
     fetch_queries(now);
     uint32_t qa[kQueriesInRegisters ? D / 16 : 1][4];
@@ -388,7 +389,7 @@ prefix_stream_kernel(const bf16* __restrict__ kc, const bf16* __restrict__ vc, c
         fetch_stage = fetch_stage + 1 == STAGES ? 0 : fetch_stage + 1;
         ++ahead.s;
         ahead.first_key += KB;
-        if (--ahead.left == 0 && ahead.s < s_end) ahead = locate(at, ahead.s, s_end, c.n_groups, c.n_rows, group, k.covered);
+        if (--ahead.left == 0 && ahead.s < s_end) ahead = locate(at, ahead.s, s_end, c.n_groups, c.n_rows, group, k.covered, k.covered_groups);
         if (ahead.s < s_end) page = lane_page(c, boxes, ahead, lane);
       }
       cp_async_commit();                           // (one a tick; an item's queries are one more, behind that of a tick)
@@ -401,7 +402,7 @@ prefix_stream_kernel(const bf16* __restrict__ kc, const bf16* __restrict__ vc, c
           for (int x = 0; x < D / 16; ++x) ldmatrix_x4(qa[x], qs + (lane & 15) * LD + x * 16 + (lane >> 4) * 8);
           __syncwarp();
           if (now.s + now.left < s_end) {
-            next = locate(at, now.s + now.left, s_end, c.n_groups, c.n_rows, group, k.covered);
+            next = locate(at, now.s + now.left, s_end, c.n_groups, c.n_rows, group, k.covered, k.covered_groups);
             fetch_queries(next);
           }
         }
@@ -444,7 +445,7 @@ prefix_stream_kernel(const bf16* __restrict__ kc, const bf16* __restrict__ vc, c
       }
       if (now.s + now.left >= s_end) break;
       if constexpr (!kQueriesInRegisters) {
-        next = locate(at, now.s + now.left, s_end, c.n_groups, c.n_rows, group, k.covered);
+        next = locate(at, now.s + now.left, s_end, c.n_groups, c.n_rows, group, k.covered, k.covered_groups);
         fetch_queries(next);
       }
       now = next;
@@ -466,7 +467,7 @@ prefix_stream_kernel(const bf16* __restrict__ kc, const bf16* __restrict__ vc, c
     const int g = group_of(at, c.n_groups, i);
     p.grouped = g >= 0;
     if (g >= 0) {
-      p.first_vector = (i - at.low[g]) * group - k.covered;
+      p.first_vector = (i - at.low[g]) * group - k.covered_of(g);
       const int tiles_here = (g + 1 < c.n_groups ? at.where[g + 1] : at.group_tiles) - at.where[g];
       const int blocks_here = tiles_here > 0 ? (at.start[g + 1] - at.start[g]) / tiles_here : 0, tile = max(p.first_vector, 0) / VT;
 #pragma unroll
@@ -521,8 +522,8 @@ B200_EXPORT long long b200_prefix_scratch_floats(int n_rows, int n_groups, int n
 
 // q, out [tokens, nh * D]; k_cache, v_cache [pages, nkv, page_size, D]; `groups`: (first row, shared keys) each.  `scratch` holds
 // b200_prefix_scratch_floats(...) floats on a 16-byte boundary (of as many `ctas`).  `covered` > 0: b200_prefix_tcgen05 has just been launched with the
-// same scratch for the first `covered` vectors of every group, in splits_shared splits (else 0 of both).  `ctas`: of the stream kernel, at
-// most one for each of the device's `sms`.
+// same scratch for the first covered % 2^16 vectors of every one of the first covered / 2^16 groups (0: of all), in splits_shared splits (else 0 of
+// both).  `ctas`: of the stream kernel, at most one for each of the device's `sms`.
 B200_EXPORT int b200_prefix_attention_mma(const void* q, const void* k_cache, const void* v_cache, void* out, float* scratch, const int* block_table,
                                           int table_stride, const int* cu_q, const int* kv_len, const int* rows, int n_rows, const int* groups,
                                           int n_groups, int nh, int nkv, int page_size, int pages, float scale, int splits_shared, int covered,
@@ -546,7 +547,8 @@ B200_EXPORT int b200_prefix_attention_mma(const void* q, const void* k_cache, co
   k.acc = scratch + align4(vectors * (D + 2));
   k.ml = reinterpret_cast<float2*>(k.acc + parts * D);
   k.row_parts = reinterpret_cast<RowParts*>(k.ml + parts);
-  k.covered = covered;
+  k.covered = covered & 0xffff;
+  k.covered_groups = covered >> 16 == 0 ? n_groups : covered >> 16;
   k.c = {block_table, cu_q, kv_len, rows, reinterpret_cast<const int2*>(groups), scratch, part_ml, err, table_stride, n_rows, n_groups, nh, nkv,
          page_size, pages, splits_shared, 0, 1, scale * 1.4426950408889634f};
   Boxes boxes;

@@ -89,7 +89,7 @@ def _plan(dtype, heads: int, kv_heads: int, dim: int, page: int, n_rows: int, n_
         shared, own = _splits(most_shared, most_own, sharing * kv_heads * tiles, n_rows * kv_heads * -(-per // _TILE), per_sm * sms)
         floats = n_rows * heads * (shared + own) * (ops.padded_head_dim(dim) + 2)
         return lib.b200_prefix_attention, None, None, (floats, shared, own, tiles, 0, 0, 0, sms), 2
-    tcgen05, tiles, two, shared, covered, stream = None, 1, 0, 0, 0, sms
+    tcgen05, tiles, two, shared, covered, stream, served = None, 1, 0, 0, 0, sms, 0
     blocks = -(-vectors // _MMA_VECTORS) * -(-most_shared // 32) * kv_heads * sharing
     if n_groups and dim == 128 and page & (page - 1) == 0 and vectors > _TENSOR_CORE_VECTORS:
         # one or two tiles a CTA, none without a block of keys for each of its streams
@@ -100,13 +100,13 @@ def _plan(dtype, heads: int, kv_heads: int, dim: int, page: int, n_rows: int, n_
             _TENSOR_CORE_BLOCKS + _TENSOR_CORE_BLOCKS_A_STEP * -(-steps // _most_ctas(steps, all_tiles, sms))
         if blocks >= least:
             ctas, stream = _share_sms(steps, two, all_tiles, n_rows * kv_heads, most_own, 4 * dim, sms)
-            shared, covered = ctas << (1 - two), tiles * (_TC_VECTORS << two)
+            shared, covered, served = ctas << (1 - two), tiles * (_TC_VECTORS << two), sharing
             tcgen05 = load_entry_points("prefix_tcgen05.cu").b200_prefix_tcgen05
     lib = load_entry_points("prefix_mma.cu", {"HEAD_DIM": dim})
     count = lib.library.b200_prefix_scratch_floats
     count.restype = ctypes.c_longlong
     floats = count(n_rows, n_groups, heads, kv_heads, shared, stream)
-    return None, tcgen05, lib.b200_prefix_attention_mma, (floats, shared, 0, tiles, two, covered, stream, sms), 2 + (tcgen05 is not None)
+    return None, tcgen05, lib.b200_prefix_attention_mma, (floats, shared, served, tiles, two, covered, stream, sms), 2 + (tcgen05 is not None)
 
 
 def pays(dtype, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, n_rows: int, n_groups: int, saved_keys: int, read_keys: int,
@@ -176,7 +176,7 @@ def prefix_attention(q, k_cache, v_cache, out, block_table, cu_q, kv_len, rows, 
     finite: they are multiplied by weights of zero).  A row of no keys gets zeros.  Each row stands in ``rows`` once; ``out`` may be ``q``.
 
     ``most_rows``, ``most_shared`` and ``most_own`` are about how many rows a group has, how many keys it shares and how many keys
-    a row has beyond them, at most, ``sharing_groups`` about how many of the groups share keys (None: all): they decide how the work is
+    a row has beyond them, at most, ``sharing_groups`` about how many of the groups, the first ones, share keys (None: all): they decide how the work is
     cut up (and what a captured graph is cut up for), not the result's meaning.  Page ids outside the pool and rows longer than
     their block table (of at most 2^30 places) set the error word (``ops.check_errors``); the other index arrays are taken at their word, as ``ops.decode_attention`` takes them."""
     if num_kv_heads <= 0 or num_heads <= 0 or num_heads % num_kv_heads:
@@ -217,8 +217,9 @@ def prefix_attention(q, k_cache, v_cache, out, block_table, cu_q, kv_len, rows, 
         if all_sizes is not None:
             rc = all_sizes(q, k_cache, v_cache, out, *common, shared, own, tiles, ops._code(q), head_dim, sms, *ends)
         else:
-            rc = tcgen05(q, k_cache, v_cache, *common, shared, tiles, two, *ends) if tcgen05 is not None else 0
-            rc = rc or mma(q, k_cache, v_cache, out, *common, shared, covered, stream, sms, *ends)
+            # (`own`: the groups that the tcgen05 kernel serves)
+            rc = tcgen05(q, k_cache, v_cache, *common, shared, tiles | own << 16, two, *ends) if tcgen05 is not None else 0
+            rc = rc or mma(q, k_cache, v_cache, out, *common, shared, covered | own << 16, stream, sms, *ends)
     ops._ok(rc, "prefix_attention", kernels)
 
 

@@ -541,3 +541,11 @@ def test_tables_and_caches_beyond_what_the_tensor_core_kernels_count():
     c.k = c.v = small
     torch.cuda.empty_cache()
     c.check(out)
+
+
+@pytest.mark.parametrize("sharing", [1, 2, 3, 4, 5, None])
+def test_tcgen05_of_the_first_groups_alone(sharing, always_tcgen05):
+    """Groups behind those that it is said to serve are the other kernel's, whether they share keys or not."""
+    c = Case([(40, 300, [2 + i for i in range(40)]), (3, 700, [1, 9, -200]), (2, 0, [50, 0]), (35, 200, [1 + i for i in range(35)]), (1, 0, [33])],
+             8, 2, 128, 16, BF16, other_tokens=1, scramble=True)
+    c.check(c.run(sharing_groups=sharing))

@@ -189,3 +189,16 @@ def test_shared_keys_are_read_once_where_that_was_measured_to_pay():
     assert pays(48, 16, page=24) and not pays(512, 450, page=24, own=600)
     # nothing saved, and nothing asked for
     assert not pays(0, 16) and pays(1, 16, least=1, own=1)
+
+
+def test_groups_that_share_nothing_get_no_ctas_of_the_tcgen05_kernel():
+    def served(n_groups, sharing):
+        got = prefix._plan(torch.bfloat16, 32, 8, 128, 16, 64, n_groups, 64, 32768, 100, sharing, True, 148)
+        assert got[1] is not None
+        return got[3][2]
+    assert [served(2, 1), served(5, 4), served(3, 3), served(9, 0)] == [1, 4, 3, 1]
+    # the entry points take the groups beside the tiles and the vectors, and refuse more groups than there are
+    none, some = ctypes.c_void_p(), ctypes.c_void_p(1 << 20)       # (never followed)
+    entry = load_cuda_library("prefix_tcgen05.cu").b200_prefix_tcgen05
+    for tiles in (1 | 3 << 16, 3 << 16, 1 << 16):
+        assert entry(some, some, some, some, some, 4, some, some, some, 2, some, 2, 8, 2, 16, 9, ctypes.c_float(0.1), 2, tiles, 0, some, none) == -2
