@@ -549,3 +549,17 @@ def test_tcgen05_of_the_first_groups_alone(sharing, always_tcgen05):
     c = Case([(40, 300, [2 + i for i in range(40)]), (3, 700, [1, 9, -200]), (2, 0, [50, 0]), (35, 200, [1 + i for i in range(35)]), (1, 0, [33])],
              8, 2, 128, 16, BF16, other_tokens=1, scramble=True)
     c.check(c.run(sharing_groups=sharing))
+
+
+@pytest.mark.parametrize("rows", [397, 398, 430])
+def test_as_many_rows_as_the_tensor_core_kernels_take_and_more(rows):
+    """400 rows and groups together: 397 and 398 rows in two groups, then the all-sizes kernel."""
+    first = rows - 50
+    c = Case([(first, 150, [1 + i % 40 for i in range(first)]), (50, 33, [1 + i for i in range(50)])], 4, 2, 64, 16, BF16, scramble=True)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("d", [130, 192, 256, 384, 512])
+def test_float32_wide_heads_in_several_groups(d):
+    c = Case([(3, 70, [1, 40, 9]), (2, 0, [5, 33]), (20, 130, [1 + i for i in range(20)]), (1, 16, [3])], 8, 2, d, 16, F32, other_tokens=1, scramble=True)
+    c.check(c.run())
