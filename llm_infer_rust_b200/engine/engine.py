@@ -430,14 +430,14 @@ class Engine:
         if graph is not None:
             logits = self._step_graph(graph, req, len(entries), device_tokens)
         else:
-            logits = self._step_eager(req, device_tokens)
+            logits = self._step_eager(req, device_tokens, groups[2] if groups else None)
         for e in entries:
             mgr.advance(e.request, mgr.length(e.request) + len(e.tokens))
         return logits
 
     def _look_for_prefixes(self, req, bucket: Optional[int], lengths: Sequence[int]) -> Optional[Tuple[int, int, int]]:
         """Decide whether the step's decode rows read the pages that they share once: how many groups of rows do so, the most keys that one
-        shares and the most that a row has beyond them (None: none does).  ``bucket``: rows of the step's graph (None: it has none);
+        shares and how many a row has beyond them at most, as the call is to be cut up (None: none does).  ``bucket``: rows of the step's graph (None: it has none);
         ``lengths``: the rows' keys."""
         mgr, g = self.cache.manager, self._prefix_group
         if g < 0 or mgr.shared_pages(g) == 0:
@@ -450,6 +450,11 @@ class Engine:
                                  for heads in self._prefix_heads):
             req.prefix_group = -1
             return None
+        # The tensor-core kernels give every warp an equal stretch of all rows' own keys: what a call is cut up for is their sum, and half of
+        # the most a row has stands for the rows' mean.  So one long row does not: 48 rows behind 16,384 keys beside one that left them
+        # after 4,096, 28 layers, cut up for that one's own keys 7.1 ms a step, so 2.1 (1.9 without it).  (All but the largest group's shared keys count as own.)
+        if all(prefix.on_tensor_cores(self.dtype, *heads, rows, places) for heads in self._prefix_heads):
+            own = min(own, 2 * -(-(sum(decoded) - saved - shared) // len(decoded)))
         return groups, shared, own
 
     @staticmethod
@@ -477,7 +482,7 @@ class Engine:
         self._prefix_graphs.move_to_end(key)
         return g
 
-    def _step_eager(self, req, device_tokens: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def _step_eager(self, req, device_tokens: Optional[torch.Tensor] = None, own_keys: Optional[int] = None) -> torch.Tensor:
         layout = self._rt.plan_batch(self.cache.manager, req)
         self._meta.reserve(layout.total_ints)
         turn, host = self._meta.next_host()
@@ -486,6 +491,8 @@ class Engine:
         if device_tokens is not None:
             dev[layout.off_tokens:layout.off_tokens + layout.num_tokens].copy_(device_tokens, non_blocking=True)
         ctx = self._context(layout, dev, host, layout.max_kv_len)
+        if own_keys is not None and ctx.shared is not None:
+            ctx.shared.most_own = own_keys
         self._launched = True
         return self.model.forward(ctx, self.cache.layer_caches, self.cache.embedding)
 

@@ -82,7 +82,7 @@ def _plan(dtype, heads: int, kv_heads: int, dim: int, page: int, n_rows: int, n_
     vectors = most_rows * per
     sharing = max(1, min(sharing, n_groups))
     # (pages of any size: powers of two in what decode attention asks for and the tcgen05 kernel fetches, not here)
-    if not taken or not ops.decode_uses_tensor_cores(dtype, heads, kv_heads, dim, 1) or n_rows + n_groups > _MOST_ENTRIES:
+    if not taken or not on_tensor_cores(dtype, heads, kv_heads, dim, n_rows, n_groups):
         lib = load_entry_points("prefix_attention.cu", {"HEAD_DIM": ops.padded_head_dim(dim)})
         tiles = -(-vectors // _TILE)
         per_sm = max(1, 227 * 1024 // (lib.b200_prefix_attention_smem() + 1024))
@@ -109,6 +109,11 @@ def _plan(dtype, heads: int, kv_heads: int, dim: int, page: int, n_rows: int, n_
     return None, tcgen05, lib.b200_prefix_attention_mma, (floats, shared, served, tiles, two, covered, stream, sms), 2 + (tcgen05 is not None)
 
 
+def on_tensor_cores(dtype, num_heads: int, num_kv_heads: int, head_dim: int, n_rows: int, n_groups: int) -> bool:
+    """Whether calls of these sizes go to the tensor-core kernels (if their tensors are aligned)."""
+    return ops.decode_uses_tensor_cores(dtype, num_heads, num_kv_heads, head_dim, 1) and n_rows + n_groups <= _MOST_ENTRIES
+
+
 def pays(dtype, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, n_rows: int, n_groups: int, saved_keys: int, read_keys: int,
          least: int) -> bool:
     """Whether ``prefix_attention`` of ``n_rows`` rows in ``n_groups`` groups is quicker than ``ops.decode_attention`` of the same rows, where it
@@ -129,7 +134,7 @@ def pays(dtype, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int
     saved = 2 * saved_keys * num_kv_heads * head_dim * dtype.itemsize
     group = num_heads // num_kv_heads
     if dtype == torch.bfloat16 and group <= ops.MMA_MAX_GROUP:
-        if ops.decode_uses_tensor_cores(dtype, num_heads, num_kv_heads, head_dim, 1) and n_rows + n_groups <= _MOST_ENTRIES:
+        if on_tensor_cores(dtype, num_heads, num_kv_heads, head_dim, n_rows, n_groups):
             return saved >= (least if group <= 2 else least * 4 // 3) and 6 * saved_keys >= read_keys
         if ops.decode_uses_tensor_cores(dtype, num_heads, num_kv_heads, head_dim, page_size) or saved_keys < 8 * read_keys:
             return False
@@ -176,7 +181,8 @@ def prefix_attention(q, k_cache, v_cache, out, block_table, cu_q, kv_len, rows, 
     finite: they are multiplied by weights of zero).  A row of no keys gets zeros.  Each row stands in ``rows`` once; ``out`` may be ``q``.
 
     ``most_rows``, ``most_shared`` and ``most_own`` are about how many rows a group has, how many keys it shares and how many keys
-    a row has beyond them, at most, ``sharing_groups`` about how many of the groups, the first ones, share keys (None: all): they decide how the work is
+    a row has beyond them, at most (where one row has far more than the others and the tensor-core kernels serve the call: twice the rows' mean),
+    ``sharing_groups`` about how many of the groups, the first ones, share keys (None: all): they decide how the work is
     cut up (and what a captured graph is cut up for), not the result's meaning.  Page ids outside the pool and rows longer than
     their block table (of at most 2^30 places) set the error word (``ops.check_errors``); the other index arrays are taken at their word, as ``ops.decode_attention`` takes them."""
     if num_kv_heads <= 0 or num_heads <= 0 or num_heads % num_kv_heads:

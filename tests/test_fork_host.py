@@ -361,3 +361,26 @@ def test_shared_pages_are_looked_for_where_a_mixer_reads_them_once(tiny):
         made = importlib.import_module(f"{kit}_kit")
         for raw in made.CONFIGS.values():
             assert group_of(getattr(made, "as_given", dict)(raw)) == -1, kit
+
+
+def test_a_long_row_is_not_what_a_call_is_cut_up_for():
+    """The rows' own keys that a step names: not those of one row that shares nothing, where the kernels share all rows' out evenly."""
+    from types import SimpleNamespace
+
+    import torch
+
+    from llm_infer_rust_b200.engine import Engine
+    m = manager(9000, slots=60)
+    m.open(1)
+    hold(m, 1, 4004)
+    m.fork(1, 2)
+    hold(m, 1, 16384)
+    for c in range(3, 50):
+        m.fork(1, c)
+    ids = [1, 2] + list(range(3, 50))
+    req = rt.BatchRequest()
+    req.ids, req.counts, req.tokens, req.want_counts, req.want_index = ids, [1] * 49, [0] * 49, [1] * 49, [0] * 49
+    for dtype, heads, own in ((torch.bfloat16, (16, 8, 128), 2 * -(-(48 + 4005) // 49)), (torch.float32, (16, 8, 128), 4005), (torch.bfloat16, (32, 1, 128), 4005)):
+        engine = SimpleNamespace(cache=SimpleNamespace(manager=m, page_sizes=[4]), _rt=rt, _prefix_group=0, _prefix_heads=[heads], dtype=dtype,
+                                 _prefix_places=Engine._prefix_places)
+        assert Engine._look_for_prefixes(engine, req, None, [m.length(r) + 1 for r in ids]) == (1, 16384, own), dtype
