@@ -725,23 +725,32 @@ class Engine:
         return [results[uid] for uid in uids]
 
     # ------------------------------------------------------------------ several answers, scores
+    def _open_own(self, ids: int) -> int:
+        """A live request of the engine's own; the first of ``ids`` ids in a row that nobody else has."""
+        first = self._own_ids
+        got = self.cache.manager.open(first)
+        if got != self._rt.Acquire.Ready:
+            raise MemoryError(f"no request can be opened: {got.name}; free pages per group: "
+                              f"{[self.cache.manager.free_pages(g) for g in range(self.cache.manager.num_groups())]}, free state slots: "
+                              f"{self.cache.manager.free_state_slots()}")
+        self._own_ids += ids
+        return first
+
     def answers(self, prompt: Sequence[int], n: int, params: Optional[SamplingParams] = None) -> List[GenerationResult]:
         """``n`` answers to one prompt (host token ids in and out).  The prompt runs once; its request is then forked, so that the answers
         hold its pages in common, and they decode side by side.  Answer i is sampled with seed ``params.seed`` + i (without a seed:
-        seeds of the engine's own), so answer 0 is what ``generate`` gives.  The requests live beside the scheduler's; a cache
-        without room for them raises MemoryError."""
+        seeds of the engine's own), so answer 0 is what ``generate`` gives (in bfloat16, whose products round by the batch, as far as no
+        two tokens lie that close).  The requests live beside the scheduler's; a cache without room for them raises MemoryError."""
         params = (params or SamplingParams()).normalized()
         prompt = [int(t) for t in prompt]
         if n < 1 or n > self.max_running_req:
             raise ValueError(f"{n} answers are refused: 1 to max_running_req ({self.max_running_req})")
         if not 1 <= len(prompt) <= self.max_seq_len:
             raise ValueError(f"a prompt of {len(prompt)} tokens is refused: 1 to {self.max_seq_len}")
-        first = self._own_ids
-        self._own_ids += n
+        first = self._open_own(n)
         seed = params.seed if params.seed is not None else (self.seed * 0x9E3779B97F4A7C15 + first * 0xD1B54A32D192ED03) & ((1 << 64) - 1)
         results = [GenerationResult([], "", None if params.logprobs is None else []) for _ in range(n)]
         request_of = {0: first}                              # of the answers that go on; the first of them has the prompt's own
-        self.open_request(first)
         try:
             portion = self.max_batch_tokens or len(prompt)
             for at in range(0, len(prompt), portion):
@@ -782,7 +791,8 @@ class Engine:
 
     def score(self, tokens: Sequence[int], top: int = 0, portion: int = 1024) -> List[TokenLogprob]:
         """The log probability of each of ``tokens`` behind the ones before it (none for the first one), with the entropy and the ``top``
-        most likely tokens of each place.  ``portion``: tokens of a step, whose logits are held at once."""
+        most likely tokens of each place.  ``portion``: tokens of a step, whose logits are held at once.  A cache without room raises
+        MemoryError."""
         tokens = [int(t) for t in tokens]
         if not 1 <= len(tokens) <= self.max_seq_len or portion < 1:
             raise ValueError(f"{len(tokens)} tokens are refused: 1 to {self.max_seq_len}, in portions of at least 1")
@@ -791,9 +801,7 @@ class Engine:
         if self.max_batch_tokens:
             portion = min(portion, self.max_batch_tokens)
         found: List[TokenLogprob] = []
-        request = self._own_ids
-        self._own_ids += 1
-        self.open_request(request)
+        request = self._open_own(1)
         try:
             for at in range(0, len(tokens) - 1, portion):
                 here = tokens[at:min(at + portion, len(tokens) - 1)]

@@ -480,3 +480,19 @@ def test_graphs_of_shared_pages_are_captured_when_they_come_again_and_kept(folde
     for bucket in (1, 2, 4):
         assert eng._prefix_graph(bucket, 1, 1 << 12, 7) is None and eng._prefix_graph(bucket, 1, 1 << 12, 7).bucket == bucket
     assert [key[0] for key in eng._prefix_graphs] == [2, 4]
+
+
+def test_answers_and_scores_without_a_slot_for_their_request(folders):
+    from llm_infer_rust_b200 import SamplingParams
+    folder, _ = folders("A", "float32")
+    eng = engine(folder, dtype="float32", page_size=4, max_running_req=2, max_total_tokens=64)
+    eng.open_request(1)
+    eng.open_request(2)
+    for call in (lambda: eng.answers([1, 2, 3], 2, SamplingParams(max_tokens=2)), lambda: eng.score([1, 2, 3])):
+        with pytest.raises(MemoryError, match="no request can be opened"):
+            call()
+    assert eng.cache.manager.live_requests() == 2 and eng.cache.manager.check() == ""
+    eng.close_request(1)
+    assert len(eng.score([1, 2, 3])) == 2 and len(eng.answers([1, 2, 3], 1, SamplingParams(max_tokens=2, ignore_eos=True))[0].tokens) == 2
+    eng.close_request(2)
+    assert len(eng.answers([1, 2, 3], 2, SamplingParams(max_tokens=2, ignore_eos=True))) == 2
