@@ -121,6 +121,14 @@ def read_prompts(args: argparse.Namespace) -> List[List[int]]:
     return prompts
 
 
+def several_answers(engine, prompts: List[List[int]], n: int, params):
+    """(prompt, result) of ``n`` answers to each prompt.  One that is empty or too long is the scheduler's, which ends it and goes on."""
+    for prompt in prompts:
+        served = 1 <= len(prompt) <= engine.max_seq_len
+        for result in engine.answers(prompt, n, params) if served else engine.generate([prompt] * n, params):
+            yield prompt, result
+
+
 def main(argv: Optional[List[str]] = None) -> int:
     args = parse_args(argv)
     if args.help:
@@ -167,7 +175,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     params = SamplingParams(args.temperature, args.top_k, args.top_p, args.ignore_eos, args.max_tokens,
                             args.seed if args.seed else None, args.logprobs)
     if args.answers > 1:
-        results = ((prompt, result) for prompt in prompts for result in engine.answers(prompt, args.answers, params))
+        results = several_answers(engine, prompts, args.answers, params)
     else:
         results = zip(prompts, engine.generate(prompts, params))
     for prompt, result in results:

@@ -496,3 +496,14 @@ def test_answers_and_scores_without_a_slot_for_their_request(folders):
     assert len(eng.score([1, 2, 3])) == 2 and len(eng.answers([1, 2, 3], 1, SamplingParams(max_tokens=2, ignore_eos=True))[0].tokens) == 2
     eng.close_request(2)
     assert len(eng.answers([1, 2, 3], 2, SamplingParams(max_tokens=2, ignore_eos=True))) == 2
+
+
+def test_command_line_goes_on_behind_a_prompt_that_is_refused(folders):
+    folder, _ = folders("A", "float32")
+    long = ",".join(["7"] * 70)
+    run = subprocess.run([sys.executable, "-m", "llm_infer_rust_b200", "--model-path", folder, "--prompt-ids", long, "--prompt-ids", "1,2,3", "--max-tokens",
+                          "4", "--ignore-eos", "--answers", "2", "--max-seq-len", "64", "--max-total-tokens", "256", "--max-running-req", "4",
+                          "--cuda-graph-bs", "0", "--log-level", "error"], cwd=ROOT, capture_output=True, text=True)
+    assert run.returncode == 0, run.stderr
+    lines = [json.loads(line) for line in run.stdout.splitlines()]
+    assert [(len(l["prompt_ids"]), len(l["output_ids"]), l["finish_reason"]) for l in lines] == [(70, 0, "abort")] * 2 + [(3, 4, "length")] * 2
