@@ -1,6 +1,6 @@
 // Decode attention behind shared prefixes (prefix.cuh) for float32, and for what the bfloat16 kernels do not take (head sizes that are
-// no multiple of 16 or above 256, more than 16 query heads a KV head, very many rows).  Compile with -DHEAD_DIM=<multiple
-// of 16, at most 512>; the real head size may be smaller.
+// no multiple of 16 or above 256, more than 16 query heads a KV head, more than 400 rows and groups, tensors off 16 bytes, tables and
+// caches that they cannot count).  Compile with -DHEAD_DIM=<multiple of 16, at most 512>; the real head size may be smaller.
 //
 // A CTA has a tile of up to 32 query vectors and walks its split of the keys in blocks of 32, two blocks of keys and values on their
 // way where they fit.  S = Q K^T (a warp eight keys) and O += P V (a warp every fourth group of eight dims) run on mma.sync in
